@@ -44,6 +44,21 @@ def make_fused_linear(w_type, K, W, n_out, Y, X, scales=None, norm_weight=None, 
     d.X, d.norm_weight, d.norm_eps, d.residual = X, norm_weight, norm_eps, residual
     return d
 
+
+
+class PagedKV(ctypes.Structure):
+    """struct hip_paged_kv of include/cccc_hip_quant.h."""
+    _fields_ = [(n, ctypes.c_int) for n in ("type", "head_dim", "n_kv_heads", "page_size", "n_pages", "n_seqs", "table_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_ulonglong) for n in ("page_stride", "scale_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("page_table", "ctx_len", "seq_start")]
+
+
+def make_paged_kv(type, head_dim, n_kv_heads, page_size, n_pages, k, v, page_table, table_stride, ctx_len, seq_start, n_seqs,
+                  k_scale=None, v_scale=None, page_stride=0, scale_stride=0) -> PagedKV:
+    return PagedKV(type, head_dim, n_kv_heads, page_size, n_pages, n_seqs, table_stride, k, v, k_scale, v_scale,
+                   page_stride, scale_stride, page_table, ctx_len, seq_start)
+
 EXPORTS = (
     "hip_convert",
     "hip_fp4_blockscale_to_bf16",
@@ -70,6 +85,10 @@ EXPORTS = (
     "hip_qk_norm_rope_kv_rows_bf16",
     "hip_attention_prefill_bf16",
     "hip_attention_prefill_fused_bf16",
+    "hip_qk_norm_rope_kv_paged_bf16",
+    "hip_kv_paged_read_bf16",
+    "hip_attention_paged_workspace_bytes",
+    "hip_attention_paged_bf16",
     "hip_add_bf16",
     "hip_swiglu_bf16",
     "hip_add_rms_norm_bf16",
@@ -155,6 +174,15 @@ class QuantLibrary:
         for name in ("hip_attention_prefill_bf16", "hip_attention_prefill_fused_bf16"):
             getattr(L, name).restype = i32
             getattr(L, name).argtypes = [vp] * 4 + [i32, i32, i32, i32, i32, i32]
+        kv, i64, u64 = ctypes.POINTER(PagedKV), ctypes.c_longlong, ctypes.c_ulonglong
+        L.hip_qk_norm_rope_kv_paged_bf16.restype = i32
+        L.hip_qk_norm_rope_kv_paged_bf16.argtypes = [kv] + [vp] * 7 + [i32, vp, i32, i32, i32, i32, i32, f32]
+        L.hip_kv_paged_read_bf16.restype = i32
+        L.hip_kv_paged_read_bf16.argtypes = [kv, vp, vp, i32, i64, i64]
+        L.hip_attention_paged_workspace_bytes.restype = u64
+        L.hip_attention_paged_workspace_bytes.argtypes = [kv, i32, i32, i32, i32, i32, i32]
+        L.hip_attention_paged_bf16.restype = i32
+        L.hip_attention_paged_bf16.argtypes = [kv, vp, vp, vp, u64] + [i32] * 8
         L.hip_add_bf16.restype = i32
         L.hip_add_bf16.argtypes = [vp, vp, vp, ctypes.c_ulonglong]
         L.hip_swiglu_bf16.restype = i32
@@ -222,6 +250,19 @@ class QuantLibrary:
 
     def quant_linear_fused(self, desc: FusedLinear) -> int:
         return self.c.hip_quant_linear_fused(ctypes.byref(desc))
+
+    def qk_norm_rope_kv_paged(self, cache: PagedKV, q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, n_positions, q_out, n_q_heads, n_tokens,
+                              ldq, ldk, ldv, eps=1e-6) -> int:
+        return self.c.hip_qk_norm_rope_kv_paged_bf16(cache, q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, n_positions, q_out, n_q_heads, n_tokens, ldq, ldk, ldv, eps)
+
+    def kv_paged_read(self, cache: PagedKV, k_out, v_out, n_tokens, token_stride, head_stride) -> int:
+        return self.c.hip_kv_paged_read_bf16(cache, k_out, v_out, n_tokens, token_stride, head_stride)
+
+    def attention_paged_workspace_bytes(self, cache: PagedKV, n_q_heads, n_tokens, max_new, max_ctx, window=0, n_sink=0) -> int:
+        return int(self.c.hip_attention_paged_workspace_bytes(cache, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink))
+
+    def attention_paged(self, cache: PagedKV, q, y, workspace, workspace_bytes, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, ldq, ldy) -> int:
+        return self.c.hip_attention_paged_bf16(cache, q, y, workspace, workspace_bytes, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, ldq, ldy)
 
     def set_sync(self, enabled: bool) -> int:
         return self.c.hip_quant_set_sync(1 if enabled else 0)

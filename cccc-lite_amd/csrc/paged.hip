@@ -1,0 +1,118 @@
+// C-ABI entry points of the paged key / value cache (kernels in paged.h and paged_attention.h).
+#include "../../include/cccc_hip_quant.h"
+#include "paged_attention.h"
+#include "runtime.h"
+#include <algorithm>
+#include <cmath>
+
+using namespace ccq;
+
+namespace
+{
+constexpr long long MOST_BLOCKS = 0xFFFFFF;        // of 256 lanes: a grid has fewer than 2^32
+
+inline bool aligned(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// The descriptor as the kernels take it; false: refused.
+bool paged_args(const hip_paged_kv* c, PagedArgs& a)
+{
+    if (!c || (c->type != CCCC_BFLOAT16 && c->type != CCCC_FP8_E4M3 && c->type != CCCC_FP8_E5M2) || (c->head_dim != 64 && c->head_dim != 128)) { return false; }
+    if (c->n_kv_heads <= 0 || c->n_kv_heads > 1024 || c->n_pages <= 0 || c->n_seqs <= 0 || c->n_seqs > (1 << 24) || c->table_stride <= 0) { return false; }
+    if (c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)) != 0) { return false; }
+    if (!c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16) || !c->page_table || !c->ctx_len || !c->seq_start) { return false; }
+    if (!aligned(c->page_table, 4) || !aligned(c->ctx_len, 4) || !aligned(c->seq_start, 4)) { return false; }
+    const bool fp8 = c->type != CCCC_BFLOAT16;
+    const size_t rows = (size_t)c->n_kv_heads * c->page_size, dense = rows * c->head_dim * (fp8 ? 1 : 2);
+    if (c->page_stride % 16 != 0 || (c->page_stride != 0 && c->page_stride < dense)) { return false; }
+    if (fp8 && (!c->k_scale || !c->v_scale || c->scale_stride % 16 != 0 || (c->scale_stride != 0 && c->scale_stride < rows))) { return false; }
+    a.k = (const uint8_t*)c->k;
+    a.v = (const uint8_t*)c->v;
+    a.k_scale = (const uint8_t*)c->k_scale;
+    a.v_scale = (const uint8_t*)c->v_scale;
+    a.table = (const int*)c->page_table;
+    a.ctx_len = (const int*)c->ctx_len;
+    a.seq_start = (const int*)c->seq_start;
+    a.page_stride = c->page_stride ? (size_t)c->page_stride : dense;
+    a.scale_stride = c->scale_stride ? (size_t)c->scale_stride : rows;
+    a.n_pages = c->n_pages;
+    a.n_kv = c->n_kv_heads;
+    a.n_seqs = c->n_seqs;
+    a.table_stride = c->table_stride;
+    a.shift = __builtin_ctz((unsigned)c->page_size);
+    a.max_ctx = (int)std::min((long long)c->table_stride << a.shift, 1LL << 30);
+    return true;
+}
+
+#define CCQ_PAGED_KERNEL(KERNEL, c)                                                                                    \
+    ((c)->head_dim == 64 ? ((c)->type == CCCC_BFLOAT16 ? KERNEL<DT_BF16, 64> : (c)->type == CCCC_FP8_E4M3 ? KERNEL<DT_E4M3, 64> : KERNEL<DT_E5M2, 64>) \
+                         : ((c)->type == CCCC_BFLOAT16 ? KERNEL<DT_BF16, 128> : (c)->type == CCCC_FP8_E4M3 ? KERNEL<DT_E4M3, 128> : KERNEL<DT_E5M2, 128>))
+
+bool attention_args(const hip_paged_kv* c, PagedArgs& a, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink)
+{
+    if (!paged_args(c, a) || n_q_heads <= 0 || n_q_heads % c->n_kv_heads != 0 || n_q_heads / c->n_kv_heads > 64) { return false; }
+    if (n_tokens < 0 || max_new <= 0 || max_ctx <= 0 || window < 0 || n_sink < 0) { return false; }
+    if ((long long)n_tokens * n_q_heads > MOST_BLOCKS) { return false; }
+    a.max_ctx = std::min(a.max_ctx, max_ctx);
+    return true;
+}
+}    // namespace
+
+int hip_qk_norm_rope_kv_paged_bf16(const hip_paged_kv* cache, const void* q, const void* k, const void* v, const void* q_norm_w, const void* k_norm_w, const void* cos_tab, const void* sin_tab,
+                                   int n_positions, void* q_out, int n_q_heads, int n_tokens, int ldq, int ldk, int ldv, float epsilon)
+{
+    PagedArgs a;
+    if (!paged_args(cache, a) || n_q_heads < 0 || n_q_heads > 65536 || n_tokens < 0) { return -1; }
+    const int dim = cache->head_dim;
+    if ((n_q_heads > 0 && (!q || !q_out)) || !k || !v || (q_norm_w == nullptr) != (k_norm_w == nullptr) || (cos_tab == nullptr) != (sin_tab == nullptr)) { return -1; }
+    if (cos_tab && n_positions <= 0) { return -1; }
+    for (const void* p : { q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, (const void*)q_out })
+    {
+        if (!aligned(p, 16)) { return -1; }
+    }
+    if ((n_q_heads > 0 && (ldq % 8 != 0 || ldq < (long long)n_q_heads * dim)) || ldk % 8 != 0 || ldv % 8 != 0 || ldk < (long long)a.n_kv * dim || ldv < (long long)a.n_kv * dim) { return -1; }
+    const int per_wg = 256 * 8 / dim;
+    const long long blocks = (long long)n_tokens * ((n_q_heads + 2 * a.n_kv + per_wg - 1) / per_wg);
+    if (blocks > MOST_BLOCKS) { return -1; }
+    if (n_tokens == 0) { return 0; }
+    const PagedAppend p = { (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)q_norm_w, (const uint16_t*)k_norm_w, (const uint16_t*)cos_tab, (const uint16_t*)sin_tab,
+                            (uint16_t*)q_out, n_q_heads, n_tokens, n_positions, (size_t)ldq, (size_t)ldk, (size_t)ldv, epsilon };
+    const auto kernel = CCQ_PAGED_KERNEL(paged_append_kernel, cache);
+    kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, p);
+    return finish("qk_norm_rope_kv_paged");
+}
+
+int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void* v_out, int n_tokens, long long token_stride, long long head_stride)
+{
+    PagedArgs a;
+    if (!paged_args(cache, a) || n_tokens < 0 || !k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16)) { return -1; }
+    if (token_stride % 8 != 0 || head_stride % 8 != 0 || token_stride < cache->head_dim || head_stride < cache->head_dim) { return -1; }
+    const int per_wg = 256 * 8 / cache->head_dim;
+    const long long blocks = (long long)n_tokens * ((2 * a.n_kv + per_wg - 1) / per_wg);
+    if (blocks > MOST_BLOCKS) { return -1; }
+    if (n_tokens == 0) { return 0; }
+    const auto kernel = CCQ_PAGED_KERNEL(paged_read_kernel, cache);
+    kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, (uint16_t*)k_out, (uint16_t*)v_out, token_stride, head_stride);
+    return finish("kv_paged_read");
+}
+
+unsigned long long hip_attention_paged_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink)
+{
+    PagedArgs a;
+    if (!attention_args(cache, a, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink)) { return 0; }
+    return 0;
+}
+
+int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, void* workspace, unsigned long long workspace_bytes, int n_q_heads, int n_tokens, int max_new, int max_ctx,
+                             int window, int n_sink, int ldq, int ldy)
+{
+    PagedArgs a;
+    if (!attention_args(cache, a, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink)) { return -1; }
+    if (!q || !y || !aligned(q, 16) || !aligned(y, 16) || !aligned(workspace, 16) || (workspace == nullptr && workspace_bytes != 0)) { return -1; }
+    const long long width = (long long)n_q_heads * cache->head_dim;
+    if (ldq % 8 != 0 || ldy % 8 != 0 || ldq < width || ldy < width) { return -1; }
+    if (n_tokens == 0) { return 0; }
+    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv, n_tokens, max_new, window, n_sink, 1.0f / sqrtf((float)cache->head_dim) };
+    const auto kernel = CCQ_PAGED_KERNEL(paged_attention_rows_kernel, cache);
+    kernel<<<(unsigned)((long long)n_tokens * ((n_q_heads + 3) / 4)), 256, 0, stream()>>>(a, p);
+    return finish("attention_paged");
+}

@@ -353,6 +353,73 @@ C_EXPORT int hip_argmax_pick_embed_bf16(const void* workspace, unsigned int n, v
                                         const void* embed_W, void* embed_y, int D, int n_rows);
 
 /*
+ * A batch of sequences on a paged key / value cache (no counterpart in the reference, whose cache is one (128, T_kv, 1, Hkv) tensor per layer for one
+ * sequence, cccc/MatrixEx.cpp:3018-3104).  The neighbours above for continuous batching: new tokens of many sequences side by side, one each, a few
+ * or a whole chunk; rows held as BF16 or, quantised as they are written, as FP8.  Activations are token-major BF16.
+ *
+ * What a call is told about the batch lies in device memory, so that a captured graph can be replayed with other lengths and pages:
+ *   seq_start int32 [n_seqs + 1]: rows seq_start[s] .. seq_start[s + 1] - 1 of the activations are the new tokens of sequence s (none: an empty range).
+ *                   Rows before the first or behind the last sequence, up to n_tokens, are left as they were.
+ *   ctx_len   int32 [n_seqs]: rows of the sequence in the cache, its new tokens included; those are the last positions.
+ *   page_table int32 [n_seqs][table_stride]: position `pos` lies in page page_table[s][pos / page_size], at row pos % page_size.  Sequences may share pages.
+ * A length beyond table_stride * page_size (for the attention also max_ctx) is cut to it.  A page outside 0 .. n_pages - 1 is never touched: its rows are not
+ * written, read back as 0 and seen by no token; likewise new tokens at negative positions (more new tokens than ctx_len).
+ *
+ * FP8 rows: codes c = fp8(x / 2^e), nearest even, one exponent byte e + 127 per row and kv head, 2^e the smallest power of two >= 2^-100 for which the row's
+ * largest finite magnitude stays within 448 (E4M3) or 57344 (E5M2); e is at most 119 or 112, beyond it codes saturate.  Powers of two cost no precision within
+ * 2^15 (E4M3) or 2^30 of the largest value, and c * 2^e is exact in BF16 (values under 2^-109 or 2^-116 become 0).  An infinity is held as NaN in E4M3 and
+ * kept in E5M2.
+ */
+typedef struct hip_paged_kv
+{
+    int type;                /* 3 (BF16), 4 (FP8_E4M3) or 5 (FP8_E5M2) */
+    int head_dim;            /* 64 or 128 */
+    int n_kv_heads;
+    int page_size;           /* rows per page: a power of two from 16 to 4096 */
+    int n_pages;
+    int n_seqs;
+    int table_stride;        /* entries per sequence in page_table */
+    void* k;                 /* pages [n_kv_heads][page_size][head_dim], 16-byte aligned */
+    void* v;
+    void* k_scale;           /* FP8: exponent bytes [n_kv_heads][page_size] per page; ignored for BF16 */
+    void* v_scale;
+    unsigned long long page_stride;  /* bytes from page to page of k and of v, a multiple of 16; 0: dense */
+    unsigned long long scale_stride; /* bytes from page to page of the exponent bytes, a multiple of 16; 0: dense */
+    const void* page_table;
+    const void* ctx_len;
+    const void* seq_start;
+} hip_paged_kv;
+
+/* Per-head RMSNorm (NULL, NULL: none) and RoPE of the new tokens' q and k and the append of k and v to the pages.  q, k and v are rows of n_q_heads and
+ * n_kv_heads heads with row pitches ldq, ldk, ldv (elements, multiples of 8), so that one projection's output [q | k | v] can be passed as it is; q_out
+ * is dense [n_tokens][n_q_heads][head_dim] (q and q_out may be the same dense buffer).  cos_tab, sin_tab BF16 [n_positions][head_dim / 2], the row of a
+ * token's position; a token at a position past n_positions is left out.  Both NULL: no rotation.  n_q_heads 0 (q, q_out NULL): keys and values only.
+ * Norm and rotation are FP32 with one rounding, to BF16 or to the codes (hip_qk_norm_rope_kv_rows_bf16 rounds between them as the reference does).
+ * 0 for n_tokens 0; pointers 16-byte aligned, else -1. */
+C_EXPORT int hip_qk_norm_rope_kv_paged_bf16(const hip_paged_kv* cache, const void* q, const void* k, const void* v,
+                                            const void* q_norm_w, const void* k_norm_w, const void* cos_tab, const void* sin_tab, int n_positions,
+                                            void* q_out, int n_q_heads, int n_tokens, int ldq, int ldk, int ldv, float epsilon);
+
+/* The cached rows of the tokens that seq_start and ctx_len name (the whole sequences with seq_start the sums of ctx_len) back as BF16, exactly: row t of kv head h
+ * to k_out + t * token_stride + h * head_stride, likewise v_out (elements, multiples of 8).  n_kv_heads * head_dim and head_dim give [n_tokens][n_kv_heads]
+ * [head_dim]; head_dim and t_kv * head_dim the contiguous cache [kv_head][t_kv][head_dim] of the entries above.  The strides must keep rows apart.
+ * Rows that are not there (see above) give 0.  k_out and v_out 16-byte aligned; 0 for n_tokens 0. */
+C_EXPORT int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void* v_out, int n_tokens, long long token_stride, long long head_stride);
+
+/* Causal GQA attention of the new tokens over the pages of their sequences, keys and values of the new tokens already appended: a token at position p sees
+ * positions 0 .. p, with window > 0 only p - window + 1 .. p and the first n_sink ones.  q [n_tokens] rows of n_q_heads heads with row pitch ldq, y likewise
+ * with ldy (multiples of 8); scale 1 / sqrt(head_dim).  FP32 scores, softmax and sums, probabilities rounded to BF16 for the product with V, one rounding
+ * of the result.  What a token does not see does not reach it, whatever it holds; a token that sees nothing, or whose scores are all minus infinity,
+ * gives 0.  Any number of query heads per kv head up to 64.
+ * max_new and max_ctx are the most new tokens and the most rows that any sequence may have (a graph: over all its replays): grids and workspace follow from
+ * them, and a sequence with more new tokens than max_new is left out.  workspace: hip_attention_paged_workspace_bytes(the same arguments) bytes, 16-byte
+ * aligned, content between calls of no matter; calls that share one must be ordered.  With fewer bytes, or NULL and 0, the keys are split over fewer workgroups.
+ * y must not overlap q.  0 for n_tokens 0. */
+C_EXPORT unsigned long long hip_attention_paged_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink);
+C_EXPORT int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, void* workspace, unsigned long long workspace_bytes,
+                                      int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink, int ldq, int ldy);
+
+/*
  * Library controls (no counterpart in the reference, which always uses the null stream and always
  * synchronises: cccc-hip/hip_functions.cpp:32-42).
  * Both switches are per host thread, like the reference's current-device pointer (cccc/GpuControl.cpp:18);
