@@ -55,6 +55,36 @@ bool attention_args(const hip_paged_kv* c, PagedArgs& a, int n_q_heads, int n_to
     a.max_ctx = std::min(a.max_ctx, max_ctx);
     return true;
 }
+// How a call's rows are split: which kernels run, and over how many ranges of keys at most.
+struct Plan
+{
+    bool rows, tiles;               // the kernel for up to 16 rows of a kv head, the one for more
+    int min_rows;                   // sequences of at most so many rows are the first one's
+    long long n_tiles;              // at most
+    int rows_split, tiles_split, n_split;
+};
+
+constexpr int TILE_ROWS = 128;
+
+Plan plan_attention(const PagedArgs& a, int group, int n_tokens, int max_new, int window, int n_sink)
+{
+    const long long most_rows = (long long)std::min(max_new, n_tokens) * group;
+    Plan plan = {};
+    plan.tiles = most_rows > 16;
+    plan.rows = !plan.tiles || (group <= 16 && a.n_seqs > 1 && n_tokens < (long long)a.n_seqs * max_new);
+    plan.min_rows = plan.tiles && plan.rows ? 16 : 0;
+    const long long rows = (long long)n_tokens * group;
+    plan.n_tiles = rows / TILE_ROWS + std::min<long long>(a.n_seqs, rows / (plan.min_rows + 1));
+    const long long wide = 2LL * cu_count();
+    const long long keys = window == 0 ? a.max_ctx : std::min<long long>(a.max_ctx, (long long)window + n_sink + max_new);
+    auto split = [&](long long workgroups, long long most) { return (int)std::max<long long>(1, std::min({ wide / std::max<long long>(workgroups, 1), most, 64LL })); };
+    plan.rows_split = plan.rows ? split((long long)a.n_seqs * a.n_kv, keys / 256) : 1;
+    plan.tiles_split = plan.tiles ? split(plan.n_tiles * a.n_kv, keys / 256) : 1;
+    plan.n_split = std::max(plan.rows_split, plan.tiles_split);
+    return plan;
+}
+
+size_t partial_bytes(int n_split, size_t outputs, int dim) { return n_split < 2 ? 0 : (outputs * ((size_t)n_split * (dim + 2) + 1) * 4 + 15) & ~(size_t)15; }
 }    // namespace
 
 int hip_qk_norm_rope_kv_paged_bf16(const hip_paged_kv* cache, const void* q, const void* k, const void* v, const void* q_norm_w, const void* k_norm_w, const void* cos_tab, const void* sin_tab,
@@ -98,8 +128,9 @@ int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void* v_out, 
 unsigned long long hip_attention_paged_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink)
 {
     PagedArgs a;
-    if (!attention_args(cache, a, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink)) { return 0; }
-    return 0;
+    if (!attention_args(cache, a, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink) || n_tokens == 0) { return 0; }
+    const Plan plan = plan_attention(a, n_q_heads / a.n_kv, n_tokens, max_new, window, n_sink);
+    return partial_bytes(plan.n_split, (size_t)n_tokens * n_q_heads, cache->head_dim);
 }
 
 int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, void* workspace, unsigned long long workspace_bytes, int n_q_heads, int n_tokens, int max_new, int max_ctx,
@@ -108,11 +139,34 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
     PagedArgs a;
     if (!attention_args(cache, a, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink)) { return -1; }
     if (!q || !y || !aligned(q, 16) || !aligned(y, 16) || !aligned(workspace, 16) || (workspace == nullptr && workspace_bytes != 0)) { return -1; }
-    const long long width = (long long)n_q_heads * cache->head_dim;
+    const int dim = cache->head_dim;
+    const long long width = (long long)n_q_heads * dim;
     if (ldq % 8 != 0 || ldy % 8 != 0 || ldq < width || ldy < width) { return -1; }
     if (n_tokens == 0) { return 0; }
-    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv, n_tokens, max_new, window, n_sink, 1.0f / sqrtf((float)cache->head_dim) };
-    const auto kernel = CCQ_PAGED_KERNEL(paged_attention_rows_kernel, cache);
-    kernel<<<(unsigned)((long long)n_tokens * ((n_q_heads + 3) / 4)), 256, 0, stream()>>>(a, p);
+    const int group = n_q_heads / a.n_kv;
+    const size_t outputs = (size_t)n_tokens * n_q_heads;
+    Plan plan = plan_attention(a, group, n_tokens, max_new, window, n_sink);
+    while (plan.n_split > 1 && partial_bytes(plan.n_split, outputs, dim) > workspace_bytes) { plan.n_split--; }
+    if (plan.n_tiles * a.n_kv > MOST_BLOCKS || (long long)a.n_seqs * a.n_kv > MOST_BLOCKS) { return -1; }
+    PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)workspace, (size_t)ldq, (size_t)ldy, n_q_heads, group, n_tokens, max_new, window, n_sink, plan.n_split, 1, plan.min_rows,
+                         1.4426950408889634f / sqrtf((float)dim) };
+    if (plan.rows)
+    {
+        p.split = std::min(plan.rows_split, plan.n_split);
+        const auto kernel = CCQ_PAGED_KERNEL(paged_attention_rows_kernel, cache);
+        kernel<<<dim3((unsigned)(a.n_seqs * a.n_kv), p.split), 256, 0, stream()>>>(a, p);
+    }
+    if (plan.tiles)
+    {
+        p.split = std::min(plan.tiles_split, plan.n_split);
+        const auto kernel = CCQ_PAGED_KERNEL(paged_attention_tile_kernel, cache);
+        kernel<<<dim3((unsigned)(plan.n_tiles * a.n_kv), p.split), 256, 0, stream()>>>(a, p);
+    }
+    if (plan.n_split > 1)
+    {
+        const unsigned blocks = (unsigned)(n_tokens * ((n_q_heads * dim + 1023) / 1024));
+        if (dim == 64) { paged_attention_combine_kernel<64><<<blocks, 256, 0, stream()>>>(a, p); }
+        else { paged_attention_combine_kernel<128><<<blocks, 256, 0, stream()>>>(a, p); }
+    }
     return finish("attention_paged");
 }

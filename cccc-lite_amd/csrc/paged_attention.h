@@ -1,6 +1,10 @@
 // Causal attention of the new tokens of a batch of sequences over their pages.
+//   y = sum_k p_k v_k / sum_k p_k,  p_k = exp(scale q k - m),  over the keys that the token sees, m a running maximum.
+// The rows of a kv head are those of the sequence's new tokens and of the query heads that share it: row r is token r / group, head r % group.
+// Two kernels take them, 16 rows or 128 at a time, each with the keys in ranges where there are few rows; a third adds the ranges.
 #pragma once
 #include "paged.h"
+#include <type_traits>
 
 namespace ccq
 {
@@ -9,72 +13,857 @@ struct PagedAttention
 {
     const uint16_t* q;
     uint16_t* y;
+    float* partial;                 // [range][token][head][dim] sums, [range][token][head] (max, sum), [token][head] ranges: only where there are ranges
     size_t ldq, ldy;
     int n_q, group, n_tokens, max_new, window, n_sink;
-    float scale;
+    int n_split;                    // most ranges of a row, as `partial` is laid out
+    int split;                      // ranges of this launch, n_split or fewer
+    int min_rows;                   // sequences of at most so many rows per kv head are the other kernel's
+    float scale;                    // 1 / sqrt(dim) log2 e
+
+    __device__ __forceinline__ size_t outputs() const { return (size_t)n_tokens * n_q; }
+    __device__ __forceinline__ float* sums(int range, size_t row, int dim) const { return partial + ((size_t)range * outputs() + row) * dim; }
+    __device__ __forceinline__ float2* stats(int range, size_t row, int dim) const { return (float2*)(partial + (size_t)n_split * outputs() * dim) + (size_t)range * outputs() + row; }
+    __device__ __forceinline__ int* ranges(size_t row, int dim) const { return (int*)(partial + (size_t)n_split * outputs() * (dim + 2)) + row; }
 };
 
-// Element d of a cached row, in FP32.
-template <int TYPE>
-__device__ __forceinline__ float paged_element(const uint8_t* row, int d, float scale)
+// The new tokens of a sequence that a call computes: tokens first .. first + n - 1 of the activations, the first of them at position pos.
+struct NewTokens
 {
-    if constexpr (TYPE == DT_BF16) { return bf16_bits_to_f32(((const uint16_t*)row)[d]); }
-    else { return (TYPE == DT_E4M3 ? e4m3_to_f32(row[d]) : e5m2_to_f32(row[d])) * scale; }
+    int first, n, pos;
+};
+
+__device__ __forceinline__ NewTokens new_tokens(const PagedArgs& a, const PagedAttention& p, int s)
+{
+    const int begin = a.seq_start[s], end = a.seq_start[s + 1];
+    const int first = max(begin, 0), n = min(end, p.n_tokens) - first;
+    if (n <= 0 || (long long)end - begin > p.max_new) { return { first, 0, 0 }; }
+    return { first, n, paged_rows(a, s) - (end - first) };
 }
 
-// One wave per (token, query head), a lane per key for the scores and one or two dims per lane for the products, 64 keys at a time with a running
-// maximum and sum.
+// The blocks of SIZE keys that tokens at positions lo .. hi see: the first `sinks` ones, then from block sinks + skip on; n in all.
+template <int SIZE>
+struct KeyBlocks
+{
+    int n, sinks, skip;
+
+    __device__ __forceinline__ KeyBlocks(const PagedAttention& p, int lo, int hi)
+    {
+        const int blocks = max(hi + SIZE, 0) / SIZE;
+        const int from = p.window == 0 ? 0 : max(lo - p.window + 1, 0) / SIZE;
+        sinks = min((int)min(((long long)p.n_sink + SIZE - 1) / SIZE, (long long)blocks), from);
+        skip = from - sinks;
+        n = blocks - skip;
+    }
+    __device__ __forceinline__ int block(int i) const { return i < sinks ? i : i + skip; }
+    // every token at positions lo .. hi sees every key of block b
+    __device__ static __forceinline__ bool plain(const PagedAttention& p, int lo, int hi, int b)
+    {
+        return b * SIZE + SIZE - 1 <= lo && (p.window == 0 || b * SIZE > hi - p.window || b * SIZE + SIZE <= p.n_sink);
+    }
+    // none of them sees any
+    __device__ static __forceinline__ bool hidden(const PagedAttention& p, int lo, int hi, int b)
+    {
+        return b * SIZE > hi || (p.window != 0 && b * SIZE + SIZE - 1 <= lo - p.window && b * SIZE >= p.n_sink);
+    }
+};
+
+__device__ __forceinline__ bool sees(const PagedAttention& p, int pos, int key) { return key <= pos && (p.window == 0 || key > pos - p.window || key < p.n_sink); }
+
+// The weights' running maximum moves only when a score exceeds it by more than this (in log2): until then they are at most 2^8, which FP32 sums
+// and BF16's exponent do not notice, and the sums are left alone.
+constexpr float PA_LAG = 8.0f;
+
+// Workgroup barrier that orders LDS traffic only: __syncthreads() waits for the loads in flight too.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+typedef short pa_b16x4 __attribute__((ext_vector_type(4)));
+typedef int pa_b32x2 __attribute__((ext_vector_type(2)));
+
+// Transposing reads of LDS, by 16 lanes each.  16 bits: lane i points at 4 elements of row i / 4, piece i % 4, and receives element i of the 4 rows.
+__device__ __forceinline__ u32x2 lds_transposed16(const uint8_t* at)
+{
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_b16x4*)at));
+}
+
+// 8 bits: lane i points at 8 elements of row i / 2, piece i % 2, and receives element i of the 8 rows.
+__device__ __forceinline__ u32x2 lds_transposed8(const uint8_t* at)
+{
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) pa_b32x2*)at));
+}
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p; }
+
+// A byte per lane to a dword per lane of LDS.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void bytes_to_lds(uint32_t lds, const uint8_t* at)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+__device__ __forceinline__ float max8(const float* s)
+{
+    return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+}
+
+// Bits of a dword's two BF16 values that are infinite or NaN, as a mask over both; and whether there are any in four dwords.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w)
+{
+    return (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u);
+}
+__device__ __forceinline__ uint32_t not_finite(const u32x4& v) { return not_finite(v[0]) | not_finite(v[1]) | not_finite(v[2]) | not_finite(v[3]); }
+
+// What is infinite or NaN among eight BF16 values, apart from the rest: the rest with zeros there, and 1 where KIND is (0: +inf, 1: -inf, 2: NaN).
+__device__ __forceinline__ u32x4 finite_part(const u32x4& v)
+{
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+    {
+        const uint32_t bad = not_finite(v[i]);
+        r[i] = v[i] & ~((bad >> 15) * 0xFFFFu);
+    }
+    return r;
+}
+__device__ __forceinline__ u32x4 where_kind(const u32x4& v, int kind)
+{
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+    {
+        r[i] = 0;
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+        {
+            const uint32_t x = v[i] >> (16 * half) & 0xFFFFu;
+            const bool is = kind == 0 ? x == 0x7F80u : kind == 1 ? x == 0xFF80u : (x & 0x7FFFu) > 0x7F80u;
+            r[i] |= is ? 0x3F80u << (16 * half) : 0u;
+        }
+    }
+    return r;
+}
+__device__ __forceinline__ float value_of_kind(int kind) { return kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf(""); }
+
+// Up to 16 rows of a kv head: single tokens, or a few.  Bound by the cached rows' way from memory.
+//   A workgroup of four waves takes a range of the sequence's blocks of 32 keys, a wave every fourth block, each with a pipeline of its own: rows go by
+// direct loads to the wave's part of LDS, STAGES blocks ahead, and nothing but the wave's own count of loads in flight is waited for.
+//   scores: v_mfma_f32_16x16x32_bf16, key rows as row operand, the 16 queries as columns: D lane (row j = lane % 16, g = lane / 16) holds keys 4 g .. + 3
+//           of 16.  FP8 keys become BF16 in registers, times their power of two (a lane's operand is one key's): exact.
+//   V p:    the eight weights of a lane (keys 4 g .. + 3 and 16 + 4 g .. + 3) are its column operand as they are; the row operand (dim, the same keys)
+//           comes from transposing reads.  FP8 values' powers of two go to the weights.
+// LDS: chunk c (16 bytes) of row r lies at c ^ swizzle(r), so that the operand reads hit all banks.
+// Grid: (sequences x kv heads) x ranges.
 template <int TYPE, int DIM>
 __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedArgs a, const PagedAttention p)
 {
-    constexpr int ROW = DIM * CODE_BYTES<TYPE>, OUT = DIM / 64;
-    __shared__ float q_s[4][DIM];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int parts = (p.n_q + 3) / 4, t = blockIdx.x / parts, head = blockIdx.x % parts * 4 + wave;
+    constexpr int KEYS = 32, STAGES = 2;
+    constexpr int ROW = DIM * CODE_BYTES<TYPE>, CHUNKS = ROW / 16, SIDE = KEYS * ROW, SCALES = TYPE == DT_BF16 ? 0 : 256, STAGE = 2 * SIDE + SCALES;
+    constexpr int ROWS_PER_LOAD = 1024 / ROW, LOADS = SIDE / 1024;
+    constexpr int SUM = DIM + 4;                                            // floats per row of the sums
+    constexpr int LDS = STAGES * STAGE * 4 > 4 * 16 * SUM * 4 ? STAGES * STAGE * 4 : 4 * 16 * SUM * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
+    __shared__ float2 stat[4][16];
+    const int kvh = blockIdx.x % a.n_kv, s = blockIdx.x / a.n_kv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int j = lane & 15, g = lane >> 4;
+    const NewTokens mine = new_tokens(a, p, s);
+    const int n_rows = mine.n * p.group;
+    if (n_rows == 0 || n_rows > 16) { return; }
+    const int last_pos = mine.pos + mine.n - 1;
+    const KeyBlocks<KEYS> blocks(p, mine.pos, last_pos);
+    const int per = max(((blocks.n + p.split - 1) / p.split + 3) & ~3, 8);
+    const int n_ranges = max((blocks.n + per - 1) / per, 1);
+    const int range = blockIdx.y, begin = range * per, end = min(blocks.n, begin + per);
+    if (range >= n_ranges) { return; }
+
+    const int row = min(j, n_rows - 1), token = row / p.group, head = kvh * p.group + row % p.group;
+    const int my_pos = mine.pos + token;
+    // FP8: eight elements 32 c + 8 g .. + 7, as for BF16
+    u32x4 qf[DIM / 32];
+#pragma unroll
+    for (int c = 0; c < DIM / 32; c++) { qf[c] = *(const u32x4*)(p.q + (size_t)(mine.first + token) * p.ldq + (size_t)head * DIM + c * 32 + g * 8); }
+
+    auto key_swizzle = [](int r) { return r / (256 / ROW) % CHUNKS; };
+    auto value_swizzle = [](int r) {
+        if constexpr (TYPE == DT_BF16) { return DIM == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
+        else { return DIM == 128 ? ((r >> 1) & 3) | ((r >> 4) & 1) << 2 : ((r >> 2) & 1) | ((r >> 4) & 1) << 1; }
+    };
+    uint8_t* const my_lds = lds + wave * STAGES * STAGE;
+    const uint32_t my_lds0 = __builtin_amdgcn_readfirstlane(lds_offset(my_lds));
+    // the wave's n-th block of the range is list entry begin + wave + 4 n
+    const int n_mine = begin + wave < end ? (end - begin - wave + 3) / 4 : 0;
+    int pages = 0;                                                          // lane l: page of rows 16 (l % 2) of the wave's block n0 + l / 2; -1: none
+    auto look_up = [&](int n0) {
+        const int i = begin + wave + 4 * (n0 + (lane >> 1));
+        const int pos = blocks.block(i) * KEYS + 16 * (lane & 1);
+        pages = i >= end || pos > last_pos ? 0 : max(paged_page(a, s, pos), -1);
+    };
+    int tag[STAGES];                                                        // per stage: bits of the half blocks that have no page
+    auto stage = [&](int n, int at) {
+        if (n % 32 == 0) { look_up(n); }
+        const int key0 = blocks.block(begin + wave + 4 * n) * KEYS;
+        int bad = 0;
+        size_t offset[2], scale_offset[2];
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+        {
+            const int page = __builtin_amdgcn_readlane(pages, (n % 32) * 2 + half);
+            bad |= page < 0 ? 1 << half : 0;
+            const size_t r = paged_row(a, kvh, key0 + 16 * half);
+            offset[half] = max(page, 0) * a.page_stride + r * ROW;
+            scale_offset[half] = max(page, 0) * a.scale_stride + r;
+        }
+        const uint32_t to = my_lds0 + at * STAGE;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++)
+        {
+            const int r = i * ROWS_PER_LOAD + lane / CHUNKS, c = lane % CHUNKS;
+            const size_t from = offset[i * ROWS_PER_LOAD / 16] - (size_t)(i * ROWS_PER_LOAD / 16 * 16 * ROW);
+            load_to_lds<true>(to + i * 1024, a.k + from, (uint32_t)(r * ROW + (c ^ key_swizzle(r)) * 16));
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; i++)
+        {
+            const int r = i * ROWS_PER_LOAD + lane / CHUNKS, c = lane % CHUNKS;
+            const size_t from = offset[i * ROWS_PER_LOAD / 16] - (size_t)(i * ROWS_PER_LOAD / 16 * 16 * ROW);
+            load_to_lds<true>(to + SIDE + i * 1024, a.v + from, (uint32_t)(r * ROW + (c ^ value_swizzle(r)) * 16));
+        }
+        if constexpr (TYPE != DT_BF16)
+        {
+            // lanes 0 .. 31: the keys' exponents, then the values'
+            bytes_to_lds(to + 2 * SIDE, (lane < 32 ? a.k_scale : a.v_scale) + (lane & 16 ? scale_offset[1] : scale_offset[0]) + (lane & 15));
+        }
+        tag[at] = bad;
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    f32x4 out[DIM / 16];
+#pragma unroll
+    for (int d = 0; d < DIM / 16; d++) { out[d] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f }; }
+
+    auto block = [&](int n, int at) {
+        const uint8_t* const kb = my_lds + at * STAGE;
+        const uint8_t* const vb = kb + SIDE;
+        const int b = blocks.block(begin + wave + 4 * n), bad = tag[at];
+        float vscale[8];
+        f32x4 acc[2] = { { 0.0f, 0.0f, 0.0f, 0.0f }, { 0.0f, 0.0f, 0.0f, 0.0f } };
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+        {
+            const int r = 16 * kt + j;
+            float kscale = 1.0f;
+            if constexpr (TYPE != DT_BF16) { kscale = bits_to_f32(*(const uint32_t*)(kb + 2 * SIDE + r * 4) << 23); }
+#pragma unroll
+            for (int c = 0; c < DIM / 32; c++)
+            {
+                u32x4 kf;
+                if constexpr (TYPE == DT_BF16) { kf = *(const u32x4*)(kb + r * ROW + ((4 * c + g) ^ key_swizzle(r)) * 16); }
+                else
+                {
+                    const u32x2 codes = *(const u32x2*)(kb + r * ROW + ((2 * c + (g >> 1)) ^ key_swizzle(r)) * 16 + (g & 1) * 8);
+                    const u32x2 lo = fp8x4_to_bf16<TYPE>(codes[0], kscale), hi = fp8x4_to_bf16<TYPE>(codes[1], kscale);
+                    kf = u32x4{ lo[0], lo[1], hi[0], hi[1] };
+                }
+                acc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[c]), acc[kt], 0, 0, 0);
+            }
+        }
+        if constexpr (TYPE != DT_BF16)
+        {
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+            {
+                const u32x4 e = *(const u32x4*)(kb + 2 * SIDE + 128 + (16 * kt + 4 * g) * 4);
+#pragma unroll
+                for (int v = 0; v < 4; v++) { vscale[4 * kt + v] = bits_to_f32(e[v] << 23); }
+            }
+        }
+        u32x4 vf[DIM / 16];
+#pragma unroll
+        for (int d = 0; d < DIM / 16; d++)
+        {
+            if constexpr (TYPE == DT_BF16)
+            {
+                const int r = 4 * g + (j >> 2);
+                const uint8_t* const at0 = vb + r * ROW + (((2 * d + ((j & 3) >> 1)) ^ value_swizzle(r)) << 4) + ((j & 1) << 3);
+                const u32x2 lo = lds_transposed16(at0), hi = lds_transposed16(at0 + 16 * ROW);      // the swizzle of row r + 16 is that of r
+                vf[d] = u32x4{ lo[0], lo[1], hi[0], hi[1] };
+            }
+            else
+            {
+                const int r = 4 * g + ((j >> 1) & 3) + (j >> 3) * 16;
+                const u32x2 codes = lds_transposed8(vb + r * ROW + ((d ^ value_swizzle(r)) << 4) + ((j & 1) << 3));
+                const u32x2 lo = fp8x4_to_bf16<TYPE>(codes[0], 1.0f), hi = fp8x4_to_bf16<TYPE>(codes[1], 1.0f);
+                vf[d] = u32x4{ lo[0], lo[1], hi[0], hi[1] };
+            }
+        }
+        const bool plain = KeyBlocks<KEYS>::plain(p, mine.pos, last_pos, b) && bad == 0;
+        float score[8];
+        uint32_t seen = 0xFFu;
+#pragma unroll
+        for (int e = 0; e < 8; e++) { score[e] = acc[e >> 2][e & 3] * p.scale; }
+        if (!plain)
+        {
+            seen = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+            {
+                const bool see = sees(p, my_pos, b * KEYS + 16 * (e >> 2) + 4 * g + (e & 3)) && !(bad >> (e >> 2) & 1);
+                seen |= see ? 1u << e : 0u;
+                score[e] = see ? score[e] : -INFINITY;
+            }
+        }
+        float top = max8(score);
+        if (__any(top > m + PA_LAG))
+        {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            const float next = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+            const float shrink = next > -INFINITY ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
+            m = next;
+            l *= shrink;
+#pragma unroll
+            for (int d = 0; d < DIM / 16; d++) { out[d] *= shrink; }
+        }
+        const float off = m > -INFINITY ? m : 0.0f;                         // no key seen yet: every weight is 2^-inf = 0
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) { w[e] = __builtin_amdgcn_exp2f(score[e] - off); }
+        l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        if constexpr (TYPE != DT_BF16)
+        {
+#pragma unroll
+            for (int e = 0; e < 8; e++) { w[e] = seen >> e & 1 ? w[e] * vscale[e] : 0.0f; }
+        }
+        const bf16x8 pb = { (__bf16)w[0], (__bf16)w[1], (__bf16)w[2], (__bf16)w[3], (__bf16)w[4], (__bf16)w[5], (__bf16)w[6], (__bf16)w[7] };
+        uint32_t odd = 0;
+        if (!plain)
+        {
+#pragma unroll
+            for (int d = 0; d < DIM / 16; d++) { odd |= not_finite(vf[d]); }
+        }
+        if (__any(odd != 0))
+        {
+            // 0 times an infinity is NaN: what is not finite is added apart, to the rows that see it
+            bf16x8 see;
+#pragma unroll
+            for (int e = 0; e < 8; e++) { see[e] = (__bf16)(float)(seen >> e & 1); }
+#pragma unroll
+            for (int d = 0; d < DIM / 16; d++)
+            {
+                out[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, finite_part(vf[d])), pb, out[d], 0, 0, 0);
+#pragma unroll 1
+                for (int kind = 0; kind < 3; kind++)
+                {
+                    const f32x4 count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, where_kind(vf[d], kind)), see, f32x4{ 0.0f, 0.0f, 0.0f, 0.0f }, 0, 0, 0);
+#pragma unroll
+                    for (int v = 0; v < 4; v++) { out[d][v] += count[v] > 0.0f ? value_of_kind(kind) : 0.0f; }
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int d = 0; d < DIM / 16; d++) { out[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[d]), pb, out[d], 0, 0, 0); }
+    };
+
+    constexpr int IN_FLIGHT = 2 * LOADS + (TYPE == DT_BF16 ? 0 : 1);        // loads per stage
+    if (0 < n_mine) { stage(0, 0); }
+    if (1 < n_mine) { stage(1, 1); }
+    for (int n = 0; n < n_mine; n += 2)
+    {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+        {
+            if (n + u >= n_mine) { break; }
+            if (n + u + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(IN_FLIGHT) : "memory"); }
+            else { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+            block(n + u, u);
+            if (n + u + 2 < n_mine)
+            {
+                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // the stage has been read
+                stage(n + u + 2, u);
+            }
+        }
+    }
+
+    // the four waves' sums of a row meet in LDS
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) { stat[wave][j] = make_float2(m, l); }
+    __syncthreads();
+    float* const sums = (float*)lds;
+#pragma unroll
+    for (int d = 0; d < DIM / 16; d++) { *(f32x4*)(sums + (wave * 16 + j) * SUM + 16 * d + 4 * g) = out[d]; }
+    __syncthreads();
+    const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (DIM / 16);
+    if (r >= n_rows) { return; }
+    float top = -INFINITY, total = 0.0f, weight[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++) { top = fmaxf(top, stat[w][r].x); }
+    const float base = top > -INFINITY ? top : 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+    {
+        weight[w] = __builtin_amdgcn_exp2f(stat[w][r].x - base);            // 2^-inf = 0 for a wave without a key
+        total += weight[w] * stat[w][r].y;
+    }
+    float sum[DIM / 16];
+#pragma unroll
+    for (int d = 0; d < DIM / 16; d++)
+    {
+        sum[d] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) { sum[d] += weight[w] > 0.0f || weight[w] != weight[w] ? weight[w] * sums[(w * 16 + r) * SUM + d0 + d] : 0.0f; }
+    }
+    const size_t at_token = mine.first + r / p.group, at_head = kvh * p.group + r % p.group, at_row = at_token * p.n_q + at_head;
+    if (p.n_split > 1 && range == 0 && d0 == 0) { *p.ranges(at_row, DIM) = n_ranges; }
+    if (n_ranges > 1)
+    {
+        float* const dst = p.sums(range, at_row, DIM) + d0;
+#pragma unroll
+        for (int d = 0; d < DIM / 16; d += 4) { *(f32x4*)(dst + d) = f32x4{ sum[d], sum[d + 1], sum[d + 2], sum[d + 3] }; }
+        if (d0 == 0) { *p.stats(range, at_row, DIM) = make_float2(top, total); }
+        return;
+    }
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int d = 0; d < DIM / 16; d++) { sum[d] = total == 0.0f ? 0.0f : sum[d] * by; }
+    uint16_t* const dst = p.y + at_token * p.ldy + at_head * DIM + d0;
+#pragma unroll
+    for (int d = 0; d < DIM / 16; d += 4) { *(u32x2*)(dst + d) = pack4(sum + d); }
+}
+
+// 128 RT rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions.
+//   A workgroup of four waves takes 128 RT rows, a wave 32 RT of them and every key of each block of 64; keys and values reach LDS as BF16, shared by
+// the waves: from a BF16 cache by direct loads, from FP8 through registers, times their powers of two (exact, once per workgroup).
+//   scores: v_mfma_f32_32x32x16_bf16, key rows as row operand, queries as columns: D lane (row j = lane % 32, h = lane / 32), register i holds key
+//           8 (i / 4) + 4 h + i % 4 of 32.
+//   V p:    registers 8 u .. + 7 of a lane are its column operand of the u-th 16 keys as they are; the row operand (dim, the same keys) comes from
+//           two transposing reads.
+// A row's statistics and sums stay in the two lanes that have it.
+// Grid: (tiles x kv heads) x ranges; which sequence a tile belongs to is found from seq_start.  The last tiles of a sequence, which see the most
+// keys, go first.
+template <int TYPE, int DIM, int RT = 1>
+__global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const PagedArgs a, const PagedAttention p)
+{
+    constexpr int KEYS = 64, ROWS = 128 * RT, ROW = DIM * 2, CHUNKS = ROW / 16, BLOCK = KEYS * ROW;
+    constexpr int CODES = DIM * CODE_BYTES<TYPE>;                           // bytes of a cached row
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * BLOCK];       // two blocks of keys, two of values
+    __shared__ __attribute__((aligned(16))) uint32_t odd_rows[2][4];        // per buffer of values and wave that staged: something infinite or NaN
+    const int kvh = blockIdx.x % a.n_kv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int j = lane & 31, h = lane >> 5;
+
+    // the sequence and tile of this workgroup: a lane per sequence, their tiles added up
+    int s = -1, tile = blockIdx.x / a.n_kv;
+    for (int base = 0; base < a.n_seqs; base += 64)
+    {
+        const int i = base + lane;
+        int tiles = 0;
+        if (i < a.n_seqs)
+        {
+            const int rows = new_tokens(a, p, i).n * p.group;
+            tiles = rows > p.min_rows ? (rows + ROWS - 1) / ROWS : 0;
+        }
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1)
+        {
+            const int below = __shfl_up(upto, o);
+            upto += lane >= o ? below : 0;
+        }
+        const unsigned long long past = __ballot(upto > tile);
+        if (past != 0)
+        {
+            const int at = __builtin_ctzll(past);
+            s = base + at;
+            tile = __builtin_amdgcn_readlane(upto, at) - 1 - tile;          // of the sequence, from its end
+            break;
+        }
+        tile -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (s < 0) { return; }
+    s = __builtin_amdgcn_readfirstlane(s);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    const NewTokens mine = new_tokens(a, p, s);
+    const int n_rows = mine.n * p.group, row0 = tile * ROWS;
+    const int tile_lo = mine.pos + row0 / p.group, tile_hi = mine.pos + min(row0 + ROWS - 1, n_rows - 1) / p.group;
+    const KeyBlocks<KEYS> blocks(p, tile_lo, tile_hi);
+    const int per = max((blocks.n + p.split - 1) / p.split, 4);
+    const int n_ranges = max((blocks.n + per - 1) / per, 1);
+    const int range = blockIdx.y, begin = range * per, end = min(blocks.n, begin + per);
+    if (range >= n_ranges) { return; }
+
+    // the wave's rows
+    const int wave_lo = mine.pos + min(row0 + wave * 32 * RT, n_rows - 1) / p.group, wave_hi = mine.pos + min(row0 + wave * 32 * RT + 32 * RT - 1, n_rows - 1) / p.group;
+    int token[RT], head[RT], my_pos[RT];
+    bool real[RT];
+    u32x4 qf[RT][DIM / 16];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+    {
+        const int r = row0 + (wave * RT + t) * 32 + j, row = min(r, n_rows - 1);
+        real[t] = r < n_rows;
+        token[t] = mine.first + row / p.group;
+        head[t] = kvh * p.group + row % p.group;
+        my_pos[t] = mine.pos + row / p.group;
+#pragma unroll
+        for (int c = 0; c < DIM / 16; c++) { qf[t][c] = *(const u32x4*)(p.q + (size_t)token[t] * p.ldq + (size_t)head[t] * DIM + c * 16 + h * 8); }
+    }
+
+    auto key_swizzle = [](int r) { return r / (256 / ROW) % CHUNKS; };
+    auto value_swizzle = [](int r) { return DIM == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
+    int pages = 0, none = 0;                    // lane l, entry 64 n + l of the range: page of the 16 rows that this wave stages; bits of the quarters without one
+    auto look_up = [&](int i0) {
+        const int i = i0 + lane, key0 = blocks.block(i) * KEYS;
+        pages = none = 0;
+        if (i >= end) { return; }
+#pragma unroll
+        for (int quarter = 0; quarter < 4; quarter++)
+        {
+            const int pos = key0 + 16 * quarter;
+            const int page = pos > tile_hi ? 0 : paged_page(a, s, pos);
+            none |= page < 0 ? 1 << quarter : 0;
+            pages = quarter == wave ? max(page, 0) : pages;
+        }
+    };
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds));
+    constexpr int PIECES = TYPE == DT_BF16 ? 1 : CODES * 16 / 1024;         // FP8: 16 bytes per lane each of the wave's 16 rows
+    struct Rows
+    {
+        u32x4 codes[PIECES];
+        uint32_t exponent[PIECES];
+    };
+    // the wave's 16 rows of entry i: on their way to LDS (BF16) or to registers
+    auto load = [&](bool values, int i, int page, uint32_t to, Rows& raw) {
+        const size_t r0 = paged_row(a, kvh, blocks.block(i) * KEYS + 16 * wave);
+        const uint8_t* const from = (values ? a.v : a.k) + page * a.page_stride + r0 * CODES;
+        if constexpr (TYPE == DT_BF16)
+        {
+#pragma unroll
+            for (int n = 0; n < ROW * 16 / 1024; n++)
+            {
+                const int r = n * (1024 / ROW) + lane / CHUNKS, c = lane % CHUNKS;
+                load_to_lds<false>(lds0 + to + n * 1024, from, (uint32_t)(r * ROW + (c ^ (values ? value_swizzle(r) : key_swizzle(r))) * 16));
+            }
+        }
+        else
+        {
+            const uint8_t* const exponents = (values ? a.v_scale : a.k_scale) + page * a.scale_stride + r0;
+#pragma unroll
+            for (int n = 0; n < PIECES; n++)
+            {
+                raw.codes[n] = *(const u32x4*)(from + n * 1024 + lane * 16);
+                raw.exponent[n] = exponents[n * (1024 / CODES) + lane / (CODES / 16)];
+            }
+        }
+    };
+    // FP8: the loaded rows to LDS as BF16; the result tells whether something is not finite
+    auto store = [&](bool values, uint32_t to, const Rows& raw) {
+        uint32_t odd = 0;
+        if constexpr (TYPE != DT_BF16)
+        {
+#pragma unroll
+            for (int n = 0; n < PIECES; n++)
+            {
+                const int r = n * (1024 / CODES) + lane / (CODES / 16), c = lane % (CODES / 16) * 2, swizzle = values ? value_swizzle(r) : key_swizzle(r);
+                const float by = bits_to_f32(raw.exponent[n] << 23);
+                u32x2 w[4];
+#pragma unroll
+                for (int d = 0; d < 4; d++) { w[d] = fp8x4_to_bf16<TYPE>(raw.codes[n][d], by); }
+                const u32x4 lo = { w[0][0], w[0][1], w[1][0], w[1][1] }, hi = { w[2][0], w[2][1], w[3][0], w[3][1] };
+                *(u32x4*)(lds + to + r * ROW + (c ^ swizzle) * 16) = lo;
+                *(u32x4*)(lds + to + r * ROW + ((c + 1) ^ swizzle) * 16) = hi;
+                odd |= not_finite(lo) | not_finite(hi);
+            }
+        }
+        return odd;
+    };
+    auto keys_at = [&](int i) { return (uint32_t)((i - begin) & 1) * BLOCK; };
+    auto values_at = [&](int i) { return (uint32_t)(2 + ((i - begin) & 1)) * BLOCK; };
+    const uint32_t part = wave * (BLOCK / 4);                               // the wave's rows of a block
+    auto tile_plain = [&](int i, int lacks) { return KeyBlocks<KEYS>::plain(p, tile_lo, tile_hi, blocks.block(i)) && lacks == 0; };
+    // in front of the barrier behind which the values of entry i are read: whether any is infinite or NaN, where that matters
+    auto note_odd = [&](int i, int lacks, uint32_t odd) {
+        if (tile_plain(i, lacks)) { return; }
+        if constexpr (TYPE == DT_BF16)
+        {
+#pragma unroll
+            for (int n = 0; n < ROW * 16 / 1024; n++) { odd |= not_finite(*(const u32x4*)(lds + values_at(i) + part + n * 1024 + lane * 16)); }
+        }
+        const bool any = __any(odd != 0);
+        if (lane == 0) { odd_rows[i & 1][wave] = any; }
+    };
+
+    int k_at[DIM / 16];                         // of chunk 2 c + h of key row j
+#pragma unroll
+    for (int c = 0; c < DIM / 16; c++) { k_at[c] = j * ROW + ((2 * c + h) ^ key_swizzle(j)) * 16; }
+    auto score_products = [&](int i, f32x16 (&acc)[RT][2]) {
+        const uint8_t* const kb = lds + keys_at(i);
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) { acc[t][kt][e] = 0.0f; }
+#pragma unroll
+        for (int c = 0; c < DIM / 16; c++)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+            {
+                const bf16x8 kf = *(const bf16x8*)(kb + k_at[c] + kt * 32 * ROW);       // the swizzle of row j + 32 is that of j
+#pragma unroll
+                for (int t = 0; t < RT; t++) { acc[t][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, qf[t][c]), acc[t][kt], 0, 0, 0); }
+            }
+    };
+
+    float m[RT], l[RT];
+    f32x16 out[RT][DIM / 32];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+    {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DIM / 32; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) { out[t][d][e] = 0.0f; }
+    }
+    // dims 32 d + 16 (lane / 16 % 2) + 4 (lane % 4) .. + 3 of key row 4 h + lane % 16 / 4 (and of rows 8 further, and of the next 16)
+    const int v_row = 4 * h + ((lane & 15) >> 2), v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    int v_at[DIM / 32];
+#pragma unroll
+    for (int d = 0; d < DIM / 32; d++) { v_at[d] = v_row * ROW + (((4 * d + v_chunk) ^ value_swizzle(v_row)) << 4) + ((lane & 1) << 3); }
+
+    auto weigh = [&](f32x16 (&acc)[RT][2], int i, int lacks, auto masked_c) {
+        constexpr bool masked = decltype(masked_c)::value;
+        const uint8_t* const vb = lds + values_at(i);
+        const int b = blocks.block(i);
+        float off[RT], sum[RT][4];
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+        {
+            if (masked)
+            {
+                // element e: key 8 (e / 4) + 4 h + e % 4 of the block
+                const int d = my_pos[t] - b * KEYS - 4 * h, from = p.window == 0 ? -0x40000000 : d - p.window, first = p.n_sink - b * KEYS - 4 * h;
+#pragma unroll
+                for (int e = 0; e < 32; e++)
+                {
+                    const int key = 8 * (e / 4) + e % 4;
+                    const bool see = key <= d && (key > from || key < first) && !(lacks >> (e / 8) & 1);
+                    acc[t][e / 16][e % 16] = see ? acc[t][e / 16][e % 16] : -INFINITY;
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 32; e++) { top = fmaxf(top, acc[t][e / 16][e % 16]); }
+            top *= p.scale;
+            if (__any(top > m[t] + PA_LAG))
+            {
+                const float next = fmaxf(m[t], fmaxf(top, __shfl_xor(top, 32)));
+                const float shrink = m[t] > -INFINITY ? __builtin_amdgcn_exp2f(m[t] - next) : 1.0f;       // sums of nothing: 0, or what is not finite
+                m[t] = next;
+                l[t] *= shrink;
+#pragma unroll
+                for (int d = 0; d < DIM / 32; d++) { out[t][d] *= shrink; }
+            }
+            off[t] = m[t] > -INFINITY ? -m[t] : 0.0f;                       // no key seen yet: every weight is 2^-inf = 0
+#pragma unroll
+            for (int n = 0; n < 4; n++) { sum[t][n] = 0.0f; }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+        {
+            bf16x8 pb[RT];
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(acc[t][u / 2][u % 2 * 8 + e], p.scale, off[t]));
+                    sum[t][e & 3] += w;
+                    pb[t][e] = (__bf16)w;
+                }
+#pragma unroll
+            for (int d = 0; d < DIM / 32; d++)
+            {
+                const u32x2 lo = lds_transposed16(vb + v_at[d] + u * 16 * ROW), hi = lds_transposed16(vb + v_at[d] + (u * 16 + 8) * ROW);
+                const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{ lo[0], lo[1], hi[0], hi[1] });
+#pragma unroll
+                for (int t = 0; t < RT; t++) { out[t][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[t], out[t][d], 0, 0, 0); }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++) { l[t] += (sum[t][0] + sum[t][1]) + (sum[t][2] + sum[t][3]); }
+    };
+    // Weight 0 times an infinity is NaN: where some rows do not see every key of entry i, what is infinite or NaN among its values is added to the sums of
+    // the rows that see it and cleared in front of the products.
+    auto set_apart = [&](int i, int lacks) {
+        const u32x4 odd = *(const u32x4*)odd_rows[i & 1];
+        if (__builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]) == 0) { return; }
+        uint8_t* const vb = lds + values_at(i);
+        const int b = blocks.block(i);
+#pragma unroll 1
+        for (int key = 0; key < KEYS; key++)
+        {
+            if (lacks >> (key / 16) & 1) { continue; }
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+            {
+                const bool see = sees(p, my_pos[t], b * KEYS + key);
+#pragma unroll
+                for (int n = 0; n < DIM / 8; n++)
+                {
+                    const int dim = 8 * n + 4 * h;
+                    const u32x2 raw = *(const u32x2*)(vb + key * ROW + (((dim / 8) ^ value_swizzle(key)) << 4) + (dim & 4) * 2);
+                    float v[4];
+                    unpack4(raw, v);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { out[t][n / 4][n % 4 * 4 + e] += see && !(fabsf(v[e]) < INFINITY) ? v[e] : 0.0f; }
+                }
+            }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int n = 0; n < ROW * 16 / 1024; n++)
+        {
+            u32x4* const at = (u32x4*)(vb + part + n * 1024 + lane * 16);
+            *at = finite_part(*at);
+        }
+        lds_barrier();
+    };
+    // loads of this wave into LDS have arrived and its accesses of LDS are done; the same, then the workgroup's barrier
+    auto arrived = []() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); };
+    auto barrier = []() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+    if (begin < end)
+    {
+        Rows raw_k, raw_v;
+        f32x16 acc[RT][2];
+        uint32_t odd = 0;
+        auto load_both = [&](int i) {
+            if (((i - begin) & 63) == 0) { look_up(i); }
+            const int page = __builtin_amdgcn_readlane(pages, (i - begin) & 63);
+            load(false, i, page, keys_at(i) + part, raw_k);
+            load(true, i, page, values_at(i) + part, raw_v);
+            return __builtin_amdgcn_readlane(none, (i - begin) & 63);
+        };
+        auto store_both = [&](int i) {
+            if constexpr (TYPE != DT_BF16)
+            {
+                store(false, keys_at(i) + part, raw_k);
+                odd = store(true, values_at(i) + part, raw_v);
+            }
+        };
+        int lacks = load_both(begin);
+        store_both(begin);
+        arrived();
+        note_odd(begin, lacks, odd);
+        barrier();
+        // entry i is in LDS
+        for (int i = begin; i < end; i++)
+        {
+            int lacks_ahead = 0;
+            if (i + 1 < end) { lacks_ahead = load_both(i + 1); }            // the buffers of entry i - 1, read before the last barrier
+            const int b = blocks.block(i);
+            if (!tile_plain(i, lacks)) { set_apart(i, lacks); }
+            if (!KeyBlocks<KEYS>::hidden(p, wave_lo, wave_hi, b))
+            {
+                score_products(i, acc);
+                if (KeyBlocks<KEYS>::plain(p, wave_lo, wave_hi, b) && lacks == 0) { weigh(acc, i, 0, std::false_type{}); }
+                else { weigh(acc, i, lacks, std::true_type{}); }
+            }
+            if (i + 1 < end)
+            {
+                store_both(i + 1);
+                arrived();
+                note_odd(i + 1, lacks_ahead, odd);
+                barrier();
+                lacks = lacks_ahead;
+            }
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+    {
+        const float total = l[t] + __shfl_xor(l[t], 32);
+        if (!real[t]) { continue; }
+        const size_t at_row = (size_t)token[t] * p.n_q + head[t];
+        if (p.n_split > 1 && range == 0 && h == 0) { *p.ranges(at_row, DIM) = n_ranges; }
+        if (n_ranges > 1)
+        {
+            float* const dst = p.sums(range, at_row, DIM) + 4 * h;
+#pragma unroll
+            for (int d = 0; d < DIM / 32; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) { *(f32x4*)(dst + 32 * d + 2 * e) = f32x4{ out[t][d][e], out[t][d][e + 1], out[t][d][e + 2], out[t][d][e + 3] }; }
+            if (h == 0) { *p.stats(range, at_row, DIM) = make_float2(m[t], total); }
+            continue;
+        }
+        uint16_t* const dst = p.y + (size_t)token[t] * p.ldy + (size_t)head[t] * DIM + 4 * h;
+        const float by = 1.0f / total;
+#pragma unroll
+        for (int d = 0; d < DIM / 32; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+            {
+                float v[4];
+#pragma unroll
+                for (int n = 0; n < 4; n++) { v[n] = total == 0.0f ? 0.0f : out[t][d][e + n] * by; }
+                *(u32x2*)(dst + 32 * d + 2 * e) = pack4(v);
+            }
+    }
+}
+
+// Sums of the key ranges of a token's heads, four dims per thread: rescaled to the largest maximum, added in the order of the ranges, divided by the
+// sum of the weights, one rounding.  Grid: tokens x workgroups over the heads.
+template <int DIM>
+__global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
+{
+    constexpr int LANES = DIM / 4, PER_WG = 256 / LANES;
+    const int parts = (p.n_q + PER_WG - 1) / PER_WG;
+    const int t = blockIdx.x / parts, head = blockIdx.x % parts * PER_WG + threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
     const int s = paged_sequence(a, t);
-    if (s < 0 || head >= p.n_q) { return; }
-    const int n_new = a.seq_start[s + 1] - a.seq_start[s], ctx = paged_rows(a, s), pos = ctx - (a.seq_start[s + 1] - t);
-    if (n_new > p.max_new) { return; }
-    const int h = head / p.group;
-    for (int d = lane; d < DIM; d += 64) { q_s[wave][d] = bf16_bits_to_f32(p.q[(size_t)t * p.ldq + (size_t)head * DIM + d]); }
-    __builtin_amdgcn_wave_barrier();
-    float m = -INFINITY, l = 0.0f, out[OUT] = {};
-    for (int base = 0; base <= pos; base += 64)
+    if (s < 0 || head >= p.n_q || new_tokens(a, p, s).n == 0) { return; }
+    const size_t row = (size_t)t * p.n_q + head;
+    const int n = *p.ranges(row, DIM);
+    if (n <= 1) { return; }                                                 // written already
+    f32x4 sum = { 0.0f, 0.0f, 0.0f, 0.0f };
+    float m = -INFINITY, l = 0.0f;
+    for (int r0 = 0; r0 < n; r0 += 8)
     {
-        const int key = base + lane;
-        const int page = key <= pos ? paged_page(a, s, key) : -1;
-        const bool seen = page >= 0 && (p.window == 0 || key > pos - p.window || key < p.n_sink);
-        const size_t row = paged_row(a, h, key);
-        float score = -INFINITY;
-        if (seen)
+        f32x4 part[8];                                                      // eight ranges requested at once
+        float2 stat[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++)
         {
-            const uint8_t* const k = a.k + page * a.page_stride + row * ROW;
-            const float scale = TYPE == DT_BF16 ? 1.0f : bits_to_f32((uint32_t)a.k_scale[page * a.scale_stride + row] << 23);
-            float sum = 0.0f;
-            for (int d = 0; d < DIM; d++) { sum += q_s[wave][d] * paged_element<TYPE>(k, d, scale); }
-            score = sum * p.scale;
+            stat[r] = *p.stats(min(r0 + r, n - 1), row, DIM);
+            part[r] = *(const f32x4*)(p.sums(min(r0 + r, n - 1), row, DIM) + d);
         }
-        float top = score;
-        for (int o = 1; o < 64; o <<= 1) { top = fmaxf(top, __shfl_xor(top, o)); }
-        const float next = fmaxf(m, top), shrink = next > -INFINITY ? expf(m - next) : 1.0f;
-        const float w = seen && (next > -INFINITY || score != score) ? expf(score - next) : 0.0f;
-        m = next;
-        l = l * shrink + wave_sum(w);
-        for (int o = 0; o < OUT; o++) { out[o] *= shrink; }
-        const unsigned long long visible = __ballot(seen);
-        for (int j = 0; j < 64; j++)
+        float top = m;
+#pragma unroll
+        for (int r = 0; r < 8; r++) { top = fmaxf(top, stat[r].x); }
+        const float base = top > -INFINITY ? top : 0.0f, shrink = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        l *= shrink;
+        sum *= shrink;
+#pragma unroll
+        for (int r = 0; r < 8; r++)
         {
-            if (!(visible >> j & 1)) { continue; }
-            const int from = __shfl(page, j);
-            const size_t r = paged_row(a, h, base + j);
-            const float scale = TYPE == DT_BF16 ? 1.0f : bits_to_f32((uint32_t)a.v_scale[from * a.scale_stride + r] << 23), weight = __shfl(w, j);
-            for (int o = 0; o < OUT; o++) { out[o] += weight * paged_element<TYPE>(a.v + from * a.page_stride + r * ROW, lane + 64 * o, scale); }
+            const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
+            if (r0 + r < n && w != 0.0f)
+            {
+                l += w * stat[r].y;
+                sum += w * part[r];
+            }
         }
     }
-    for (int o = 0; o < OUT; o++)
-    {
-        p.y[(size_t)t * p.ldy + (size_t)head * DIM + lane + 64 * o] = (uint16_t)f32_to_bf16_bits(l == 0.0f ? 0.0f : out[o] / l);
-    }
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) { v[e] = l == 0.0f ? 0.0f : sum[e] / l; }
+    *(u32x2*)(p.y + (size_t)t * p.ldy + (size_t)head * DIM + d) = pack4(v);
 }
 
 }    // namespace ccq
