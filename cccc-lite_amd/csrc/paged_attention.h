@@ -534,17 +534,21 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
         u32x4 codes[PIECES];
         uint32_t exponent[PIECES];
     };
+    const uint32_t key_from = lane * 16 ^ key_swizzle(lane / CHUNKS) * 16, value_from = lane * 16 ^ value_swizzle(lane / CHUNKS) * 16;
     // the wave's 16 rows of entry i: on their way to LDS (BF16) or to registers
     auto load = [&](bool values, int i, int page, uint32_t to, Rows& raw) {
         const size_t r0 = paged_row(a, kvh, blocks.block(i) * KEYS + 16 * wave);
         const uint8_t* const from = (values ? a.v : a.k) + page * a.page_stride + r0 * CODES;
         if constexpr (TYPE == DT_BF16)
         {
+            // rows n (1024 / ROW) + lane / CHUNKS: with n a swizzle changes by a constant in bits of its own
+            uint32_t at = values ? value_from : key_from;
+            asm volatile("" : "+v"(at));                                    // worked out anew: registers are short
 #pragma unroll
             for (int n = 0; n < ROW * 16 / 1024; n++)
             {
-                const int r = n * (1024 / ROW) + lane / CHUNKS, c = lane % CHUNKS;
-                load_to_lds<false>(lds0 + to + n * 1024, from, (uint32_t)(r * ROW + (c ^ (values ? value_swizzle(r) : key_swizzle(r))) * 16));
+                constexpr int R = 1024 / ROW;
+                load_to_lds<false>(lds0 + to + n * 1024, from + n * 1024, values ? at : at ^ (uint32_t)(key_swizzle(n * R) * 16));
             }
         }
         else
@@ -595,25 +599,19 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
         if (lane == 0) { odd_rows[i & 1][wave] = any; }
     };
 
-    int k_at[DIM / 16];                         // of chunk 2 c + h of key row j
-#pragma unroll
-    for (int c = 0; c < DIM / 16; c++) { k_at[c] = j * ROW + ((2 * c + h) ^ key_swizzle(j)) * 16; }
+    const uint32_t k_at = j * ROW + (h ^ key_swizzle(j)) * 16;             // of chunk h of key row j; chunk 2 c + h at k_at ^ 32 c
     auto score_products = [&](int i, f32x16 (&acc)[RT][2]) {
-        const uint8_t* const kb = lds + keys_at(i);
-#pragma unroll
-        for (int t = 0; t < RT; t++)
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) { acc[t][kt][e] = 0.0f; }
+        uint32_t at = k_at + keys_at(i);
+        asm volatile("" : "+v"(at));
+        const f32x16 zero = {};
 #pragma unroll
         for (int c = 0; c < DIM / 16; c++)
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
             {
-                const bf16x8 kf = *(const bf16x8*)(kb + k_at[c] + kt * 32 * ROW);       // the swizzle of row j + 32 is that of j
+                const bf16x8 kf = *(const bf16x8*)(lds + (at ^ (32 * c)) + kt * 32 * ROW);       // the swizzle of row j + 32 is that of j
 #pragma unroll
-                for (int t = 0; t < RT; t++) { acc[t][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, qf[t][c]), acc[t][kt], 0, 0, 0); }
+                for (int t = 0; t < RT; t++) { acc[t][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, qf[t][c]), c == 0 ? zero : acc[t][kt], 0, 0, 0); }
             }
     };
 
@@ -631,30 +629,31 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
     }
     // dims 32 d + 16 (lane / 16 % 2) + 4 (lane % 4) .. + 3 of key row 4 h + lane % 16 / 4 (and of rows 8 further, and of the next 16)
     const int v_row = 4 * h + ((lane & 15) >> 2), v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    int v_at[DIM / 32];
-#pragma unroll
-    for (int d = 0; d < DIM / 32; d++) { v_at[d] = v_row * ROW + (((4 * d + v_chunk) ^ value_swizzle(v_row)) << 4) + ((lane & 1) << 3); }
+    const uint32_t v_at = v_row * ROW + ((v_chunk ^ value_swizzle(v_row)) << 4) + ((lane & 1) << 3);     // dims 32 d on at v_at ^ 64 d
 
-    auto weigh = [&](f32x16 (&acc)[RT][2], int i, int lacks, auto masked_c) {
-        constexpr bool masked = decltype(masked_c)::value;
-        const uint8_t* const vb = lds + values_at(i);
-        const int b = blocks.block(i);
+    // scores of keys that a row does not see
+    auto mask = [&](f32x16 (&acc)[RT][2], int b, int lacks) {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+        {
+            // element e: key 8 (e / 4) + 4 h + e % 4 of the block
+            const int d = my_pos[t] - b * KEYS - 4 * h, from = p.window == 0 ? -0x40000000 : d - p.window, first = p.n_sink - b * KEYS - 4 * h;
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+            {
+                const int key = 8 * (e / 4) + e % 4;
+                const bool see = key <= d && (key > from || key < first) && !(lacks >> (e / 8) & 1);
+                acc[t][e / 16][e % 16] = see ? acc[t][e / 16][e % 16] : -INFINITY;
+            }
+        }
+    };
+    auto weigh = [&](f32x16 (&acc)[RT][2], int i) {
+        uint32_t at = v_at + values_at(i);
+        asm volatile("" : "+v"(at));
         float off[RT], sum[RT][4];
 #pragma unroll
         for (int t = 0; t < RT; t++)
         {
-            if (masked)
-            {
-                // element e: key 8 (e / 4) + 4 h + e % 4 of the block
-                const int d = my_pos[t] - b * KEYS - 4 * h, from = p.window == 0 ? -0x40000000 : d - p.window, first = p.n_sink - b * KEYS - 4 * h;
-#pragma unroll
-                for (int e = 0; e < 32; e++)
-                {
-                    const int key = 8 * (e / 4) + e % 4;
-                    const bool see = key <= d && (key > from || key < first) && !(lacks >> (e / 8) & 1);
-                    acc[t][e / 16][e % 16] = see ? acc[t][e / 16][e % 16] : -INFINITY;
-                }
-            }
             float top = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 32; e++) { top = fmaxf(top, acc[t][e / 16][e % 16]); }
@@ -688,7 +687,7 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
 #pragma unroll
             for (int d = 0; d < DIM / 32; d++)
             {
-                const u32x2 lo = lds_transposed16(vb + v_at[d] + u * 16 * ROW), hi = lds_transposed16(vb + v_at[d] + (u * 16 + 8) * ROW);
+                const u32x2 lo = lds_transposed16(lds + (at ^ (64 * d)) + u * 16 * ROW), hi = lds_transposed16(lds + (at ^ (64 * d)) + (u * 16 + 8) * ROW);
                 const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{ lo[0], lo[1], hi[0], hi[1] });
 #pragma unroll
                 for (int t = 0; t < RT; t++) { out[t][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[t], out[t][d], 0, 0, 0); }
@@ -771,8 +770,8 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
             if (!KeyBlocks<KEYS>::hidden(p, wave_lo, wave_hi, b))
             {
                 score_products(i, acc);
-                if (KeyBlocks<KEYS>::plain(p, wave_lo, wave_hi, b) && lacks == 0) { weigh(acc, i, 0, std::false_type{}); }
-                else { weigh(acc, i, lacks, std::true_type{}); }
+                if (!KeyBlocks<KEYS>::plain(p, wave_lo, wave_hi, b) || lacks != 0) { mask(acc, b, lacks); }
+                weigh(acc, i);
             }
             if (i + 1 < end)
             {
