@@ -55,36 +55,35 @@ bool attention_args(const hip_paged_kv* c, PagedArgs& a, int n_q_heads, int n_to
     a.max_ctx = std::min(a.max_ctx, max_ctx);
     return true;
 }
-// How a call's rows are split: which kernels run, and over how many ranges of keys at most.
+// How a call's rows are taken: in tiles, as sequences of up to 16 rows per kv head, or both, each over so many ranges of keys at most.
 struct Plan
 {
-    bool rows, tiles;               // the kernel for up to 16 rows of a kv head, the one for more
-    int min_rows;                   // sequences of at most so many rows are the first one's
-    long long n_tiles;              // at most
-    int rows_split, tiles_split, n_split;
+    long long tiles;                // at most
+    bool rows;
+    int min_rows, tile_split, row_split, n_split;
 };
 
-constexpr int TILE_ROWS = 128;
-
+// Sequences of up to 16 rows per kv head have a form of their own, also beside longer ones -- unless every sequence has max_new tokens, as far as their
+// number tells.
 Plan plan_attention(const PagedArgs& a, int group, int n_tokens, int max_new, int window, int n_sink)
 {
-    const long long most_rows = (long long)std::min(max_new, n_tokens) * group;
-    Plan plan = {};
-    plan.tiles = most_rows > 16;
-    plan.rows = !plan.tiles || (group <= 16 && a.n_seqs > 1 && n_tokens < (long long)a.n_seqs * max_new);
-    plan.min_rows = plan.tiles && plan.rows ? 16 : 0;
-    const long long rows = (long long)n_tokens * group;
-    plan.n_tiles = rows / TILE_ROWS + std::min<long long>(a.n_seqs, rows / (plan.min_rows + 1));
-    const long long wide = 2LL * cu_count();
+    const long long most_rows = (long long)std::min(max_new, n_tokens) * group, rows = (long long)n_tokens * group;
+    Plan plan = { 0, true, 0, 1, 1, 1 };
+    if (most_rows > PA_ROWS)
+    {
+        plan.rows = group <= PA_ROWS && n_tokens < (long long)a.n_seqs * max_new;
+        plan.min_rows = plan.rows ? PA_ROWS : 0;
+        plan.tiles = rows / PA_TILE + std::min<long long>(a.n_seqs, rows / (plan.min_rows + 1));
+    }
     const long long keys = window == 0 ? a.max_ctx : std::min<long long>(a.max_ctx, (long long)window + n_sink + max_new);
-    auto split = [&](long long workgroups, long long most) { return (int)std::max<long long>(1, std::min({ wide / std::max<long long>(workgroups, 1), most, 64LL })); };
-    plan.rows_split = plan.rows ? split((long long)a.n_seqs * a.n_kv, keys / 256) : 1;
-    plan.tiles_split = plan.tiles ? split(plan.n_tiles * a.n_kv, keys / 256) : 1;
-    plan.n_split = std::max(plan.rows_split, plan.tiles_split);
+    auto split = [&](long long workgroups) { return (int)std::max<long long>(1, std::min({ 2LL * cu_count() / std::max<long long>(workgroups, 1), keys / 256, 64LL })); };
+    plan.tile_split = split(plan.tiles * a.n_kv);
+    plan.row_split = split((long long)a.n_seqs * a.n_kv);
+    plan.n_split = std::max(plan.tiles ? plan.tile_split : 1, plan.rows ? plan.row_split : 1);
     return plan;
 }
 
-size_t partial_bytes(int n_split, size_t outputs, int dim) { return n_split < 2 ? 0 : (outputs * ((size_t)n_split * (dim + 2) + 1) * 4 + 15) & ~(size_t)15; }
+size_t partial_bytes(int n_split, size_t outputs, int dim) { return n_split < 2 ? 0 : (outputs * (size_t)n_split * (dim + 2) * 4 + 15) & ~(size_t)15; }
 }    // namespace
 
 int hip_qk_norm_rope_kv_paged_bf16(const hip_paged_kv* cache, const void* q, const void* k, const void* v, const void* q_norm_w, const void* k_norm_w, const void* cos_tab, const void* sin_tab,
@@ -147,26 +146,19 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
     const size_t outputs = (size_t)n_tokens * n_q_heads;
     Plan plan = plan_attention(a, group, n_tokens, max_new, window, n_sink);
     while (plan.n_split > 1 && partial_bytes(plan.n_split, outputs, dim) > workspace_bytes) { plan.n_split--; }
-    if (plan.n_tiles * a.n_kv > MOST_BLOCKS || (long long)a.n_seqs * a.n_kv > MOST_BLOCKS) { return -1; }
-    PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)workspace, (size_t)ldq, (size_t)ldy, n_q_heads, group, n_tokens, max_new, window, n_sink, plan.n_split, 1, plan.min_rows,
-                         1.4426950408889634f / sqrtf((float)dim) };
-    if (plan.rows)
+    const int tile_split = std::min(plan.tile_split, plan.n_split), row_split = std::min(plan.row_split, plan.n_split);
+    const long long tiles = plan.tiles * a.n_kv, sequences = plan.rows ? (long long)a.n_seqs * a.n_kv : 0;
+    const long long blocks = tiles * tile_split + sequences * row_split;
+    const long long sums = (tile_split > 1 ? tiles * (PA_TILE / 16) : 0) + (row_split > 1 ? sequences : 0);
+    if (blocks > MOST_BLOCKS || sums > MOST_BLOCKS) { return -1; }
+    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)workspace, (size_t)ldq, (size_t)ldy, n_q_heads, group, n_tokens, max_new, window, n_sink, plan.n_split,
+                               (int)plan.tiles, tile_split, row_split, plan.min_rows, 1.4426950408889634f / sqrtf((float)dim) };
+    const auto kernel = CCQ_PAGED_KERNEL(paged_attention_kernel, cache);
+    kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, p);
+    if (sums > 0)
     {
-        p.split = std::min(plan.rows_split, plan.n_split);
-        const auto kernel = CCQ_PAGED_KERNEL(paged_attention_rows_kernel, cache);
-        kernel<<<dim3((unsigned)(a.n_seqs * a.n_kv), p.split), 256, 0, stream()>>>(a, p);
-    }
-    if (plan.tiles)
-    {
-        p.split = std::min(plan.tiles_split, plan.n_split);
-        const auto kernel = CCQ_PAGED_KERNEL(paged_attention_tile_kernel, cache);
-        kernel<<<dim3((unsigned)(plan.n_tiles * a.n_kv), p.split), 256, 0, stream()>>>(a, p);
-    }
-    if (plan.n_split > 1)
-    {
-        const unsigned blocks = (unsigned)(n_tokens * ((n_q_heads * dim + 1023) / 1024));
-        if (dim == 64) { paged_attention_combine_kernel<64><<<blocks, 256, 0, stream()>>>(a, p); }
-        else { paged_attention_combine_kernel<128><<<blocks, 256, 0, stream()>>>(a, p); }
+        if (dim == 64) { paged_attention_combine_kernel<64><<<(unsigned)sums, 256, 0, stream()>>>(a, p); }
+        else { paged_attention_combine_kernel<128><<<(unsigned)sums, 256, 0, stream()>>>(a, p); }
     }
     return finish("attention_paged");
 }

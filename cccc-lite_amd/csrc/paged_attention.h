@@ -13,18 +13,18 @@ struct PagedAttention
 {
     const uint16_t* q;
     uint16_t* y;
-    float* partial;                 // [range][token][head][dim] sums, [range][token][head] (max, sum), [token][head] ranges: only where there are ranges
+    float* partial;                 // [range][token][head][dim] sums, then [range][token][head] (max, sum): only where there are ranges
     size_t ldq, ldy;
     int n_q, group, n_tokens, max_new, window, n_sink;
-    int n_split;                    // most ranges of a row, as `partial` is laid out
-    int split;                      // ranges of this launch, n_split or fewer
-    int min_rows;                   // sequences of at most so many rows per kv head are the other kernel's
-    float scale;                    // 1 / sqrt(dim) log2 e
+    int n_split;                    // ranges of keys that `partial` is laid out for
+    int tiles, tile_split;          // tiles of 128 rows (at most) and the most ranges of each
+    int row_split;                  // most ranges of a sequence of at most 16 rows per kv head
+    int min_rows;                   // sequences of at most so many rows per kv head are not cut into tiles
+    float scale;                    // log2 e / sqrt(dim)
 
     __device__ __forceinline__ size_t outputs() const { return (size_t)n_tokens * n_q; }
     __device__ __forceinline__ float* sums(int range, size_t row, int dim) const { return partial + ((size_t)range * outputs() + row) * dim; }
     __device__ __forceinline__ float2* stats(int range, size_t row, int dim) const { return (float2*)(partial + (size_t)n_split * outputs() * dim) + (size_t)range * outputs() + row; }
-    __device__ __forceinline__ int* ranges(size_t row, int dim) const { return (int*)(partial + (size_t)n_split * outputs() * (dim + 2)) + row; }
 };
 
 // The new tokens of a sequence that a call computes: tokens first .. first + n - 1 of the activations, the first of them at position pos.
@@ -45,8 +45,9 @@ __device__ __forceinline__ NewTokens new_tokens(const PagedArgs& a, const PagedA
 template <int SIZE>
 struct KeyBlocks
 {
-    int n, sinks, skip;
+    int n = 0, sinks = 0, skip = 0;
 
+    __device__ __forceinline__ KeyBlocks() {}
     __device__ __forceinline__ KeyBlocks(const PagedAttention& p, int lo, int hi)
     {
         const int blocks = max(hi + SIZE, 0) / SIZE;
@@ -69,6 +70,75 @@ struct KeyBlocks
 };
 
 __device__ __forceinline__ bool sees(const PagedAttention& p, int pos, int key) { return key <= pos && (p.window == 0 || key > pos - p.window || key < p.n_sink); }
+
+// Rows row0 .. of a sequence that a workgroup takes (s < 0: none), the positions of their tokens and the keys they see, in ranges of `per` blocks.
+template <int SIZE, int ROWS>
+struct Rows
+{
+    int s = -1, row0, n_rows, lo, hi, per, n_ranges;
+    NewTokens mine;
+    KeyBlocks<SIZE> blocks;
+
+    __device__ __forceinline__ void cut(const PagedAttention& p, int split, int multiple, int least)
+    {
+        lo = mine.pos + row0 / p.group;
+        hi = mine.pos + min(row0 + ROWS - 1, n_rows - 1) / p.group;
+        blocks = KeyBlocks<SIZE>(p, lo, hi);
+        per = max(((blocks.n + split - 1) / split + multiple - 1) / multiple * multiple, least);
+        n_ranges = max((blocks.n + per - 1) / per, 1);
+    }
+};
+
+constexpr int PA_ROWS = 16, PA_ROWS_KEYS = 32, PA_TILE = 128, PA_TILE_KEYS = 64;
+
+// A sequence of up to 16 rows per kv head.
+__device__ __forceinline__ Rows<PA_ROWS_KEYS, PA_ROWS> sequence_rows(const PagedArgs& a, const PagedAttention& p, int s)
+{
+    Rows<PA_ROWS_KEYS, PA_ROWS> r;
+    r.mine = new_tokens(a, p, s);
+    r.row0 = 0;
+    r.n_rows = r.mine.n * p.group;
+    if (r.n_rows == 0 || r.n_rows > PA_ROWS) { return r; }
+    r.s = s;
+    r.cut(p, p.row_split, 4, 8);
+    return r;
+}
+
+// Tile `tile` of those of all sequences, a sequence's last ones first: they see the most keys.  Called by whole waves: a lane per sequence, their tiles added up.
+__device__ __forceinline__ Rows<PA_TILE_KEYS, PA_TILE> tile_rows(const PagedArgs& a, const PagedAttention& p, int tile)
+{
+    Rows<PA_TILE_KEYS, PA_TILE> r;
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.n_seqs; base += 64)
+    {
+        int tiles = 0;
+        if (base + lane < a.n_seqs)
+        {
+            const int rows = new_tokens(a, p, base + lane).n * p.group;
+            tiles = rows > p.min_rows ? (rows + PA_TILE - 1) / PA_TILE : 0;
+        }
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1)
+        {
+            const int below = __shfl_up(upto, o);
+            upto += lane >= o ? below : 0;
+        }
+        const unsigned long long past = __ballot(upto > tile);
+        if (past != 0)
+        {
+            const int at = __builtin_ctzll(past);
+            r.s = __builtin_amdgcn_readfirstlane(base + at);
+            r.mine = new_tokens(a, p, r.s);
+            r.row0 = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(upto, at) - 1 - tile) * PA_TILE;
+            r.n_rows = r.mine.n * p.group;
+            r.cut(p, p.tile_split, 1, 4);
+            return r;
+        }
+        tile -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return r;
+}
 
 // The weights' running maximum moves only when a score exceeds it by more than this (in log2): until then they are at most 2^8, which FP32 sums
 // and BF16's exponent do not notice, and the sums are left alone.
@@ -148,40 +218,39 @@ __device__ __forceinline__ float value_of_kind(int kind) { return kind == 0 ? IN
 
 // Up to 16 rows of a kv head: single tokens, or a few.  Bound by the cached rows' way from memory.
 //   A workgroup of four waves takes a range of the sequence's blocks of 32 keys, a wave every fourth block, each with a pipeline of its own: rows go by
-// direct loads to the wave's part of LDS, STAGES blocks ahead, and nothing but the wave's own count of loads in flight is waited for.
+// direct loads to the wave's part of LDS, keys and values STAGES blocks ahead each, and nothing but the wave's own count of loads in flight is waited for.
 //   scores: v_mfma_f32_16x16x32_bf16, key rows as row operand, the 16 queries as columns: D lane (row j = lane % 16, g = lane / 16) holds keys 4 g .. + 3
 //           of 16.  FP8 keys become BF16 in registers, times their power of two (a lane's operand is one key's): exact.
 //   V p:    the eight weights of a lane (keys 4 g .. + 3 and 16 + 4 g .. + 3) are its column operand as they are; the row operand (dim, the same keys)
 //           comes from transposing reads.  FP8 values' powers of two go to the weights.
 // LDS: chunk c (16 bytes) of row r lies at c ^ swizzle(r), so that the operand reads hit all banks.
-// Grid: (sequences x kv heads) x ranges.
 template <int TYPE, int DIM>
-__global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedArgs a, const PagedAttention p)
+struct RowsForm
 {
-    constexpr int KEYS = 32, STAGES = 2;
-    constexpr int ROW = DIM * CODE_BYTES<TYPE>, CHUNKS = ROW / 16, SIDE = KEYS * ROW, SCALES = TYPE == DT_BF16 ? 0 : 256, STAGE = 2 * SIDE + SCALES;
-    constexpr int ROWS_PER_LOAD = 1024 / ROW, LOADS = SIDE / 1024;
-    constexpr int SUM = DIM + 4;                                            // floats per row of the sums
-    constexpr int LDS = STAGES * STAGE * 4 > 4 * 16 * SUM * 4 ? STAGES * STAGE * 4 : 4 * 16 * SUM * 4;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS];
-    __shared__ float2 stat[4][16];
-    const int kvh = blockIdx.x % a.n_kv, s = blockIdx.x / a.n_kv;
+    static constexpr int KEYS = PA_ROWS_KEYS, STAGES = DIM * CODE_BYTES<TYPE> == 256 ? 1 : 2;
+    static constexpr int ROW = DIM * CODE_BYTES<TYPE>, SIDE = KEYS * ROW, SCALES = TYPE == DT_BF16 ? 0 : 256, WAVE = STAGES * (2 * SIDE + SCALES);
+    static constexpr int SUM = DIM + 4;                                     // floats per row of the sums
+    static constexpr int STAT = 4 * (WAVE > PA_ROWS * SUM * 4 ? WAVE : PA_ROWS * SUM * 4), LDS = STAT + 4 * PA_ROWS * 8;
+};
+
+template <int TYPE, int DIM>
+__device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int s, int kvh, int range)
+{
+    typedef RowsForm<TYPE, DIM> F;
+    constexpr int KEYS = F::KEYS, STAGES = F::STAGES, ROW = F::ROW, SIDE = F::SIDE, SUM = F::SUM, CHUNKS = ROW / 16;
+    constexpr int ROWS_PER_LOAD = 1024 / ROW, LOADS = SIDE / 1024, KEY_LOADS = LOADS + (TYPE == DT_BF16 ? 0 : 1);
+    float2* const stat = (float2*)(lds + F::STAT);                          // [wave][row] (max, sum)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 15, g = lane >> 4;
-    const NewTokens mine = new_tokens(a, p, s);
-    const int n_rows = mine.n * p.group;
-    if (n_rows == 0 || n_rows > 16) { return; }
-    const int last_pos = mine.pos + mine.n - 1;
-    const KeyBlocks<KEYS> blocks(p, mine.pos, last_pos);
-    const int per = max(((blocks.n + p.split - 1) / p.split + 3) & ~3, 8);
-    const int n_ranges = max((blocks.n + per - 1) / per, 1);
-    const int range = blockIdx.y, begin = range * per, end = min(blocks.n, begin + per);
-    if (range >= n_ranges) { return; }
+    const auto rows = sequence_rows(a, p, s);
+    if (rows.s < 0 || range >= rows.n_ranges) { return; }
+    const NewTokens mine = rows.mine;
+    const auto& blocks = rows.blocks;
+    const int n_rows = rows.n_rows, begin = range * rows.per, end = min(blocks.n, begin + rows.per);
 
     const int row = min(j, n_rows - 1), token = row / p.group, head = kvh * p.group + row % p.group;
     const int my_pos = mine.pos + token;
-    // FP8: eight elements 32 c + 8 g .. + 7, as for BF16
-    u32x4 qf[DIM / 32];
+    u32x4 qf[DIM / 32];                                                     // elements 32 c + 8 g .. + 7
 #pragma unroll
     for (int c = 0; c < DIM / 32; c++) { qf[c] = *(const u32x4*)(p.q + (size_t)(mine.first + token) * p.ldq + (size_t)head * DIM + c * 32 + g * 8); }
 
@@ -190,52 +259,42 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
         if constexpr (TYPE == DT_BF16) { return DIM == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
         else { return DIM == 128 ? ((r >> 1) & 3) | ((r >> 4) & 1) << 2 : ((r >> 2) & 1) | ((r >> 4) & 1) << 1; }
     };
-    uint8_t* const my_lds = lds + wave * STAGES * STAGE;
+    // the wave's LDS: key blocks, value blocks, exponents (lanes 0 .. 31 keys', then values')
+    uint8_t* const my_lds = lds + wave * F::WAVE;
     const uint32_t my_lds0 = __builtin_amdgcn_readfirstlane(lds_offset(my_lds));
+    constexpr int VALUES = STAGES * SIDE, EXPONENTS = 2 * VALUES;
     // the wave's n-th block of the range is list entry begin + wave + 4 n
     const int n_mine = begin + wave < end ? (end - begin - wave + 3) / 4 : 0;
-    int pages = 0;                                                          // lane l: page of rows 16 (l % 2) of the wave's block n0 + l / 2; -1: none
+    auto block_of = [&](int n) { return blocks.block(begin + wave + 4 * n); };
+    int pages = 0;                                                          // lane l: page of rows 16 (l % 2) .. + 15 of the wave's block 32 k + l / 2; -1: none
     auto look_up = [&](int n0) {
         const int i = begin + wave + 4 * (n0 + (lane >> 1));
         const int pos = blocks.block(i) * KEYS + 16 * (lane & 1);
-        pages = i >= end || pos > last_pos ? 0 : max(paged_page(a, s, pos), -1);
+        pages = i >= end || pos > rows.hi ? 0 : max(paged_page(a, s, pos), -1);
     };
-    int tag[STAGES];                                                        // per stage: bits of the half blocks that have no page
-    auto stage = [&](int n, int at) {
-        if (n % 32 == 0) { look_up(n); }
-        const int key0 = blocks.block(begin + wave + 4 * n) * KEYS;
-        int bad = 0;
-        size_t offset[2], scale_offset[2];
+    // half blocks (16 rows) of entry n: their page, and where they begin
+    auto page_of = [&](int n, int half) { return __builtin_amdgcn_readlane(pages, (n % 32) * 2 + half); };
+    auto stage = [&](int n, bool values) {
+        const int key0 = block_of(n) * KEYS;
+        const uint32_t to = my_lds0 + (values ? VALUES : 0) + n % STAGES * SIDE;
+        size_t exponent_at[2];
 #pragma unroll
         for (int half = 0; half < 2; half++)
         {
-            const int page = __builtin_amdgcn_readlane(pages, (n % 32) * 2 + half);
-            bad |= page < 0 ? 1 << half : 0;
-            const size_t r = paged_row(a, kvh, key0 + 16 * half);
-            offset[half] = max(page, 0) * a.page_stride + r * ROW;
-            scale_offset[half] = max(page, 0) * a.scale_stride + r;
-        }
-        const uint32_t to = my_lds0 + at * STAGE;
+            const size_t page = max(page_of(n, half), 0), r0 = paged_row(a, kvh, key0 + 16 * half);
+            const uint8_t* const from = (values ? a.v : a.k) + page * a.page_stride + r0 * ROW;
+            exponent_at[half] = page * a.scale_stride + r0;
 #pragma unroll
-        for (int i = 0; i < LOADS; i++)
-        {
-            const int r = i * ROWS_PER_LOAD + lane / CHUNKS, c = lane % CHUNKS;
-            const size_t from = offset[i * ROWS_PER_LOAD / 16] - (size_t)(i * ROWS_PER_LOAD / 16 * 16 * ROW);
-            load_to_lds<true>(to + i * 1024, a.k + from, (uint32_t)(r * ROW + (c ^ key_swizzle(r)) * 16));
-        }
-#pragma unroll
-        for (int i = 0; i < LOADS; i++)
-        {
-            const int r = i * ROWS_PER_LOAD + lane / CHUNKS, c = lane % CHUNKS;
-            const size_t from = offset[i * ROWS_PER_LOAD / 16] - (size_t)(i * ROWS_PER_LOAD / 16 * 16 * ROW);
-            load_to_lds<true>(to + SIDE + i * 1024, a.v + from, (uint32_t)(r * ROW + (c ^ value_swizzle(r)) * 16));
+            for (int i = 0; i < LOADS / 2; i++)
+            {
+                const int in = i * ROWS_PER_LOAD + lane / CHUNKS, r = 16 * half + in, c = lane % CHUNKS;
+                load_to_lds<true>(to + (half * LOADS / 2 + i) * 1024, from, (uint32_t)(in * ROW + (c ^ (values ? value_swizzle(r) : key_swizzle(r))) * 16));
+            }
         }
         if constexpr (TYPE != DT_BF16)
         {
-            // lanes 0 .. 31: the keys' exponents, then the values'
-            bytes_to_lds(to + 2 * SIDE, (lane < 32 ? a.k_scale : a.v_scale) + (lane & 16 ? scale_offset[1] : scale_offset[0]) + (lane & 15));
+            if (!values) { bytes_to_lds(my_lds0 + EXPONENTS + n % STAGES * F::SCALES, (lane < 32 ? a.k_scale : a.v_scale) + (lane & 16 ? exponent_at[1] : exponent_at[0]) + (lane & 15)); }
         }
-        tag[at] = bad;
     };
 
     float m = -INFINITY, l = 0.0f;
@@ -243,18 +302,26 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
 #pragma unroll
     for (int d = 0; d < DIM / 16; d++) { out[d] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f }; }
 
-    auto block = [&](int n, int at) {
-        const uint8_t* const kb = my_lds + at * STAGE;
-        const uint8_t* const vb = kb + SIDE;
-        const int b = blocks.block(begin + wave + 4 * n), bad = tag[at];
-        float vscale[8];
+    auto block = [&](int n) {
+        const uint8_t* const kb = my_lds + n % STAGES * SIDE;
+        const uint8_t* const vb = my_lds + VALUES + n % STAGES * SIDE;
+        const uint8_t* const exponents = my_lds + EXPONENTS + n % STAGES * F::SCALES;
+        const int b = block_of(n), bad = (page_of(n, 0) < 0 ? 1 : 0) | (page_of(n, 1) < 0 ? 2 : 0);
+        // what was asked for behind the keys of n may still be on its way
+        if (STAGES == 2 && n + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * LOADS + KEY_LOADS) : "memory"); }
+        else { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS) : "memory"); }
         f32x4 acc[2] = { { 0.0f, 0.0f, 0.0f, 0.0f }, { 0.0f, 0.0f, 0.0f, 0.0f } };
+        u32x4 value_exponents[2];
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
         {
             const int r = 16 * kt + j;
             float kscale = 1.0f;
-            if constexpr (TYPE != DT_BF16) { kscale = bits_to_f32(*(const uint32_t*)(kb + 2 * SIDE + r * 4) << 23); }
+            if constexpr (TYPE != DT_BF16)
+            {
+                kscale = bits_to_f32(*(const uint32_t*)(exponents + r * 4) << 23);
+                value_exponents[kt] = *(const u32x4*)(exponents + 128 + (16 * kt + 4 * g) * 4);
+            }
 #pragma unroll
             for (int c = 0; c < DIM / 32; c++)
             {
@@ -269,16 +336,16 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
                 acc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[c]), acc[kt], 0, 0, 0);
             }
         }
-        if constexpr (TYPE != DT_BF16)
+        if (n + STAGES < n_mine)
         {
-#pragma unroll
-            for (int kt = 0; kt < 2; kt++)
-            {
-                const u32x4 e = *(const u32x4*)(kb + 2 * SIDE + 128 + (16 * kt + 4 * g) * 4);
-#pragma unroll
-                for (int v = 0; v < 4; v++) { vscale[4 * kt + v] = bits_to_f32(e[v] << 23); }
-            }
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");           // the keys have been read
+            if ((n + STAGES) % 32 == 0) { look_up(n + STAGES); }
+            stage(n + STAGES, false);
         }
+        if (STAGES == 2 && n + 2 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS + 2 * KEY_LOADS) : "memory"); }
+        else if (STAGES == 2 && n + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS + KEY_LOADS) : "memory"); }
+        else if (STAGES == 1 && n + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(KEY_LOADS) : "memory"); }
+        else { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
         u32x4 vf[DIM / 16];
 #pragma unroll
         for (int d = 0; d < DIM / 16; d++)
@@ -298,7 +365,12 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
                 vf[d] = u32x4{ lo[0], lo[1], hi[0], hi[1] };
             }
         }
-        const bool plain = KeyBlocks<KEYS>::plain(p, mine.pos, last_pos, b) && bad == 0;
+        if (n + STAGES < n_mine)
+        {
+            asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");           // the values have been read
+            stage(n + STAGES, true);
+        }
+        const bool plain = KeyBlocks<KEYS>::plain(p, rows.lo, rows.hi, b) && bad == 0;
         float score[8];
         uint32_t seen = 0xFFu;
 #pragma unroll
@@ -319,7 +391,7 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
         {
             top = fmaxf(top, __shfl_xor(top, 16));
             const float next = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
-            const float shrink = next > -INFINITY ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
+            const float shrink = m > -INFINITY ? __builtin_amdgcn_exp2f(m - next) : 1.0f;         // sums of nothing: 0, or what is not finite
             m = next;
             l *= shrink;
 #pragma unroll
@@ -333,7 +405,7 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
         if constexpr (TYPE != DT_BF16)
         {
 #pragma unroll
-            for (int e = 0; e < 8; e++) { w[e] = seen >> e & 1 ? w[e] * vscale[e] : 0.0f; }
+            for (int e = 0; e < 8; e++) { w[e] = seen >> e & 1 ? w[e] * bits_to_f32(value_exponents[e >> 2][e & 3] << 23) : 0.0f; }
         }
         const bf16x8 pb = { (__bf16)w[0], (__bf16)w[1], (__bf16)w[2], (__bf16)w[3], (__bf16)w[4], (__bf16)w[5], (__bf16)w[6], (__bf16)w[7] };
         uint32_t odd = 0;
@@ -366,30 +438,23 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
         for (int d = 0; d < DIM / 16; d++) { out[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[d]), pb, out[d], 0, 0, 0); }
     };
 
-    constexpr int IN_FLIGHT = 2 * LOADS + (TYPE == DT_BF16 ? 0 : 1);        // loads per stage
-    if (0 < n_mine) { stage(0, 0); }
-    if (1 < n_mine) { stage(1, 1); }
-    for (int n = 0; n < n_mine; n += 2)
+    if (n_mine > 0)
     {
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-        {
-            if (n + u >= n_mine) { break; }
-            if (n + u + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(IN_FLIGHT) : "memory"); }
-            else { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
-            block(n + u, u);
-            if (n + u + 2 < n_mine)
-            {
-                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");       // the stage has been read
-                stage(n + u + 2, u);
-            }
-        }
+        look_up(0);
+        stage(0, false);
+        stage(0, true);
     }
+    if (STAGES == 2 && n_mine > 1)
+    {
+        stage(1, false);
+        stage(1, true);
+    }
+    for (int n = 0; n < n_mine; n++) { block(n); }
 
     // the four waves' sums of a row meet in LDS
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (g == 0) { stat[wave][j] = make_float2(m, l); }
+    if (g == 0) { stat[wave * 16 + j] = make_float2(m, l); }
     __syncthreads();
     float* const sums = (float*)lds;
 #pragma unroll
@@ -399,13 +464,13 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
     if (r >= n_rows) { return; }
     float top = -INFINITY, total = 0.0f, weight[4];
 #pragma unroll
-    for (int w = 0; w < 4; w++) { top = fmaxf(top, stat[w][r].x); }
+    for (int w = 0; w < 4; w++) { top = fmaxf(top, stat[w * 16 + r].x); }
     const float base = top > -INFINITY ? top : 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; w++)
     {
-        weight[w] = __builtin_amdgcn_exp2f(stat[w][r].x - base);            // 2^-inf = 0 for a wave without a key
-        total += weight[w] * stat[w][r].y;
+        weight[w] = __builtin_amdgcn_exp2f(stat[w * 16 + r].x - base);            // 2^-inf = 0 for a wave without a key
+        total += weight[w] * stat[w * 16 + r].y;
     }
     float sum[DIM / 16];
 #pragma unroll
@@ -416,8 +481,7 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
         for (int w = 0; w < 4; w++) { sum[d] += weight[w] > 0.0f || weight[w] != weight[w] ? weight[w] * sums[(w * 16 + r) * SUM + d0 + d] : 0.0f; }
     }
     const size_t at_token = mine.first + r / p.group, at_head = kvh * p.group + r % p.group, at_row = at_token * p.n_q + at_head;
-    if (p.n_split > 1 && range == 0 && d0 == 0) { *p.ranges(at_row, DIM) = n_ranges; }
-    if (n_ranges > 1)
+    if (rows.n_ranges > 1)
     {
         float* const dst = p.sums(range, at_row, DIM) + d0;
 #pragma unroll
@@ -441,58 +505,28 @@ __global__ __launch_bounds__(256) void paged_attention_rows_kernel(const PagedAr
 //   V p:    registers 8 u .. + 7 of a lane are its column operand of the u-th 16 keys as they are; the row operand (dim, the same keys) comes from
 //           two transposing reads.
 // A row's statistics and sums stay in the two lanes that have it.
-// Grid: (tiles x kv heads) x ranges; which sequence a tile belongs to is found from seq_start.  The last tiles of a sequence, which see the most
-// keys, go first.
-template <int TYPE, int DIM, int RT = 1>
-__global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const PagedArgs a, const PagedAttention p)
+template <int TYPE, int DIM>
+struct TileForm
 {
-    constexpr int KEYS = 64, ROWS = 128 * RT, ROW = DIM * 2, CHUNKS = ROW / 16, BLOCK = KEYS * ROW;
+    static constexpr int BLOCK = PA_TILE_KEYS * DIM * 2;
+    static constexpr int ODD = 4 * BLOCK, LDS = ODD + 32;                   // two blocks of keys, two of values
+};
+
+template <int TYPE, int DIM>
+__device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int tile, int kvh, int range)
+{
+    typedef TileForm<TYPE, DIM> F;
+    constexpr int RT = 1, KEYS = PA_TILE_KEYS, ROW = DIM * 2, CHUNKS = ROW / 16, BLOCK = F::BLOCK;
     constexpr int CODES = DIM * CODE_BYTES<TYPE>;                           // bytes of a cached row
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * BLOCK];       // two blocks of keys, two of values
-    __shared__ __attribute__((aligned(16))) uint32_t odd_rows[2][4];        // per buffer of values and wave that staged: something infinite or NaN
-    const int kvh = blockIdx.x % a.n_kv;
+    uint32_t* const odd_rows = (uint32_t*)(lds + F::ODD);                   // per buffer of values and wave that staged: something infinite or NaN
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 31, h = lane >> 5;
-
-    // the sequence and tile of this workgroup: a lane per sequence, their tiles added up
-    int s = -1, tile = blockIdx.x / a.n_kv;
-    for (int base = 0; base < a.n_seqs; base += 64)
-    {
-        const int i = base + lane;
-        int tiles = 0;
-        if (i < a.n_seqs)
-        {
-            const int rows = new_tokens(a, p, i).n * p.group;
-            tiles = rows > p.min_rows ? (rows + ROWS - 1) / ROWS : 0;
-        }
-        int upto = tiles;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1)
-        {
-            const int below = __shfl_up(upto, o);
-            upto += lane >= o ? below : 0;
-        }
-        const unsigned long long past = __ballot(upto > tile);
-        if (past != 0)
-        {
-            const int at = __builtin_ctzll(past);
-            s = base + at;
-            tile = __builtin_amdgcn_readlane(upto, at) - 1 - tile;          // of the sequence, from its end
-            break;
-        }
-        tile -= __builtin_amdgcn_readlane(upto, 63);
-    }
-    if (s < 0) { return; }
-    s = __builtin_amdgcn_readfirstlane(s);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    const NewTokens mine = new_tokens(a, p, s);
-    const int n_rows = mine.n * p.group, row0 = tile * ROWS;
-    const int tile_lo = mine.pos + row0 / p.group, tile_hi = mine.pos + min(row0 + ROWS - 1, n_rows - 1) / p.group;
-    const KeyBlocks<KEYS> blocks(p, tile_lo, tile_hi);
-    const int per = max((blocks.n + p.split - 1) / p.split, 4);
-    const int n_ranges = max((blocks.n + per - 1) / per, 1);
-    const int range = blockIdx.y, begin = range * per, end = min(blocks.n, begin + per);
-    if (range >= n_ranges) { return; }
+    const auto rows = tile_rows(a, p, tile);
+    if (rows.s < 0 || range >= rows.n_ranges) { return; }
+    const NewTokens mine = rows.mine;
+    const auto& blocks = rows.blocks;
+    const int s = rows.s, n_rows = rows.n_rows, row0 = rows.row0, tile_lo = rows.lo, tile_hi = rows.hi;
+    const int begin = range * rows.per, end = min(blocks.n, begin + rows.per);
 
     // the wave's rows
     const int wave_lo = mine.pos + min(row0 + wave * 32 * RT, n_rows - 1) / p.group, wave_hi = mine.pos + min(row0 + wave * 32 * RT + 32 * RT - 1, n_rows - 1) / p.group;
@@ -529,14 +563,14 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
     };
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds));
     constexpr int PIECES = TYPE == DT_BF16 ? 1 : CODES * 16 / 1024;         // FP8: 16 bytes per lane each of the wave's 16 rows
-    struct Rows
+    struct Staged
     {
         u32x4 codes[PIECES];
         uint32_t exponent[PIECES];
     };
     const uint32_t key_from = lane * 16 ^ key_swizzle(lane / CHUNKS) * 16, value_from = lane * 16 ^ value_swizzle(lane / CHUNKS) * 16;
     // the wave's 16 rows of entry i: on their way to LDS (BF16) or to registers
-    auto load = [&](bool values, int i, int page, uint32_t to, Rows& raw) {
+    auto load = [&](bool values, int i, int page, uint32_t to, Staged& raw) {
         const size_t r0 = paged_row(a, kvh, blocks.block(i) * KEYS + 16 * wave);
         const uint8_t* const from = (values ? a.v : a.k) + page * a.page_stride + r0 * CODES;
         if constexpr (TYPE == DT_BF16)
@@ -563,7 +597,7 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
         }
     };
     // FP8: the loaded rows to LDS as BF16; the result tells whether something is not finite
-    auto store = [&](bool values, uint32_t to, const Rows& raw) {
+    auto store = [&](bool values, uint32_t to, const Staged& raw) {
         uint32_t odd = 0;
         if constexpr (TYPE != DT_BF16)
         {
@@ -596,7 +630,7 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
             for (int n = 0; n < ROW * 16 / 1024; n++) { odd |= not_finite(*(const u32x4*)(lds + values_at(i) + part + n * 1024 + lane * 16)); }
         }
         const bool any = __any(odd != 0);
-        if (lane == 0) { odd_rows[i & 1][wave] = any; }
+        if (lane == 0) { odd_rows[(i & 1) * 4 + wave] = any; }
     };
 
     const uint32_t k_at = j * ROW + (h ^ key_swizzle(j)) * 16;             // of chunk h of key row j; chunk 2 c + h at k_at ^ 32 c
@@ -699,7 +733,7 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
     // Weight 0 times an infinity is NaN: where some rows do not see every key of entry i, what is infinite or NaN among its values is added to the sums of
     // the rows that see it and cleared in front of the products.
     auto set_apart = [&](int i, int lacks) {
-        const u32x4 odd = *(const u32x4*)odd_rows[i & 1];
+        const u32x4 odd = *(const u32x4*)(odd_rows + (i & 1) * 4);
         if (__builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]) == 0) { return; }
         uint8_t* const vb = lds + values_at(i);
         const int b = blocks.block(i);
@@ -738,7 +772,7 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
 
     if (begin < end)
     {
-        Rows raw_k, raw_v;
+        Staged raw_k, raw_v;
         f32x16 acc[RT][2];
         uint32_t odd = 0;
         auto load_both = [&](int i) {
@@ -790,8 +824,7 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
         const float total = l[t] + __shfl_xor(l[t], 32);
         if (!real[t]) { continue; }
         const size_t at_row = (size_t)token[t] * p.n_q + head[t];
-        if (p.n_split > 1 && range == 0 && h == 0) { *p.ranges(at_row, DIM) = n_ranges; }
-        if (n_ranges > 1)
+        if (rows.n_ranges > 1)
         {
             float* const dst = p.sums(range, at_row, DIM) + 4 * h;
 #pragma unroll
@@ -816,30 +849,66 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_tile_kernel(const
     }
 }
 
-// Sums of the key ranges of a token's heads, four dims per thread: rescaled to the largest maximum, added in the order of the ranges, divided by the
-// sum of the weights, one rounding.  Grid: tokens x workgroups over the heads.
+// Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then ranges x sequences x kv heads.
+template <int TYPE, int DIM>
+__global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs a, const PagedAttention p)
+{
+    typedef RowsForm<TYPE, DIM> R;
+    typedef TileForm<TYPE, DIM> T;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS > T::LDS ? R::LDS : T::LDS];
+    static_assert(sizeof(lds) <= 80 * 1024, "two workgroups on a CU");
+    const int tiles = p.tiles * a.n_kv, n_tiles = tiles * p.tile_split;
+    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
+    else
+    {
+        const int at = blockIdx.x - n_tiles, sequences = a.n_seqs * a.n_kv;
+        attend_rows<TYPE, DIM>(a, p, lds, at % sequences / a.n_kv, at % a.n_kv, at / sequences);
+    }
+}
+
+// Sums of the key ranges of 16 rows, DIM / 16 dims of a row per thread: rescaled to the largest maximum, added in the order of the ranges, divided by the
+// sum of the weights, one rounding.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads where tiles have ranges, then
+// sequences x kv heads where those do.
 template <int DIM>
 __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
 {
-    constexpr int LANES = DIM / 4, PER_WG = 256 / LANES;
-    const int parts = (p.n_q + PER_WG - 1) / PER_WG;
-    const int t = blockIdx.x / parts, head = blockIdx.x % parts * PER_WG + threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
-    const int s = paged_sequence(a, t);
-    if (s < 0 || head >= p.n_q || new_tokens(a, p, s).n == 0) { return; }
-    const size_t row = (size_t)t * p.n_q + head;
-    const int n = *p.ranges(row, DIM);
-    if (n <= 1) { return; }                                                 // written already
-    f32x4 sum = { 0.0f, 0.0f, 0.0f, 0.0f };
+    constexpr int PER = DIM / 16, PARTS = PA_TILE / 16;
+    const int n_tiles = p.tile_split > 1 ? p.tiles * PARTS * a.n_kv : 0, kvh = blockIdx.x % a.n_kv;
+    NewTokens mine;
+    int row, n;
+    if ((int)blockIdx.x < n_tiles)
+    {
+        const int at = blockIdx.x / a.n_kv;
+        const auto rows = tile_rows(a, p, at / PARTS);
+        row = rows.row0 + at % PARTS * 16 + (threadIdx.x >> 4);
+        if (rows.s < 0 || row >= rows.n_rows) { return; }
+        mine = rows.mine;
+        n = rows.n_ranges;
+    }
+    else
+    {
+        const auto rows = sequence_rows(a, p, (blockIdx.x - n_tiles) / a.n_kv);
+        row = threadIdx.x >> 4;
+        if (rows.s < 0 || row >= rows.n_rows) { return; }
+        mine = rows.mine;
+        n = rows.n_ranges;
+    }
+    if (n <= 1) { return; }
+    const size_t token = mine.first + row / p.group, head = kvh * p.group + row % p.group, at_row = token * p.n_q + head;
+    const int d0 = (threadIdx.x & 15) * PER;
+    f32x4 sum[PER / 4] = {};
     float m = -INFINITY, l = 0.0f;
     for (int r0 = 0; r0 < n; r0 += 8)
     {
-        f32x4 part[8];                                                      // eight ranges requested at once
+        f32x4 part[8][PER / 4];                                             // eight ranges requested at once
         float2 stat[8];
 #pragma unroll
         for (int r = 0; r < 8; r++)
         {
-            stat[r] = *p.stats(min(r0 + r, n - 1), row, DIM);
-            part[r] = *(const f32x4*)(p.sums(min(r0 + r, n - 1), row, DIM) + d);
+            const int range = min(r0 + r, n - 1);
+            stat[r] = *p.stats(range, at_row, DIM);
+#pragma unroll
+            for (int d = 0; d < PER / 4; d++) { part[r][d] = *(const f32x4*)(p.sums(range, at_row, DIM) + d0 + 4 * d); }
         }
         float top = m;
 #pragma unroll
@@ -847,22 +916,29 @@ __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const Page
         const float base = top > -INFINITY ? top : 0.0f, shrink = __builtin_amdgcn_exp2f(m - base);
         m = top;
         l *= shrink;
-        sum *= shrink;
+#pragma unroll
+        for (int d = 0; d < PER / 4; d++) { sum[d] *= shrink; }
 #pragma unroll
         for (int r = 0; r < 8; r++)
         {
             const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
-            if (r0 + r < n && w != 0.0f)
+            if (r0 + r < n && w != 0.0f)                                    // a range without a key has weight 0
             {
                 l += w * stat[r].y;
-                sum += w * part[r];
+#pragma unroll
+                for (int d = 0; d < PER / 4; d++) { sum[d] += w * part[r][d]; }
             }
         }
     }
-    float v[4];
+    uint16_t* const dst = p.y + token * p.ldy + head * DIM + d0;
 #pragma unroll
-    for (int e = 0; e < 4; e++) { v[e] = l == 0.0f ? 0.0f : sum[e] / l; }
-    *(u32x2*)(p.y + (size_t)t * p.ldy + (size_t)head * DIM + d) = pack4(v);
+    for (int d = 0; d < PER / 4; d++)
+    {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) { v[e] = l == 0.0f ? 0.0f : sum[d][e] / l; }
+        *(u32x2*)(dst + 4 * d) = pack4(v);
+    }
 }
 
 }    // namespace ccq
