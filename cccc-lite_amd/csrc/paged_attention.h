@@ -27,6 +27,9 @@ struct PagedAttention
     __device__ __forceinline__ float2* stats(int range, size_t row, int dim) const { return (float2*)(partial + (size_t)n_split * outputs() * dim) + (size_t)range * outputs() + row; }
 };
 
+// a value that all lanes have, in a scalar register
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // The new tokens of a sequence that a call computes: tokens first .. first + n - 1 of the activations, the first of them at position pos.
 struct NewTokens
 {
@@ -62,11 +65,6 @@ struct KeyBlocks
     {
         return b * SIZE + SIZE - 1 <= lo && (p.window == 0 || b * SIZE > hi - p.window || b * SIZE + SIZE <= p.n_sink);
     }
-    // none of them sees any
-    __device__ static __forceinline__ bool hidden(const PagedAttention& p, int lo, int hi, int b)
-    {
-        return b * SIZE > hi || (p.window != 0 && b * SIZE + SIZE - 1 <= lo - p.window && b * SIZE >= p.n_sink);
-    }
 };
 
 __device__ __forceinline__ bool sees(const PagedAttention& p, int pos, int key) { return key <= pos && (p.window == 0 || key > pos - p.window || key < p.n_sink); }
@@ -81,15 +79,18 @@ struct Rows
 
     __device__ __forceinline__ void cut(const PagedAttention& p, int split, int multiple, int least)
     {
-        lo = mine.pos + row0 / p.group;
-        hi = mine.pos + min(row0 + ROWS - 1, n_rows - 1) / p.group;
+        lo = uniform(mine.pos + row0 / p.group);
+        hi = uniform(mine.pos + min(row0 + ROWS - 1, n_rows - 1) / p.group);
         blocks = KeyBlocks<SIZE>(p, lo, hi);
+        blocks.n = uniform(blocks.n);
+        blocks.sinks = uniform(blocks.sinks);
+        blocks.skip = uniform(blocks.skip);
         per = max(((blocks.n + split - 1) / split + multiple - 1) / multiple * multiple, least);
         n_ranges = max((blocks.n + per - 1) / per, 1);
     }
 };
 
-constexpr int PA_ROWS = 16, PA_ROWS_KEYS = 32, PA_TILE = 128, PA_TILE_KEYS = 64;
+constexpr int PA_ROWS = 16, PA_ROWS_KEYS = 32, PA_TILE_KEYS = 64;
 
 // A sequence of up to 16 rows per kv head.
 __device__ __forceinline__ Rows<PA_ROWS_KEYS, PA_ROWS> sequence_rows(const PagedArgs& a, const PagedAttention& p, int s)
@@ -97,7 +98,7 @@ __device__ __forceinline__ Rows<PA_ROWS_KEYS, PA_ROWS> sequence_rows(const Paged
     Rows<PA_ROWS_KEYS, PA_ROWS> r;
     r.mine = new_tokens(a, p, s);
     r.row0 = 0;
-    r.n_rows = r.mine.n * p.group;
+    r.n_rows = uniform(r.mine.n * p.group);
     if (r.n_rows == 0 || r.n_rows > PA_ROWS) { return r; }
     r.s = s;
     r.cut(p, p.row_split, 4, 8);
@@ -105,9 +106,10 @@ __device__ __forceinline__ Rows<PA_ROWS_KEYS, PA_ROWS> sequence_rows(const Paged
 }
 
 // Tile `tile` of those of all sequences, a sequence's last ones first: they see the most keys.  Called by whole waves: a lane per sequence, their tiles added up.
-__device__ __forceinline__ Rows<PA_TILE_KEYS, PA_TILE> tile_rows(const PagedArgs& a, const PagedAttention& p, int tile)
+template <int TILE>
+__device__ __forceinline__ Rows<PA_TILE_KEYS, TILE> tile_rows(const PagedArgs& a, const PagedAttention& p, int tile)
 {
-    Rows<PA_TILE_KEYS, PA_TILE> r;
+    Rows<PA_TILE_KEYS, TILE> r;
     const int lane = threadIdx.x & 63;
     for (int base = 0; base < a.n_seqs; base += 64)
     {
@@ -115,7 +117,7 @@ __device__ __forceinline__ Rows<PA_TILE_KEYS, PA_TILE> tile_rows(const PagedArgs
         if (base + lane < a.n_seqs)
         {
             const int rows = new_tokens(a, p, base + lane).n * p.group;
-            tiles = rows > p.min_rows ? (rows + PA_TILE - 1) / PA_TILE : 0;
+            tiles = rows > p.min_rows ? (rows + TILE - 1) / TILE : 0;
         }
         int upto = tiles;
 #pragma unroll
@@ -130,8 +132,8 @@ __device__ __forceinline__ Rows<PA_TILE_KEYS, PA_TILE> tile_rows(const PagedArgs
             const int at = __builtin_ctzll(past);
             r.s = __builtin_amdgcn_readfirstlane(base + at);
             r.mine = new_tokens(a, p, r.s);
-            r.row0 = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(upto, at) - 1 - tile) * PA_TILE;
-            r.n_rows = r.mine.n * p.group;
+            r.row0 = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(upto, at) - 1 - tile) * TILE;
+            r.n_rows = uniform(r.mine.n * p.group);
             r.cut(p, p.tile_split, 1, 4);
             return r;
         }
@@ -164,9 +166,14 @@ __device__ __forceinline__ u32x2 lds_transposed8(const uint8_t* at)
 
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p; }
 
-// A byte per lane to a dword per lane of LDS.
+// A byte per lane to a dword per lane of LDS; and, unless `wanted` is 0, a KiB from base + off to LDS.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void kib_to_lds(uint32_t wanted, uint32_t lds, const uint8_t* base, uint32_t off)
+{
+    asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 .Lkib_to_lds%=\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n.Lkib_to_lds%=:"
+                 : : "s"(wanted), "s"(lds), "v"(off), "s"(base) : "memory", "m0", "scc");
+}
 __device__ __forceinline__ void bytes_to_lds(uint32_t lds, const uint8_t* at)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
@@ -512,16 +519,16 @@ struct TileForm
     static constexpr int ODD = 4 * BLOCK, LDS = ODD + 32;                   // two blocks of keys, two of values
 };
 
-template <int TYPE, int DIM>
+template <int TYPE, int DIM, int RT>
 __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int tile, int kvh, int range)
 {
     typedef TileForm<TYPE, DIM> F;
-    constexpr int RT = 1, KEYS = PA_TILE_KEYS, ROW = DIM * 2, CHUNKS = ROW / 16, BLOCK = F::BLOCK;
+    constexpr int KEYS = PA_TILE_KEYS, ROW = DIM * 2, CHUNKS = ROW / 16, BLOCK = F::BLOCK;
     constexpr int CODES = DIM * CODE_BYTES<TYPE>;                           // bytes of a cached row
     uint32_t* const odd_rows = (uint32_t*)(lds + F::ODD);                   // per buffer of values and wave that staged: something infinite or NaN
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 31, h = lane >> 5;
-    const auto rows = tile_rows(a, p, tile);
+    const auto rows = tile_rows<128 * RT>(a, p, tile);
     if (rows.s < 0 || range >= rows.n_ranges) { return; }
     const NewTokens mine = rows.mine;
     const auto& blocks = rows.blocks;
@@ -529,7 +536,6 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     const int begin = range * rows.per, end = min(blocks.n, begin + rows.per);
 
     // the wave's rows
-    const int wave_lo = mine.pos + min(row0 + wave * 32 * RT, n_rows - 1) / p.group, wave_hi = mine.pos + min(row0 + wave * 32 * RT + 32 * RT - 1, n_rows - 1) / p.group;
     int token[RT], head[RT], my_pos[RT];
     bool real[RT];
     u32x4 qf[RT][DIM / 16];
@@ -547,88 +553,98 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
 
     auto key_swizzle = [](int r) { return r / (256 / ROW) % CHUNKS; };
     auto value_swizzle = [](int r) { return DIM == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
-    int pages = 0, none = 0;                    // lane l, entry 64 n + l of the range: page of the 16 rows that this wave stages; bits of the quarters without one
+    // lane l, entry 64 n + l of the range: where the 16 rows that this wave stages begin in the pool (and their exponents), and above bit 60 which
+    // quarters of the entry have no page
+    size_t rows_from = 0, exponents_from = 0;
     auto look_up = [&](int i0) {
         const int i = i0 + lane, key0 = blocks.block(i) * KEYS;
-        pages = none = 0;
-        if (i >= end) { return; }
-#pragma unroll
-        for (int quarter = 0; quarter < 4; quarter++)
+        size_t lacks = 0;
+        int mine_page = 0;
+        if (i < end)
         {
-            const int pos = key0 + 16 * quarter;
-            const int page = pos > tile_hi ? 0 : paged_page(a, s, pos);
-            none |= page < 0 ? 1 << quarter : 0;
-            pages = quarter == wave ? max(page, 0) : pages;
+#pragma unroll
+            for (int quarter = 0; quarter < 4; quarter++)
+            {
+                const int pos = key0 + 16 * quarter;
+                const int page = pos > tile_hi ? 0 : paged_page(a, s, pos);
+                lacks |= page < 0 ? (size_t)1 << (60 + quarter) : 0;
+                mine_page = quarter == wave ? max(page, 0) : mine_page;
+            }
         }
+        const size_t r0 = paged_row(a, kvh, key0 + 16 * wave);
+        rows_from = mine_page * a.page_stride + r0 * CODES | lacks;
+        exponents_from = mine_page * a.scale_stride + r0;
+    };
+    auto of_entry = [&](size_t v, int i) {
+        const int at = (i - begin) & 63;
+        return (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), at) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, at);
     };
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds));
-    constexpr int PIECES = TYPE == DT_BF16 ? 1 : CODES * 16 / 1024;         // FP8: 16 bytes per lane each of the wave's 16 rows
+    // FP8: lane group q (DIM / 8 lanes, eight codes each) takes rows PIECES q .. of the wave's 16
+    constexpr int LANES = DIM / 8, PIECES = DIM / 32;
     struct Staged
     {
-        u32x4 codes[PIECES];
-        uint32_t exponent[PIECES];
+        u32x2 codes[PIECES];
+        uint32_t exponents;
     };
     const uint32_t key_from = lane * 16 ^ key_swizzle(lane / CHUNKS) * 16, value_from = lane * 16 ^ value_swizzle(lane / CHUNKS) * 16;
-    // the wave's 16 rows of entry i: on their way to LDS (BF16) or to registers
-    auto load = [&](bool values, int i, int page, uint32_t to, Staged& raw) {
-        const size_t r0 = paged_row(a, kvh, blocks.block(i) * KEYS + 16 * wave);
-        const uint8_t* const from = (values ? a.v : a.k) + page * a.page_stride + r0 * CODES;
+    const uint32_t code_from = lane / LANES * PIECES * CODES + lane % LANES * 8;
+    const int code_row = lane / LANES * PIECES;
+    const uint32_t key_to = code_row * ROW + (lane % LANES ^ key_swizzle(code_row)) * 16, value_to = code_row * ROW + (lane % LANES ^ value_swizzle(code_row)) * 16;
+    // The wave's 16 rows of an entry in PIECES parts: on their way to LDS (BF16) or to registers, and from there to LDS as BF16 (FP8).
+    struct Source
+    {
+        const uint8_t* rows;
+        const uint8_t* exponents;
+    };
+    auto source = [&](bool values, size_t from, size_t exponents) {
+        return Source{ (values ? a.v : a.k) + (from & ((size_t)1 << 60) - 1), (values ? a.v_scale : a.k_scale) + exponents };
+    };
+    auto load = [&](bool values, int n, uint32_t wanted, const Source& of, uint32_t to, Staged& raw) {
         if constexpr (TYPE == DT_BF16)
         {
-            // rows n (1024 / ROW) + lane / CHUNKS: with n a swizzle changes by a constant in bits of its own
-            uint32_t at = values ? value_from : key_from;
+            // rows n (1024 / ROW) + lane / CHUNKS: with n the keys' swizzle changes by 4 n, the values' not at all
+            uint32_t at = values ? value_from : key_from ^ 64 * n;
             asm volatile("" : "+v"(at));                                    // worked out anew: registers are short
-#pragma unroll
-            for (int n = 0; n < ROW * 16 / 1024; n++)
-            {
-                constexpr int R = 1024 / ROW;
-                load_to_lds<false>(lds0 + to + n * 1024, from + n * 1024, values ? at : at ^ (uint32_t)(key_swizzle(n * R) * 16));
-            }
+            kib_to_lds(uniform((int)wanted), lds0 + to + n * 1024, of.rows + n * 1024, at);
         }
         else
         {
-            const uint8_t* const exponents = (values ? a.v_scale : a.k_scale) + page * a.scale_stride + r0;
-#pragma unroll
-            for (int n = 0; n < PIECES; n++)
+            uint32_t at = code_from;
+            asm volatile("" : "+v"(at));
+            raw.codes[n] = *(const u32x2*)(of.rows + at + n * CODES);
+            if (n == 0)
             {
-                raw.codes[n] = *(const u32x4*)(from + n * 1024 + lane * 16);
-                raw.exponent[n] = exponents[n * (1024 / CODES) + lane / (CODES / 16)];
+                if constexpr (DIM == 128) { raw.exponents = *(const uint32_t*)(of.exponents + lane / LANES * 4); }
+                else { raw.exponents = *(const uint16_t*)(of.exponents + lane / LANES * 2); }
             }
         }
     };
-    // FP8: the loaded rows to LDS as BF16; the result tells whether something is not finite
-    auto store = [&](bool values, uint32_t to, const Staged& raw) {
-        uint32_t odd = 0;
+    auto store = [&](bool values, int n, uint32_t to, const Staged& raw) {
         if constexpr (TYPE != DT_BF16)
         {
-#pragma unroll
-            for (int n = 0; n < PIECES; n++)
-            {
-                const int r = n * (1024 / CODES) + lane / (CODES / 16), c = lane % (CODES / 16) * 2, swizzle = values ? value_swizzle(r) : key_swizzle(r);
-                const float by = bits_to_f32(raw.exponent[n] << 23);
-                u32x2 w[4];
-#pragma unroll
-                for (int d = 0; d < 4; d++) { w[d] = fp8x4_to_bf16<TYPE>(raw.codes[n][d], by); }
-                const u32x4 lo = { w[0][0], w[0][1], w[1][0], w[1][1] }, hi = { w[2][0], w[2][1], w[3][0], w[3][1] };
-                *(u32x4*)(lds + to + r * ROW + (c ^ swizzle) * 16) = lo;
-                *(u32x4*)(lds + to + r * ROW + ((c + 1) ^ swizzle) * 16) = hi;
-                odd |= not_finite(lo) | not_finite(hi);
-            }
+            uint32_t at = values ? value_to : key_to;
+            asm volatile("" : "+v"(at));
+            const float by = bits_to_f32((raw.exponents >> (8 * n) & 255u) << 23);
+            const u32x2 lo = fp8x4_to_bf16<TYPE>(raw.codes[n][0], by), hi = fp8x4_to_bf16<TYPE>(raw.codes[n][1], by);
+            // row PIECES q + n: n is in the row's low bits, which the swizzles take as they are
+            *(u32x4*)(lds + to + (at ^ (values ? value_swizzle(n) : key_swizzle(n)) * 16) + n * ROW) = u32x4{ lo[0], lo[1], hi[0], hi[1] };
         }
-        return odd;
     };
     auto keys_at = [&](int i) { return (uint32_t)((i - begin) & 1) * BLOCK; };
     auto values_at = [&](int i) { return (uint32_t)(2 + ((i - begin) & 1)) * BLOCK; };
     const uint32_t part = wave * (BLOCK / 4);                               // the wave's rows of a block
-    auto tile_plain = [&](int i, int lacks) { return KeyBlocks<KEYS>::plain(p, tile_lo, tile_hi, blocks.block(i)) && lacks == 0; };
-    // in front of the barrier behind which the values of entry i are read: whether any is infinite or NaN, where that matters
-    auto note_odd = [&](int i, int lacks, uint32_t odd) {
-        if (tile_plain(i, lacks)) { return; }
-        if constexpr (TYPE == DT_BF16)
-        {
+    // entries plain_from .. plain_to - 1: every row of the tile sees every key
+    int plain_from = 0, plain_to = (tile_lo + 1) / KEYS;
+    if (p.window != 0) { plain_from = (tile_hi - p.window + KEYS) / KEYS; }
+    plain_from = max(plain_from - blocks.skip, tile_hi < p.window || p.window == 0 ? 0 : blocks.sinks);
+    plain_to -= blocks.skip;
+    auto masked = [&](int i, size_t from) { return i < plain_from || i >= plain_to || from >> 60 != 0; };
+    // in front of the barrier behind which the values of entry i are read: whether any of this wave's rows is infinite or NaN, where that matters
+    auto note_odd = [&](int i) {
+        uint32_t odd = 0;
 #pragma unroll
-            for (int n = 0; n < ROW * 16 / 1024; n++) { odd |= not_finite(*(const u32x4*)(lds + values_at(i) + part + n * 1024 + lane * 16)); }
-        }
+        for (int n = 0; n < PIECES; n++) { odd |= not_finite(*(const u32x4*)(lds + values_at(i) + part + n * 1024 + lane * 16)); }
         const bool any = __any(odd != 0);
         if (lane == 0) { odd_rows[(i & 1) * 4 + wave] = any; }
     };
@@ -681,20 +697,27 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
             }
         }
     };
-    auto weigh = [&](f32x16 (&acc)[RT][2], int i) {
-        uint32_t at = v_at + values_at(i);
-        asm volatile("" : "+v"(at));
-        float off[RT], sum[RT][4];
+    // largest raw score of a row
+    float top[RT];
+    auto find_top = [&](const f32x16 (&acc)[RT][2]) {
 #pragma unroll
         for (int t = 0; t < RT; t++)
         {
-            float top = -INFINITY;
+            top[t] = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 32; e++) { top = fmaxf(top, acc[t][e / 16][e % 16]); }
-            top *= p.scale;
-            if (__any(top > m[t] + PA_LAG))
+            for (int e = 0; e < 32; e++) { top[t] = fmaxf(top[t], acc[t][e / 16][e % 16]); }
+        }
+    };
+    // the running maximum; sums rescaled where it moves
+    float off[RT];
+    auto raise = [&]() {
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+        {
+            const float least = top[t] * p.scale;
+            if (__any(least > m[t] + PA_LAG))
             {
-                const float next = fmaxf(m[t], fmaxf(top, __shfl_xor(top, 32)));
+                const float next = fmaxf(m[t], fmaxf(least, __shfl_xor(least, 32)));
                 const float shrink = m[t] > -INFINITY ? __builtin_amdgcn_exp2f(m[t] - next) : 1.0f;       // sums of nothing: 0, or what is not finite
                 m[t] = next;
                 l[t] *= shrink;
@@ -702,33 +725,79 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
                 for (int d = 0; d < DIM / 32; d++) { out[t][d] *= shrink; }
             }
             off[t] = m[t] > -INFINITY ? -m[t] : 0.0f;                       // no key seen yet: every weight is 2^-inf = 0
-#pragma unroll
-            for (int n = 0; n < 4; n++) { sum[t][n] = 0.0f; }
         }
+    };
+    // The weights of entry i under the products of entry i + 1, then the products of the weights under the largest scores of i + 1: in each step the
+    // vector unit has work for as long as the matrix core has.
+    auto advance = [&](int i, const f32x16 (&cur)[RT][2], f32x16 (&next)[RT][2], auto loads, auto stores) {
+        constexpr int STEPS = DIM / 16, WEIGHTS = 32 / STEPS, PAIRS = DIM / 64;
+        uint32_t key_at = k_at + keys_at(i + 1), value_at = v_at + values_at(i);
+        asm volatile("" : "+v"(key_at), "+v"(value_at));
+        auto keys = [&](int c, int kt) { return *(const bf16x8*)(lds + (key_at ^ (32 * c)) + kt * 32 * ROW); };      // the swizzle of row j + 32 is that of j
+        auto values = [&](int u, int d) {
+            const u32x2 lo = lds_transposed16(lds + (value_at ^ (64 * d)) + u * 16 * ROW), hi = lds_transposed16(lds + (value_at ^ (64 * d)) + (u * 16 + 8) * ROW);
+            return __builtin_bit_cast(bf16x8, u32x4{ lo[0], lo[1], hi[0], hi[1] });
+        };
+        const f32x16 zero = {};
+        constexpr int AHEAD = 2, N_VALUES = 4 * PAIRS;    // steps that operands are read ahead
+        bf16x8 pb[RT][4], kf[STEPS][2], vf[N_VALUES][2];
+        float sum[RT][2] = {};
+        auto read = [&](int step) {                                         // operands of a step, counted through
 #pragma unroll
-        for (int u = 0; u < 4; u++)
+            for (int n = 0; n < 2; n++)
+            {
+                if (step < STEPS) { kf[step][n] = keys(step, n); }
+                else if (step < STEPS + N_VALUES) { vf[step - STEPS][n] = values((step - STEPS) / PAIRS, (step - STEPS) % PAIRS * 2 + n); }
+            }
+        };
+#pragma unroll
+        for (int c = 0; c < AHEAD; c++) { read(c); }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < STEPS; c++)
         {
-            bf16x8 pb[RT];
+            read(c + AHEAD);
+            loads(c);
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int t = 0; t < RT; t++) { next[t][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[c][kt], __builtin_bit_cast(bf16x8, qf[t][c]), c == 0 ? zero : next[t][kt], 0, 0, 0); }
 #pragma unroll
             for (int t = 0; t < RT; t++)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(acc[t][u / 2][u % 2 * 8 + e], p.scale, off[t]));
-                    sum[t][e & 3] += w;
-                    pb[t][e] = (__bf16)w;
-                }
-#pragma unroll
-            for (int d = 0; d < DIM / 32; d++)
             {
-                const u32x2 lo = lds_transposed16(lds + (at ^ (64 * d)) + u * 16 * ROW), hi = lds_transposed16(lds + (at ^ (64 * d)) + (u * 16 + 8) * ROW);
-                const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{ lo[0], lo[1], hi[0], hi[1] });
 #pragma unroll
-                for (int t = 0; t < RT; t++) { out[t][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[t], out[t][d], 0, 0, 0); }
+                for (int e = c * WEIGHTS; e < (c + 1) * WEIGHTS; e++)
+                {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(cur[t][e / 16][e % 16], p.scale, off[t]));
+                    sum[t][e & 1] += w;
+                    pb[t][e / 8][e % 8] = (__bf16)w;
+                }
+                asm volatile("" : "+v"(sum[t][0]), "+v"(sum[t][1]));        // added here, not when somebody asks
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int t = 0; t < RT; t++) { l[t] += (sum[t][0] + sum[t][1]) + (sum[t][2] + sum[t][3]); }
+        for (int n = 0; n < N_VALUES; n++)
+        {
+            const int u = n / PAIRS, d = n % PAIRS * 2;
+            read(STEPS + n + AHEAD);
+            stores(n);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int t = 0; t < RT; t++) { out[t][d + k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n][k], pb[t][u], out[t][d + k], 0, 0, 0); }
+#pragma unroll
+            for (int t = 0; t < RT; t++)
+            {
+                if (n == 0) { top[t] = -INFINITY; }
+#pragma unroll
+                for (int e = n * (8 / PAIRS); e < (n + 1) * (8 / PAIRS); e++) { top[t] = fmaxf(top[t], next[t][e / 16][e % 16]); }
+                asm volatile("" : "+v"(top[t]));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++) { l[t] += sum[t][0] + sum[t][1]; }
     };
     // Weight 0 times an infinity is NaN: where some rows do not see every key of entry i, what is infinite or NaN among its values is added to the sums of
     // the rows that see it and cleared in front of the products.
@@ -773,48 +842,81 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     if (begin < end)
     {
         Staged raw_k, raw_v;
-        f32x16 acc[RT][2];
-        uint32_t odd = 0;
-        auto load_both = [&](int i) {
-            if (((i - begin) & 63) == 0) { look_up(i); }
-            const int page = __builtin_amdgcn_readlane(pages, (i - begin) & 63);
-            load(false, i, page, keys_at(i) + part, raw_k);
-            load(true, i, page, values_at(i) + part, raw_v);
-            return __builtin_amdgcn_readlane(none, (i - begin) & 63);
+        f32x16 cur[RT][2], next[RT][2];
+        look_up(begin);
+        // where the values of the next entry begin, and whether this one and the next are masked (for what they lack)
+        size_t from = of_entry(rows_from, begin), exponents = TYPE == DT_BF16 ? 0 : of_entry(exponents_from, begin);
+        bool is_masked = masked(begin, from), next_masked = false;
+        int lacks = (int)(from >> 60), next_lacks = 0;
+        auto fetch = [&](bool values, uint32_t to, Staged& raw) {
+            const Source of = source(values, from, exponents);
+#pragma unroll
+            for (int n = 0; n < PIECES; n++) { load(values, n, 1, of, to, raw); }
+#pragma unroll
+            for (int n = 0; n < PIECES; n++) { store(values, n, to, raw); }
         };
-        auto store_both = [&](int i) {
-            if constexpr (TYPE != DT_BF16)
-            {
-                store(false, keys_at(i) + part, raw_k);
-                odd = store(true, values_at(i) + part, raw_v);
-            }
-        };
-        int lacks = load_both(begin);
-        store_both(begin);
-        arrived();
-        note_odd(begin, lacks, odd);
-        barrier();
-        // entry i is in LDS
-        for (int i = begin; i < end; i++)
+        fetch(false, keys_at(begin) + part, raw_k);
+        fetch(true, values_at(begin) + part, raw_v);
+        if (begin + 1 < end)
         {
-            int lacks_ahead = 0;
-            if (i + 1 < end) { lacks_ahead = load_both(i + 1); }            // the buffers of entry i - 1, read before the last barrier
-            const int b = blocks.block(i);
-            if (!tile_plain(i, lacks)) { set_apart(i, lacks); }
-            if (!KeyBlocks<KEYS>::hidden(p, wave_lo, wave_hi, b))
+            from = of_entry(rows_from, begin + 1);
+            if constexpr (TYPE != DT_BF16) { exponents = of_entry(exponents_from, begin + 1); }
+            next_masked = masked(begin + 1, from);
+            next_lacks = (int)(from >> 60);
+            fetch(false, keys_at(begin + 1) + part, raw_k);
+        }
+        arrived();
+        if (is_masked) { note_odd(begin); }
+        barrier();
+        score_products(begin, cur);
+        find_top(cur);
+        // entry i: its values and the keys of i + 1 are in LDS, `cur` holds its raw scores
+        auto entry = [&](int i, f32x16 (&cur)[RT][2], f32x16 (&next)[RT][2]) {
+            // behind the last entry: its rows again (FP8) or none (BF16), and scores of what lies there, for nobody
+            const int ahead = min(i + 2, end - 1);
+            if (((i + 2 - begin) & 63) == 0 && i + 2 < end) { look_up(i + 2); }
+            const size_t from_ahead = of_entry(rows_from, ahead), exponents_ahead = TYPE == DT_BF16 ? 0 : of_entry(exponents_from, ahead);
+            const Source key_rows = source(false, from_ahead, exponents_ahead), value_rows = source(true, from, exponents);
+            const uint32_t keys_to = keys_at(i) + part, values_to = values_at(i + 1) + part;       // keys of i + 2: those of i were read before the last barrier
+            if (is_masked)
             {
-                score_products(i, acc);
-                if (!KeyBlocks<KEYS>::plain(p, wave_lo, wave_hi, b) || lacks != 0) { mask(acc, b, lacks); }
-                weigh(acc, i);
+                set_apart(i, lacks);
+                mask(cur, blocks.block(i), lacks);
+                find_top(cur);
             }
-            if (i + 1 < end)
-            {
-                store_both(i + 1);
-                arrived();
-                note_odd(i + 1, lacks_ahead, odd);
-                barrier();
-                lacks = lacks_ahead;
-            }
+            raise();
+            // a workgroup's loads all at once would hold up its waves: one or two with every step
+            constexpr int STEPS = DIM / 16, PER = 2 * PIECES * 2 / STEPS;
+            auto loads = [&](int step) {
+#pragma unroll
+                for (int n = step * PER; n < (step + 1) * PER; n++)
+                {
+                    if (n < PIECES) { load(false, n, i + 2 < end, key_rows, keys_to, raw_k); }
+                    else if (n < 2 * PIECES) { load(true, n - PIECES, i + 1 < end, value_rows, values_to, raw_v); }
+                }
+            };
+            auto stores = [&](int step) {
+                constexpr int FROM = 4 * (DIM / 64) - 2 * PIECES;
+                const int n = step - FROM;
+                if (n < 0) { return; }
+                if (n < PIECES) { store(false, n, keys_to, raw_k); }
+                else { store(true, n - PIECES, values_to, raw_v); }
+            };
+            advance(i, cur, next, loads, stores);
+            arrived();
+            if (next_masked && i + 1 < end) { note_odd(i + 1); }
+            barrier();
+            is_masked = next_masked;
+            lacks = next_lacks;
+            from = from_ahead;
+            exponents = exponents_ahead;
+            next_masked = masked(i + 2, from);
+            next_lacks = (int)(from >> 60);
+        };
+        for (int i = begin; i < end; i += 2)
+        {
+            entry(i, cur, next);
+            if (i + 1 < end) { entry(i + 1, next, cur); }
         }
     }
 
@@ -850,15 +952,15 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
 }
 
 // Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then ranges x sequences x kv heads.
-template <int TYPE, int DIM>
-__global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs a, const PagedAttention p)
+template <int TYPE, int DIM, int RT>
+__global__ __launch_bounds__(256, 3 - RT) void paged_attention_kernel(const PagedArgs a, const PagedAttention p)
 {
     typedef RowsForm<TYPE, DIM> R;
     typedef TileForm<TYPE, DIM> T;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS > T::LDS ? R::LDS : T::LDS];
     static_assert(sizeof(lds) <= 80 * 1024, "two workgroups on a CU");
     const int tiles = p.tiles * a.n_kv, n_tiles = tiles * p.tile_split;
-    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
+    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM, RT>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
     else
     {
         const int at = blockIdx.x - n_tiles, sequences = a.n_seqs * a.n_kv;
@@ -869,17 +971,17 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs
 // Sums of the key ranges of 16 rows, DIM / 16 dims of a row per thread: rescaled to the largest maximum, added in the order of the ranges, divided by the
 // sum of the weights, one rounding.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads where tiles have ranges, then
 // sequences x kv heads where those do.
-template <int DIM>
+template <int DIM, int RT>
 __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
 {
-    constexpr int PER = DIM / 16, PARTS = PA_TILE / 16;
+    constexpr int PER = DIM / 16, PARTS = 8 * RT;
     const int n_tiles = p.tile_split > 1 ? p.tiles * PARTS * a.n_kv : 0, kvh = blockIdx.x % a.n_kv;
     NewTokens mine;
     int row, n;
     if ((int)blockIdx.x < n_tiles)
     {
         const int at = blockIdx.x / a.n_kv;
-        const auto rows = tile_rows(a, p, at / PARTS);
+        const auto rows = tile_rows<128 * RT>(a, p, at / PARTS);
         row = rows.row0 + at % PARTS * 16 + (threadIdx.x >> 4);
         if (rows.s < 0 || row >= rows.n_rows) { return; }
         mine = rows.mine;
