@@ -47,11 +47,6 @@ bool paged_args(const hip_paged_kv* c, PagedArgs& a)
     ((c)->head_dim == 64 ? ((c)->type == CCCC_BFLOAT16 ? KERNEL<DT_BF16, 64> : (c)->type == CCCC_FP8_E4M3 ? KERNEL<DT_E4M3, 64> : KERNEL<DT_E5M2, 64>) \
                          : ((c)->type == CCCC_BFLOAT16 ? KERNEL<DT_BF16, 128> : (c)->type == CCCC_FP8_E4M3 ? KERNEL<DT_E4M3, 128> : KERNEL<DT_E5M2, 128>))
 
-template <int TYPE, int DIM>
-constexpr auto paged_attention_128 = paged_attention_kernel<TYPE, DIM, 1>;
-template <int TYPE, int DIM>
-constexpr auto paged_attention_256 = paged_attention_kernel<TYPE, DIM, 2>;
-
 bool attention_args(const hip_paged_kv* c, PagedArgs& a, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink)
 {
     if (!paged_args(c, a) || n_q_heads <= 0 || n_q_heads % c->n_kv_heads != 0 || n_q_heads / c->n_kv_heads > 64) { return false; }
@@ -80,12 +75,15 @@ Plan plan_attention(const PagedArgs& a, int group, int n_tokens, int max_new, in
         plan.rows = group <= PA_ROWS && n_tokens < (long long)a.n_seqs * max_new;
         plan.min_rows = plan.rows ? PA_ROWS : 0;
         if (getenv("PA_RT")) { plan.tile = 128 * atoi(getenv("PA_RT")); }
-        plan.tiles = rows / plan.tile + std::min<long long>(a.n_seqs, rows / (plan.min_rows + 1));
+        const long long cut = std::min<long long>(a.n_seqs, rows / (plan.min_rows + 1));       // sequences, at most
+        plan.tiles = (rows - cut) / plan.tile + cut;
     }
     const long long keys = window == 0 ? a.max_ctx : std::min<long long>(a.max_ctx, (long long)window + n_sink + max_new);
     auto split = [&](long long workgroups) { return (int)std::max<long long>(1, std::min({ 2LL * cu_count() / std::max<long long>(workgroups, 1), keys / 256, 64LL })); };
     plan.tile_split = split(plan.tiles * a.n_kv * (plan.tile / 128));
     plan.row_split = split((long long)a.n_seqs * a.n_kv);
+    if (getenv("PA_TS")) { plan.tile_split = atoi(getenv("PA_TS")); }
+    if (getenv("PA_RS")) { plan.row_split = atoi(getenv("PA_RS")); }
     plan.n_split = std::max(plan.tiles ? plan.tile_split : 1, plan.rows ? plan.row_split : 1);
     return plan;
 }
@@ -159,13 +157,12 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
     const long long sums = (tile_split > 1 ? tiles * (plan.tile / 16) : 0) + (row_split > 1 ? sequences : 0);
     if (blocks > MOST_BLOCKS || sums > MOST_BLOCKS) { return -1; }
     const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)workspace, (size_t)ldq, (size_t)ldy, n_q_heads, group, n_tokens, max_new, window, n_sink, plan.n_split,
-                               (int)plan.tiles, tile_split, row_split, plan.min_rows, 1.4426950408889634f / sqrtf((float)dim) };
-    const auto kernel = plan.tile == 128 ? CCQ_PAGED_KERNEL(paged_attention_128, cache) : CCQ_PAGED_KERNEL(paged_attention_256, cache);
+                               (int)plan.tiles, tile_split, row_split, plan.min_rows, getenv("PA_SNAKE") ? 1 : 0, 1.4426950408889634f / sqrtf((float)dim) };
+    const auto kernel = CCQ_PAGED_KERNEL(paged_attention_kernel, cache);
     kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, p);
     if (sums > 0)
     {
-        const auto combine = plan.tile == 128 ? (dim == 64 ? paged_attention_combine_kernel<64, 1> : paged_attention_combine_kernel<128, 1>)
-                                              : (dim == 64 ? paged_attention_combine_kernel<64, 2> : paged_attention_combine_kernel<128, 2>);
+        const auto combine = dim == 64 ? paged_attention_combine_kernel<64, 64, 1> : cache->type == CCCC_BFLOAT16 ? paged_attention_combine_kernel<128, 32, 1> : paged_attention_combine_kernel<128, 64, 1>;
         combine<<<(unsigned)sums, 256, 0, stream()>>>(a, p);
     }
     return finish("attention_paged");

@@ -20,6 +20,7 @@ struct PagedAttention
     int tiles, tile_split;          // tiles of 128 rows (at most) and the most ranges of each
     int row_split;                  // most ranges of a sequence of at most 16 rows per kv head
     int min_rows;                   // sequences of at most so many rows per kv head are not cut into tiles
+    int snake;
     float scale;                    // log2 e / sqrt(dim)
 
     __device__ __forceinline__ size_t outputs() const { return (size_t)n_tokens * n_q; }
@@ -60,11 +61,6 @@ struct KeyBlocks
         n = blocks - skip;
     }
     __device__ __forceinline__ int block(int i) const { return i < sinks ? i : i + skip; }
-    // every token at positions lo .. hi sees every key of block b
-    __device__ static __forceinline__ bool plain(const PagedAttention& p, int lo, int hi, int b)
-    {
-        return b * SIZE + SIZE - 1 <= lo && (p.window == 0 || b * SIZE > hi - p.window || b * SIZE + SIZE <= p.n_sink);
-    }
 };
 
 __device__ __forceinline__ bool sees(const PagedAttention& p, int pos, int key) { return key <= pos && (p.window == 0 || key > pos - p.window || key < p.n_sink); }
@@ -90,27 +86,30 @@ struct Rows
     }
 };
 
-constexpr int PA_ROWS = 16, PA_ROWS_KEYS = 32, PA_TILE_KEYS = 64;
+constexpr int PA_ROWS = 16, PA_TILE_KEYS = 64;
 
 // A sequence of up to 16 rows per kv head.
-__device__ __forceinline__ Rows<PA_ROWS_KEYS, PA_ROWS> sequence_rows(const PagedArgs& a, const PagedAttention& p, int s)
+template <int KEYS>
+__device__ __forceinline__ Rows<KEYS, PA_ROWS> sequence_rows(const PagedArgs& a, const PagedAttention& p, int s)
 {
-    Rows<PA_ROWS_KEYS, PA_ROWS> r;
+    Rows<KEYS, PA_ROWS> r;
     r.mine = new_tokens(a, p, s);
     r.row0 = 0;
     r.n_rows = uniform(r.mine.n * p.group);
     if (r.n_rows == 0 || r.n_rows > PA_ROWS) { return r; }
     r.s = s;
-    r.cut(p, p.row_split, 4, 8);
+    r.cut(p, p.row_split, 4, 256 / KEYS);
     return r;
 }
 
-// Tile `tile` of those of all sequences, a sequence's last ones first: they see the most keys.  Called by whole waves: a lane per sequence, their tiles added up.
+// Tile `tile` of those of all sequences, a sequence's last ones first: they see the most keys.  Where a CU gets two workgroups in all, the second half of
+// the tiles comes in the other order, so that a long one has a short one beside it.  Called by whole waves: a lane per sequence, their tiles added up.
 template <int TILE>
 __device__ __forceinline__ Rows<PA_TILE_KEYS, TILE> tile_rows(const PagedArgs& a, const PagedAttention& p, int tile)
 {
     Rows<PA_TILE_KEYS, TILE> r;
     const int lane = threadIdx.x & 63;
+    if (p.snake && tile >= (p.tiles + 1) / 2) { tile = p.tiles - 1 - (tile - (p.tiles + 1) / 2); }
     for (int base = 0; base < a.n_seqs; base += 64)
     {
         int tiles = 0;
@@ -174,16 +173,29 @@ __device__ __forceinline__ void kib_to_lds(uint32_t wanted, uint32_t lds, const 
     asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 .Lkib_to_lds%=\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n.Lkib_to_lds%=:"
                  : : "s"(wanted), "s"(lds), "v"(off), "s"(base) : "memory", "m0", "scc");
 }
+// N KiB in a row, lane l's 16 bytes of the n-th at off[n] (the instruction's own offset counts on both sides).
+template <int N>
+__device__ __forceinline__ void kibs_to_lds(uint32_t lds, const uint8_t* base, const uint32_t (&off)[N])
+{
+    static_assert(N == 1 || N == 2 || N == 4, "16 rows");
+    if constexpr (N == 1) { asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" : : "s"(lds), "v"(off[0]), "s"(base) : "memory", "m0"); }
+    else if constexpr (N == 2)
+    {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3 nt\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024 nt"
+                     : : "s"(lds), "v"(off[0]), "v"(off[1]), "s"(base) : "memory", "m0");
+    }
+    else
+    {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5 nt\n\tglobal_load_lds_dwordx4 %2, %5 offset:1024 nt\n\t"
+                     "global_load_lds_dwordx4 %3, %5 offset:2048 nt\n\tglobal_load_lds_dwordx4 %4, %5 offset:3072 nt"
+                     : : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory", "m0");
+    }
+}
 __device__ __forceinline__ void bytes_to_lds(uint32_t lds, const uint8_t* at)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
 }
 #pragma clang diagnostic pop
-
-__device__ __forceinline__ float max8(const float* s)
-{
-    return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-}
 
 // Bits of a dword's two BF16 values that are infinite or NaN, as a mask over both; and whether there are any in four dwords.
 __device__ __forceinline__ uint32_t not_finite(uint32_t w)
@@ -192,50 +204,36 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w)
 }
 __device__ __forceinline__ uint32_t not_finite(const u32x4& v) { return not_finite(v[0]) | not_finite(v[1]) | not_finite(v[2]) | not_finite(v[3]); }
 
-// What is infinite or NaN among eight BF16 values, apart from the rest: the rest with zeros there, and 1 where KIND is (0: +inf, 1: -inf, 2: NaN).
+// The same with zeros there.
 __device__ __forceinline__ u32x4 finite_part(const u32x4& v)
 {
     u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-    {
-        const uint32_t bad = not_finite(v[i]);
-        r[i] = v[i] & ~((bad >> 15) * 0xFFFFu);
-    }
+    for (int i = 0; i < 4; i++) { r[i] = v[i] & ~((not_finite(v[i]) >> 15) * 0xFFFFu); }
     return r;
 }
-__device__ __forceinline__ u32x4 where_kind(const u32x4& v, int kind)
+
+// Bit 7 of each byte of a dword that is an infinite or NaN code.
+template <int TYPE>
+__device__ __forceinline__ uint32_t codes_not_finite(uint32_t w)
 {
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-    {
-        r[i] = 0;
-#pragma unroll
-        for (int half = 0; half < 2; half++)
-        {
-            const uint32_t x = v[i] >> (16 * half) & 0xFFFFu;
-            const bool is = kind == 0 ? x == 0x7F80u : kind == 1 ? x == 0xFF80u : (x & 0x7FFFu) > 0x7F80u;
-            r[i] |= is ? 0x3F80u << (16 * half) : 0u;
-        }
-    }
-    return r;
+    if constexpr (TYPE == DT_E4M3) { return (w & 0x7F7F7F7Fu) + 0x01010101u & 0x80808080u; }
+    else { return (w & 0x7C7C7C7Cu) + 0x04040404u & 0x80808080u; }
 }
-__device__ __forceinline__ float value_of_kind(int kind) { return kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf(""); }
 
 // Up to 16 rows of a kv head: single tokens, or a few.  Bound by the cached rows' way from memory.
-//   A workgroup of four waves takes a range of the sequence's blocks of 32 keys, a wave every fourth block, each with a pipeline of its own: rows go by
+//   A workgroup of four waves takes a range of the sequence's blocks of KEYS keys, a wave every fourth block, each with a pipeline of its own: rows go by
 // direct loads to the wave's part of LDS, keys and values STAGES blocks ahead each, and nothing but the wave's own count of loads in flight is waited for.
 //   scores: v_mfma_f32_16x16x32_bf16, key rows as row operand, the 16 queries as columns: D lane (row j = lane % 16, g = lane / 16) holds keys 4 g .. + 3
 //           of 16.  FP8 keys become BF16 in registers, times their power of two (a lane's operand is one key's): exact.
-//   V p:    the eight weights of a lane (keys 4 g .. + 3 and 16 + 4 g .. + 3) are its column operand as they are; the row operand (dim, the same keys)
-//           comes from transposing reads.  FP8 values' powers of two go to the weights.
+//   V p:    the eight weights of a lane in 32 keys (4 g .. + 3 and 16 + 4 g .. + 3) are its column operand as they are; the row operand (dim, the same
+//           keys) comes from transposing reads.  FP8 values' powers of two go to the weights.
 // LDS: chunk c (16 bytes) of row r lies at c ^ swizzle(r), so that the operand reads hit all banks.
 template <int TYPE, int DIM>
 struct RowsForm
 {
-    static constexpr int KEYS = PA_ROWS_KEYS, STAGES = DIM * CODE_BYTES<TYPE> == 256 ? 1 : 2;
-    static constexpr int ROW = DIM * CODE_BYTES<TYPE>, SIDE = KEYS * ROW, SCALES = TYPE == DT_BF16 ? 0 : 256, WAVE = STAGES * (2 * SIDE + SCALES);
+    static constexpr int ROW = DIM * CODE_BYTES<TYPE>, KEYS = ROW == 256 ? 32 : 64, STAGES = ROW == 64 ? 2 : 1;
+    static constexpr int SIDE = KEYS * ROW, EXPONENTS = TYPE == DT_BF16 ? 0 : 2 * KEYS * 4, WAVE = STAGES * (2 * SIDE + EXPONENTS);
     static constexpr int SUM = DIM + 4;                                     // floats per row of the sums
     static constexpr int STAT = 4 * (WAVE > PA_ROWS * SUM * 4 ? WAVE : PA_ROWS * SUM * 4), LDS = STAT + 4 * PA_ROWS * 8;
 };
@@ -245,11 +243,11 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
 {
     typedef RowsForm<TYPE, DIM> F;
     constexpr int KEYS = F::KEYS, STAGES = F::STAGES, ROW = F::ROW, SIDE = F::SIDE, SUM = F::SUM, CHUNKS = ROW / 16;
-    constexpr int ROWS_PER_LOAD = 1024 / ROW, LOADS = SIDE / 1024, KEY_LOADS = LOADS + (TYPE == DT_BF16 ? 0 : 1);
+    constexpr int TILES = KEYS / 16, LOADS = SIDE / 1024, PART_LOADS = LOADS / TILES, KEY_LOADS = LOADS + (TYPE == DT_BF16 ? 0 : 2);
     float2* const stat = (float2*)(lds + F::STAT);                          // [wave][row] (max, sum)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 15, g = lane >> 4;
-    const auto rows = sequence_rows(a, p, s);
+    const auto rows = sequence_rows<KEYS>(a, p, s);
     if (rows.s < 0 || range >= rows.n_ranges) { return; }
     const NewTokens mine = rows.mine;
     const auto& blocks = rows.blocks;
@@ -266,43 +264,60 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         if constexpr (TYPE == DT_BF16) { return DIM == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
         else { return DIM == 128 ? ((r >> 1) & 3) | ((r >> 4) & 1) << 2 : ((r >> 2) & 1) | ((r >> 4) & 1) << 1; }
     };
-    // the wave's LDS: key blocks, value blocks, exponents (lanes 0 .. 31 keys', then values')
+    // the wave's LDS: key blocks, value blocks, exponents (keys', then values')
     uint8_t* const my_lds = lds + wave * F::WAVE;
     const uint32_t my_lds0 = __builtin_amdgcn_readfirstlane(lds_offset(my_lds));
     constexpr int VALUES = STAGES * SIDE, EXPONENTS = 2 * VALUES;
     // the wave's n-th block of the range is list entry begin + wave + 4 n
     const int n_mine = begin + wave < end ? (end - begin - wave + 3) / 4 : 0;
-    auto block_of = [&](int n) { return blocks.block(begin + wave + 4 * n); };
-    int pages = 0;                                                          // lane l: page of rows 16 (l % 2) .. + 15 of the wave's block 32 k + l / 2; -1: none
+    // lane l: where rows 16 (l % TILES) .. + 15 of the wave's block k 64 / TILES + l / TILES begin in the pool (and their exponents); bit 63: they have no page
+    constexpr int BATCH = 64 / TILES;
+    size_t rows_from = 0, exponents_from = 0;
     auto look_up = [&](int n0) {
-        const int i = begin + wave + 4 * (n0 + (lane >> 1));
-        const int pos = blocks.block(i) * KEYS + 16 * (lane & 1);
-        pages = i >= end || pos > rows.hi ? 0 : max(paged_page(a, s, pos), -1);
+        const int i = begin + wave + 4 * (n0 + lane / TILES);
+        const int pos = blocks.block(i) * KEYS + 16 * (lane % TILES);
+        const int page = i >= end || pos > rows.hi ? 0 : paged_page(a, s, pos);
+        const size_t r0 = paged_row(a, kvh, pos);
+        rows_from = max(page, 0) * a.page_stride + r0 * ROW | (page < 0 ? (size_t)1 << 63 : 0);
+        exponents_from = max(page, 0) * a.scale_stride + r0;
     };
-    // half blocks (16 rows) of entry n: their page, and where they begin
-    auto page_of = [&](int n, int half) { return __builtin_amdgcn_readlane(pages, (n % 32) * 2 + half); };
+    auto of_part = [&](size_t v, int n, int part) {
+        const int at = n % BATCH * TILES + part;
+        return (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), at) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, at);
+    };
+    const uint32_t key_off = lane * 16 ^ key_swizzle(lane / CHUNKS) * 16, value_off = lane * 16 ^ value_swizzle(lane / CHUNKS) * 16;
     auto stage = [&](int n, bool values) {
-        const int key0 = block_of(n) * KEYS;
-        const uint32_t to = my_lds0 + (values ? VALUES : 0) + n % STAGES * SIDE;
-        size_t exponent_at[2];
 #pragma unroll
-        for (int half = 0; half < 2; half++)
+        for (int part = 0; part < TILES; part++)
         {
-            const size_t page = max(page_of(n, half), 0), r0 = paged_row(a, kvh, key0 + 16 * half);
-            const uint8_t* const from = (values ? a.v : a.k) + page * a.page_stride + r0 * ROW;
-            exponent_at[half] = page * a.scale_stride + r0;
+            const size_t from = of_part(rows_from, n, part) & ~((size_t)1 << 63);
+            uint32_t off[PART_LOADS];
 #pragma unroll
-            for (int i = 0; i < LOADS / 2; i++)
+            for (int i = 0; i < PART_LOADS; i++)
             {
-                const int in = i * ROWS_PER_LOAD + lane / CHUNKS, r = 16 * half + in, c = lane % CHUNKS;
-                load_to_lds<true>(to + (half * LOADS / 2 + i) * 1024, from, (uint32_t)(in * ROW + (c ^ (values ? value_swizzle(r) : key_swizzle(r))) * 16));
+                // row 16 part + i 1024 / ROW + lane / CHUNKS: the first two terms change bits of the swizzle that the lane's row does not reach
+                const int r = 16 * part + i * (1024 / ROW);
+                off[i] = values ? value_off ^ (uint32_t)(value_swizzle(r) * 16) : key_off ^ (uint32_t)(key_swizzle(r) * 16);
             }
+            kibs_to_lds(my_lds0 + (values ? VALUES : 0) + n % STAGES * SIDE + part * 16 * ROW, (values ? a.v : a.k) + from, off);
         }
         if constexpr (TYPE != DT_BF16)
         {
-            if (!values) { bytes_to_lds(my_lds0 + EXPONENTS + n % STAGES * F::SCALES, (lane < 32 ? a.k_scale : a.v_scale) + (lane & 16 ? exponent_at[1] : exponent_at[0]) + (lane & 15)); }
+            if (!values)
+            {
+                // lane l: the exponent of row l
+                const int at = n % BATCH * TILES + g;
+                const size_t from = (size_t)(uint32_t)__shfl((int)(exponents_from >> 32), at) << 32 | (uint32_t)__shfl((int)exponents_from, at);
+                bytes_to_lds(my_lds0 + EXPONENTS + n % STAGES * F::EXPONENTS, a.k_scale + from + j);
+                bytes_to_lds(my_lds0 + EXPONENTS + n % STAGES * F::EXPONENTS + KEYS * 4, a.v_scale + from + j);
+            }
         }
     };
+    // list entries plain_from .. plain_to - 1: every row sees every key
+    int plain_from = 0, plain_to = (rows.lo + 1) / KEYS;
+    if (p.window != 0) { plain_from = (rows.hi - p.window + KEYS) / KEYS; }
+    plain_from = uniform(max(plain_from - blocks.skip, rows.hi < p.window || p.window == 0 ? 0 : blocks.sinks));
+    plain_to = uniform(plain_to - blocks.skip);
 
     float m = -INFINITY, l = 0.0f;
     f32x4 out[DIM / 16];
@@ -312,22 +327,26 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
     auto block = [&](int n) {
         const uint8_t* const kb = my_lds + n % STAGES * SIDE;
         const uint8_t* const vb = my_lds + VALUES + n % STAGES * SIDE;
-        const uint8_t* const exponents = my_lds + EXPONENTS + n % STAGES * F::SCALES;
-        const int b = block_of(n), bad = (page_of(n, 0) < 0 ? 1 : 0) | (page_of(n, 1) < 0 ? 2 : 0);
+        const uint8_t* const exponents = my_lds + EXPONENTS + n % STAGES * F::EXPONENTS;
+        const int entry = begin + wave + 4 * n;
+        int lacks = 0;
+#pragma unroll
+        for (int part = 0; part < TILES; part++) { lacks |= (int)((uint32_t)__builtin_amdgcn_readlane((int)(rows_from >> 32), n % BATCH * TILES + part) >> 31) << part; }
         // what was asked for behind the keys of n may still be on its way
         if (STAGES == 2 && n + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * LOADS + KEY_LOADS) : "memory"); }
         else { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS) : "memory"); }
-        f32x4 acc[2] = { { 0.0f, 0.0f, 0.0f, 0.0f }, { 0.0f, 0.0f, 0.0f, 0.0f } };
-        u32x4 value_exponents[2];
+        f32x4 acc[TILES];
+        u32x4 value_exponents[TILES];
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++)
+        for (int kt = 0; kt < TILES; kt++)
         {
+            acc[kt] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f };
             const int r = 16 * kt + j;
             float kscale = 1.0f;
             if constexpr (TYPE != DT_BF16)
             {
                 kscale = bits_to_f32(*(const uint32_t*)(exponents + r * 4) << 23);
-                value_exponents[kt] = *(const u32x4*)(exponents + 128 + (16 * kt + 4 * g) * 4);
+                value_exponents[kt] = *(const u32x4*)(exponents + KEYS * 4 + (16 * kt + 4 * g) * 4);
             }
 #pragma unroll
             for (int c = 0; c < DIM / 32; c++)
@@ -346,30 +365,93 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         if (n + STAGES < n_mine)
         {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");           // the keys have been read
-            if ((n + STAGES) % 32 == 0) { look_up(n + STAGES); }
+            if ((n + STAGES) % BATCH == 0) { look_up(n + STAGES); }
             stage(n + STAGES, false);
         }
         if (STAGES == 2 && n + 2 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS + 2 * KEY_LOADS) : "memory"); }
         else if (STAGES == 2 && n + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS + KEY_LOADS) : "memory"); }
         else if (STAGES == 1 && n + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(KEY_LOADS) : "memory"); }
         else { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
-        u32x4 vf[DIM / 16];
+        // values as they lie there: eight of a dim, BF16 or codes
+        constexpr int WORDS = TYPE == DT_BF16 ? 4 : 2, STEPS = TILES / 2;
+        uint32_t raw[STEPS][DIM / 16][WORDS];
 #pragma unroll
-        for (int d = 0; d < DIM / 16; d++)
-        {
-            if constexpr (TYPE == DT_BF16)
+        for (int u = 0; u < STEPS; u++)
+#pragma unroll
+            for (int d = 0; d < DIM / 16; d++)
             {
-                const int r = 4 * g + (j >> 2);
-                const uint8_t* const at0 = vb + r * ROW + (((2 * d + ((j & 3) >> 1)) ^ value_swizzle(r)) << 4) + ((j & 1) << 3);
-                const u32x2 lo = lds_transposed16(at0), hi = lds_transposed16(at0 + 16 * ROW);      // the swizzle of row r + 16 is that of r
-                vf[d] = u32x4{ lo[0], lo[1], hi[0], hi[1] };
+                if constexpr (TYPE == DT_BF16)
+                {
+                    const int r = 32 * u + 4 * g + (j >> 2);
+                    const uint8_t* const at0 = vb + r * ROW + (((2 * d + ((j & 3) >> 1)) ^ value_swizzle(r)) << 4) + ((j & 1) << 3);
+                    const u32x2 lo = lds_transposed16(at0), hi = lds_transposed16(at0 + 16 * ROW);      // the swizzle of row r + 16 is that of r
+                    raw[u][d][0] = lo[0], raw[u][d][1] = lo[1], raw[u][d][2] = hi[0], raw[u][d][3] = hi[1];
+                }
+                else
+                {
+                    const int r = 32 * u + 4 * g + ((j >> 1) & 3) + (j >> 3) * 16;
+                    const u32x2 codes = lds_transposed8(vb + r * ROW + ((d ^ value_swizzle(r)) << 4) + ((j & 1) << 3));
+                    raw[u][d][0] = codes[0], raw[u][d][1] = codes[1];
+                }
             }
+        auto values = [&](int u, int d) {
+            if constexpr (TYPE == DT_BF16) { return u32x4{ raw[u][d][0], raw[u][d][1], raw[u][d][2], raw[u][d][3] }; }
             else
             {
-                const int r = 4 * g + ((j >> 1) & 3) + (j >> 3) * 16;
-                const u32x2 codes = lds_transposed8(vb + r * ROW + ((d ^ value_swizzle(r)) << 4) + ((j & 1) << 3));
-                const u32x2 lo = fp8x4_to_bf16<TYPE>(codes[0], 1.0f), hi = fp8x4_to_bf16<TYPE>(codes[1], 1.0f);
-                vf[d] = u32x4{ lo[0], lo[1], hi[0], hi[1] };
+                const u32x2 lo = fp8x4_to_bf16<TYPE>(raw[u][d][0], 1.0f), hi = fp8x4_to_bf16<TYPE>(raw[u][d][1], 1.0f);
+                return u32x4{ lo[0], lo[1], hi[0], hi[1] };
+            }
+        };
+        const bool plain = entry >= plain_from && entry < plain_to && lacks == 0;
+        if (!plain)
+        {
+            const int b = blocks.block(entry);
+#pragma unroll
+            for (int e = 0; e < 4 * TILES; e++)
+            {
+                const bool see = sees(p, my_pos, b * KEYS + 16 * (e >> 2) + 4 * g + (e & 3)) && !(lacks >> (e >> 2) & 1);
+                acc[e >> 2][e & 3] = see ? acc[e >> 2][e & 3] : -INFINITY;
+                if constexpr (TYPE != DT_BF16) { value_exponents[e >> 2][e & 3] = see ? value_exponents[e >> 2][e & 3] : 0; }     // one that nobody wrote may be an infinity's
+            }
+            // Weight 0 times an infinity is NaN: what is infinite or NaN is added to the sums of the rows that see it and cleared in front of the products.
+            uint32_t odd = 0;
+#pragma unroll
+            for (int u = 0; u < STEPS; u++)
+#pragma unroll
+                for (int d = 0; d < DIM / 16; d++)
+#pragma unroll
+                    for (int i = 0; i < WORDS; i++) { odd |= TYPE == DT_BF16 ? not_finite(raw[u][d][i]) : codes_not_finite<TYPE>(raw[u][d][i]); }
+            if (__any(odd != 0))
+            {
+#pragma unroll 1
+                for (int key = 0; key < KEYS; key++)
+                {
+                    const bool see = sees(p, my_pos, b * KEYS + key) && !(lacks >> (key / 16) & 1);
+#pragma unroll
+                    for (int d = 0; d < DIM / 16; d++)
+                    {
+                        // dims 16 d + 4 g .. + 3
+                        const int byte = (16 * d + 4 * g) * CODE_BYTES<TYPE>;
+                        const uint8_t* const from = vb + key * ROW + ((byte / 16 ^ value_swizzle(key)) << 4) + byte % 16;
+                        u32x2 w;
+                        if constexpr (TYPE == DT_BF16) { w = *(const u32x2*)from; }
+                        else { w = fp8x4_to_bf16<TYPE>(*(const uint32_t*)from, 1.0f); }
+                        float v[4];
+                        unpack4(w, v);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) { out[d][e] += see && !(fabsf(v[e]) < INFINITY) ? v[e] : 0.0f; }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < STEPS; u++)
+#pragma unroll
+                    for (int d = 0; d < DIM / 16; d++)
+#pragma unroll
+                        for (int i = 0; i < WORDS; i++)
+                        {
+                            const uint32_t w = raw[u][d][i];
+                            raw[u][d][i] = w & ~(TYPE == DT_BF16 ? (not_finite(w) >> 15) * 0xFFFFu : (codes_not_finite<TYPE>(w) >> 7) * 0xFFu);
+                        }
             }
         }
         if (n + STAGES < n_mine)
@@ -377,23 +459,10 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");           // the values have been read
             stage(n + STAGES, true);
         }
-        const bool plain = KeyBlocks<KEYS>::plain(p, rows.lo, rows.hi, b) && bad == 0;
-        float score[8];
-        uint32_t seen = 0xFFu;
+        float top = acc[0][0];
 #pragma unroll
-        for (int e = 0; e < 8; e++) { score[e] = acc[e >> 2][e & 3] * p.scale; }
-        if (!plain)
-        {
-            seen = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-            {
-                const bool see = sees(p, my_pos, b * KEYS + 16 * (e >> 2) + 4 * g + (e & 3)) && !(bad >> (e >> 2) & 1);
-                seen |= see ? 1u << e : 0u;
-                score[e] = see ? score[e] : -INFINITY;
-            }
-        }
-        float top = max8(score);
+        for (int e = 1; e < 4 * TILES; e++) { top = fmaxf(top, acc[e >> 2][e & 3]); }
+        top *= p.scale;
         if (__any(top > m + PA_LAG))
         {
             top = fmaxf(top, __shfl_xor(top, 16));
@@ -404,45 +473,22 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
 #pragma unroll
             for (int d = 0; d < DIM / 16; d++) { out[d] *= shrink; }
         }
-        const float off = m > -INFINITY ? m : 0.0f;                         // no key seen yet: every weight is 2^-inf = 0
-        float w[8];
+        const float off = m > -INFINITY ? -m : 0.0f;                        // no key seen yet: every weight is 2^-inf = 0
+        float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+        bf16x8 pb[STEPS];
 #pragma unroll
-        for (int e = 0; e < 8; e++) { w[e] = __builtin_amdgcn_exp2f(score[e] - off); }
-        l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-        if constexpr (TYPE != DT_BF16)
+        for (int e = 0; e < 4 * TILES; e++)
         {
-#pragma unroll
-            for (int e = 0; e < 8; e++) { w[e] = seen >> e & 1 ? w[e] * bits_to_f32(value_exponents[e >> 2][e & 3] << 23) : 0.0f; }
+            float w = __builtin_amdgcn_exp2f(fmaf(acc[e >> 2][e & 3], p.scale, off));
+            sum[e & 3] += w;
+            if constexpr (TYPE != DT_BF16) { w *= bits_to_f32(value_exponents[e >> 2][e & 3] << 23); }
+            pb[e >> 3][e & 7] = (__bf16)w;
         }
-        const bf16x8 pb = { (__bf16)w[0], (__bf16)w[1], (__bf16)w[2], (__bf16)w[3], (__bf16)w[4], (__bf16)w[5], (__bf16)w[6], (__bf16)w[7] };
-        uint32_t odd = 0;
-        if (!plain)
-        {
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-            for (int d = 0; d < DIM / 16; d++) { odd |= not_finite(vf[d]); }
-        }
-        if (__any(odd != 0))
-        {
-            // 0 times an infinity is NaN: what is not finite is added apart, to the rows that see it
-            bf16x8 see;
+        for (int u = 0; u < STEPS; u++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) { see[e] = (__bf16)(float)(seen >> e & 1); }
-#pragma unroll
-            for (int d = 0; d < DIM / 16; d++)
-            {
-                out[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, finite_part(vf[d])), pb, out[d], 0, 0, 0);
-#pragma unroll 1
-                for (int kind = 0; kind < 3; kind++)
-                {
-                    const f32x4 count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, where_kind(vf[d], kind)), see, f32x4{ 0.0f, 0.0f, 0.0f, 0.0f }, 0, 0, 0);
-#pragma unroll
-                    for (int v = 0; v < 4; v++) { out[d][v] += count[v] > 0.0f ? value_of_kind(kind) : 0.0f; }
-                }
-            }
-            return;
-        }
-#pragma unroll
-        for (int d = 0; d < DIM / 16; d++) { out[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[d]), pb, out[d], 0, 0, 0); }
+            for (int d = 0; d < DIM / 16; d++) { out[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, values(u, d)), pb[u], out[d], 0, 0, 0); }
     };
 
     if (n_mine > 0)
@@ -952,15 +998,15 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
 }
 
 // Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then ranges x sequences x kv heads.
-template <int TYPE, int DIM, int RT>
-__global__ __launch_bounds__(256, 3 - RT) void paged_attention_kernel(const PagedArgs a, const PagedAttention p)
+template <int TYPE, int DIM>
+__global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs a, const PagedAttention p)
 {
     typedef RowsForm<TYPE, DIM> R;
     typedef TileForm<TYPE, DIM> T;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS > T::LDS ? R::LDS : T::LDS];
     static_assert(sizeof(lds) <= 80 * 1024, "two workgroups on a CU");
     const int tiles = p.tiles * a.n_kv, n_tiles = tiles * p.tile_split;
-    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM, RT>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
+    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM, 1>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
     else
     {
         const int at = blockIdx.x - n_tiles, sequences = a.n_seqs * a.n_kv;
@@ -971,7 +1017,7 @@ __global__ __launch_bounds__(256, 3 - RT) void paged_attention_kernel(const Page
 // Sums of the key ranges of 16 rows, DIM / 16 dims of a row per thread: rescaled to the largest maximum, added in the order of the ranges, divided by the
 // sum of the weights, one rounding.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads where tiles have ranges, then
 // sequences x kv heads where those do.
-template <int DIM, int RT>
+template <int DIM, int KEYS, int RT>
 __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
 {
     constexpr int PER = DIM / 16, PARTS = 8 * RT;
@@ -989,7 +1035,7 @@ __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const Page
     }
     else
     {
-        const auto rows = sequence_rows(a, p, (blockIdx.x - n_tiles) / a.n_kv);
+        const auto rows = sequence_rows<KEYS>(a, p, (blockIdx.x - n_tiles) / a.n_kv);
         row = threadIdx.x >> 4;
         if (rows.s < 0 || row >= rows.n_rows) { return; }
         mine = rows.mine;
@@ -1000,12 +1046,12 @@ __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const Page
     const int d0 = (threadIdx.x & 15) * PER;
     f32x4 sum[PER / 4] = {};
     float m = -INFINITY, l = 0.0f;
-    for (int r0 = 0; r0 < n; r0 += 8)
+    for (int r0 = 0; r0 < n; r0 += 4)
     {
-        f32x4 part[8][PER / 4];                                             // eight ranges requested at once
-        float2 stat[8];
+        f32x4 part[4][PER / 4];                                             // four ranges requested at once
+        float2 stat[4];
 #pragma unroll
-        for (int r = 0; r < 8; r++)
+        for (int r = 0; r < 4; r++)
         {
             const int range = min(r0 + r, n - 1);
             stat[r] = *p.stats(range, at_row, DIM);
@@ -1014,14 +1060,14 @@ __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const Page
         }
         float top = m;
 #pragma unroll
-        for (int r = 0; r < 8; r++) { top = fmaxf(top, stat[r].x); }
+        for (int r = 0; r < 4; r++) { top = fmaxf(top, stat[r].x); }
         const float base = top > -INFINITY ? top : 0.0f, shrink = __builtin_amdgcn_exp2f(m - base);
         m = top;
         l *= shrink;
 #pragma unroll
         for (int d = 0; d < PER / 4; d++) { sum[d] *= shrink; }
 #pragma unroll
-        for (int r = 0; r < 8; r++)
+        for (int r = 0; r < 4; r++)
         {
             const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
             if (r0 + r < n && w != 0.0f)                                    // a range without a key has weight 0
