@@ -47,6 +47,9 @@ bool paged_args(const hip_paged_kv* c, PagedArgs& a)
     ((c)->head_dim == 64 ? ((c)->type == CCCC_BFLOAT16 ? KERNEL<DT_BF16, 64> : (c)->type == CCCC_FP8_E4M3 ? KERNEL<DT_E4M3, 64> : KERNEL<DT_E5M2, 64>) \
                          : ((c)->type == CCCC_BFLOAT16 ? KERNEL<DT_BF16, 128> : (c)->type == CCCC_FP8_E4M3 ? KERNEL<DT_E4M3, 128> : KERNEL<DT_E5M2, 128>))
 
+// keys of a block of paged_attention_kernel's rows (RowsForm)
+int keys_per_block(const hip_paged_kv* c) { return c->type == CCCC_BFLOAT16 && c->head_dim == 128 ? 32 : 64; }
+
 bool attention_args(const hip_paged_kv* c, PagedArgs& a, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink)
 {
     if (!paged_args(c, a) || n_q_heads <= 0 || n_q_heads % c->n_kv_heads != 0 || n_q_heads / c->n_kv_heads > 64) { return false; }
@@ -55,40 +58,47 @@ bool attention_args(const hip_paged_kv* c, PagedArgs& a, int n_q_heads, int n_to
     a.max_ctx = std::min(a.max_ctx, max_ctx);
     return true;
 }
-// How a call's rows are taken: in tiles, as sequences of up to 16 rows per kv head, or both, each over so many ranges of keys at most.
+// How a call's rows are taken: in tiles, each over so many ranges of keys at most; as sequences of up to 16 rows per kv head, whose keys are shared out over
+// so many workgroups (0: one each); or both.
 struct Plan
 {
-    long long tiles;                // at most
+    int tiles, tile_split;          // at most
     bool rows;
-    int tile;                       // rows of a tile
-    int min_rows, tile_split, row_split, n_split;
+    int min_rows, row_chunks;
+    size_t tile_bytes, row_bytes;   // of partial sums
 };
 
-// Sequences of up to 16 rows per kv head have a form of their own, also beside longer ones -- unless every sequence has max_new tokens, as far as their
-// number tells.
-Plan plan_attention(const PagedArgs& a, int group, int n_tokens, int max_new, int window, int n_sink)
+// False: more than a launch can have.
+bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, int n_tokens, int max_new, int window, int n_sink, Plan& plan)
 {
-    const long long most_rows = (long long)std::min(max_new, n_tokens) * group, rows = (long long)n_tokens * group;
-    Plan plan = { 0, true, 128, 0, 1, 1, 1 };
-    if (most_rows > PA_ROWS)
+    const int group = n_q / a.n_kv;
+    const long long rows = (long long)n_tokens * group, slots = 2LL * cu_count();
+    // Sequences of up to 16 rows per kv head have a form of their own, also beside longer ones -- unless every sequence has max_new tokens, as far as
+    // their number tells.
+    plan = { 0, 1, true, 0, 0, 0, 0 };
+    const long long keys = window == 0 ? a.max_ctx : std::min<long long>(a.max_ctx, (long long)window + n_sink + max_new);
+    if ((long long)std::min(max_new, n_tokens) * group > PA_ROWS)
     {
         plan.rows = group <= PA_ROWS && n_tokens < (long long)a.n_seqs * max_new;
         plan.min_rows = plan.rows ? PA_ROWS : 0;
-        if (getenv("PA_RT")) { plan.tile = 128 * atoi(getenv("PA_RT")); }
         const long long cut = std::min<long long>(a.n_seqs, rows / (plan.min_rows + 1));       // sequences, at most
-        plan.tiles = (rows - cut) / plan.tile + cut;
+        const long long tiles = (rows - cut) / 128 + cut;
+        if (tiles * a.n_kv * 64 > MOST_BLOCKS) { return false; }
+        plan.tiles = (int)tiles;
+        plan.tile_split = (int)std::max<long long>(1, std::min({ slots / (tiles * a.n_kv), keys / 256, 64LL }));
+        if (getenv("PA_TS")) { plan.tile_split = atoi(getenv("PA_TS")); }
+        plan.tile_bytes = plan.tile_split > 1 ? ((size_t)n_tokens * n_q * plan.tile_split * (dim + 2) * 4 + 15) & ~(size_t)15 : 0;
     }
-    const long long keys = window == 0 ? a.max_ctx : std::min<long long>(a.max_ctx, (long long)window + n_sink + max_new);
-    auto split = [&](long long workgroups) { return (int)std::max<long long>(1, std::min({ 2LL * cu_count() / std::max<long long>(workgroups, 1), keys / 256, 64LL })); };
-    plan.tile_split = split(plan.tiles * a.n_kv * (plan.tile / 128));
-    plan.row_split = split((long long)a.n_seqs * a.n_kv);
-    if (getenv("PA_TS")) { plan.tile_split = atoi(getenv("PA_TS")); }
-    if (getenv("PA_RS")) { plan.row_split = atoi(getenv("PA_RS")); }
-    plan.n_split = std::max(plan.tiles ? plan.tile_split : 1, plan.rows ? plan.row_split : 1);
-    return plan;
+    if (plan.rows)
+    {
+        const long long shares = (long long)a.n_seqs * ((a.max_ctx + 4LL * keys_per_block) / (4 * keys_per_block) + 1);
+        if ((long long)a.n_seqs * a.n_kv * 2 > MOST_BLOCKS || shares > 0x3FFFFFFFLL) { return false; }
+        plan.row_chunks = (int)std::max<long long>(1, std::min<long long>(slots / a.n_kv, (long long)a.n_seqs * ((keys + 255) / 256 + 1)));
+        if (getenv("PA_RS")) { plan.row_chunks = atoi(getenv("PA_RS")); }
+        plan.row_bytes = (size_t)plan.row_chunks * 2 * a.n_kv * PA_ROWS * (dim + 2) * 4;
+    }
+    return true;
 }
-
-size_t partial_bytes(int n_split, size_t outputs, int dim) { return n_split < 2 ? 0 : (outputs * (size_t)n_split * (dim + 2) * 4 + 15) & ~(size_t)15; }
 }    // namespace
 
 int hip_qk_norm_rope_kv_paged_bf16(const hip_paged_kv* cache, const void* q, const void* k, const void* v, const void* q_norm_w, const void* k_norm_w, const void* cos_tab, const void* sin_tab,
@@ -133,8 +143,8 @@ unsigned long long hip_attention_paged_workspace_bytes(const hip_paged_kv* cache
 {
     PagedArgs a;
     if (!attention_args(cache, a, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink) || n_tokens == 0) { return 0; }
-    const Plan plan = plan_attention(a, n_q_heads / a.n_kv, n_tokens, max_new, window, n_sink);
-    return partial_bytes(plan.n_split, (size_t)n_tokens * n_q_heads, cache->head_dim);
+    Plan plan;
+    return plan_attention(a, keys_per_block(cache), n_q_heads, cache->head_dim, n_tokens, max_new, window, n_sink, plan) ? plan.tile_bytes + plan.row_bytes : 0;
 }
 
 int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, void* workspace, unsigned long long workspace_bytes, int n_q_heads, int n_tokens, int max_new, int max_ctx,
@@ -147,22 +157,25 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
     const long long width = (long long)n_q_heads * dim;
     if (ldq % 8 != 0 || ldy % 8 != 0 || ldq < width || ldy < width) { return -1; }
     if (n_tokens == 0) { return 0; }
-    const int group = n_q_heads / a.n_kv;
-    const size_t outputs = (size_t)n_tokens * n_q_heads;
-    Plan plan = plan_attention(a, group, n_tokens, max_new, window, n_sink);
-    while (plan.n_split > 1 && partial_bytes(plan.n_split, outputs, dim) > workspace_bytes) { plan.n_split--; }
-    const int tile_split = std::min(plan.tile_split, plan.n_split), row_split = std::min(plan.row_split, plan.n_split);
-    const long long tiles = plan.tiles * a.n_kv, sequences = plan.rows ? (long long)a.n_seqs * a.n_kv : 0;
-    const long long blocks = tiles * tile_split + sequences * row_split;
-    const long long sums = (tile_split > 1 ? tiles * (plan.tile / 16) : 0) + (row_split > 1 ? sequences : 0);
-    if (blocks > MOST_BLOCKS || sums > MOST_BLOCKS) { return -1; }
-    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)workspace, (size_t)ldq, (size_t)ldy, n_q_heads, group, n_tokens, max_new, window, n_sink, plan.n_split,
-                               (int)plan.tiles, tile_split, row_split, plan.min_rows, getenv("PA_SNAKE") ? 1 : 0, 1.4426950408889634f / sqrtf((float)dim) };
+    Plan plan;
+    if (!plan_attention(a, keys_per_block(cache), n_q_heads, dim, n_tokens, max_new, window, n_sink, plan)) { return -1; }
+    // too little workspace: tiles and sequences in one piece each
+    if (workspace_bytes < plan.tile_bytes + plan.row_bytes)
+    {
+        plan.tile_split = 1;
+        plan.tile_bytes = 0;
+        if (workspace_bytes < plan.row_bytes) { plan.row_chunks = 0; }
+    }
+    const long long tiles = (long long)plan.tiles * a.n_kv * plan.tile_split, chunks = plan.rows ? (long long)(plan.row_chunks ? plan.row_chunks : a.n_seqs) * a.n_kv : 0;
+    const long long sums = (plan.tile_split > 1 ? (long long)plan.tiles * a.n_kv * 8 : 0) + (plan.row_chunks > 0 ? (long long)a.n_seqs * a.n_kv : 0);
+    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)workspace, (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv, n_tokens, max_new, window, n_sink, plan.tile_split,
+                               plan.tiles, plan.tile_split, plan.row_chunks, (float*)((char*)workspace + plan.tile_bytes), plan.min_rows, getenv("PA_SNAKE") ? 1 : 0,
+                               1.4426950408889634f / sqrtf((float)dim) };
     const auto kernel = CCQ_PAGED_KERNEL(paged_attention_kernel, cache);
-    kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, p);
+    kernel<<<(unsigned)(tiles + chunks), 256, 0, stream()>>>(a, p);
     if (sums > 0)
     {
-        const auto combine = dim == 64 ? paged_attention_combine_kernel<64, 64, 1> : cache->type == CCCC_BFLOAT16 ? paged_attention_combine_kernel<128, 32, 1> : paged_attention_combine_kernel<128, 64, 1>;
+        const auto combine = dim == 64 ? paged_attention_combine_kernel<64, 64> : keys_per_block(cache) == 32 ? paged_attention_combine_kernel<128, 32> : paged_attention_combine_kernel<128, 64>;
         combine<<<(unsigned)sums, 256, 0, stream()>>>(a, p);
     }
     return finish("attention_paged");

@@ -18,11 +18,17 @@ struct PagedAttention
     int n_q, group, n_tokens, max_new, window, n_sink;
     int n_split;                    // ranges of keys that `partial` is laid out for
     int tiles, tile_split;          // tiles of 128 rows (at most) and the most ranges of each
-    int row_split;                  // most ranges of a sequence of at most 16 rows per kv head
+    int row_chunks;                 // workgroups per kv head that share the keys of all sequences of at most 16 rows per kv head; 0: one for each of those
+    float* row_partial;             // [chunk][2][kv head][16][dim] sums, then (max, sum) likewise
     int min_rows;                   // sequences of at most so many rows per kv head are not cut into tiles
     int snake;
     float scale;                    // log2 e / sqrt(dim)
 
+    __device__ __forceinline__ float* row_sums(int slot, int kvh, int n_kv, int row, int dim) const { return row_partial + (((size_t)slot * n_kv + kvh) * 16 + row) * dim; }
+    __device__ __forceinline__ float2* row_stats(int slot, int kvh, int n_kv, int row, int dim) const
+    {
+        return (float2*)(row_partial + (size_t)row_chunks * 2 * n_kv * 16 * dim) + ((size_t)slot * n_kv + kvh) * 16 + row;
+    }
     __device__ __forceinline__ size_t outputs() const { return (size_t)n_tokens * n_q; }
     __device__ __forceinline__ float* sums(int range, size_t row, int dim) const { return partial + ((size_t)range * outputs() + row) * dim; }
     __device__ __forceinline__ float2* stats(int range, size_t row, int dim) const { return (float2*)(partial + (size_t)n_split * outputs() * dim) + (size_t)range * outputs() + row; }
@@ -88,19 +94,57 @@ struct Rows
 
 constexpr int PA_ROWS = 16, PA_TILE_KEYS = 64;
 
-// A sequence of up to 16 rows per kv head.
+// Sequences of up to 16 rows per kv head: their keys laid end to end in shares of four blocks (a block per wave), cut into chunks of equal length, a
+// workgroup each.  Lengths that differ leave no workgroup with more than another, and a sequence is cut where chunks end and nowhere else.
 template <int KEYS>
-__device__ __forceinline__ Rows<KEYS, PA_ROWS> sequence_rows(const PagedArgs& a, const PagedAttention& p, int s)
+struct Shares
 {
-    Rows<KEYS, PA_ROWS> r;
-    r.mine = new_tokens(a, p, s);
-    r.row0 = 0;
-    r.n_rows = uniform(r.mine.n * p.group);
-    if (r.n_rows == 0 || r.n_rows > PA_ROWS) { return r; }
-    r.s = s;
-    r.cut(p, p.row_split, 4, 256 / KEYS);
-    return r;
-}
+    int total = 0, chunk = 1;                                               // shares of all, and of a chunk
+    int mine = 0, upto = 0, base = 0, before = 0;                           // of sequence base + lane; with those before it in the batch; of earlier batches
+
+    __device__ __forceinline__ static KeyBlocks<KEYS> keys(const PagedAttention& p, const NewTokens& n) { return KeyBlocks<KEYS>(p, n.pos, n.pos + n.n - 1); }
+    __device__ __forceinline__ static int shares(const PagedArgs& a, const PagedAttention& p, int s)
+    {
+        if (s >= a.n_seqs) { return 0; }
+        const NewTokens n = new_tokens(a, p, s);
+        const int rows = n.n * p.group;
+        return rows == 0 || rows > PA_ROWS ? 0 : max((keys(p, n).n + 3) / 4, 1);
+    }
+    // whole waves
+    __device__ __forceinline__ void take(const PagedArgs& a, const PagedAttention& p)
+    {
+        const int lane = threadIdx.x & 63;
+        for (int b = 0; b < a.n_seqs; b += 64)
+        {
+            int v = shares(a, p, b + lane);
+            if (b == 0) { mine = v; }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) { v += __shfl_xor(v, o); }
+            total += uniform(v);
+        }
+        chunk = max((total + p.row_chunks - 1) / p.row_chunks, KEYS == 32 ? 2 : 1);
+        add_up();
+    }
+    __device__ __forceinline__ void add_up()
+    {
+        const int lane = threadIdx.x & 63;
+        upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1)
+        {
+            const int below = __shfl_up(upto, o);
+            upto += lane >= o ? below : 0;
+        }
+    }
+    __device__ __forceinline__ int batch_end() const { return before + __builtin_amdgcn_readlane(upto, 63); }
+    __device__ __forceinline__ void next_batch(const PagedArgs& a, const PagedAttention& p)
+    {
+        before = batch_end();
+        base += 64;
+        mine = shares(a, p, base + (int)(threadIdx.x & 63));
+        add_up();
+    }
+};
 
 // Tile `tile` of those of all sequences, a sequence's last ones first: they see the most keys.  Where a CU gets two workgroups in all, the second half of
 // the tiles comes in the other order, so that a long one has a short one beside it.  Called by whole waves: a lane per sequence, their tiles added up.
@@ -239,7 +283,7 @@ struct RowsForm
 };
 
 template <int TYPE, int DIM>
-__device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int s, int kvh, int range)
+__device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int s, int kvh, int from_share, int to_share, int slot)
 {
     typedef RowsForm<TYPE, DIM> F;
     constexpr int KEYS = F::KEYS, STAGES = F::STAGES, ROW = F::ROW, SIDE = F::SIDE, SUM = F::SUM, CHUNKS = ROW / 16;
@@ -247,11 +291,10 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
     float2* const stat = (float2*)(lds + F::STAT);                          // [wave][row] (max, sum)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 15, g = lane >> 4;
-    const auto rows = sequence_rows<KEYS>(a, p, s);
-    if (rows.s < 0 || range >= rows.n_ranges) { return; }
-    const NewTokens mine = rows.mine;
-    const auto& blocks = rows.blocks;
-    const int n_rows = rows.n_rows, begin = range * rows.per, end = min(blocks.n, begin + rows.per);
+    const NewTokens mine = new_tokens(a, p, s);
+    const auto blocks = Shares<KEYS>::keys(p, mine);
+    const int n_rows = uniform(mine.n * p.group), lo = uniform(mine.pos), hi = uniform(mine.pos + mine.n - 1);
+    const int begin = from_share * 4, end = uniform(min(blocks.n, to_share * 4));
 
     const int row = min(j, n_rows - 1), token = row / p.group, head = kvh * p.group + row % p.group;
     const int my_pos = mine.pos + token;
@@ -276,7 +319,7 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
     auto look_up = [&](int n0) {
         const int i = begin + wave + 4 * (n0 + lane / TILES);
         const int pos = blocks.block(i) * KEYS + 16 * (lane % TILES);
-        const int page = i >= end || pos > rows.hi ? 0 : paged_page(a, s, pos);
+        const int page = i >= end || pos > hi ? 0 : paged_page(a, s, pos);
         const size_t r0 = paged_row(a, kvh, pos);
         rows_from = max(page, 0) * a.page_stride + r0 * ROW | (page < 0 ? (size_t)1 << 63 : 0);
         exponents_from = max(page, 0) * a.scale_stride + r0;
@@ -314,9 +357,9 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         }
     };
     // list entries plain_from .. plain_to - 1: every row sees every key
-    int plain_from = 0, plain_to = (rows.lo + 1) / KEYS;
-    if (p.window != 0) { plain_from = (rows.hi - p.window + KEYS) / KEYS; }
-    plain_from = uniform(max(plain_from - blocks.skip, rows.hi < p.window || p.window == 0 ? 0 : blocks.sinks));
+    int plain_from = 0, plain_to = (lo + 1) / KEYS;
+    if (p.window != 0) { plain_from = (hi - p.window + KEYS) / KEYS; }
+    plain_from = uniform(max(plain_from - blocks.skip, hi < p.window || p.window == 0 ? 0 : blocks.sinks));
     plain_to = uniform(plain_to - blocks.skip);
 
     float m = -INFINITY, l = 0.0f;
@@ -514,40 +557,70 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
     for (int d = 0; d < DIM / 16; d++) { *(f32x4*)(sums + (wave * 16 + j) * SUM + 16 * d + 4 * g) = out[d]; }
     __syncthreads();
     const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (DIM / 16);
-    if (r >= n_rows) { return; }
-    float top = -INFINITY, total = 0.0f, weight[4];
-#pragma unroll
-    for (int w = 0; w < 4; w++) { top = fmaxf(top, stat[w * 16 + r].x); }
-    const float base = top > -INFINITY ? top : 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++)
+    if (r < n_rows)
     {
-        weight[w] = __builtin_amdgcn_exp2f(stat[w * 16 + r].x - base);            // 2^-inf = 0 for a wave without a key
-        total += weight[w] * stat[w * 16 + r].y;
-    }
-    float sum[DIM / 16];
+        float top = -INFINITY, total = 0.0f, weight[4];
 #pragma unroll
-    for (int d = 0; d < DIM / 16; d++)
+        for (int w = 0; w < 4; w++) { top = fmaxf(top, stat[w * 16 + r].x); }
+        const float base = top > -INFINITY ? top : 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+        {
+            weight[w] = __builtin_amdgcn_exp2f(stat[w * 16 + r].x - base);  // 2^-inf = 0 for a wave without a key
+            total += weight[w] * stat[w * 16 + r].y;
+        }
+        float sum[DIM / 16];
+#pragma unroll
+        for (int d = 0; d < DIM / 16; d++)
+        {
+            sum[d] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) { sum[d] += weight[w] != 0.0f ? weight[w] * sums[(w * 16 + r) * SUM + d0 + d] : 0.0f; }
+        }
+        if (slot >= 0)
+        {
+            float* const dst = p.row_sums(slot, kvh, a.n_kv, r, DIM) + d0;
+#pragma unroll
+            for (int d = 0; d < DIM / 16; d += 4) { *(f32x4*)(dst + d) = f32x4{ sum[d], sum[d + 1], sum[d + 2], sum[d + 3] }; }
+            if (d0 == 0) { *p.row_stats(slot, kvh, a.n_kv, r, DIM) = make_float2(top, total); }
+        }
+        else
+        {
+            const float by = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (int d = 0; d < DIM / 16; d++) { sum[d] = total == 0.0f ? 0.0f : sum[d] * by; }
+            uint16_t* const dst = p.y + (size_t)(mine.first + r / p.group) * p.ldy + (size_t)(kvh * p.group + r % p.group) * DIM + d0;
+#pragma unroll
+            for (int d = 0; d < DIM / 16; d += 4) { *(u32x2*)(dst + d) = pack4(sum + d); }
+        }
+    }
+    __syncthreads();                                                        // the next sequence's rows come to the same LDS
+}
+
+// The c-th chunk of the keys of a kv head: the end of one sequence, whole ones, the beginning of another.
+template <int TYPE, int DIM>
+__device__ __forceinline__ void attend_chunk(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int c, int kvh)
+{
+    constexpr int KEYS = RowsForm<TYPE, DIM>::KEYS;
+    const bool alone = p.row_chunks == 0;                                   // the workgroup of sequence c
+    Shares<KEYS> all;
+    if (!alone) { all.take(a, p); }
+    const int begin = alone ? 0 : c * all.chunk, end = alone ? uniform(Shares<KEYS>::shares(a, p, c)) : min(begin + all.chunk, all.total);
+    for (int at = begin; at < end;)
     {
-        sum[d] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) { sum[d] += weight[w] > 0.0f || weight[w] != weight[w] ? weight[w] * sums[(w * 16 + r) * SUM + d0 + d] : 0.0f; }
+        int s = c, n = end, first = 0;                                      // the sequence, its shares and where they begin
+        if (!alone)
+        {
+            while (all.batch_end() <= at) { all.next_batch(a, p); }
+            const int of = __builtin_ctzll(__ballot(all.before + all.upto > at));
+            s = all.base + of;
+            n = __builtin_amdgcn_readlane(all.mine, of);
+            first = all.before + __builtin_amdgcn_readlane(all.upto, of) - n;
+        }
+        const int from = at - first, to = min(end - first, n);
+        attend_rows<TYPE, DIM>(a, p, lds, s, kvh, from, to, to - from == n ? -1 : 2 * c + (at > begin ? 1 : 0));
+        at = first + to;
     }
-    const size_t at_token = mine.first + r / p.group, at_head = kvh * p.group + r % p.group, at_row = at_token * p.n_q + at_head;
-    if (rows.n_ranges > 1)
-    {
-        float* const dst = p.sums(range, at_row, DIM) + d0;
-#pragma unroll
-        for (int d = 0; d < DIM / 16; d += 4) { *(f32x4*)(dst + d) = f32x4{ sum[d], sum[d + 1], sum[d + 2], sum[d + 3] }; }
-        if (d0 == 0) { *p.stats(range, at_row, DIM) = make_float2(top, total); }
-        return;
-    }
-    const float by = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-    for (int d = 0; d < DIM / 16; d++) { sum[d] = total == 0.0f ? 0.0f : sum[d] * by; }
-    uint16_t* const dst = p.y + at_token * p.ldy + at_head * DIM + d0;
-#pragma unroll
-    for (int d = 0; d < DIM / 16; d += 4) { *(u32x2*)(dst + d) = pack4(sum + d); }
 }
 
 // 128 RT rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions.
@@ -997,7 +1070,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     }
 }
 
-// Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then ranges x sequences x kv heads.
+// Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then chunks x kv heads.
 template <int TYPE, int DIM>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs a, const PagedAttention p)
 {
@@ -1007,27 +1080,24 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs
     static_assert(sizeof(lds) <= 80 * 1024, "two workgroups on a CU");
     const int tiles = p.tiles * a.n_kv, n_tiles = tiles * p.tile_split;
     if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM, 1>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
-    else
-    {
-        const int at = blockIdx.x - n_tiles, sequences = a.n_seqs * a.n_kv;
-        attend_rows<TYPE, DIM>(a, p, lds, at % sequences / a.n_kv, at % a.n_kv, at / sequences);
-    }
+    else { attend_chunk<TYPE, DIM>(a, p, lds, (blockIdx.x - n_tiles) / a.n_kv, (blockIdx.x - n_tiles) % a.n_kv); }
 }
 
-// Sums of the key ranges of 16 rows, DIM / 16 dims of a row per thread: rescaled to the largest maximum, added in the order of the ranges, divided by the
-// sum of the weights, one rounding.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads where tiles have ranges, then
-// sequences x kv heads where those do.
-template <int DIM, int KEYS, int RT>
+// Sums of the parts of 16 rows, DIM / 16 dims of a row per thread: rescaled to the largest maximum, added in order, divided by the sum of the weights,
+// one rounding.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads where tiles have ranges, then sequences x kv heads where
+// those are cut.
+template <int DIM, int KEYS>
 __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
 {
-    constexpr int PER = DIM / 16, PARTS = 8 * RT;
+    constexpr int PER = DIM / 16, PARTS = 8;
     const int n_tiles = p.tile_split > 1 ? p.tiles * PARTS * a.n_kv : 0, kvh = blockIdx.x % a.n_kv;
+    const bool tiled = (int)blockIdx.x < n_tiles;
     NewTokens mine;
-    int row, n;
-    if ((int)blockIdx.x < n_tiles)
+    int row, n, first = 0, first_slot = 0;
+    if (tiled)
     {
         const int at = blockIdx.x / a.n_kv;
-        const auto rows = tile_rows<128 * RT>(a, p, at / PARTS);
+        const auto rows = tile_rows<128>(a, p, at / PARTS);
         row = rows.row0 + at % PARTS * 16 + (threadIdx.x >> 4);
         if (rows.s < 0 || row >= rows.n_rows) { return; }
         mine = rows.mine;
@@ -1035,11 +1105,17 @@ __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const Page
     }
     else
     {
-        const auto rows = sequence_rows<KEYS>(a, p, (blockIdx.x - n_tiles) / a.n_kv);
+        const int s = (blockIdx.x - n_tiles) / a.n_kv;
+        Shares<KEYS> all;
+        all.take(a, p);
+        while (all.base + 64 <= s) { all.next_batch(a, p); }
+        const int shares = __builtin_amdgcn_readlane(all.mine, s & 63), begin = all.before + __builtin_amdgcn_readlane(all.upto, s & 63) - shares;
         row = threadIdx.x >> 4;
-        if (rows.s < 0 || row >= rows.n_rows) { return; }
-        mine = rows.mine;
-        n = rows.n_ranges;
+        mine = new_tokens(a, p, s);
+        if (shares == 0 || row >= mine.n * p.group) { return; }
+        first = begin / all.chunk;
+        first_slot = 2 * first + (begin > first * all.chunk ? 1 : 0);
+        n = (begin + shares - 1) / all.chunk - first + 1;
     }
     if (n <= 1) { return; }
     const size_t token = mine.first + row / p.group, head = kvh * p.group + row % p.group, at_row = token * p.n_q + head;
@@ -1048,15 +1124,16 @@ __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const Page
     float m = -INFINITY, l = 0.0f;
     for (int r0 = 0; r0 < n; r0 += 4)
     {
-        f32x4 part[4][PER / 4];                                             // four ranges requested at once
+        f32x4 part[4][PER / 4];                                             // four parts requested at once
         float2 stat[4];
 #pragma unroll
         for (int r = 0; r < 4; r++)
         {
-            const int range = min(r0 + r, n - 1);
-            stat[r] = *p.stats(range, at_row, DIM);
+            const int at = min(r0 + r, n - 1), slot = at == 0 ? first_slot : 2 * (first + at);
+            stat[r] = tiled ? *p.stats(at, at_row, DIM) : *p.row_stats(slot, kvh, a.n_kv, row, DIM);
+            const float* const from = (tiled ? p.sums(at, at_row, DIM) : p.row_sums(slot, kvh, a.n_kv, row, DIM)) + d0;
 #pragma unroll
-            for (int d = 0; d < PER / 4; d++) { part[r][d] = *(const f32x4*)(p.sums(range, at_row, DIM) + d0 + 4 * d); }
+            for (int d = 0; d < PER / 4; d++) { part[r][d] = *(const f32x4*)(from + 4 * d); }
         }
         float top = m;
 #pragma unroll
@@ -1070,7 +1147,7 @@ __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const Page
         for (int r = 0; r < 4; r++)
         {
             const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
-            if (r0 + r < n && w != 0.0f)                                    // a range without a key has weight 0
+            if (r0 + r < n && w != 0.0f)                                    // a part without a key has weight 0
             {
                 l += w * stat[r].y;
 #pragma unroll
