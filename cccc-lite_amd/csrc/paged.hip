@@ -3,6 +3,8 @@
 #include "paged_attention.h"
 #include "runtime.h"
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <cmath>
 
 using namespace ccq;
@@ -95,9 +97,18 @@ bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, in
         if ((long long)a.n_seqs * a.n_kv * 2 > MOST_BLOCKS || shares > 0x3FFFFFFFLL) { return false; }
         plan.row_chunks = (int)std::max<long long>(1, std::min<long long>(slots / a.n_kv, (long long)a.n_seqs * ((keys + 255) / 256 + 1)));
         if (getenv("PA_RS")) { plan.row_chunks = atoi(getenv("PA_RS")); }
-        plan.row_bytes = (size_t)plan.row_chunks * 2 * a.n_kv * PA_ROWS * (dim + 2) * 4;
+        plan.row_bytes = (size_t)plan.row_chunks * 2 * a.n_kv * (PA_ROWS * (dim + 2) * 4 + 8);
     }
     return true;
+}
+
+// A name for a call's counters that no other call has: what lies in a workspace before is not taken for counts of this one.
+unsigned long long name_call()
+{
+    static std::atomic<unsigned long long> next{ (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9E3779B97F4A7C15ull };
+    unsigned long long name;
+    do { name = next.fetch_add(0x9E3779B97F4A7C15ull) >> 16; } while (name == 0);
+    return name;
 }
 }    // namespace
 
@@ -167,16 +178,19 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
         if (workspace_bytes < plan.row_bytes) { plan.row_chunks = 0; }
     }
     const long long tiles = (long long)plan.tiles * a.n_kv * plan.tile_split, chunks = plan.rows ? (long long)(plan.row_chunks ? plan.row_chunks : a.n_seqs) * a.n_kv : 0;
-    const long long sums = (plan.tile_split > 1 ? (long long)plan.tiles * a.n_kv * 8 : 0) + (plan.row_chunks > 0 ? (long long)a.n_seqs * a.n_kv : 0);
-    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)workspace, (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv, n_tokens, max_new, window, n_sink, plan.tile_split,
-                               plan.tiles, plan.tile_split, plan.row_chunks, (float*)((char*)workspace + plan.tile_bytes), plan.min_rows, getenv("PA_SNAKE") ? 1 : 0,
-                               1.4426950408889634f / sqrtf((float)dim) };
+    // the workspace: chunks' words, sums and statistics, then the tiles'
+    const size_t words = (size_t)plan.row_chunks * 2 * a.n_kv;
+    char* const chunk_sums = (char*)workspace + words * 8;
+    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)((char*)workspace + (plan.row_chunks ? plan.row_bytes : 0)), (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv,
+                               n_tokens, max_new, window, n_sink, plan.tile_split, plan.tiles, plan.tile_split, plan.row_chunks, (float*)chunk_sums, (unsigned long long*)workspace,
+                               plan.row_chunks ? name_call() : 0, plan.min_rows, 1, 1.4426950408889634f / sqrtf((float)dim) };
     const auto kernel = CCQ_PAGED_KERNEL(paged_attention_kernel, cache);
     kernel<<<(unsigned)(tiles + chunks), 256, 0, stream()>>>(a, p);
-    if (sums > 0)
+    if (plan.tile_split > 1)
     {
-        const auto combine = dim == 64 ? paged_attention_combine_kernel<64, 64> : keys_per_block(cache) == 32 ? paged_attention_combine_kernel<128, 32> : paged_attention_combine_kernel<128, 64>;
-        combine<<<(unsigned)sums, 256, 0, stream()>>>(a, p);
+        const unsigned blocks = (unsigned)(plan.tiles * a.n_kv * 8);
+        if (dim == 64) { paged_attention_combine_kernel<64><<<blocks, 256, 0, stream()>>>(a, p); }
+        else { paged_attention_combine_kernel<128><<<blocks, 256, 0, stream()>>>(a, p); }
     }
     return finish("attention_paged");
 }

@@ -20,14 +20,16 @@ struct PagedAttention
     int tiles, tile_split;          // tiles of 128 rows (at most) and the most ranges of each
     int row_chunks;                 // workgroups per kv head that share the keys of all sequences of at most 16 rows per kv head; 0: one for each of those
     float* row_partial;             // [chunk][2][kv head][16][dim] sums, then (max, sum) likewise
+    unsigned long long* there;      // [chunk][2][kv head]: whose part is there
+    unsigned long long call;        // of this call alone, 48 bits
     int min_rows;                   // sequences of at most so many rows per kv head are not cut into tiles
     int snake;
     float scale;                    // log2 e / sqrt(dim)
 
     __device__ __forceinline__ float* row_sums(int slot, int kvh, int n_kv, int row, int dim) const { return row_partial + (((size_t)slot * n_kv + kvh) * 16 + row) * dim; }
-    __device__ __forceinline__ float2* row_stats(int slot, int kvh, int n_kv, int row, int dim) const
+    __device__ __forceinline__ float* row_stats(int slot, int kvh, int n_kv, int row, int dim) const
     {
-        return (float2*)(row_partial + (size_t)row_chunks * 2 * n_kv * 16 * dim) + ((size_t)slot * n_kv + kvh) * 16 + row;
+        return row_partial + (size_t)row_chunks * 2 * n_kv * 16 * dim + (((size_t)slot * n_kv + kvh) * 16 + row) * 2;
     }
     __device__ __forceinline__ size_t outputs() const { return (size_t)n_tokens * n_q; }
     __device__ __forceinline__ float* sums(int range, size_t row, int dim) const { return partial + ((size_t)range * outputs() + row) * dim; }
@@ -99,7 +101,7 @@ constexpr int PA_ROWS = 16, PA_TILE_KEYS = 64;
 template <int KEYS>
 struct Shares
 {
-    int total = 0, chunk = 1;                                               // shares of all, and of a chunk
+    int total = 0, chunk = 0x7FFFFFFF;                                               // shares of all, and of a chunk
     int mine = 0, upto = 0, base = 0, before = 0;                           // of sequence base + lane; with those before it in the batch; of earlier batches
 
     __device__ __forceinline__ static KeyBlocks<KEYS> keys(const PagedAttention& p, const NewTokens& n) { return KeyBlocks<KEYS>(p, n.pos, n.pos + n.n - 1); }
@@ -265,6 +267,85 @@ __device__ __forceinline__ uint32_t codes_not_finite(uint32_t w)
     else { return (w & 0x7C7C7C7Cu) + 0x04040404u & 0x80808080u; }
 }
 
+// Parts pass between workgroups of different XCDs, whose L2s do not know of each other: they are written through and read past them by relaxed atomics of the
+// device's scope.  (Plain stores between fences, which write back and drop a whole L2, cost 15 us and more a call.)
+__device__ __forceinline__ void store_part(float* to, float x, float y)
+{
+    __hip_atomic_store((unsigned long long*)to, (unsigned long long)f32_to_bits(y) << 32 | f32_to_bits(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_part(const float* from)
+{
+    const unsigned long long v = __hip_atomic_load((const unsigned long long*)from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(bits_to_f32((uint32_t)v), bits_to_f32((uint32_t)(v >> 32)));
+}
+
+// Whether the n parts that belong together are all there, this workgroup's own, just stored, among them.  A part is there when its word holds the name of this
+// call, whatever lay there before; flag(i) is the i-th one's word, `own` this workgroup's.  Each workgroup sets its word and then looks at all of them, so at least the
+// last one finds them set; where several do, all write the same result.  (A counter instead, with a compare and swap per workgroup, took 0.8 us for each.)
+template <class Flag>
+__device__ __forceinline__ bool all_there(unsigned long long* own, unsigned long long call, int n, uint32_t* lds_result, Flag flag)
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                        // the wave's stores are there
+    __syncthreads();
+    if (threadIdx.x < 64)
+    {
+        if (threadIdx.x == 0) { __hip_atomic_store(own, call, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        bool all = true;
+        for (int i = threadIdx.x; i < n; i += 64) { all = all && __hip_atomic_load(flag(i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == call; }
+        all = __all(all);
+        if (threadIdx.x == 0) { *lds_result = all; }
+    }
+    __syncthreads();
+    return *lds_result != 0;
+}
+
+// DIM / 16 dims of a row from its n parts: rescaled to the largest maximum, added in order, divided by the sum of the weights, one rounding.
+// part(i, sums, stat) tells where the i-th one's sums and (max, sum) are.  PLAIN: parts of an earlier launch.
+template <int DIM, bool PLAIN = false, class Part>
+__device__ __forceinline__ void add_parts(int n, uint16_t* y, Part part)
+{
+    constexpr int PER = DIM / 16;
+    float sum[PER] = {};
+    float m = -INFINITY, l = 0.0f;
+    for (int r0 = 0; r0 < n; r0 += 4)
+    {
+        float2 v[4][PER / 2], stat[4];                                      // four parts requested at once
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+        {
+            const float *from, *at;
+            part(min(r0 + r, n - 1), from, at);
+            stat[r] = PLAIN ? *(const float2*)at : load_part(at);
+#pragma unroll
+            for (int d = 0; d < PER / 2; d++) { v[r][d] = PLAIN ? *(const float2*)(from + 2 * d) : load_part(from + 2 * d); }
+        }
+        float top = m;
+#pragma unroll
+        for (int r = 0; r < 4; r++) { top = fmaxf(top, stat[r].x); }
+        const float base = top > -INFINITY ? top : 0.0f, shrink = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        l *= shrink;
+#pragma unroll
+        for (int d = 0; d < PER; d++) { sum[d] *= shrink; }
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+        {
+            const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
+            if (r0 + r < n && w != 0.0f)                                    // a part without a key has weight 0
+            {
+                l += w * stat[r].y;
+#pragma unroll
+                for (int d = 0; d < PER; d++) { sum[d] += w * (d % 2 ? v[r][d / 2].y : v[r][d / 2].x); }
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < PER; d++) { sum[d] = l == 0.0f ? 0.0f : sum[d] / l; }
+#pragma unroll
+    for (int d = 0; d < PER; d += 4) { *(u32x2*)(y + d) = pack4(sum + d); }
+}
+
 // Up to 16 rows of a kv head: single tokens, or a few.  Bound by the cached rows' way from memory.
 //   A workgroup of four waves takes a range of the sequence's blocks of KEYS keys, a wave every fourth block, each with a pipeline of its own: rows go by
 // direct loads to the wave's part of LDS, keys and values STAGES blocks ahead each, and nothing but the wave's own count of loads in flight is waited for.
@@ -283,7 +364,7 @@ struct RowsForm
 };
 
 template <int TYPE, int DIM>
-__device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int s, int kvh, int from_share, int to_share, int slot)
+__device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int s, int kvh, int from_share, int to_share, int slot, int first_chunk, int first_slot, int n_parts)
 {
     typedef RowsForm<TYPE, DIM> F;
     constexpr int KEYS = F::KEYS, STAGES = F::STAGES, ROW = F::ROW, SIDE = F::SIDE, SUM = F::SUM, CHUNKS = ROW / 16;
@@ -581,8 +662,8 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         {
             float* const dst = p.row_sums(slot, kvh, a.n_kv, r, DIM) + d0;
 #pragma unroll
-            for (int d = 0; d < DIM / 16; d += 4) { *(f32x4*)(dst + d) = f32x4{ sum[d], sum[d + 1], sum[d + 2], sum[d + 3] }; }
-            if (d0 == 0) { *p.row_stats(slot, kvh, a.n_kv, r, DIM) = make_float2(top, total); }
+            for (int d = 0; d < DIM / 16; d += 2) { store_part(dst + d, sum[d], sum[d + 1]); }
+            if (d0 == 0) { store_part(p.row_stats(slot, kvh, a.n_kv, r, DIM), top, total); }
         }
         else
         {
@@ -592,6 +673,23 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
             uint16_t* const dst = p.y + (size_t)(mine.first + r / p.group) * p.ldy + (size_t)(kvh * p.group + r % p.group) * DIM + d0;
 #pragma unroll
             for (int d = 0; d < DIM / 16; d += 4) { *(u32x2*)(dst + d) = pack4(sum + d); }
+        }
+    }
+    if (slot >= 0)
+    {
+        auto slot_of = [&](int i) { return i == 0 ? first_slot : 2 * (first_chunk + i); };
+        auto flag = [&](int i) { return p.there + (size_t)slot_of(i) * a.n_kv + kvh; };
+        if (all_there(p.there + (size_t)slot * a.n_kv + kvh, p.call, n_parts, (uint32_t*)stat, flag))
+        {
+            if (r < n_rows)
+            {
+                add_parts<DIM>(n_parts, p.y + (size_t)(mine.first + r / p.group) * p.ldy + (size_t)(kvh * p.group + r % p.group) * DIM + d0, [&](int i, const float*& from, const float*& at) {
+                    from = p.row_sums(slot_of(i), kvh, a.n_kv, r, DIM) + d0;
+                    at = p.row_stats(slot_of(i), kvh, a.n_kv, r, DIM);
+                });
+            }
+            // a captured call may be replayed under its name
+            for (int i = threadIdx.x; i < n_parts; i += 256) { __hip_atomic_store(flag(i), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
         }
     }
     __syncthreads();                                                        // the next sequence's rows come to the same LDS
@@ -618,7 +716,8 @@ __device__ __forceinline__ void attend_chunk(const PagedArgs& a, const PagedAtte
             first = all.before + __builtin_amdgcn_readlane(all.upto, of) - n;
         }
         const int from = at - first, to = min(end - first, n);
-        attend_rows<TYPE, DIM>(a, p, lds, s, kvh, from, to, to - from == n ? -1 : 2 * c + (at > begin ? 1 : 0));
+        const int first_chunk = first / all.chunk, n_parts = (first + n - 1) / all.chunk - first_chunk + 1;
+        attend_rows<TYPE, DIM>(a, p, lds, s, kvh, from, to, to - from == n ? -1 : 2 * c + (at > begin ? 1 : 0), first_chunk, 2 * first_chunk + (first > first_chunk * all.chunk ? 1 : 0), n_parts);
         at = first + to;
     }
 }
@@ -1083,87 +1182,20 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs
     else { attend_chunk<TYPE, DIM>(a, p, lds, (blockIdx.x - n_tiles) / a.n_kv, (blockIdx.x - n_tiles) % a.n_kv); }
 }
 
-// Sums of the parts of 16 rows, DIM / 16 dims of a row per thread: rescaled to the largest maximum, added in order, divided by the sum of the weights,
-// one rounding.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads where tiles have ranges, then sequences x kv heads where
-// those are cut.
-template <int DIM, int KEYS>
+// The tiles' ranges added, 16 rows per workgroup and DIM / 16 dims of a row per thread.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads.
+template <int DIM>
 __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
 {
-    constexpr int PER = DIM / 16, PARTS = 8;
-    const int n_tiles = p.tile_split > 1 ? p.tiles * PARTS * a.n_kv : 0, kvh = blockIdx.x % a.n_kv;
-    const bool tiled = (int)blockIdx.x < n_tiles;
-    NewTokens mine;
-    int row, n, first = 0, first_slot = 0;
-    if (tiled)
-    {
-        const int at = blockIdx.x / a.n_kv;
-        const auto rows = tile_rows<128>(a, p, at / PARTS);
-        row = rows.row0 + at % PARTS * 16 + (threadIdx.x >> 4);
-        if (rows.s < 0 || row >= rows.n_rows) { return; }
-        mine = rows.mine;
-        n = rows.n_ranges;
-    }
-    else
-    {
-        const int s = (blockIdx.x - n_tiles) / a.n_kv;
-        Shares<KEYS> all;
-        all.take(a, p);
-        while (all.base + 64 <= s) { all.next_batch(a, p); }
-        const int shares = __builtin_amdgcn_readlane(all.mine, s & 63), begin = all.before + __builtin_amdgcn_readlane(all.upto, s & 63) - shares;
-        row = threadIdx.x >> 4;
-        mine = new_tokens(a, p, s);
-        if (shares == 0 || row >= mine.n * p.group) { return; }
-        first = begin / all.chunk;
-        first_slot = 2 * first + (begin > first * all.chunk ? 1 : 0);
-        n = (begin + shares - 1) / all.chunk - first + 1;
-    }
-    if (n <= 1) { return; }
-    const size_t token = mine.first + row / p.group, head = kvh * p.group + row % p.group, at_row = token * p.n_q + head;
-    const int d0 = (threadIdx.x & 15) * PER;
-    f32x4 sum[PER / 4] = {};
-    float m = -INFINITY, l = 0.0f;
-    for (int r0 = 0; r0 < n; r0 += 4)
-    {
-        f32x4 part[4][PER / 4];                                             // four parts requested at once
-        float2 stat[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-        {
-            const int at = min(r0 + r, n - 1), slot = at == 0 ? first_slot : 2 * (first + at);
-            stat[r] = tiled ? *p.stats(at, at_row, DIM) : *p.row_stats(slot, kvh, a.n_kv, row, DIM);
-            const float* const from = (tiled ? p.sums(at, at_row, DIM) : p.row_sums(slot, kvh, a.n_kv, row, DIM)) + d0;
-#pragma unroll
-            for (int d = 0; d < PER / 4; d++) { part[r][d] = *(const f32x4*)(from + 4 * d); }
-        }
-        float top = m;
-#pragma unroll
-        for (int r = 0; r < 4; r++) { top = fmaxf(top, stat[r].x); }
-        const float base = top > -INFINITY ? top : 0.0f, shrink = __builtin_amdgcn_exp2f(m - base);
-        m = top;
-        l *= shrink;
-#pragma unroll
-        for (int d = 0; d < PER / 4; d++) { sum[d] *= shrink; }
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-        {
-            const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
-            if (r0 + r < n && w != 0.0f)                                    // a part without a key has weight 0
-            {
-                l += w * stat[r].y;
-#pragma unroll
-                for (int d = 0; d < PER / 4; d++) { sum[d] += w * part[r][d]; }
-            }
-        }
-    }
-    uint16_t* const dst = p.y + token * p.ldy + head * DIM + d0;
-#pragma unroll
-    for (int d = 0; d < PER / 4; d++)
-    {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) { v[e] = l == 0.0f ? 0.0f : sum[d][e] / l; }
-        *(u32x2*)(dst + 4 * d) = pack4(v);
-    }
+    const int kvh = blockIdx.x % a.n_kv, at = blockIdx.x / a.n_kv;
+    const auto rows = tile_rows<128>(a, p, at / 8);
+    const int row = rows.row0 + at % 8 * 16 + (threadIdx.x >> 4);
+    if (rows.s < 0 || row >= rows.n_rows || rows.n_ranges <= 1) { return; }
+    const size_t token = rows.mine.first + row / p.group, head = kvh * p.group + row % p.group, at_row = token * p.n_q + head;
+    const int d0 = (threadIdx.x & 15) * (DIM / 16);
+    add_parts<DIM, true>(rows.n_ranges, p.y + token * p.ldy + head * DIM + d0, [&](int i, const float*& from, const float*& stat) {
+        from = p.sums(i, at_row, DIM) + d0;
+        stat = (const float*)p.stats(i, at_row, DIM);
+    });
 }
 
 }    // namespace ccq
