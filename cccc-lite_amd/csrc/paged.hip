@@ -66,7 +66,7 @@ struct Plan
 {
     int tiles, tile_split;          // at most
     bool rows;
-    int min_rows, row_chunks;
+    int min_rows, row_slots, row_parts;
     size_t tile_bytes, row_bytes;   // of partial sums
 };
 
@@ -77,7 +77,7 @@ bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, in
     const long long rows = (long long)n_tokens * group, slots = 2LL * cu_count();
     // Sequences of up to 16 rows per kv head have a form of their own, also beside longer ones -- unless every sequence has max_new tokens, as far as
     // their number tells.
-    plan = { 0, 1, true, 0, 0, 0, 0 };
+    plan = { 0, 1, true, 0, 0, 0, 0, 0 };
     const long long keys = window == 0 ? a.max_ctx : std::min<long long>(a.max_ctx, (long long)window + n_sink + max_new);
     if ((long long)std::min(max_new, n_tokens) * group > PA_ROWS)
     {
@@ -93,11 +93,13 @@ bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, in
     }
     if (plan.rows)
     {
-        const long long shares = (long long)a.n_seqs * ((a.max_ctx + 4LL * keys_per_block) / (4 * keys_per_block) + 1);
-        if ((long long)a.n_seqs * a.n_kv * 2 > MOST_BLOCKS || shares > 0x3FFFFFFFLL) { return false; }
-        plan.row_chunks = (int)std::max<long long>(1, std::min<long long>(slots / a.n_kv, (long long)a.n_seqs * ((keys + 255) / 256 + 1)));
-        if (getenv("PA_RS")) { plan.row_chunks = atoi(getenv("PA_RS")); }
-        plan.row_bytes = (size_t)plan.row_chunks * 2 * a.n_kv * (PA_ROWS * (dim + 2) * 4 + 8);
+        // shares of four blocks (Parts): of a sequence at most, with a block at either end and one more for the first keys in part; all fit 32 bits
+        const long long shares = (keys / keys_per_block + 3 + 3) / 4 + 1, all = shares * a.n_seqs, part = keys_per_block == 32 ? 2 : 1;
+        const long long at_once = std::max<long long>(1, slots / a.n_kv);
+        if (all > 0x3FFFFFFFLL || (a.n_seqs + 3 * at_once + 1) * a.n_kv * 2 > MOST_BLOCKS) { return false; }
+        plan.row_slots = (int)at_once;
+        plan.row_parts = (int)(a.n_seqs + std::max<long long>(1, std::min(3 * at_once, all / part)));
+        plan.row_bytes = (size_t)plan.row_parts * a.n_kv * (PA_ROWS * (dim + 2) * 4 + 8);
     }
     return true;
 }
@@ -175,17 +177,17 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
     {
         plan.tile_split = 1;
         plan.tile_bytes = 0;
-        if (workspace_bytes < plan.row_bytes) { plan.row_chunks = 0; }
+        if (workspace_bytes < plan.row_bytes) { plan.row_parts = 0; }
     }
-    const long long tiles = (long long)plan.tiles * a.n_kv * plan.tile_split, chunks = plan.rows ? (long long)(plan.row_chunks ? plan.row_chunks : a.n_seqs) * a.n_kv : 0;
-    // the workspace: chunks' words, sums and statistics, then the tiles'
-    const size_t words = (size_t)plan.row_chunks * 2 * a.n_kv;
-    char* const chunk_sums = (char*)workspace + words * 8;
-    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)((char*)workspace + (plan.row_chunks ? plan.row_bytes : 0)), (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv,
-                               n_tokens, max_new, window, n_sink, plan.tile_split, plan.tiles, plan.tile_split, plan.row_chunks, (float*)chunk_sums, (unsigned long long*)workspace,
-                               plan.row_chunks ? name_call() : 0, plan.min_rows, 1, 1.4426950408889634f / sqrtf((float)dim) };
+    const long long tiles = (long long)plan.tiles * a.n_kv * plan.tile_split, parts = plan.rows ? (long long)(plan.row_parts ? plan.row_parts : a.n_seqs) * a.n_kv : 0;
+    // the workspace: the parts' words, sums and statistics, then the tiles'
+    const size_t words = (size_t)plan.row_parts * a.n_kv;
+    char* const part_sums = (char*)workspace + words * 8;
+    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)((char*)workspace + (plan.row_parts ? plan.row_bytes : 0)), (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv,
+                               n_tokens, max_new, window, n_sink, plan.tile_split, plan.tiles, plan.tile_split, plan.row_slots, plan.row_parts, (float*)part_sums, (unsigned long long*)workspace,
+                               plan.row_parts ? name_call() : 0, plan.min_rows, 1, 1.4426950408889634f / sqrtf((float)dim) };
     const auto kernel = CCQ_PAGED_KERNEL(paged_attention_kernel, cache);
-    kernel<<<(unsigned)(tiles + chunks), 256, 0, stream()>>>(a, p);
+    kernel<<<(unsigned)(tiles + parts), 256, 0, stream()>>>(a, p);
     if (plan.tile_split > 1)
     {
         const unsigned blocks = (unsigned)(plan.tiles * a.n_kv * 8);

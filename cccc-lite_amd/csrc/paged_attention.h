@@ -18,9 +18,10 @@ struct PagedAttention
     int n_q, group, n_tokens, max_new, window, n_sink;
     int n_split;                    // ranges of keys that `partial` is laid out for
     int tiles, tile_split;          // tiles of 128 rows (at most) and the most ranges of each
-    int row_chunks;                 // workgroups per kv head that share the keys of all sequences of at most 16 rows per kv head; 0: one for each of those
-    float* row_partial;             // [chunk][2][kv head][16][dim] sums, then (max, sum) likewise
-    unsigned long long* there;      // [chunk][2][kv head]: whose part is there
+    int row_slots;                  // workgroups per kv head that the GPU runs at once
+    int row_parts;                  // workgroups per kv head for the parts of all sequences of at most 16 rows per kv head; 0: one for each sequence
+    float* row_partial;             // [part][kv head][16][dim] sums, then (max, sum) likewise
+    unsigned long long* there;      // [part][kv head]: the name of the call whose part is there
     unsigned long long call;        // of this call alone, 48 bits
     int min_rows;                   // sequences of at most so many rows per kv head are not cut into tiles
     int snake;
@@ -29,7 +30,7 @@ struct PagedAttention
     __device__ __forceinline__ float* row_sums(int slot, int kvh, int n_kv, int row, int dim) const { return row_partial + (((size_t)slot * n_kv + kvh) * 16 + row) * dim; }
     __device__ __forceinline__ float* row_stats(int slot, int kvh, int n_kv, int row, int dim) const
     {
-        return row_partial + (size_t)row_chunks * 2 * n_kv * 16 * dim + (((size_t)slot * n_kv + kvh) * 16 + row) * 2;
+        return row_partial + (size_t)row_parts * n_kv * 16 * dim + (((size_t)slot * n_kv + kvh) * 16 + row) * 2;
     }
     __device__ __forceinline__ size_t outputs() const { return (size_t)n_tokens * n_q; }
     __device__ __forceinline__ float* sums(int range, size_t row, int dim) const { return partial + ((size_t)range * outputs() + row) * dim; }
@@ -38,6 +39,17 @@ struct PagedAttention
 
 // a value that all lanes have, in a scalar register
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// the sum of a value over the lanes up to this one
+__device__ __forceinline__ int add_up_lanes(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);         // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);         // row_bcast 15 to rows 1 and 3
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // row_bcast 31 to rows 2 and 3
+}
 
 // The new tokens of a sequence that a call computes: tokens first .. first + n - 1 of the activations, the first of them at position pos.
 struct NewTokens
@@ -96,55 +108,60 @@ struct Rows
 
 constexpr int PA_ROWS = 16, PA_TILE_KEYS = 64;
 
-// Sequences of up to 16 rows per kv head: their keys laid end to end in shares of four blocks (a block per wave), cut into chunks of equal length, a
-// workgroup each.  Lengths that differ leave no workgroup with more than another, and a sequence is cut where chunks end and nowhere else.
+// Sequences of up to 16 rows per kv head: the keys of each in shares of four blocks (a block per wave), cut into parts of about the same number of shares, a
+// workgroup each.  How many shares a part has follows from those of all sequences, so that long and short ones leave no workgroup with much more than
+// another: about two workgroups' worth of an even split, since a part costs some 5 us besides its keys, but not over PA_PART, which evens out what is
+// left over at the end.  (MI355X, 32 / 8 heads, E4M3, parts of a sequence: 64 sequences of 1000 to 8000 keys 1 113 us, 3 111, 6 123; 16 of 4100 keys 1 35, 2 31,
+// 4 32; 8 of 4000 keys 1 32, 2 24, 4 20.3, 8 20.5.)
+constexpr int PA_PART = 9;
 template <int KEYS>
-struct Shares
+struct Parts
 {
-    int total = 0, chunk = 0x7FFFFFFF;                                               // shares of all, and of a chunk
-    int mine = 0, upto = 0, base = 0, before = 0;                           // of sequence base + lane; with those before it in the batch; of earlier batches
+    int per = 1;                                                            // shares of a part
+    int base = 0, before = 0;                                               // the batch of sequences base + lane, and parts of those before it
+    int shares = 0, parts = 0, upto = 0;                                    // of the lane's sequence, and parts with those before it in the batch
+    NewTokens mine = { 0, 0, 0 };                                           // the lane's
 
     __device__ __forceinline__ static KeyBlocks<KEYS> keys(const PagedAttention& p, const NewTokens& n) { return KeyBlocks<KEYS>(p, n.pos, n.pos + n.n - 1); }
-    __device__ __forceinline__ static int shares(const PagedArgs& a, const PagedAttention& p, int s)
+    __device__ __forceinline__ static int shares_of(const PagedAttention& p, const NewTokens& n)
     {
-        if (s >= a.n_seqs) { return 0; }
-        const NewTokens n = new_tokens(a, p, s);
         const int rows = n.n * p.group;
         return rows == 0 || rows > PA_ROWS ? 0 : max((keys(p, n).n + 3) / 4, 1);
     }
-    // whole waves
+    __device__ __forceinline__ int batch_end() const { return before + __builtin_amdgcn_readlane(upto, 63); }
+    // whole waves from here on
+    __device__ __forceinline__ void load(const PagedArgs& a, const PagedAttention& p)
+    {
+        const int s = base + (int)(threadIdx.x & 63);
+        mine = s < a.n_seqs ? new_tokens(a, p, s) : NewTokens{ 0, 0, 0 };
+        shares = shares_of(p, mine);
+    }
+    __device__ __forceinline__ void cut()
+    {
+        parts = (shares + per - 1) / per;
+        upto = add_up_lanes(parts);
+    }
     __device__ __forceinline__ void take(const PagedArgs& a, const PagedAttention& p)
     {
-        const int lane = threadIdx.x & 63;
-        for (int b = 0; b < a.n_seqs; b += 64)
+        int total = 0;
+        for (base = 0; base < a.n_seqs; base += 64)
         {
-            int v = shares(a, p, b + lane);
-            if (b == 0) { mine = v; }
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) { v += __shfl_xor(v, o); }
-            total += uniform(v);
+            load(a, p);
+            total += __builtin_amdgcn_readlane(add_up_lanes(shares), 63);
         }
-        chunk = max((total + p.row_chunks - 1) / p.row_chunks, KEYS == 32 ? 2 : 1);
-        add_up();
+        auto split = [&](int n) { return (total + n - 1) / n; };
+        per = max(max(split(3 * p.row_slots), min(PA_PART, split((p.row_slots + 1) / 2))), KEYS == 32 ? 2 : 1);
+        per = max(per, split(max(p.row_parts - a.n_seqs, 1)));              // no more parts than workgroups
+        base = 0;
+        if (a.n_seqs > 64) { load(a, p); }
+        cut();
     }
-    __device__ __forceinline__ void add_up()
-    {
-        const int lane = threadIdx.x & 63;
-        upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1)
-        {
-            const int below = __shfl_up(upto, o);
-            upto += lane >= o ? below : 0;
-        }
-    }
-    __device__ __forceinline__ int batch_end() const { return before + __builtin_amdgcn_readlane(upto, 63); }
-    __device__ __forceinline__ void next_batch(const PagedArgs& a, const PagedAttention& p)
+    __device__ __forceinline__ void next(const PagedArgs& a, const PagedAttention& p)
     {
         before = batch_end();
         base += 64;
-        mine = shares(a, p, base + (int)(threadIdx.x & 63));
-        add_up();
+        load(a, p);
+        cut();
     }
 };
 
@@ -158,25 +175,15 @@ __device__ __forceinline__ Rows<PA_TILE_KEYS, TILE> tile_rows(const PagedArgs& a
     if (p.snake && tile >= (p.tiles + 1) / 2) { tile = p.tiles - 1 - (tile - (p.tiles + 1) / 2); }
     for (int base = 0; base < a.n_seqs; base += 64)
     {
-        int tiles = 0;
-        if (base + lane < a.n_seqs)
-        {
-            const int rows = new_tokens(a, p, base + lane).n * p.group;
-            tiles = rows > p.min_rows ? (rows + TILE - 1) / TILE : 0;
-        }
-        int upto = tiles;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1)
-        {
-            const int below = __shfl_up(upto, o);
-            upto += lane >= o ? below : 0;
-        }
+        const NewTokens mine = base + lane < a.n_seqs ? new_tokens(a, p, base + lane) : NewTokens{ 0, 0, 0 };
+        const int rows = mine.n * p.group, tiles = rows > p.min_rows ? (rows + TILE - 1) / TILE : 0;
+        const int upto = add_up_lanes(tiles);
         const unsigned long long past = __ballot(upto > tile);
         if (past != 0)
         {
             const int at = __builtin_ctzll(past);
             r.s = __builtin_amdgcn_readfirstlane(base + at);
-            r.mine = new_tokens(a, p, r.s);
+            r.mine = { __builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.n, at), __builtin_amdgcn_readlane(mine.pos, at) };
             r.row0 = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(upto, at) - 1 - tile) * TILE;
             r.n_rows = uniform(r.mine.n * p.group);
             r.cut(p, p.tile_split, 1, 4);
@@ -364,7 +371,7 @@ struct RowsForm
 };
 
 template <int TYPE, int DIM>
-__device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int s, int kvh, int from_share, int to_share, int slot, int first_chunk, int first_slot, int n_parts)
+__device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int s, const NewTokens& mine, int kvh, int from_share, int to_share, int slot, int part, int n_parts)
 {
     typedef RowsForm<TYPE, DIM> F;
     constexpr int KEYS = F::KEYS, STAGES = F::STAGES, ROW = F::ROW, SIDE = F::SIDE, SUM = F::SUM, CHUNKS = ROW / 16;
@@ -372,8 +379,7 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
     float2* const stat = (float2*)(lds + F::STAT);                          // [wave][row] (max, sum)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 15, g = lane >> 4;
-    const NewTokens mine = new_tokens(a, p, s);
-    const auto blocks = Shares<KEYS>::keys(p, mine);
+    const auto blocks = Parts<KEYS>::keys(p, mine);
     const int n_rows = uniform(mine.n * p.group), lo = uniform(mine.pos), hi = uniform(mine.pos + mine.n - 1);
     const int begin = from_share * 4, end = uniform(min(blocks.n, to_share * 4));
 
@@ -658,7 +664,7 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
 #pragma unroll
             for (int w = 0; w < 4; w++) { sum[d] += weight[w] != 0.0f ? weight[w] * sums[(w * 16 + r) * SUM + d0 + d] : 0.0f; }
         }
-        if (slot >= 0)
+        if (n_parts > 1)
         {
             float* const dst = p.row_sums(slot, kvh, a.n_kv, r, DIM) + d0;
 #pragma unroll
@@ -675,9 +681,9 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
             for (int d = 0; d < DIM / 16; d += 4) { *(u32x2*)(dst + d) = pack4(sum + d); }
         }
     }
-    if (slot >= 0)
+    if (n_parts > 1)
     {
-        auto slot_of = [&](int i) { return i == 0 ? first_slot : 2 * (first_chunk + i); };
+        auto slot_of = [&](int i) { return slot - part + i; };
         auto flag = [&](int i) { return p.there + (size_t)slot_of(i) * a.n_kv + kvh; };
         if (all_there(p.there + (size_t)slot * a.n_kv + kvh, p.call, n_parts, (uint32_t*)stat, flag))
         {
@@ -692,34 +698,37 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
             for (int i = threadIdx.x; i < n_parts; i += 256) { __hip_atomic_store(flag(i), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
         }
     }
-    __syncthreads();                                                        // the next sequence's rows come to the same LDS
 }
 
-// The c-th chunk of the keys of a kv head: the end of one sequence, whole ones, the beginning of another.
+// Part c of a kv head's, or with row_parts 0 all of sequence c.
 template <int TYPE, int DIM>
-__device__ __forceinline__ void attend_chunk(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int c, int kvh)
+__device__ __forceinline__ void attend_part(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int c, int kvh)
 {
     constexpr int KEYS = RowsForm<TYPE, DIM>::KEYS;
-    const bool alone = p.row_chunks == 0;                                   // the workgroup of sequence c
-    Shares<KEYS> all;
-    if (!alone) { all.take(a, p); }
-    const int begin = alone ? 0 : c * all.chunk, end = alone ? uniform(Shares<KEYS>::shares(a, p, c)) : min(begin + all.chunk, all.total);
-    for (int at = begin; at < end;)
+    int s = c, part = 0, parts = 1, shares;
+    NewTokens mine;
+    if (p.row_parts == 0)
     {
-        int s = c, n = end, first = 0;                                      // the sequence, its shares and where they begin
-        if (!alone)
-        {
-            while (all.batch_end() <= at) { all.next_batch(a, p); }
-            const int of = __builtin_ctzll(__ballot(all.before + all.upto > at));
-            s = all.base + of;
-            n = __builtin_amdgcn_readlane(all.mine, of);
-            first = all.before + __builtin_amdgcn_readlane(all.upto, of) - n;
-        }
-        const int from = at - first, to = min(end - first, n);
-        const int first_chunk = first / all.chunk, n_parts = (first + n - 1) / all.chunk - first_chunk + 1;
-        attend_rows<TYPE, DIM>(a, p, lds, s, kvh, from, to, to - from == n ? -1 : 2 * c + (at > begin ? 1 : 0), first_chunk, 2 * first_chunk + (first > first_chunk * all.chunk ? 1 : 0), n_parts);
-        at = first + to;
+        mine = new_tokens(a, p, c);
+        shares = uniform(Parts<KEYS>::shares_of(p, mine));
     }
+    else
+    {
+        Parts<KEYS> all;
+        all.take(a, p);
+        while (all.batch_end() <= c)
+        {
+            if (all.base + 64 >= a.n_seqs) { return; }
+            all.next(a, p);
+        }
+        const int of = __builtin_ctzll(__ballot(all.before + all.upto > c));
+        s = all.base + of;
+        parts = __builtin_amdgcn_readlane(all.parts, of);
+        part = c - (all.before + __builtin_amdgcn_readlane(all.upto, of) - parts);
+        shares = __builtin_amdgcn_readlane(all.shares, of);
+        mine = { __builtin_amdgcn_readlane(all.mine.first, of), __builtin_amdgcn_readlane(all.mine.n, of), __builtin_amdgcn_readlane(all.mine.pos, of) };
+    }
+    if (shares > 0) { attend_rows<TYPE, DIM>(a, p, lds, s, mine, kvh, (int)((long long)shares * part / parts), (int)((long long)shares * (part + 1) / parts), c, part, parts); }
 }
 
 // 128 RT rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions.
@@ -1169,7 +1178,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     }
 }
 
-// Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then chunks x kv heads.
+// Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then parts x kv heads.
 template <int TYPE, int DIM>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs a, const PagedAttention p)
 {
@@ -1179,7 +1188,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs
     static_assert(sizeof(lds) <= 80 * 1024, "two workgroups on a CU");
     const int tiles = p.tiles * a.n_kv, n_tiles = tiles * p.tile_split;
     if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM, 1>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
-    else { attend_chunk<TYPE, DIM>(a, p, lds, (blockIdx.x - n_tiles) / a.n_kv, (blockIdx.x - n_tiles) % a.n_kv); }
+    else { attend_part<TYPE, DIM>(a, p, lds, (blockIdx.x - n_tiles) / a.n_kv, (blockIdx.x - n_tiles) % a.n_kv); }
 }
 
 // The tiles' ranges added, 16 rows per workgroup and DIM / 16 dims of a row per thread.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads.
