@@ -21,19 +21,44 @@ struct PagedArgs
     int max_ctx;                    // rows a sequence may have: the table's, and the caller's limit
 };
 
-// Sequence of activation row t, or -1.  Called by whole waves with one t: a lane per sequence, so one trip to memory per 64 of them.
-// Ranges that are not in order name no sequence, or one whose range has t: a row index never leaves the range that was looked at.
-__device__ __forceinline__ int paged_sequence(const PagedArgs& a, int t)
+// Where activation rows t0 .. t0 + N - 1 belong: sequence (-1: to none), position, page (-1: none).  Called by whole waves with one t0: a lane per sequence,
+// so one trip to memory per 64 of them, then one each for the N rows' lengths and pages.  Ranges that are not in order name no sequence, or one whose
+// range has t: a row index never leaves the range that was looked at.
+template <int N>
+struct PagedPlaces
 {
-    int s = -1;
-    for (int base = 0; base <= a.n_seqs; base += 64)
+    int s[N], pos[N], page[N];
+
+    __device__ __forceinline__ PagedPlaces(const PagedArgs& a, int t0)
     {
-        const int i = base + (threadIdx.x & 63);
-        s += __builtin_popcountll(__ballot(i <= a.n_seqs && a.seq_start[i] <= t));
+#pragma unroll
+        for (int n = 0; n < N; n++) { s[n] = -1; }
+        for (int base = 0; base <= a.n_seqs; base += 64)
+        {
+            const int i = base + (threadIdx.x & 63), start = i <= a.n_seqs ? a.seq_start[i] : 0x7FFFFFFF;
+#pragma unroll
+            for (int n = 0; n < N; n++) { s[n] += __builtin_popcountll(__ballot(start <= t0 + n)); }
+        }
+        int at[N], begin[N], end[N], rows[N];
+#pragma unroll
+        for (int n = 0; n < N; n++)
+        {
+            at[n] = min(max(s[n], 0), a.n_seqs - 1);
+            begin[n] = a.seq_start[at[n]];
+            end[n] = a.seq_start[at[n] + 1];
+            rows[n] = a.ctx_len[at[n]];
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++)
+        {
+            if (at[n] != s[n] || begin[n] > t0 + n || end[n] <= t0 + n) { s[n] = -1; }
+            pos[n] = min(rows[n], a.max_ctx) - (end[n] - (t0 + n));
+            page[n] = s[n] < 0 || pos[n] < 0 ? -1 : a.table[(size_t)at[n] * a.table_stride + (pos[n] >> a.shift)];
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) { page[n] = page[n] < a.n_pages ? max(page[n], -1) : -1; }
     }
-    if (s < 0 || s >= a.n_seqs || a.seq_start[s] > t || a.seq_start[s + 1] <= t) { return -1; }
-    return s;
-}
+};
 
 // Rows of a sequence in the cache.
 __device__ __forceinline__ int paged_rows(const PagedArgs& a, int s) { return min(a.ctx_len[s], a.max_ctx); }
@@ -115,118 +140,162 @@ __device__ __forceinline__ u32x2 pack4(const float* f)
     return u32x2{ f32_to_bf16_bits(f[0]) | f32_to_bf16_bits(f[1]) << 16, f32_to_bf16_bits(f[2]) | f32_to_bf16_bits(f[3]) << 16 };
 }
 
-// Norm, rotation and append of one head of one token by DIM / 8 lanes: lane i holds elements 4 i .. + 3 of both halves of the head, so that the
-// rotation needs no neighbour.  Grid: tokens x workgroups of 256 lanes over the n_q + 2 n_kv heads.
-template <int TYPE, int DIM>
+// Norm, rotation and append of a head by DIM / 8 lanes: lane i holds elements 4 i .. + 3 of both halves of the head, so that the rotation needs no
+// neighbour.  A lane takes the same head of TOKENS tokens: rows that do not hang on where their token belongs are asked for first, and the trips that tell
+// it are shared.  Grid: tokens / TOKENS x workgroups of 256 lanes over the n_q + 2 n_kv heads.
+template <int TYPE, int DIM, int TOKENS>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedArgs a, const PagedAppend p)
 {
     constexpr int LANES = DIM / 8, PER_WG = 256 / LANES, TOP = TYPE == DT_E4M3 ? 8 : 15;
     constexpr float LARGEST = TYPE == DT_E4M3 ? 448.0f : 57344.0f;
     const int heads = p.n_q + 2 * a.n_kv, parts = (heads + PER_WG - 1) / PER_WG;
-    const int t = blockIdx.x / parts, head = blockIdx.x % parts * PER_WG + threadIdx.x / LANES, i = threadIdx.x % LANES;
-    const int s = paged_sequence(a, t);
-    if (s < 0) { return; }
-    const int pos = paged_rows(a, s) - (a.seq_start[s + 1] - t);
-    if (pos < 0 || (p.cos_tab && pos >= p.n_positions) || head >= heads) { return; }
+    const int t0 = blockIdx.x / parts * TOKENS, head = min(blockIdx.x % parts * PER_WG + (int)threadIdx.x / LANES, heads - 1), i = threadIdx.x % LANES;
+    const bool spare = blockIdx.x % parts * PER_WG + threadIdx.x / LANES >= (unsigned)heads;
     const bool is_q = head < p.n_q, is_v = head >= p.n_q + a.n_kv;
     const int h = is_q ? head : is_v ? head - p.n_q - a.n_kv : head - p.n_q;
-    const uint16_t* const src = (is_q ? p.q + (size_t)t * p.ldq : is_v ? p.v + (size_t)t * p.ldv : p.k + (size_t)t * p.ldk) + (size_t)h * DIM + i * 4;
-    float x[8];
-    unpack4(*(const u32x2*)src, x);
-    unpack4(*(const u32x2*)(src + DIM / 2), x + 4);
+    const uint16_t* const src = (is_q ? p.q : is_v ? p.v : p.k) + (size_t)h * DIM + i * 4;
+    const size_t ld = is_q ? p.ldq : is_v ? p.ldv : p.ldk;
+    u32x2 raw[TOKENS][2];
+#pragma unroll
+    for (int n = 0; n < TOKENS; n++)
+    {
+        const uint16_t* const row = src + (size_t)min(t0 + n, p.n_tokens - 1) * ld;
+        raw[n][0] = *(const u32x2*)row;
+        raw[n][1] = *(const u32x2*)(row + DIM / 2);
+    }
     const uint16_t* const nw = is_v ? nullptr : is_q ? p.q_norm_w : p.k_norm_w;
+    float w[8] = {};
     if (nw)
     {
-        float w[8], sum = 0.0f;
         unpack4(*(const u32x2*)(nw + i * 4), w);
         unpack4(*(const u32x2*)(nw + i * 4 + DIM / 2), w + 4);
-#pragma unroll
-        for (int e = 0; e < 8; e++) { sum += x[e] * x[e]; }
-        sum = reduce_lanes<LANES>(sum, [](float u, float v) { return u + v; });
-        const float invstd = rsqrtf(sum / (float)DIM + p.eps);
-#pragma unroll
-        for (int e = 0; e < 8; e++) { x[e] = x[e] * invstd * w[e]; }
     }
-    if (p.cos_tab && !is_v)
+    const PagedPlaces<TOKENS> at(a, t0);
+    u32x2 cs[TOKENS], sn[TOKENS];
+    const bool turns = p.cos_tab && !is_v;
+    if (turns)
     {
-        float c[4], sn[4];
-        unpack4(*(const u32x2*)(p.cos_tab + (size_t)pos * (DIM / 2) + i * 4), c);
-        unpack4(*(const u32x2*)(p.sin_tab + (size_t)pos * (DIM / 2) + i * 4), sn);
 #pragma unroll
-        for (int e = 0; e < 4; e++)
+        for (int n = 0; n < TOKENS; n++)
         {
-            const float lo = x[e], hi = x[e + 4];
-            x[e] = lo * c[e] - hi * sn[e];
-            x[e + 4] = hi * c[e] + lo * sn[e];
+            const size_t from = (size_t)min(max(at.pos[n], 0), p.n_positions - 1) * (DIM / 2) + i * 4;
+            cs[n] = *(const u32x2*)(p.cos_tab + from);
+            sn[n] = *(const u32x2*)(p.sin_tab + from);
         }
     }
-    if (is_q)
-    {
-        uint16_t* const dst = p.q_out + ((size_t)t * p.n_q + h) * DIM + i * 4;
-        *(u32x2*)dst = pack4(x);
-        *(u32x2*)(dst + DIM / 2) = pack4(x + 4);
-        return;
-    }
-    const int page = paged_page(a, s, pos);
-    if (page < 0) { return; }
-    const size_t row = paged_row(a, h, pos);
-    uint8_t* const dst = const_cast<uint8_t*>(is_v ? a.v : a.k) + page * a.page_stride + row * (DIM * CODE_BYTES<TYPE>);
-    if constexpr (TYPE == DT_BF16)
-    {
-        *(u32x2*)(dst + i * 8) = pack4(x);
-        *(u32x2*)(dst + i * 8 + DIM) = pack4(x + 4);
-    }
-    else
-    {
-        float most = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) { most = fmaxf(most, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f); }
-        most = reduce_lanes<LANES>(most, [](float u, float v) { return fmaxf(u, v); });
-        // most = m 2^k, 1 <= m < 2: both types' largest value is 1.75 2^TOP
-        const uint32_t bits = f32_to_bits(most);
-        int e2 = (int)(bits >> 23) - 127 - TOP + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-        e2 = min(max(e2, -100), 127 - TOP);
-        const float by = bits_to_f32((uint32_t)(127 - e2) << 23);
-#pragma unroll
-        for (int e = 0; e < 8; e++)
+    for (int n = 0; n < TOKENS; n++)
+    {
+        const int t = t0 + n, pos = at.pos[n];
+        if (at.s[n] < 0 || t >= p.n_tokens || pos < 0 || (p.cos_tab && pos >= p.n_positions) || spare) { continue; }
+        float x[8];
+        unpack4(raw[n][0], x);
+        unpack4(raw[n][1], x + 4);
+        if (nw)
         {
-            const float y = x[e] * by;
-            x[e] = fabsf(y) < INFINITY ? fminf(fmaxf(y, -LARGEST), LARGEST) : y;      // saturates at the largest exponent only
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) { sum += x[e] * x[e]; }
+            sum = reduce_lanes<LANES>(sum, [](float u, float v) { return u + v; });
+            const float invstd = rsqrtf(sum / (float)DIM + p.eps);
+#pragma unroll
+            for (int e = 0; e < 8; e++) { x[e] = x[e] * invstd * w[e]; }
         }
-        *(uint32_t*)(dst + i * 4) = f32x4_to_fp8<TYPE>(x[0], x[1], x[2], x[3]);
-        *(uint32_t*)(dst + i * 4 + DIM / 2) = f32x4_to_fp8<TYPE>(x[4], x[5], x[6], x[7]);
-        if (i == 0) { const_cast<uint8_t*>(is_v ? a.v_scale : a.k_scale)[page * a.scale_stride + row] = (uint8_t)(e2 + 127); }
+        if (turns)
+        {
+            float c[4], s[4];
+            unpack4(cs[n], c);
+            unpack4(sn[n], s);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+            {
+                const float lo = x[e], hi = x[e + 4];
+                x[e] = lo * c[e] - hi * s[e];
+                x[e + 4] = hi * c[e] + lo * s[e];
+            }
+        }
+        if (is_q)
+        {
+            uint16_t* const dst = p.q_out + ((size_t)t * p.n_q + h) * DIM + i * 4;
+            *(u32x2*)dst = pack4(x);
+            *(u32x2*)(dst + DIM / 2) = pack4(x + 4);
+            continue;
+        }
+        const int page = at.page[n];
+        if (page < 0) { continue; }
+        const size_t row = paged_row(a, h, pos);
+        uint8_t* const dst = const_cast<uint8_t*>(is_v ? a.v : a.k) + page * a.page_stride + row * (DIM * CODE_BYTES<TYPE>);
+        if constexpr (TYPE == DT_BF16)
+        {
+            *(u32x2*)(dst + i * 8) = pack4(x);
+            *(u32x2*)(dst + i * 8 + DIM) = pack4(x + 4);
+        }
+        else
+        {
+            float most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) { most = fmaxf(most, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f); }
+            most = reduce_lanes<LANES>(most, [](float u, float v) { return fmaxf(u, v); });
+            // most = m 2^k, 1 <= m < 2: both types' largest value is 1.75 2^TOP
+            const uint32_t bits = f32_to_bits(most);
+            int e2 = (int)(bits >> 23) - 127 - TOP + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+            e2 = min(max(e2, -100), 127 - TOP);
+            const float by = bits_to_f32((uint32_t)(127 - e2) << 23);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+            {
+                const float y = x[e] * by;
+                x[e] = fabsf(y) < INFINITY ? fminf(fmaxf(y, -LARGEST), LARGEST) : y;      // saturates at the largest exponent only
+            }
+            *(uint32_t*)(dst + i * 4) = f32x4_to_fp8<TYPE>(x[0], x[1], x[2], x[3]);
+            *(uint32_t*)(dst + i * 4 + DIM / 2) = f32x4_to_fp8<TYPE>(x[4], x[5], x[6], x[7]);
+            if (i == 0) { const_cast<uint8_t*>(is_v ? a.v_scale : a.k_scale)[page * a.scale_stride + row] = (uint8_t)(e2 + 127); }
+        }
     }
 }
 
-// Rows back as BF16: DIM / 8 lanes per row of eight values each.  Grid: tokens x workgroups of 256 lanes over the 2 n_kv rows of a token.
-template <int TYPE, int DIM>
-__global__ __launch_bounds__(256) void paged_read_kernel(const PagedArgs a, uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, long long token_stride, long long head_stride)
+// Rows back as BF16: DIM / 8 lanes per row of eight values each, the same row of TOKENS tokens per lane.  Grid: tokens / TOKENS x workgroups of 256 lanes over
+// the 2 n_kv rows of a token.
+template <int TYPE, int DIM, int TOKENS>
+__global__ __launch_bounds__(256) void paged_read_kernel(const PagedArgs a, uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int n_tokens, long long token_stride, long long head_stride)
 {
-    constexpr int LANES = DIM / 8, PER_WG = 256 / LANES;
+    constexpr int LANES = DIM / 8, PER_WG = 256 / LANES, BYTES = 8 * CODE_BYTES<TYPE>;
     const int parts = (2 * a.n_kv + PER_WG - 1) / PER_WG;
-    const int t = blockIdx.x / parts, at = blockIdx.x % parts * PER_WG + threadIdx.x / LANES, i = threadIdx.x % LANES;
-    const int s = paged_sequence(a, t);
-    if (s < 0 || at >= 2 * a.n_kv) { return; }
-    const bool is_v = at >= a.n_kv;
-    const int h = is_v ? at - a.n_kv : at;
-    const int pos = paged_rows(a, s) - (a.seq_start[s + 1] - t);
-    const int page = pos < 0 ? -1 : paged_page(a, s, pos);
-    u32x4 out = { 0, 0, 0, 0 };
-    if (page >= 0)
+    const int t0 = blockIdx.x / parts * TOKENS, of = blockIdx.x % parts * PER_WG + threadIdx.x / LANES, i = threadIdx.x % LANES;
+    const PagedPlaces<TOKENS> at(a, t0);
+    if (of >= 2 * a.n_kv) { return; }
+    const bool is_v = of >= a.n_kv;
+    const int h = is_v ? of - a.n_kv : of;
+    u32x4 codes[TOKENS];
+    uint32_t exponent[TOKENS];
+#pragma unroll
+    for (int n = 0; n < TOKENS; n++)
     {
-        const size_t row = paged_row(a, h, pos);
-        const uint8_t* const src = (is_v ? a.v : a.k) + page * a.page_stride + row * (DIM * CODE_BYTES<TYPE>) + i * 8 * CODE_BYTES<TYPE>;
-        if constexpr (TYPE == DT_BF16) { out = *(const u32x4*)src; }
+        // a row without a page: any that is there
+        const size_t page = max(at.page[n], 0), row = paged_row(a, h, max(at.pos[n], 0));
+        const uint8_t* const src = (is_v ? a.v : a.k) + page * a.page_stride + row * (DIM * CODE_BYTES<TYPE>) + i * BYTES;
+        if constexpr (TYPE == DT_BF16) { codes[n] = *(const u32x4*)src; }
         else
         {
-            const u32x2 codes = *(const u32x2*)src;
-            const float scale = bits_to_f32((uint32_t)(is_v ? a.v_scale : a.k_scale)[page * a.scale_stride + row] << 23);
-            const u32x2 lo = fp8x4_to_bf16<TYPE>(codes[0], scale), hi = fp8x4_to_bf16<TYPE>(codes[1], scale);
-            out = u32x4{ lo[0], lo[1], hi[0], hi[1] };
+            const u32x2 c = *(const u32x2*)src;
+            codes[n] = u32x4{ c[0], c[1], 0, 0 };
+            exponent[n] = (is_v ? a.v_scale : a.k_scale)[page * a.scale_stride + row];
         }
     }
-    *(u32x4*)((is_v ? v_out : k_out) + t * token_stride + h * head_stride + i * 8) = out;
+#pragma unroll
+    for (int n = 0; n < TOKENS; n++)
+    {
+        if (at.s[n] < 0 || t0 + n >= n_tokens) { continue; }
+        u32x4 out = codes[n];
+        if constexpr (TYPE != DT_BF16)
+        {
+            const float scale = bits_to_f32(exponent[n] << 23);
+            const u32x2 lo = fp8x4_to_bf16<TYPE>(codes[n][0], scale), hi = fp8x4_to_bf16<TYPE>(codes[n][1], scale);
+            out = u32x4{ lo[0], lo[1], hi[0], hi[1] };
+        }
+        if (at.page[n] < 0) { out = u32x4{ 0, 0, 0, 0 }; }
+        *(u32x4*)((is_v ? v_out : k_out) + (t0 + n) * token_stride + h * head_stride + i * 8) = out;
+    }
 }
 
 }    // namespace ccq

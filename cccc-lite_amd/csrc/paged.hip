@@ -49,6 +49,18 @@ bool paged_args(const hip_paged_kv* c, PagedArgs& a)
     ((c)->head_dim == 64 ? ((c)->type == CCCC_BFLOAT16 ? KERNEL<DT_BF16, 64> : (c)->type == CCCC_FP8_E4M3 ? KERNEL<DT_E4M3, 64> : KERNEL<DT_E5M2, 64>) \
                          : ((c)->type == CCCC_BFLOAT16 ? KERNEL<DT_BF16, 128> : (c)->type == CCCC_FP8_E4M3 ? KERNEL<DT_E4M3, 128> : KERNEL<DT_E5M2, 128>))
 
+// Tokens per workgroup of the append and the read back: one up to 32 workgroups per CU, which then share their trips to memory.  MI355X, 32 / 8 heads, E4M3, one / these,
+// us: append of 512 tokens 5.1 / 6.8, 2048 (6144 workgroups) 12.8 / 13.5, 8192 48.6 / 41.7; read of 2048 rows 4.7 / 5.5, 8192 (8192 workgroups) 12.0 / 10.9, 32000 54.6 / 43.2.
+constexpr int APPEND_TOKENS = 4, READ_TOKENS = 8;
+template <int TYPE, int DIM>
+constexpr auto append_one = paged_append_kernel<TYPE, DIM, 1>;
+template <int TYPE, int DIM>
+constexpr auto append_many = paged_append_kernel<TYPE, DIM, APPEND_TOKENS>;
+template <int TYPE, int DIM>
+constexpr auto read_one = paged_read_kernel<TYPE, DIM, 1>;
+template <int TYPE, int DIM>
+constexpr auto read_many = paged_read_kernel<TYPE, DIM, READ_TOKENS>;
+
 // keys of a block of paged_attention_kernel's rows (RowsForm)
 int keys_per_block(const hip_paged_kv* c) { return c->type == CCCC_BFLOAT16 && c->head_dim == 128 ? 32 : 64; }
 
@@ -70,6 +82,28 @@ struct Plan
     size_t tile_bytes, row_bytes;   // of partial sums
 };
 
+// Ranges of keys for tiles that are few workgroups.  A tile takes 5 us and 1.35 per block of 64 keys where a CU has one workgroup, 2.15 for two side by side (heads of
+// 64: 0.6 of it); ranges add 10 us for the launch that adds them and for the start of more workgroups, and 0.3 per MB of FP32 sums written and read.  5 % to gain
+// at least.  Measured with 1 / 2 / 4 / 8 / 16 ranges, 32 / 8 heads BF16: 512 tokens behind 3000 71.5 / 52.0 / 50.2, 1024 behind 500 37.2 / 46.0, 1024 behind 3000 80.1 / 83.7,
+// 128 behind 3000 61.4 / 40.7 / 29.7 / 27.8 / 30.9, 64 behind 8000 - / - / 47.4 / 33.9 / 30.1, 512 from 0 18.2 / 20.1.
+int tile_ranges(long long workgroups, int blocks, size_t outputs, int dim)
+{
+    const double cus = cu_count(), mb = (double)outputs * (dim + 2) * 4.0 * 1e-6;
+    int best = 1;
+    double least = 0.0;
+    for (int n = 1; n <= 64 && n <= std::max(blocks / 4, 1); n++)
+    {
+        const double all = (double)workgroups * n, rounds = std::max(1.0, all / (2.0 * cus));
+        const double time = 5.0 + std::ceil((double)blocks / n) * rounds * (all > cus ? 2.15 : 1.35) * (dim == 64 ? 0.6 : 1.0) + (n > 1 ? 10.0 + 0.3 * mb * n : 0.0);
+        if (n == 1 || time < 0.95 * least)
+        {
+            best = n;
+            least = time;
+        }
+    }
+    return best;
+}
+
 // False: more than a launch can have.
 bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, int n_tokens, int max_new, int window, int n_sink, Plan& plan)
 {
@@ -87,8 +121,7 @@ bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, in
         const long long tiles = (rows - cut) / 128 + cut;
         if (tiles * a.n_kv * 64 > MOST_BLOCKS) { return false; }
         plan.tiles = (int)tiles;
-        plan.tile_split = (int)std::max<long long>(1, std::min({ slots / (tiles * a.n_kv), keys / 256, 64LL }));
-        if (getenv("PA_TS")) { plan.tile_split = atoi(getenv("PA_TS")); }
+        plan.tile_split = tile_ranges(tiles * a.n_kv, (int)((keys + PA_TILE_KEYS - 1) / PA_TILE_KEYS), (size_t)n_tokens * n_q, dim);
         plan.tile_bytes = plan.tile_split > 1 ? ((size_t)n_tokens * n_q * plan.tile_split * (dim + 2) * 4 + 15) & ~(size_t)15 : 0;
     }
     if (plan.rows)
@@ -128,13 +161,22 @@ int hip_qk_norm_rope_kv_paged_bf16(const hip_paged_kv* cache, const void* q, con
     }
     if ((n_q_heads > 0 && (ldq % 8 != 0 || ldq < (long long)n_q_heads * dim)) || ldk % 8 != 0 || ldv % 8 != 0 || ldk < (long long)a.n_kv * dim || ldv < (long long)a.n_kv * dim) { return -1; }
     const int per_wg = 256 * 8 / dim;
-    const long long blocks = (long long)n_tokens * ((n_q_heads + 2 * a.n_kv + per_wg - 1) / per_wg);
+    const int parts = (n_q_heads + 2 * a.n_kv + per_wg - 1) / per_wg;
+    const long long blocks = (long long)n_tokens * parts;
     if (blocks > MOST_BLOCKS) { return -1; }
     if (n_tokens == 0) { return 0; }
     const PagedAppend p = { (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (const uint16_t*)q_norm_w, (const uint16_t*)k_norm_w, (const uint16_t*)cos_tab, (const uint16_t*)sin_tab,
                             (uint16_t*)q_out, n_q_heads, n_tokens, n_positions, (size_t)ldq, (size_t)ldk, (size_t)ldv, epsilon };
-    const auto kernel = CCQ_PAGED_KERNEL(paged_append_kernel, cache);
-    kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, p);
+    if (blocks < 32LL * cu_count())
+    {
+        const auto kernel = CCQ_PAGED_KERNEL(append_one, cache);
+        kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, p);
+    }
+    else
+    {
+        const auto kernel = CCQ_PAGED_KERNEL(append_many, cache);
+        kernel<<<(unsigned)((n_tokens + APPEND_TOKENS - 1) / APPEND_TOKENS * parts), 256, 0, stream()>>>(a, p);
+    }
     return finish("qk_norm_rope_kv_paged");
 }
 
@@ -144,11 +186,20 @@ int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void* v_out, 
     if (!paged_args(cache, a) || n_tokens < 0 || !k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16)) { return -1; }
     if (token_stride % 8 != 0 || head_stride % 8 != 0 || token_stride < cache->head_dim || head_stride < cache->head_dim) { return -1; }
     const int per_wg = 256 * 8 / cache->head_dim;
-    const long long blocks = (long long)n_tokens * ((2 * a.n_kv + per_wg - 1) / per_wg);
+    const int parts = (2 * a.n_kv + per_wg - 1) / per_wg;
+    const long long blocks = (long long)n_tokens * parts;
     if (blocks > MOST_BLOCKS) { return -1; }
     if (n_tokens == 0) { return 0; }
-    const auto kernel = CCQ_PAGED_KERNEL(paged_read_kernel, cache);
-    kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, (uint16_t*)k_out, (uint16_t*)v_out, token_stride, head_stride);
+    if (blocks < 32LL * cu_count())
+    {
+        const auto kernel = CCQ_PAGED_KERNEL(read_one, cache);
+        kernel<<<(unsigned)blocks, 256, 0, stream()>>>(a, (uint16_t*)k_out, (uint16_t*)v_out, n_tokens, token_stride, head_stride);
+    }
+    else
+    {
+        const auto kernel = CCQ_PAGED_KERNEL(read_many, cache);
+        kernel<<<(unsigned)((n_tokens + READ_TOKENS - 1) / READ_TOKENS * parts), 256, 0, stream()>>>(a, (uint16_t*)k_out, (uint16_t*)v_out, n_tokens, token_stride, head_stride);
+    }
     return finish("kv_paged_read");
 }
 
@@ -185,7 +236,7 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
     char* const part_sums = (char*)workspace + words * 8;
     const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)((char*)workspace + (plan.row_parts ? plan.row_bytes : 0)), (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv,
                                n_tokens, max_new, window, n_sink, plan.tile_split, plan.tiles, plan.tile_split, plan.row_slots, plan.row_parts, (float*)part_sums, (unsigned long long*)workspace,
-                               plan.row_parts ? name_call() : 0, plan.min_rows, 1, 1.4426950408889634f / sqrtf((float)dim) };
+                               plan.row_parts ? name_call() : 0, plan.min_rows, tiles <= 2LL * cu_count() ? 1 : 0, 1.4426950408889634f / sqrtf((float)dim) };
     const auto kernel = CCQ_PAGED_KERNEL(paged_attention_kernel, cache);
     kernel<<<(unsigned)(tiles + parts), 256, 0, stream()>>>(a, p);
     if (plan.tile_split > 1)

@@ -113,7 +113,7 @@ constexpr int PA_ROWS = 16, PA_TILE_KEYS = 64;
 // another: about two workgroups' worth of an even split, since a part costs some 5 us besides its keys, but not over PA_PART, which evens out what is
 // left over at the end.  (MI355X, 32 / 8 heads, E4M3, parts of a sequence: 64 sequences of 1000 to 8000 keys 1 113 us, 3 111, 6 123; 16 of 4100 keys 1 35, 2 31,
 // 4 32; 8 of 4000 keys 1 32, 2 24, 4 20.3, 8 20.5.)
-constexpr int PA_PART = 9;
+constexpr int PA_PART = 20;
 template <int KEYS>
 struct Parts
 {
