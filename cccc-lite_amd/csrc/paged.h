@@ -52,7 +52,7 @@ struct PagedPlaces
         for (int n = 0; n < N; n++)
         {
             if (at[n] != s[n] || begin[n] > t0 + n || end[n] <= t0 + n) { s[n] = -1; }
-            pos[n] = min(rows[n], a.max_ctx) - (end[n] - (t0 + n));
+            pos[n] = max(min(rows[n], a.max_ctx), 0) - (end[n] - (t0 + n));
             page[n] = s[n] < 0 || pos[n] < 0 ? -1 : a.table[(size_t)at[n] * a.table_stride + (pos[n] >> a.shift)];
         }
 #pragma unroll
@@ -61,7 +61,7 @@ struct PagedPlaces
 };
 
 // Rows of a sequence in the cache.
-__device__ __forceinline__ int paged_rows(const PagedArgs& a, int s) { return min(a.ctx_len[s], a.max_ctx); }
+__device__ __forceinline__ int paged_rows(const PagedArgs& a, int s) { return max(min(a.ctx_len[s], a.max_ctx), 0); }
 
 // Page of position pos >= 0, or -1.
 __device__ __forceinline__ int paged_page(const PagedArgs& a, int s, int pos)

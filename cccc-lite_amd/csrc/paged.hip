@@ -64,12 +64,16 @@ constexpr auto read_many = paged_read_kernel<TYPE, DIM, READ_TOKENS>;
 // keys of a block of paged_attention_kernel's rows (RowsForm)
 int keys_per_block(const hip_paged_kv* c) { return c->type == CCCC_BFLOAT16 && c->head_dim == 128 ? 32 : 64; }
 
-bool attention_args(const hip_paged_kv* c, PagedArgs& a, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink)
+bool attention_args(const hip_paged_kv* c, PagedArgs& a, int n_q_heads, int n_tokens, int& max_new, int max_ctx, int& window, int& n_sink)
 {
     if (!paged_args(c, a) || n_q_heads <= 0 || n_q_heads % c->n_kv_heads != 0 || n_q_heads / c->n_kv_heads > 64) { return false; }
     if (n_tokens < 0 || max_new <= 0 || max_ctx <= 0 || window < 0 || n_sink < 0) { return false; }
     if ((long long)n_tokens * n_q_heads > MOST_BLOCKS) { return false; }
     a.max_ctx = std::min(a.max_ctx, max_ctx);
+    // sums and differences of positions stay within 32 bits
+    max_new = std::min(max_new, 1 << 24);
+    n_sink = std::min(n_sink, a.max_ctx);
+    window = window >= a.max_ctx ? 0 : window;          // all keys
     return true;
 }
 // How a call's rows are taken: in tiles, each over so many ranges of keys at most; as sequences of up to 16 rows per kv head, whose keys are shared out over

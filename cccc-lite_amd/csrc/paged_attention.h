@@ -60,9 +60,10 @@ struct NewTokens
 __device__ __forceinline__ NewTokens new_tokens(const PagedArgs& a, const PagedAttention& p, int s)
 {
     const int begin = a.seq_start[s], end = a.seq_start[s + 1];
-    const int first = max(begin, 0), n = min(end, p.n_tokens) - first;
-    if (n <= 0 || (long long)end - begin > p.max_new) { return { first, 0, 0 }; }
-    return { first, n, paged_rows(a, s) - (end - first) };
+    const int first = max(begin, 0), last = min(end, p.n_tokens);
+    // (compared and not subtracted: ranges may hold anything)
+    if (last <= first || (long long)end - begin > p.max_new) { return { 0, 0, 0 }; }
+    return { first, last - first, paged_rows(a, s) - (end - first) };
 }
 
 // The blocks of SIZE keys that tokens at positions lo .. hi see: the first `sinks` ones, then from block sinks + skip on; n in all.
