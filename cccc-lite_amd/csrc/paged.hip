@@ -136,7 +136,7 @@ bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, in
         if (all > 0x3FFFFFFFLL || (a.n_seqs + 3 * at_once + 1) * a.n_kv * 2 > MOST_BLOCKS) { return false; }
         plan.row_slots = (int)at_once;
         plan.row_parts = (int)(a.n_seqs + std::max<long long>(1, std::min(3 * at_once, all / part)));
-        plan.row_bytes = (size_t)plan.row_parts * a.n_kv * (PA_ROWS * (dim + 2) * 4 + 8);
+        plan.row_bytes = ((size_t)plan.row_parts * a.n_kv * (PA_ROWS * (dim + 2) * 4 + 8) + 15) & ~(size_t)15;
     }
     return true;
 }
@@ -239,7 +239,7 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
     const size_t words = (size_t)plan.row_parts * a.n_kv;
     char* const part_sums = (char*)workspace + words * 8;
     const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)((char*)workspace + (plan.row_parts ? plan.row_bytes : 0)), (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv,
-                               n_tokens, max_new, window, n_sink, plan.tile_split, plan.tiles, plan.tile_split, plan.row_slots, plan.row_parts, (float*)part_sums, (unsigned long long*)workspace,
+                               n_tokens, max_new, window, n_sink, plan.tiles, plan.tile_split, plan.row_slots, plan.row_parts, (float*)part_sums, (unsigned long long*)workspace,
                                plan.row_parts ? name_call() : 0, plan.min_rows, tiles <= 2LL * cu_count() ? 1 : 0, 1.4426950408889634f / sqrtf((float)dim) };
     const auto kernel = CCQ_PAGED_KERNEL(paged_attention_kernel, cache);
     kernel<<<(unsigned)(tiles + parts), 256, 0, stream()>>>(a, p);

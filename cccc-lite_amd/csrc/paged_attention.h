@@ -4,7 +4,6 @@
 // Two kernels take them, 16 rows or 128 at a time, each with the keys in ranges where there are few rows; a third adds the ranges.
 #pragma once
 #include "paged.h"
-#include <type_traits>
 
 namespace ccq
 {
@@ -13,10 +12,9 @@ struct PagedAttention
 {
     const uint16_t* q;
     uint16_t* y;
-    float* partial;                 // [range][token][head][dim] sums, then [range][token][head] (max, sum): only where there are ranges
+    float* partial;                 // of tiles with ranges: [range][token][head][dim] sums, then [range][token][head] (max, sum)
     size_t ldq, ldy;
     int n_q, group, n_tokens, max_new, window, n_sink;
-    int n_split;                    // ranges of keys that `partial` is laid out for
     int tiles, tile_split;          // tiles of 128 rows (at most) and the most ranges of each
     int row_slots;                  // workgroups per kv head that the GPU runs at once
     int row_parts;                  // workgroups per kv head for the parts of all sequences of at most 16 rows per kv head; 0: one for each sequence
@@ -24,7 +22,7 @@ struct PagedAttention
     unsigned long long* there;      // [part][kv head]: the name of the call whose part is there
     unsigned long long call;        // of this call alone, 48 bits
     int min_rows;                   // sequences of at most so many rows per kv head are not cut into tiles
-    int snake;
+    int snake;                      // the second half of the tiles in the other order
     float scale;                    // log2 e / sqrt(dim)
 
     __device__ __forceinline__ float* row_sums(int slot, int kvh, int n_kv, int row, int dim) const { return row_partial + (((size_t)slot * n_kv + kvh) * 16 + row) * dim; }
@@ -34,7 +32,7 @@ struct PagedAttention
     }
     __device__ __forceinline__ size_t outputs() const { return (size_t)n_tokens * n_q; }
     __device__ __forceinline__ float* sums(int range, size_t row, int dim) const { return partial + ((size_t)range * outputs() + row) * dim; }
-    __device__ __forceinline__ float2* stats(int range, size_t row, int dim) const { return (float2*)(partial + (size_t)n_split * outputs() * dim) + (size_t)range * outputs() + row; }
+    __device__ __forceinline__ float2* stats(int range, size_t row, int dim) const { return (float2*)(partial + (size_t)tile_split * outputs() * dim) + (size_t)range * outputs() + row; }
 };
 
 // a value that all lanes have, in a scalar register
@@ -59,11 +57,11 @@ struct NewTokens
 
 __device__ __forceinline__ NewTokens new_tokens(const PagedArgs& a, const PagedAttention& p, int s)
 {
-    const int begin = a.seq_start[s], end = a.seq_start[s + 1];
+    const int begin = a.seq_start[s], end = a.seq_start[s + 1], rows = paged_rows(a, s);       // one trip
     const int first = max(begin, 0), last = min(end, p.n_tokens);
     // (compared and not subtracted: ranges may hold anything)
     if (last <= first || (long long)end - begin > p.max_new) { return { 0, 0, 0 }; }
-    return { first, last - first, paged_rows(a, s) - (end - first) };
+    return { first, last - first, rows - (end - first) };
 }
 
 // The blocks of SIZE keys that tokens at positions lo .. hi see: the first `sinks` ones, then from block sinks + skip on; n in all.
@@ -86,28 +84,7 @@ struct KeyBlocks
 
 __device__ __forceinline__ bool sees(const PagedAttention& p, int pos, int key) { return key <= pos && (p.window == 0 || key > pos - p.window || key < p.n_sink); }
 
-// Rows row0 .. of a sequence that a workgroup takes (s < 0: none), the positions of their tokens and the keys they see, in ranges of `per` blocks.
-template <int SIZE, int ROWS>
-struct Rows
-{
-    int s = -1, row0, n_rows, lo, hi, per, n_ranges;
-    NewTokens mine;
-    KeyBlocks<SIZE> blocks;
-
-    __device__ __forceinline__ void cut(const PagedAttention& p, int split, int multiple, int least)
-    {
-        lo = uniform(mine.pos + row0 / p.group);
-        hi = uniform(mine.pos + min(row0 + ROWS - 1, n_rows - 1) / p.group);
-        blocks = KeyBlocks<SIZE>(p, lo, hi);
-        blocks.n = uniform(blocks.n);
-        blocks.sinks = uniform(blocks.sinks);
-        blocks.skip = uniform(blocks.skip);
-        per = max(((blocks.n + split - 1) / split + multiple - 1) / multiple * multiple, least);
-        n_ranges = max((blocks.n + per - 1) / per, 1);
-    }
-};
-
-constexpr int PA_ROWS = 16, PA_TILE_KEYS = 64;
+constexpr int PA_ROWS = 16, PA_TILE = 128, PA_TILE_KEYS = 64;
 
 // Sequences of up to 16 rows per kv head: the keys of each in shares of four blocks (a block per wave), cut into parts of about the same number of shares, a
 // workgroup each.  How many shares a part has follows from those of all sequences, so that long and short ones leave no workgroup with much more than
@@ -166,28 +143,42 @@ struct Parts
     }
 };
 
+// A tile: rows row0 .. + 127 of sequence s (< 0: none), the positions of their tokens and the keys they see, in n_ranges ranges of `per` blocks.
+struct Tile
+{
+    int s = -1, row0 = 0, n_rows = 0, lo = 0, hi = 0, per = 1, n_ranges = 1;
+    NewTokens mine = { 0, 0, 0 };
+    KeyBlocks<PA_TILE_KEYS> blocks;
+};
+
 // Tile `tile` of those of all sequences, a sequence's last ones first: they see the most keys.  Where a CU gets two workgroups in all, the second half of
 // the tiles comes in the other order, so that a long one has a short one beside it.  Called by whole waves: a lane per sequence, their tiles added up.
-template <int TILE>
-__device__ __forceinline__ Rows<PA_TILE_KEYS, TILE> tile_rows(const PagedArgs& a, const PagedAttention& p, int tile)
+__device__ __forceinline__ Tile find_tile(const PagedArgs& a, const PagedAttention& p, int tile)
 {
-    Rows<PA_TILE_KEYS, TILE> r;
+    Tile r;
     const int lane = threadIdx.x & 63;
     if (p.snake && tile >= (p.tiles + 1) / 2) { tile = p.tiles - 1 - (tile - (p.tiles + 1) / 2); }
     for (int base = 0; base < a.n_seqs; base += 64)
     {
         const NewTokens mine = base + lane < a.n_seqs ? new_tokens(a, p, base + lane) : NewTokens{ 0, 0, 0 };
-        const int rows = mine.n * p.group, tiles = rows > p.min_rows ? (rows + TILE - 1) / TILE : 0;
+        const int rows = mine.n * p.group, tiles = rows > p.min_rows ? (rows + PA_TILE - 1) / PA_TILE : 0;
         const int upto = add_up_lanes(tiles);
         const unsigned long long past = __ballot(upto > tile);
         if (past != 0)
         {
             const int at = __builtin_ctzll(past);
-            r.s = __builtin_amdgcn_readfirstlane(base + at);
+            r.s = uniform(base + at);
             r.mine = { __builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.n, at), __builtin_amdgcn_readlane(mine.pos, at) };
-            r.row0 = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(upto, at) - 1 - tile) * TILE;
+            r.row0 = uniform(__builtin_amdgcn_readlane(upto, at) - 1 - tile) * PA_TILE;
             r.n_rows = uniform(r.mine.n * p.group);
-            r.cut(p, p.tile_split, 1, 4);
+            r.lo = uniform(r.mine.pos + r.row0 / p.group);
+            r.hi = uniform(r.mine.pos + min(r.row0 + PA_TILE - 1, r.n_rows - 1) / p.group);
+            r.blocks = KeyBlocks<PA_TILE_KEYS>(p, r.lo, r.hi);
+            r.blocks.n = uniform(r.blocks.n);
+            r.blocks.sinks = uniform(r.blocks.sinks);
+            r.blocks.skip = uniform(r.blocks.skip);
+            r.per = max((r.blocks.n + p.tile_split - 1) / p.tile_split, 4);
+            r.n_ranges = max((r.blocks.n + r.per - 1) / r.per, 1);
             return r;
         }
         tile -= __builtin_amdgcn_readlane(upto, 63);
@@ -313,31 +304,44 @@ __device__ __forceinline__ bool all_there(unsigned long long* own, unsigned long
 template <int DIM, bool PLAIN = false, class Part>
 __device__ __forceinline__ void add_parts(int n, uint16_t* y, Part part)
 {
-    constexpr int PER = DIM / 16;
+    constexpr int PER = DIM / 16, AT_ONCE = PLAIN ? 4 : 8;
     float sum[PER] = {};
     float m = -INFINITY, l = 0.0f;
-    for (int r0 = 0; r0 < n; r0 += 4)
+    for (int r0 = 0; r0 < n; r0 += AT_ONCE)
     {
-        float2 v[4][PER / 2], stat[4];                                      // four parts requested at once
+        float2 v[AT_ONCE][PER / 2], stat[AT_ONCE];                          // parts requested at once
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int r = 0; r < AT_ONCE; r++)
         {
             const float *from, *at;
             part(min(r0 + r, n - 1), from, at);
             stat[r] = PLAIN ? *(const float2*)at : load_part(at);
 #pragma unroll
-            for (int d = 0; d < PER / 2; d++) { v[r][d] = PLAIN ? *(const float2*)(from + 2 * d) : load_part(from + 2 * d); }
+            for (int d = 0; d < PER / 2; d += 2)
+            {
+                if (PLAIN)
+                {
+                    const f32x4 four = *(const f32x4*)(from + 2 * d);
+                    v[r][d] = make_float2(four[0], four[1]);
+                    v[r][d + 1] = make_float2(four[2], four[3]);
+                }
+                else
+                {
+                    v[r][d] = load_part(from + 2 * d);
+                    v[r][d + 1] = load_part(from + 2 * d + 2);
+                }
+            }
         }
         float top = m;
 #pragma unroll
-        for (int r = 0; r < 4; r++) { top = fmaxf(top, stat[r].x); }
+        for (int r = 0; r < AT_ONCE; r++) { top = fmaxf(top, stat[r].x); }
         const float base = top > -INFINITY ? top : 0.0f, shrink = __builtin_amdgcn_exp2f(m - base);
         m = top;
         l *= shrink;
 #pragma unroll
         for (int d = 0; d < PER; d++) { sum[d] *= shrink; }
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int r = 0; r < AT_ONCE; r++)
         {
             const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
             if (r0 + r < n && w != 0.0f)                                    // a part without a key has weight 0
@@ -732,8 +736,8 @@ __device__ __forceinline__ void attend_part(const PagedArgs& a, const PagedAtten
     if (shares > 0) { attend_rows<TYPE, DIM>(a, p, lds, s, mine, kvh, (int)((long long)shares * part / parts), (int)((long long)shares * (part + 1) / parts), c, part, parts); }
 }
 
-// 128 RT rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions.
-//   A workgroup of four waves takes 128 RT rows, a wave 32 RT of them and every key of each block of 64; keys and values reach LDS as BF16, shared by
+// 128 rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions.
+//   A workgroup of four waves takes 128 rows, a wave 32 of them and every key of each block of 64; keys and values reach LDS as BF16, shared by
 // the waves: from a BF16 cache by direct loads, from FP8 through registers, times their powers of two (exact, once per workgroup).
 //   scores: v_mfma_f32_32x32x16_bf16, key rows as row operand, queries as columns: D lane (row j = lane % 32, h = lane / 32), register i holds key
 //           8 (i / 4) + 4 h + i % 4 of 32.
@@ -747,7 +751,7 @@ struct TileForm
     static constexpr int ODD = 4 * BLOCK, LDS = ODD + 32;                   // two blocks of keys, two of values
 };
 
-template <int TYPE, int DIM, int RT>
+template <int TYPE, int DIM>
 __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int tile, int kvh, int range)
 {
     typedef TileForm<TYPE, DIM> F;
@@ -756,7 +760,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     uint32_t* const odd_rows = (uint32_t*)(lds + F::ODD);                   // per buffer of values and wave that staged: something infinite or NaN
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 31, h = lane >> 5;
-    const auto rows = tile_rows<128 * RT>(a, p, tile);
+    const Tile rows = find_tile(a, p, tile);
     if (rows.s < 0 || range >= rows.n_ranges) { return; }
     const NewTokens mine = rows.mine;
     const auto& blocks = rows.blocks;
@@ -764,20 +768,12 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     const int begin = range * rows.per, end = min(blocks.n, begin + rows.per);
 
     // the wave's rows
-    int token[RT], head[RT], my_pos[RT];
-    bool real[RT];
-    u32x4 qf[RT][DIM / 16];
+    const int r = row0 + wave * 32 + j, row = min(r, n_rows - 1);
+    const bool real = r < n_rows;
+    const int token = mine.first + row / p.group, head = kvh * p.group + row % p.group, my_pos = mine.pos + row / p.group;
+    u32x4 qf[DIM / 16];
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-    {
-        const int r = row0 + (wave * RT + t) * 32 + j, row = min(r, n_rows - 1);
-        real[t] = r < n_rows;
-        token[t] = mine.first + row / p.group;
-        head[t] = kvh * p.group + row % p.group;
-        my_pos[t] = mine.pos + row / p.group;
-#pragma unroll
-        for (int c = 0; c < DIM / 16; c++) { qf[t][c] = *(const u32x4*)(p.q + (size_t)token[t] * p.ldq + (size_t)head[t] * DIM + c * 16 + h * 8); }
-    }
+    for (int c = 0; c < DIM / 16; c++) { qf[c] = *(const u32x4*)(p.q + (size_t)token * p.ldq + (size_t)head * DIM + c * 16 + h * 8); }
 
     auto key_swizzle = [](int r) { return r / (256 / ROW) % CHUNKS; };
     auto value_swizzle = [](int r) { return DIM == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
@@ -787,16 +783,17 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     auto look_up = [&](int i0) {
         const int i = i0 + lane, key0 = blocks.block(i) * KEYS;
         size_t lacks = 0;
-        int mine_page = 0;
+        int mine_page = 0, page[4];
+        const int last = max(tile_hi, 0);
+#pragma unroll
+        for (int quarter = 0; quarter < 4; quarter++) { page[quarter] = paged_page(a, s, min(key0 + 16 * quarter, last)); }      // four loads, one trip
         if (i < end)
         {
 #pragma unroll
             for (int quarter = 0; quarter < 4; quarter++)
             {
-                const int pos = key0 + 16 * quarter;
-                const int page = pos > tile_hi ? 0 : paged_page(a, s, pos);
-                lacks |= page < 0 ? (size_t)1 << (60 + quarter) : 0;
-                mine_page = quarter == wave ? max(page, 0) : mine_page;
+                lacks |= page[quarter] < 0 && key0 + 16 * quarter <= tile_hi ? (size_t)1 << (60 + quarter) : 0;
+                mine_page = quarter == wave ? max(page[quarter], 0) : mine_page;
             }
         }
         const size_t r0 = paged_row(a, kvh, key0 + 16 * wave);
@@ -878,7 +875,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     };
 
     const uint32_t k_at = j * ROW + (h ^ key_swizzle(j)) * 16;             // of chunk h of key row j; chunk 2 c + h at k_at ^ 32 c
-    auto score_products = [&](int i, f32x16 (&acc)[RT][2]) {
+    auto score_products = [&](int i, f32x16 (&acc)[2]) {
         uint32_t at = k_at + keys_at(i);
         asm volatile("" : "+v"(at));
         const f32x16 zero = {};
@@ -888,76 +885,57 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
             for (int kt = 0; kt < 2; kt++)
             {
                 const bf16x8 kf = *(const bf16x8*)(lds + (at ^ (32 * c)) + kt * 32 * ROW);       // the swizzle of row j + 32 is that of j
-#pragma unroll
-                for (int t = 0; t < RT; t++) { acc[t][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, qf[t][c]), c == 0 ? zero : acc[t][kt], 0, 0, 0); }
+                acc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, qf[c]), c == 0 ? zero : acc[kt], 0, 0, 0);
             }
     };
 
-    float m[RT], l[RT];
-    f32x16 out[RT][DIM / 32];
+    float m = -INFINITY, l = 0.0f;
+    f32x16 out[DIM / 32];
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-    {
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
+    for (int d = 0; d < DIM / 32; d++)
 #pragma unroll
-        for (int d = 0; d < DIM / 32; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) { out[t][d][e] = 0.0f; }
-    }
+        for (int e = 0; e < 16; e++) { out[d][e] = 0.0f; }
     // dims 32 d + 16 (lane / 16 % 2) + 4 (lane % 4) .. + 3 of key row 4 h + lane % 16 / 4 (and of rows 8 further, and of the next 16)
     const int v_row = 4 * h + ((lane & 15) >> 2), v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     const uint32_t v_at = v_row * ROW + ((v_chunk ^ value_swizzle(v_row)) << 4) + ((lane & 1) << 3);     // dims 32 d on at v_at ^ 64 d
 
     // scores of keys that a row does not see
-    auto mask = [&](f32x16 (&acc)[RT][2], int b, int lacks) {
+    auto mask = [&](f32x16 (&acc)[2], int b, int lacks) {
+        // element e: key 8 (e / 4) + 4 h + e % 4 of the block
+        const int last = my_pos - b * KEYS - 4 * h, from = p.window == 0 ? -0x40000000 : last - p.window, sinks = p.n_sink - b * KEYS - 4 * h;
 #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int e = 0; e < 32; e++)
         {
-            // element e: key 8 (e / 4) + 4 h + e % 4 of the block
-            const int d = my_pos[t] - b * KEYS - 4 * h, from = p.window == 0 ? -0x40000000 : d - p.window, first = p.n_sink - b * KEYS - 4 * h;
-#pragma unroll
-            for (int e = 0; e < 32; e++)
-            {
-                const int key = 8 * (e / 4) + e % 4;
-                const bool see = key <= d && (key > from || key < first) && !(lacks >> (e / 8) & 1);
-                acc[t][e / 16][e % 16] = see ? acc[t][e / 16][e % 16] : -INFINITY;
-            }
+            const int key = 8 * (e / 4) + e % 4;
+            const bool see = key <= last && (key > from || key < sinks) && !(lacks >> (e / 8) & 1);
+            acc[e / 16][e % 16] = see ? acc[e / 16][e % 16] : -INFINITY;
         }
     };
     // largest raw score of a row
-    float top[RT];
-    auto find_top = [&](const f32x16 (&acc)[RT][2]) {
+    float top;
+    auto find_top = [&](const f32x16 (&acc)[2]) {
+        top = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < RT; t++)
-        {
-            top[t] = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 32; e++) { top[t] = fmaxf(top[t], acc[t][e / 16][e % 16]); }
-        }
+        for (int e = 0; e < 32; e++) { top = fmaxf(top, acc[e / 16][e % 16]); }
     };
     // the running maximum; sums rescaled where it moves
-    float off[RT];
+    float off;
     auto raise = [&]() {
-#pragma unroll
-        for (int t = 0; t < RT; t++)
+        const float least = top * p.scale;
+        if (__any(least > m + PA_LAG))
         {
-            const float least = top[t] * p.scale;
-            if (__any(least > m[t] + PA_LAG))
-            {
-                const float next = fmaxf(m[t], fmaxf(least, __shfl_xor(least, 32)));
-                const float shrink = m[t] > -INFINITY ? __builtin_amdgcn_exp2f(m[t] - next) : 1.0f;       // sums of nothing: 0, or what is not finite
-                m[t] = next;
-                l[t] *= shrink;
+            const float next = fmaxf(m, fmaxf(least, __shfl_xor(least, 32)));
+            const float shrink = m > -INFINITY ? __builtin_amdgcn_exp2f(m - next) : 1.0f;       // sums of nothing: 0, or what is not finite
+            m = next;
+            l *= shrink;
 #pragma unroll
-                for (int d = 0; d < DIM / 32; d++) { out[t][d] *= shrink; }
-            }
-            off[t] = m[t] > -INFINITY ? -m[t] : 0.0f;                       // no key seen yet: every weight is 2^-inf = 0
+            for (int d = 0; d < DIM / 32; d++) { out[d] *= shrink; }
         }
+        off = m > -INFINITY ? -m : 0.0f;                       // no key seen yet: every weight is 2^-inf = 0
     };
     // The weights of entry i under the products of entry i + 1, then the products of the weights under the largest scores of i + 1: in each step the
     // vector unit has work for as long as the matrix core has.
-    auto advance = [&](int i, const f32x16 (&cur)[RT][2], f32x16 (&next)[RT][2], auto loads, auto stores) {
+    auto advance = [&](int i, const f32x16 (&cur)[2], f32x16 (&next)[2], auto loads, auto stores) {
         constexpr int STEPS = DIM / 16, WEIGHTS = 32 / STEPS, PAIRS = DIM / 64;
         uint32_t key_at = k_at + keys_at(i + 1), value_at = v_at + values_at(i);
         asm volatile("" : "+v"(key_at), "+v"(value_at));
@@ -968,8 +946,8 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
         };
         const f32x16 zero = {};
         constexpr int AHEAD = 2, N_VALUES = 4 * PAIRS;    // steps that operands are read ahead
-        bf16x8 pb[RT][4], kf[STEPS][2], vf[N_VALUES][2];
-        float sum[RT][2] = {};
+        bf16x8 pb[4], kf[STEPS][2], vf[N_VALUES][2];
+        float sum[2] = {};
         auto read = [&](int step) {                                         // operands of a step, counted through
 #pragma unroll
             for (int n = 0; n < 2; n++)
@@ -988,20 +966,15 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
             loads(c);
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
+                { next[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[c][kt], __builtin_bit_cast(bf16x8, qf[c]), c == 0 ? zero : next[kt], 0, 0, 0); }
 #pragma unroll
-                for (int t = 0; t < RT; t++) { next[t][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[c][kt], __builtin_bit_cast(bf16x8, qf[t][c]), c == 0 ? zero : next[t][kt], 0, 0, 0); }
-#pragma unroll
-            for (int t = 0; t < RT; t++)
+            for (int e = c * WEIGHTS; e < (c + 1) * WEIGHTS; e++)
             {
-#pragma unroll
-                for (int e = c * WEIGHTS; e < (c + 1) * WEIGHTS; e++)
-                {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(cur[t][e / 16][e % 16], p.scale, off[t]));
-                    sum[t][e & 1] += w;
-                    pb[t][e / 8][e % 8] = (__bf16)w;
-                }
-                asm volatile("" : "+v"(sum[t][0]), "+v"(sum[t][1]));        // added here, not when somebody asks
+                const float w = __builtin_amdgcn_exp2f(fmaf(cur[e / 16][e % 16], p.scale, off));
+                sum[e & 1] += w;
+                pb[e / 8][e % 8] = (__bf16)w;
             }
+            asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));        // added here, not when somebody asks
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -1012,20 +985,14 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
             stores(n);
 #pragma unroll
             for (int k = 0; k < 2; k++)
+                { out[d + k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n][k], pb[u], out[d + k], 0, 0, 0); }
+            if (n == 0) { top = -INFINITY; }
 #pragma unroll
-                for (int t = 0; t < RT; t++) { out[t][d + k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n][k], pb[t][u], out[t][d + k], 0, 0, 0); }
-#pragma unroll
-            for (int t = 0; t < RT; t++)
-            {
-                if (n == 0) { top[t] = -INFINITY; }
-#pragma unroll
-                for (int e = n * (8 / PAIRS); e < (n + 1) * (8 / PAIRS); e++) { top[t] = fmaxf(top[t], next[t][e / 16][e % 16]); }
-                asm volatile("" : "+v"(top[t]));
-            }
+            for (int e = n * (8 / PAIRS); e < (n + 1) * (8 / PAIRS); e++) { top = fmaxf(top, next[e / 16][e % 16]); }
+            asm volatile("" : "+v"(top));
             __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int t = 0; t < RT; t++) { l[t] += sum[t][0] + sum[t][1]; }
+        l += sum[0] + sum[1];
     };
     // Weight 0 times an infinity is NaN: where some rows do not see every key of entry i, what is infinite or NaN among its values is added to the sums of
     // the rows that see it and cleared in front of the products.
@@ -1038,20 +1005,16 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
         for (int key = 0; key < KEYS; key++)
         {
             if (lacks >> (key / 16) & 1) { continue; }
+            const bool see = sees(p, my_pos, b * KEYS + key);
 #pragma unroll
-            for (int t = 0; t < RT; t++)
+            for (int n = 0; n < DIM / 8; n++)
             {
-                const bool see = sees(p, my_pos[t], b * KEYS + key);
+                const int dim = 8 * n + 4 * h;
+                const u32x2 raw = *(const u32x2*)(vb + key * ROW + (((dim / 8) ^ value_swizzle(key)) << 4) + (dim & 4) * 2);
+                float v[4];
+                unpack4(raw, v);
 #pragma unroll
-                for (int n = 0; n < DIM / 8; n++)
-                {
-                    const int dim = 8 * n + 4 * h;
-                    const u32x2 raw = *(const u32x2*)(vb + key * ROW + (((dim / 8) ^ value_swizzle(key)) << 4) + (dim & 4) * 2);
-                    float v[4];
-                    unpack4(raw, v);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) { out[t][n / 4][n % 4 * 4 + e] += see && !(fabsf(v[e]) < INFINITY) ? v[e] : 0.0f; }
-                }
+                for (int e = 0; e < 4; e++) { out[n / 4][n % 4 * 4 + e] += see && !(fabsf(v[e]) < INFINITY) ? v[e] : 0.0f; }
             }
         }
         lds_barrier();
@@ -1070,18 +1033,18 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     if (begin < end)
     {
         Staged raw_k, raw_v;
-        f32x16 cur[RT][2], next[RT][2];
+        f32x16 cur[2], next[2];
         look_up(begin);
         // where the values of the next entry begin, and whether this one and the next are masked (for what they lack)
         size_t from = of_entry(rows_from, begin), exponents = TYPE == DT_BF16 ? 0 : of_entry(exponents_from, begin);
         bool is_masked = masked(begin, from), next_masked = false;
         int lacks = (int)(from >> 60), next_lacks = 0;
+        // the first entry and the keys of the second, all asked for at once
+        Staged raw_next;
         auto fetch = [&](bool values, uint32_t to, Staged& raw) {
             const Source of = source(values, from, exponents);
 #pragma unroll
             for (int n = 0; n < PIECES; n++) { load(values, n, 1, of, to, raw); }
-#pragma unroll
-            for (int n = 0; n < PIECES; n++) { store(values, n, to, raw); }
         };
         fetch(false, keys_at(begin) + part, raw_k);
         fetch(true, values_at(begin) + part, raw_v);
@@ -1091,7 +1054,14 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
             if constexpr (TYPE != DT_BF16) { exponents = of_entry(exponents_from, begin + 1); }
             next_masked = masked(begin + 1, from);
             next_lacks = (int)(from >> 60);
-            fetch(false, keys_at(begin + 1) + part, raw_k);
+        }
+        fetch(false, keys_at(begin + 1) + part, raw_next);
+#pragma unroll
+        for (int n = 0; n < PIECES; n++)
+        {
+            store(false, n, keys_at(begin) + part, raw_k);
+            store(true, n, values_at(begin) + part, raw_v);
+            store(false, n, keys_at(begin + 1) + part, raw_next);
         }
         arrived();
         if (is_masked) { note_odd(begin); }
@@ -1099,7 +1069,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
         score_products(begin, cur);
         find_top(cur);
         // entry i: its values and the keys of i + 1 are in LDS, `cur` holds its raw scores
-        auto entry = [&](int i, f32x16 (&cur)[RT][2], f32x16 (&next)[RT][2]) {
+        auto entry = [&](int i, f32x16 (&cur)[2], f32x16 (&next)[2]) {
             // behind the last entry: its rows again (FP8) or none (BF16), and scores of what lies there, for nobody
             const int ahead = min(i + 2, end - 1);
             if (((i + 2 - begin) & 63) == 0 && i + 2 < end) { look_up(i + 2); }
@@ -1148,35 +1118,31 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
         }
     }
 
-#pragma unroll
-    for (int t = 0; t < RT; t++)
+    const float total = l + __shfl_xor(l, 32);
+    if (!real) { return; }
+    const size_t at_row = (size_t)token * p.n_q + head;
+    if (rows.n_ranges > 1)
     {
-        const float total = l[t] + __shfl_xor(l[t], 32);
-        if (!real[t]) { continue; }
-        const size_t at_row = (size_t)token[t] * p.n_q + head[t];
-        if (rows.n_ranges > 1)
-        {
-            float* const dst = p.sums(range, at_row, DIM) + 4 * h;
-#pragma unroll
-            for (int d = 0; d < DIM / 32; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) { *(f32x4*)(dst + 32 * d + 2 * e) = f32x4{ out[t][d][e], out[t][d][e + 1], out[t][d][e + 2], out[t][d][e + 3] }; }
-            if (h == 0) { *p.stats(range, at_row, DIM) = make_float2(m[t], total); }
-            continue;
-        }
-        uint16_t* const dst = p.y + (size_t)token[t] * p.ldy + (size_t)head[t] * DIM + 4 * h;
-        const float by = 1.0f / total;
+        float* const dst = p.sums(range, at_row, DIM) + 4 * h;
 #pragma unroll
         for (int d = 0; d < DIM / 32; d++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-            {
-                float v[4];
-#pragma unroll
-                for (int n = 0; n < 4; n++) { v[n] = total == 0.0f ? 0.0f : out[t][d][e + n] * by; }
-                *(u32x2*)(dst + 32 * d + 2 * e) = pack4(v);
-            }
+            for (int e = 0; e < 16; e += 4) { *(f32x4*)(dst + 32 * d + 2 * e) = f32x4{ out[d][e], out[d][e + 1], out[d][e + 2], out[d][e + 3] }; }
+        if (h == 0) { *p.stats(range, at_row, DIM) = make_float2(m, total); }
+        return;
     }
+    uint16_t* const dst = p.y + (size_t)token * p.ldy + (size_t)head * DIM + 4 * h;
+    const float by = 1.0f / total;
+#pragma unroll
+    for (int d = 0; d < DIM / 32; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+        {
+            float v[4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) { v[n] = total == 0.0f ? 0.0f : out[d][e + n] * by; }
+            *(u32x2*)(dst + 32 * d + 2 * e) = pack4(v);
+        }
 }
 
 // Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then parts x kv heads.
@@ -1188,7 +1154,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs
     __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS > T::LDS ? R::LDS : T::LDS];
     static_assert(sizeof(lds) <= 80 * 1024, "two workgroups on a CU");
     const int tiles = p.tiles * a.n_kv, n_tiles = tiles * p.tile_split;
-    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM, 1>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
+    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
     else { attend_part<TYPE, DIM>(a, p, lds, (blockIdx.x - n_tiles) / a.n_kv, (blockIdx.x - n_tiles) % a.n_kv); }
 }
 
@@ -1197,7 +1163,7 @@ template <int DIM>
 __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
 {
     const int kvh = blockIdx.x % a.n_kv, at = blockIdx.x / a.n_kv;
-    const auto rows = tile_rows<128>(a, p, at / 8);
+    const Tile rows = find_tile(a, p, at / 8);
     const int row = rows.row0 + at % 8 * 16 + (threadIdx.x >> 4);
     if (rows.s < 0 || row >= rows.n_rows || rows.n_ranges <= 1) { return; }
     const size_t token = rows.mine.first + row / p.group, head = kvh * p.group + row % p.group, at_row = token * p.n_q + head;
