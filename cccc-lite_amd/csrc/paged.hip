@@ -26,6 +26,7 @@ bool paged_args(const hip_paged_kv* c, PagedArgs& a)
     const bool fp8 = c->type != CCCC_BFLOAT16;
     const size_t rows = (size_t)c->n_kv_heads * c->page_size, dense = rows * c->head_dim * (fp8 ? 1 : 2);
     if (c->page_stride % 16 != 0 || (c->page_stride != 0 && c->page_stride < dense)) { return false; }
+    if (fp8 && (!aligned(c->k_scale, 16) || !aligned(c->v_scale, 16))) { return false; }
     if (fp8 && (!c->k_scale || !c->v_scale || c->scale_stride % 16 != 0 || (c->scale_stride != 0 && c->scale_stride < rows))) { return false; }
     a.k = (const uint8_t*)c->k;
     a.v = (const uint8_t*)c->v;
@@ -164,6 +165,7 @@ int hip_qk_norm_rope_kv_paged_bf16(const hip_paged_kv* cache, const void* q, con
         if (!aligned(p, 16)) { return -1; }
     }
     if ((n_q_heads > 0 && (ldq % 8 != 0 || ldq < (long long)n_q_heads * dim)) || ldk % 8 != 0 || ldv % 8 != 0 || ldk < (long long)a.n_kv * dim || ldv < (long long)a.n_kv * dim) { return -1; }
+    if (n_q_heads > 0 && q_out == q && n_tokens > 1 && ldq != (long long)n_q_heads * dim) { return -1; }       // a row's result would land on another's input
     const int per_wg = 256 * 8 / dim;
     const int parts = (n_q_heads + 2 * a.n_kv + per_wg - 1) / per_wg;
     const long long blocks = (long long)n_tokens * parts;
@@ -225,6 +227,7 @@ int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, 
     const long long width = (long long)n_q_heads * dim;
     if (ldq % 8 != 0 || ldy % 8 != 0 || ldq < width || ldy < width) { return -1; }
     if (n_tokens == 0) { return 0; }
+    if (y == q) { return -1; }
     Plan plan;
     if (!plan_attention(a, keys_per_block(cache), n_q_heads, dim, n_tokens, max_new, window, n_sink, plan)) { return -1; }
     // too little workspace: tiles and sequences in one piece each

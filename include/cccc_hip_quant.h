@@ -381,7 +381,7 @@ typedef struct hip_paged_kv
     int table_stride;        /* entries per sequence in page_table */
     void* k;                 /* pages [n_kv_heads][page_size][head_dim], 16-byte aligned */
     void* v;
-    void* k_scale;           /* FP8: exponent bytes [n_kv_heads][page_size] per page; ignored for BF16 */
+    void* k_scale;           /* FP8: exponent bytes [n_kv_heads][page_size] per page, 16-byte aligned; ignored for BF16 */
     void* v_scale;
     unsigned long long page_stride;  /* bytes from page to page of k and of v, a multiple of 16; 0: dense */
     unsigned long long scale_stride; /* bytes from page to page of the exponent bytes, a multiple of 16; 0: dense */
@@ -392,7 +392,7 @@ typedef struct hip_paged_kv
 
 /* Per-head RMSNorm (NULL, NULL: none) and RoPE of the new tokens' q and k and the append of k and v to the pages.  q, k and v are rows of n_q_heads and
  * n_kv_heads heads with row pitches ldq, ldk, ldv (elements, multiples of 8), so that one projection's output [q | k | v] can be passed as it is; q_out
- * is dense [n_tokens][n_q_heads][head_dim] (q and q_out may be the same dense buffer).  cos_tab, sin_tab BF16 [n_positions][head_dim / 2], the row of a
+ * is dense [n_tokens][n_q_heads][head_dim] (q and q_out may be the same buffer if q is dense too; other overlaps are not allowed).  cos_tab, sin_tab BF16 [n_positions][head_dim / 2], the row of a
  * token's position; a token at a position past n_positions is left out.  Both NULL: no rotation.  n_q_heads 0 (q, q_out NULL): keys and values only.
  * Norm and rotation are FP32 with one rounding, to BF16 or to the codes (hip_qk_norm_rope_kv_rows_bf16 rounds between them as the reference does).
  * 0 for n_tokens 0; pointers 16-byte aligned, else -1. */
@@ -409,7 +409,7 @@ C_EXPORT int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void
 /* Causal GQA attention of the new tokens over the pages of their sequences, keys and values of the new tokens already appended: a token at position p sees
  * positions 0 .. p, with window > 0 only p - window + 1 .. p and the first n_sink ones.  q [n_tokens] rows of n_q_heads heads with row pitch ldq, y likewise
  * with ldy (multiples of 8); scale 1 / sqrt(head_dim).  FP32 scores, softmax and sums, probabilities rounded to BF16 for the product with V, one rounding
- * of the result.  What a token does not see does not reach it, whatever it holds; a token that sees nothing, or whose scores are all minus infinity,
+ * of the result; sums are divided last: they stay finite for |v| up to 2^90.  What a token does not see does not reach it, whatever it holds; a token that sees nothing, or whose scores are all minus infinity,
  * gives 0.  Any number of query heads per kv head up to 64.
  * max_new and max_ctx are the most new tokens and the most rows that any sequence may have (a graph: over all its replays): grids and workspace follow from
  * them, and a sequence with more new tokens than max_new is left out.  workspace: hip_attention_paged_workspace_bytes(the same arguments) bytes, 16-byte

@@ -66,3 +66,28 @@ def test_attention_arguments(setup):
     assert lib.c.hip_attention_paged_bf16(None, p, p, None, 0, 4, 1, 1, 16, 0, 0, 512, 512) == -1
     assert call(n=0) == 0 and not raw.any()
     assert lib.attention_paged_workspace_bytes(make(**good), 3, 1, 1, 16) == 0
+
+
+@pytest.mark.parametrize("kind", [4, 5])
+@pytest.mark.parametrize("name", ["k_scale", "v_scale"])
+def test_alignment_of_exponents(setup, name, kind):
+    lib, make, good, p, raw = setup
+    for off in (1, 2, 8):
+        c = make(**(good | {"type": kind, name: p + off}))
+        assert lib.qk_norm_rope_kv_paged(c, p, p, p, None, None, None, None, 0, p, 4, 1, 512, 256, 256) == -1
+        assert lib.kv_paged_read(c, p, p, 1, 256, 128) == -1
+        assert lib.attention_paged(c, p, p + 1024, None, 0, 4, 1, 1, 16, 0, 0, 512, 512) == -1
+        assert lib.attention_paged_workspace_bytes(c, 4, 1, 1, 16) == 0
+    # of a BF16 cache they are not looked at
+    c = make(**(good | {"type": 3, name: p + 1}))
+    assert lib.kv_paged_read(c, p, p, 0, 256, 128) == 0 and lib.attention_paged_workspace_bytes(c, 4, 1, 1, 16) > 0
+    assert not raw.any()
+
+
+def test_results_over_inputs(setup):
+    """Queries of a wider projection are not rotated onto themselves, where one row's dense result lies on another's queries; attention does not write over its queries."""
+    lib, make, good, p, raw = setup
+    c = make(**good)
+    assert lib.qk_norm_rope_kv_paged(c, p, p + 1024, p + 1536, None, None, None, None, 0, p, 4, 2, 1024, 1024, 1024) == -1
+    assert lib.attention_paged(c, p, p, None, 0, 4, 1, 1, 16, 0, 0, 512, 512) == -1
+    assert not raw.any()
