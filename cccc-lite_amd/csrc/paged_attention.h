@@ -1,7 +1,9 @@
 // Causal attention of the new tokens of a batch of sequences over their pages.
 //   y = sum_k p_k v_k / sum_k p_k,  p_k = exp(scale q k - m),  over the keys that the token sees, m a running maximum.
 // The rows of a kv head are those of the sequence's new tokens and of the query heads that share it: row r is token r / group, head r % group.
-// Two kernels take them, 16 rows or 128 at a time, each with the keys in ranges where there are few rows; a third adds the ranges.
+// One kernel with two forms: sequences of up to 16 rows per kv head (RowsForm), their keys in parts that the last workgroup of a sequence adds up, and tiles of
+// 128 rows of longer ones (TileForm), with ranges of keys where tiles are few, which a second launch adds.  The same sequences in tiles alone, MI355X us: 64 of one
+// token on 1000 to 8000 E4M3 rows 219 for 111, 16 with a window of 4096 48 for 32, one on 4096 BF16 rows 16.7 for 15.1, 8 of five tokens on 500 to 3000 16.9 for 16.9.
 #pragma once
 #include "paged.h"
 
@@ -90,7 +92,8 @@ constexpr int PA_ROWS = 16, PA_TILE = 128, PA_TILE_KEYS = 64;
 // workgroup each.  How many shares a part has follows from those of all sequences, so that long and short ones leave no workgroup with much more than
 // another: about two workgroups' worth of an even split, since a part costs some 5 us besides its keys, but not over PA_PART, which evens out what is
 // left over at the end.  (MI355X, 32 / 8 heads, E4M3, parts of a sequence: 64 sequences of 1000 to 8000 keys 1 113 us, 3 111, 6 123; 16 of 4100 keys 1 35, 2 31,
-// 4 32; 8 of 4000 keys 1 32, 2 24, 4 20.3, 8 20.5.)
+// 4 32; 8 of 4000 keys 1 32, 2 24, 4 20.3, 8 20.5.  PA_PART 9 / 14 / 20 / 32: 64 sequences of 1000 to 8000 keys 111.5 / 109.7 / 109.3 / 114.7 us, 64 of 4500
+// 105.2 / 105.2 / 97.3 / 96.9, 16 of 500 to 16000 46.8 / 54.2 / 54.3 / 54.2, 4 of 32000 BF16 97.8 / 99.2 / 91.9 / 86.0, 64 BF16 191.9 / 189.8 / 193.6 / 197.3.)
 constexpr int PA_PART = 20;
 template <int KEYS>
 struct Parts
@@ -152,7 +155,8 @@ struct Tile
 };
 
 // Tile `tile` of those of all sequences, a sequence's last ones first: they see the most keys.  Where a CU gets two workgroups in all, the second half of
-// the tiles comes in the other order, so that a long one has a short one beside it.  Called by whole waves: a lane per sequence, their tiles added up.
+// the tiles comes in the other order, so that a long one has a short one beside it (MI355X, 512 tiles of 2048 tokens behind 6000: 249 us for 256; with more
+// tiles than that a CU takes the next one when it is done, and the order from long to short is the better one: 2000 tiles of four prompts 142 us for 146).  Called by whole waves: a lane per sequence, their tiles added up.
 __device__ __forceinline__ Tile find_tile(const PagedArgs& a, const PagedAttention& p, int tile)
 {
     Tile r;
@@ -210,7 +214,7 @@ __device__ __forceinline__ u32x2 lds_transposed8(const uint8_t* at)
 
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p; }
 
-// A byte per lane to a dword per lane of LDS; and, unless `wanted` is 0, a KiB from base + off to LDS.
+// Loads from memory into LDS; whoever reads waits for them.  Unless `wanted` is 0, a KiB from base + off:
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void kib_to_lds(uint32_t wanted, uint32_t lds, const uint8_t* base, uint32_t off)
@@ -236,6 +240,7 @@ __device__ __forceinline__ void kibs_to_lds(uint32_t lds, const uint8_t* base, c
                      : : "s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base) : "memory", "m0");
     }
 }
+// a byte per lane to a dword per lane:
 __device__ __forceinline__ void bytes_to_lds(uint32_t lds, const uint8_t* at)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" : : "s"(lds), "v"(at) : "memory", "m0");
@@ -358,13 +363,15 @@ __device__ __forceinline__ void add_parts(int n, uint16_t* y, Part part)
     for (int d = 0; d < PER; d += 4) { *(u32x2*)(y + d) = pack4(sum + d); }
 }
 
-// Up to 16 rows of a kv head: single tokens, or a few.  Bound by the cached rows' way from memory.
+// Up to 16 rows of a kv head: single tokens, or a few.  Bound by the cached rows' way from memory: 64 sequences of 1000 to 8000 E4M3 rows 110 us, 5.3 TB/s (a large
+// copy: 5.1); few or short ones by the chain of launch, place, page, row, flags and parts: one sequence of 4096 BF16 rows 15 us, of which the rows' way takes 3.
 //   A workgroup of four waves takes a range of the sequence's blocks of KEYS keys, a wave every fourth block, each with a pipeline of its own: rows go by
 // direct loads to the wave's part of LDS, keys and values STAGES blocks ahead each, and nothing but the wave's own count of loads in flight is waited for.
 //   scores: v_mfma_f32_16x16x32_bf16, key rows as row operand, the 16 queries as columns: D lane (row j = lane % 16, g = lane / 16) holds keys 4 g .. + 3
 //           of 16.  FP8 keys become BF16 in registers, times their power of two (a lane's operand is one key's): exact.
 //   V p:    the eight weights of a lane in 32 keys (4 g .. + 3 and 16 + 4 g .. + 3) are its column operand as they are; the row operand (dim, the same
 //           keys) comes from transposing reads.  FP8 values' powers of two go to the weights.
+// Rows are read once per kv head and kept out of the way of what is read again (nt): 64 sequences 114 us for 124 without.
 // LDS: chunk c (16 bytes) of row r lies at c ^ swizzle(r), so that the operand reads hit all banks.
 template <int TYPE, int DIM>
 struct RowsForm
@@ -736,7 +743,10 @@ __device__ __forceinline__ void attend_part(const PagedArgs& a, const PagedAtten
     if (shares > 0) { attend_rows<TYPE, DIM>(a, p, lds, s, mine, kvh, (int)((long long)shares * part / parts), (int)((long long)shares * (part + 1) / parts), c, part, parts); }
 }
 
-// 128 rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions.
+// 128 rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions: for a block of 64 keys of 128 dims a wave
+// has 1024 cycles of products, about as many of weights, masks' tests and addresses, and 4 x 254 on the way from LDS that its workgroup shares.  Two workgroups on a
+// CU fill each other's gaps (a block of both 2.15 us, a lone one 1.35): 2048 tokens behind 6000 E4M3 rows 236 us, 1000 TFLOP/s of the 1413 that a
+// large product reaches.  (64 rows per wave, half the way from LDS, do not fit a wave's registers: three times as long.)
 //   A workgroup of four waves takes 128 rows, a wave 32 of them and every key of each block of 64; keys and values reach LDS as BF16, shared by
 // the waves: from a BF16 cache by direct loads, from FP8 through registers, times their powers of two (exact, once per workgroup).
 //   scores: v_mfma_f32_32x32x16_bf16, key rows as row operand, queries as columns: D lane (row j = lane % 32, h = lane / 32), register i holds key
@@ -934,7 +944,9 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
         off = m > -INFINITY ? -m : 0.0f;                       // no key seen yet: every weight is 2^-inf = 0
     };
     // The weights of entry i under the products of entry i + 1, then the products of the weights under the largest scores of i + 1: in each step the
-    // vector unit has work for as long as the matrix core has.
+    // vector unit has work for as long as the matrix core has.  A wave goes before its SIMD's other one from the scores until half of the values' products, so
+    // that the two fall into different halves (MI355X, 2048 tokens behind 6000 E4M3 rows 241 -> 236 us, windowed prompts 144 -> 141; before it in the values'
+    // products instead 247).
     auto advance = [&](int i, const f32x16 (&cur)[2], f32x16 (&next)[2], auto loads, auto stores) {
         constexpr int STEPS = DIM / 16, WEIGHTS = 32 / STEPS, PAIRS = DIM / 64;
         uint32_t key_at = k_at + keys_at(i + 1), value_at = v_at + values_at(i);
@@ -958,6 +970,9 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
         };
 #pragma unroll
         for (int c = 0; c < AHEAD; c++) { read(c); }
+        __builtin_amdgcn_sched_barrier(0);
+        raise();                                                            // while they are on their way
+        __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < STEPS; c++)
@@ -987,6 +1002,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
             for (int k = 0; k < 2; k++)
                 { out[d + k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n][k], pb[u], out[d + k], 0, 0, 0); }
             if (n == 0) { top = -INFINITY; }
+            if (n == N_VALUES / 2) { __builtin_amdgcn_s_setprio(0); }
 #pragma unroll
             for (int e = n * (8 / PAIRS); e < (n + 1) * (8 / PAIRS); e++) { top = fmaxf(top, next[e / 16][e % 16]); }
             asm volatile("" : "+v"(top));
@@ -1082,7 +1098,6 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
                 mask(cur, blocks.block(i), lacks);
                 find_top(cur);
             }
-            raise();
             // a workgroup's loads all at once would hold up its waves: one or two with every step
             constexpr int STEPS = DIM / 16, PER = 2 * PIECES * 2 / STEPS;
             auto loads = [&](int step) {
