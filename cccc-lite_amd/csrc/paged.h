@@ -22,7 +22,7 @@ struct PagedArgs
 };
 
 // Where activation rows t0 .. t0 + N - 1 belong: sequence (-1: to none), position, page (-1: none).  Called by whole waves with one t0: a lane per sequence,
-// so one trip to memory per 64 of them, then one each for the N rows' lengths and pages.  Ranges that are not in order name no sequence, or one whose
+// so one trip to memory for the first 64 and for each 256 more, then one each for the N rows' lengths and pages.  Ranges that are not in order name no sequence, or one whose
 // range has t: a row index never leaves the range that was looked at.
 template <int N>
 struct PagedPlaces
@@ -33,11 +33,19 @@ struct PagedPlaces
     {
 #pragma unroll
         for (int n = 0; n < N; n++) { s[n] = -1; }
-        for (int base = 0; base <= a.n_seqs; base += 64)
-        {
-            const int i = base + (threadIdx.x & 63), start = i <= a.n_seqs ? a.seq_start[i] : 0x7FFFFFFF;
+        auto count = [&](int i, int start) {
 #pragma unroll
-            for (int n = 0; n < N; n++) { s[n] += __builtin_popcountll(__ballot(start <= t0 + n)); }
+            for (int n = 0; n < N; n++) { s[n] += __builtin_popcountll(__ballot(i <= a.n_seqs && start <= t0 + n)); }
+        };
+        const int lane = threadIdx.x & 63;
+        count(lane, a.seq_start[min(lane, a.n_seqs)]);
+        for (int base = 64; base <= a.n_seqs; base += 256)
+        {
+            int start[4];
+#pragma unroll
+            for (int b = 0; b < 4; b++) { start[b] = a.seq_start[min(base + 64 * b + lane, a.n_seqs)]; }
+#pragma unroll
+            for (int b = 0; b < 4; b++) { count(base + 64 * b + lane, start[b]); }
         }
         int at[N], begin[N], end[N], rows[N];
 #pragma unroll

@@ -19,7 +19,7 @@ inline bool aligned(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1))
 bool paged_args(const hip_paged_kv* c, PagedArgs& a)
 {
     if (!c || (c->type != CCCC_BFLOAT16 && c->type != CCCC_FP8_E4M3 && c->type != CCCC_FP8_E5M2) || (c->head_dim != 64 && c->head_dim != 128)) { return false; }
-    if (c->n_kv_heads <= 0 || c->n_kv_heads > 1024 || c->n_pages <= 0 || c->n_seqs <= 0 || c->n_seqs > (1 << 24) || c->table_stride <= 0) { return false; }
+    if (c->n_kv_heads <= 0 || c->n_kv_heads > 1024 || c->n_pages <= 0 || c->n_seqs <= 0 || c->n_seqs > 65536 || c->table_stride <= 0) { return false; }
     if (c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)) != 0) { return false; }
     if (!c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16) || !c->page_table || !c->ctx_len || !c->seq_start) { return false; }
     if (!aligned(c->page_table, 4) || !aligned(c->ctx_len, 4) || !aligned(c->seq_start, 4)) { return false; }
@@ -135,6 +135,7 @@ bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, in
         const long long shares = (keys / keys_per_block + 3 + 3) / 4 + 1, all = shares * a.n_seqs, part = keys_per_block == 32 ? 2 : 1;
         const long long at_once = std::max<long long>(1, slots / a.n_kv);
         if (all > 0x3FFFFFFFLL || (a.n_seqs + 3 * at_once + 1) * a.n_kv * 2 > MOST_BLOCKS) { return false; }
+        if (a.n_seqs > PA_CUT_SEQS) { return true; }
         plan.row_slots = (int)at_once;
         plan.row_parts = (int)(a.n_seqs + std::max<long long>(1, std::min(3 * at_once, all / part)));
         plan.row_bytes = ((size_t)plan.row_parts * a.n_kv * (PA_ROWS * (dim + 2) * 4 + 8) + 15) & ~(size_t)15;

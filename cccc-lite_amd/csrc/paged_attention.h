@@ -57,14 +57,27 @@ struct NewTokens
     int first, n, pos;
 };
 
-__device__ __forceinline__ NewTokens new_tokens(const PagedArgs& a, const PagedAttention& p, int s)
+// What a lane has to read for them of sequence s (any from 0 on; beyond the last: none): asked for first where several are, in one trip.
+struct SeqWords
 {
-    const int begin = a.seq_start[s], end = a.seq_start[s + 1], rows = paged_rows(a, s);       // one trip
-    const int first = max(begin, 0), last = min(end, p.n_tokens);
-    // (compared and not subtracted: ranges may hold anything)
-    if (last <= first || (long long)end - begin > p.max_new) { return { 0, 0, 0 }; }
-    return { first, last - first, rows - (end - first) };
-}
+    int begin = 0, end = 0, rows = 0;
+
+    __device__ __forceinline__ SeqWords() {}
+    __device__ __forceinline__ SeqWords(const PagedArgs& a, int s)
+    {
+        const int at = min(s, a.n_seqs - 1);
+        begin = a.seq_start[at];
+        end = a.seq_start[at + 1];
+        rows = a.ctx_len[at];
+    }
+    __device__ __forceinline__ NewTokens tokens(const PagedArgs& a, const PagedAttention& p, int s) const
+    {
+        const int first = max(begin, 0), last = min(end, p.n_tokens);
+        // (compared and not subtracted: ranges may hold anything)
+        if (s >= a.n_seqs || last <= first || (long long)end - begin > p.max_new) { return { 0, 0, 0 }; }
+        return { first, last - first, max(min(rows, a.max_ctx), 0) - (end - first) };
+    }
+};
 
 // The blocks of SIZE keys that tokens at positions lo .. hi see: the first `sinks` ones, then from block sinks + skip on; n in all.
 template <int SIZE>
@@ -95,13 +108,17 @@ constexpr int PA_ROWS = 16, PA_TILE = 128, PA_TILE_KEYS = 64;
 // 4 32; 8 of 4000 keys 1 32, 2 24, 4 20.3, 8 20.5.  PA_PART 9 / 14 / 20 / 32: 64 sequences of 1000 to 8000 keys 111.5 / 109.7 / 109.3 / 114.7 us, 64 of 4500
 // 105.2 / 105.2 / 97.3 / 96.9, 16 of 500 to 16000 46.8 / 54.2 / 54.3 / 54.2, 4 of 32000 BF16 97.8 / 99.2 / 91.9 / 86.0, 64 BF16 191.9 / 189.8 / 193.6 / 197.3.)
 constexpr int PA_PART = 20;
+
+// The most sequences whose keys are cut into parts: more are a workgroup each, enough of them to fill the GPU, and nobody has to look at all of them.
+// MI355X, 32 / 8 heads E4M3 us, cut / one each: 64 of 100 to 8000 105 / 107, 256 355 / 363, 256 of 200 to 2000 109 / 106; 8 / 1 heads, 100
+// to 8000: 64 24 / 52, 128 35 / 54, 256 64 / 60.  Beyond, with a trip to memory for each 64 sequences: 512 of 200 to 2000 257 / 199, 1024 606 / 381.
+constexpr int PA_CUT_SEQS = 256;
+
 template <int KEYS>
 struct Parts
 {
-    int per = 1;                                                            // shares of a part
-    int base = 0, before = 0;                                               // the batch of sequences base + lane, and parts of those before it
-    int shares = 0, parts = 0, upto = 0;                                    // of the lane's sequence, and parts with those before it in the batch
-    NewTokens mine = { 0, 0, 0 };                                           // the lane's
+    int s = -1, part = 0, parts = 1, shares = 0;                            // part `part` of the `parts` that the shares of sequence s are in; s < 0: none
+    NewTokens mine = { 0, 0, 0 };
 
     __device__ __forceinline__ static KeyBlocks<KEYS> keys(const PagedAttention& p, const NewTokens& n) { return KeyBlocks<KEYS>(p, n.pos, n.pos + n.n - 1); }
     __device__ __forceinline__ static int shares_of(const PagedAttention& p, const NewTokens& n)
@@ -109,40 +126,50 @@ struct Parts
         const int rows = n.n * p.group;
         return rows == 0 || rows > PA_ROWS ? 0 : max((keys(p, n).n + 3) / 4, 1);
     }
-    __device__ __forceinline__ int batch_end() const { return before + __builtin_amdgcn_readlane(upto, 63); }
-    // whole waves from here on
-    __device__ __forceinline__ void load(const PagedArgs& a, const PagedAttention& p)
+    // Part c of all.  Whole waves, four sequences per lane.
+    __device__ __forceinline__ Parts(const PagedArgs& a, const PagedAttention& p, int c)
     {
-        const int s = base + (int)(threadIdx.x & 63);
-        mine = s < a.n_seqs ? new_tokens(a, p, s) : NewTokens{ 0, 0, 0 };
-        shares = shares_of(p, mine);
-    }
-    __device__ __forceinline__ void cut()
-    {
-        parts = (shares + per - 1) / per;
-        upto = add_up_lanes(parts);
-    }
-    __device__ __forceinline__ void take(const PagedArgs& a, const PagedAttention& p)
-    {
-        int total = 0;
-        for (base = 0; base < a.n_seqs; base += 64)
+        constexpr int BATCHES = PA_CUT_SEQS / 64;
+        const int lane = threadIdx.x & 63;
+        SeqWords words[BATCHES];
+        NewTokens tokens[BATCHES];
+        int have[BATCHES], total = 0;
+        words[0] = SeqWords(a, lane);
+        if (a.n_seqs > 64)
         {
-            load(a, p);
-            total += __builtin_amdgcn_readlane(add_up_lanes(shares), 63);
+#pragma unroll
+            for (int b = 1; b < BATCHES; b++) { words[b] = SeqWords(a, 64 * b + lane); }
+        }
+#pragma unroll
+        for (int b = 0; b < BATCHES; b++)
+        {
+            if (b != 0 && a.n_seqs <= 64 * b) { break; }
+            tokens[b] = words[b].tokens(a, p, 64 * b + lane);
+            have[b] = shares_of(p, tokens[b]);
+            total += __builtin_amdgcn_readlane(add_up_lanes(have[b]), 63);
         }
         auto split = [&](int n) { return (total + n - 1) / n; };
-        per = max(max(split(3 * p.row_slots), min(PA_PART, split((p.row_slots + 1) / 2))), KEYS == 32 ? 2 : 1);
+        int per = max(max(split(3 * p.row_slots), min(PA_PART, split((p.row_slots + 1) / 2))), KEYS == 32 ? 2 : 1);
         per = max(per, split(max(p.row_parts - a.n_seqs, 1)));              // no more parts than workgroups
-        base = 0;
-        if (a.n_seqs > 64) { load(a, p); }
-        cut();
-    }
-    __device__ __forceinline__ void next(const PagedArgs& a, const PagedAttention& p)
-    {
-        before = batch_end();
-        base += 64;
-        load(a, p);
-        cut();
+        int before = 0;
+#pragma unroll
+        for (int b = 0; b < BATCHES; b++)
+        {
+            if (b != 0 && a.n_seqs <= 64 * b) { break; }
+            const int n = (have[b] + per - 1) / per, upto = before + add_up_lanes(n);
+            const unsigned long long past = __ballot(upto > c);
+            if (past != 0)
+            {
+                const int of = __builtin_ctzll(past);
+                s = 64 * b + of;
+                parts = __builtin_amdgcn_readlane(n, of);
+                part = c - (__builtin_amdgcn_readlane(upto, of) - parts);
+                shares = __builtin_amdgcn_readlane(have[b], of);
+                mine = { __builtin_amdgcn_readlane(tokens[b].first, of), __builtin_amdgcn_readlane(tokens[b].n, of), __builtin_amdgcn_readlane(tokens[b].pos, of) };
+                break;
+            }
+            before = __builtin_amdgcn_readlane(upto, 63);
+        }
     }
 };
 
@@ -156,37 +183,52 @@ struct Tile
 
 // Tile `tile` of those of all sequences, a sequence's last ones first: they see the most keys.  Where a CU gets two workgroups in all, the second half of
 // the tiles comes in the other order, so that a long one has a short one beside it (MI355X, 512 tiles of 2048 tokens behind 6000: 249 us for 256; with more
-// tiles than that a CU takes the next one when it is done, and the order from long to short is the better one: 2000 tiles of four prompts 142 us for 146).  Called by whole waves: a lane per sequence, their tiles added up.
+// tiles than that a CU takes the next one when it is done, and the order from long to short is the better one: 2000 tiles of four prompts 142 us for 146).  Called by whole waves: a lane per
+// sequence, 256 of them per trip to memory, their tiles added up.
 __device__ __forceinline__ Tile find_tile(const PagedArgs& a, const PagedAttention& p, int tile)
 {
     Tile r;
     const int lane = threadIdx.x & 63;
     if (p.snake && tile >= (p.tiles + 1) / 2) { tile = p.tiles - 1 - (tile - (p.tiles + 1) / 2); }
-    for (int base = 0; base < a.n_seqs; base += 64)
+    for (int base = 0; base < a.n_seqs; base += 256)
     {
-        const NewTokens mine = base + lane < a.n_seqs ? new_tokens(a, p, base + lane) : NewTokens{ 0, 0, 0 };
-        const int rows = mine.n * p.group, tiles = rows > p.min_rows ? (rows + PA_TILE - 1) / PA_TILE : 0;
-        const int upto = add_up_lanes(tiles);
-        const unsigned long long past = __ballot(upto > tile);
-        if (past != 0)
+        SeqWords words[4];                                                  // of 256 sequences, in one trip
+        words[0] = SeqWords(a, base + lane);
+        if (base + 64 < a.n_seqs)
         {
-            const int at = __builtin_ctzll(past);
-            r.s = uniform(base + at);
-            r.mine = { __builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.n, at), __builtin_amdgcn_readlane(mine.pos, at) };
-            r.row0 = uniform(__builtin_amdgcn_readlane(upto, at) - 1 - tile) * PA_TILE;
-            r.n_rows = uniform(r.mine.n * p.group);
-            r.lo = uniform(r.mine.pos + r.row0 / p.group);
-            r.hi = uniform(r.mine.pos + min(r.row0 + PA_TILE - 1, r.n_rows - 1) / p.group);
-            r.blocks = KeyBlocks<PA_TILE_KEYS>(p, r.lo, r.hi);
-            r.blocks.n = uniform(r.blocks.n);
-            r.blocks.sinks = uniform(r.blocks.sinks);
-            r.blocks.skip = uniform(r.blocks.skip);
-            r.per = max((r.blocks.n + p.tile_split - 1) / p.tile_split, 4);
-            r.n_ranges = max((r.blocks.n + r.per - 1) / r.per, 1);
-            return r;
+#pragma unroll
+            for (int b = 1; b < 4; b++) { words[b] = SeqWords(a, base + 64 * b + lane); }
         }
-        tile -= __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+        {
+            if (base + 64 * b >= a.n_seqs) { break; }
+            const NewTokens mine = words[b].tokens(a, p, base + 64 * b + lane);
+            const int rows = mine.n * p.group, tiles = rows > p.min_rows ? (rows + PA_TILE - 1) / PA_TILE : 0;
+            const int upto = add_up_lanes(tiles);
+            const unsigned long long past = __ballot(upto > tile);
+            if (past != 0)
+            {
+                const int at = __builtin_ctzll(past);
+                r.s = uniform(base + 64 * b + at);
+                r.mine = { __builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.n, at), __builtin_amdgcn_readlane(mine.pos, at) };
+                r.row0 = uniform(__builtin_amdgcn_readlane(upto, at) - 1 - tile) * PA_TILE;
+                break;
+            }
+            tile -= __builtin_amdgcn_readlane(upto, 63);
+        }
+        if (r.s >= 0) { break; }
     }
+    if (r.s < 0) { return r; }
+    r.n_rows = uniform(r.mine.n * p.group);
+    r.lo = uniform(r.mine.pos + r.row0 / p.group);
+    r.hi = uniform(r.mine.pos + min(r.row0 + PA_TILE - 1, r.n_rows - 1) / p.group);
+    r.blocks = KeyBlocks<PA_TILE_KEYS>(p, r.lo, r.hi);
+    r.blocks.n = uniform(r.blocks.n);
+    r.blocks.sinks = uniform(r.blocks.sinks);
+    r.blocks.skip = uniform(r.blocks.skip);
+    r.per = max((r.blocks.n + p.tile_split - 1) / p.tile_split, 4);
+    r.n_ranges = max((r.blocks.n + r.per - 1) / r.per, 1);
     return r;
 }
 
@@ -716,31 +758,16 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
 template <int TYPE, int DIM>
 __device__ __forceinline__ void attend_part(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int c, int kvh)
 {
-    constexpr int KEYS = RowsForm<TYPE, DIM>::KEYS;
-    int s = c, part = 0, parts = 1, shares;
-    NewTokens mine;
+    typedef Parts<RowsForm<TYPE, DIM>::KEYS> P;
     if (p.row_parts == 0)
     {
-        mine = new_tokens(a, p, c);
-        shares = uniform(Parts<KEYS>::shares_of(p, mine));
+        const NewTokens mine = SeqWords(a, c).tokens(a, p, c);
+        const int shares = uniform(P::shares_of(p, mine));
+        if (shares > 0) { attend_rows<TYPE, DIM>(a, p, lds, c, mine, kvh, 0, shares, 0, 0, 1); }
+        return;
     }
-    else
-    {
-        Parts<KEYS> all;
-        all.take(a, p);
-        while (all.batch_end() <= c)
-        {
-            if (all.base + 64 >= a.n_seqs) { return; }
-            all.next(a, p);
-        }
-        const int of = __builtin_ctzll(__ballot(all.before + all.upto > c));
-        s = all.base + of;
-        parts = __builtin_amdgcn_readlane(all.parts, of);
-        part = c - (all.before + __builtin_amdgcn_readlane(all.upto, of) - parts);
-        shares = __builtin_amdgcn_readlane(all.shares, of);
-        mine = { __builtin_amdgcn_readlane(all.mine.first, of), __builtin_amdgcn_readlane(all.mine.n, of), __builtin_amdgcn_readlane(all.mine.pos, of) };
-    }
-    if (shares > 0) { attend_rows<TYPE, DIM>(a, p, lds, s, mine, kvh, (int)((long long)shares * part / parts), (int)((long long)shares * (part + 1) / parts), c, part, parts); }
+    const P of(a, p, c);
+    if (of.s >= 0) { attend_rows<TYPE, DIM>(a, p, lds, of.s, of.mine, kvh, (int)((long long)of.shares * of.part / of.parts), (int)((long long)of.shares * (of.part + 1) / of.parts), c, of.part, of.parts); }
 }
 
 // 128 rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions: for a block of 64 keys of 128 dims a wave

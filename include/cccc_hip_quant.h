@@ -377,7 +377,7 @@ typedef struct hip_paged_kv
     int n_kv_heads;
     int page_size;           /* rows per page: a power of two from 16 to 4096 */
     int n_pages;
-    int n_seqs;
+    int n_seqs;              /* up to 65536 */
     int table_stride;        /* entries per sequence in page_table */
     void* k;                 /* pages [n_kv_heads][page_size][head_dim], 16-byte aligned */
     void* v;

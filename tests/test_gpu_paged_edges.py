@@ -344,3 +344,32 @@ def test_beside_the_contiguous_cache(gpu, pkg):
     b.pool = {n: b.download(n) for n in ("k", "v")}
     ref, bound = attend(b, f(mine), n_q)
     assert (np.abs(got - ref) <= bound).all()
+
+
+@pytest.mark.parametrize("n_seqs,kind,long,chunk", [(255, E4M3, 0, 0), (256, BF16, 255, 0), (257, E5M2, 256, 0), (257, BF16, 3, 40), (256, E4M3, 200, 70), (600, E4M3, 599, 0), (700, E5M2, 320, 65)])
+def test_hundreds_of_sequences(gpu, pkg, n_seqs, kind, long, chunk):
+    """Both sides of the most sequences whose keys are cut into parts, one much longer than the rest; a chunk far down the list; every operator."""
+    rng = np.random.default_rng(n_seqs + kind)
+    new = [int(n) for n in rng.integers(0, 3, n_seqs)]
+    new[long] = 1
+    if chunk: new[n_seqs - 9] = chunk
+    ctx = [n + int(c) for n, c in zip(new, rng.integers(0, 60, n_seqs))]
+    ctx[long] = 1500
+    b = Batch(n_seqs, kind, 64, 2, 16, new, ctx).upload(*gpu[:2])
+    check_attend(gpu, pkg, b, 4)
+    torch, dev, lib = gpu
+    out = torch.zeros(2, b.tokens, 2, 64, dtype=torch.int16, device=dev)
+    assert lib.kv_paged_read(b.descriptor(pkg), ptr(out[0]), ptr(out[1]), b.tokens, 128, 64) == 0
+    back, values = from_bf16(out.cpu().numpy().view(np.uint16)), {n: b.values(n) for n in ("k", "v")}
+    for t, s, pos in b.slots():
+        for i, name in enumerate(("k", "v")): assert np.array_equal(back[i, t], values[name][b.table[s, pos // 16], :, pos % 16])
+    # the rows appended to an empty pool, BF16, no norm and no rotation: what was put in lies at the tokens' places and nothing else changed
+    e = Batch(n_seqs, BF16, 64, 2, 16, new, ctx).upload(torch, dev)
+    for name in ("k", "v"): e.dev[name].zero_()
+    rows = put(torch, dev, to_bf16(rng.standard_normal((e.tokens, 4, 64))))
+    assert lib.qk_norm_rope_kv_paged(e.descriptor(pkg), None, ptr(rows), ptr(rows) + 256, None, None, None, None, 0, None, 0, e.tokens, 0, 256, 256) == 0
+    got, want = {n: e.dev[n].cpu().numpy() for n in ("k", "v")}, {n: np.zeros_like(e.dev[n].cpu().numpy()) for n in ("k", "v")}
+    x = rows.cpu().numpy().reshape(e.tokens, 2, 2, 64)
+    for t, s, pos in e.slots():
+        for i, name in enumerate(("k", "v")): want[name][e.table[s, pos // 16], :, pos % 16] = x[t, i]
+    for name in ("k", "v"): assert np.array_equal(got[name].reshape(want[name].shape), want[name])

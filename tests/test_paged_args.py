@@ -91,3 +91,14 @@ def test_results_over_inputs(setup):
     assert lib.qk_norm_rope_kv_paged(c, p, p + 1024, p + 1536, None, None, None, None, 0, p, 4, 2, 1024, 1024, 1024) == -1
     assert lib.attention_paged(c, p, p, None, 0, 4, 1, 1, 16, 0, 0, 512, 512) == -1
     assert not raw.any()
+
+
+def test_most_sequences(setup):
+    lib, make, good, p, raw = setup
+    assert lib.attention_paged_workspace_bytes(make(**(good | dict(n_seqs=256))), 4, 256, 1, 16) > 0
+    for n, status in ((65536, 0), (65537, -1), (2 ** 31 - 1, -1)):
+        c = make(**(good | dict(n_seqs=n)))
+        assert lib.qk_norm_rope_kv_paged(c, p, p, p, None, None, None, None, 0, p, 4, 0, 512, 256, 256) == status
+        assert lib.kv_paged_read(c, p, p, 0, 256, 128) == status
+        assert lib.attention_paged(c, p, p, None, 0, 4, 0, 1, 16, 0, 0, 512, 512) == status
+    assert not raw.any()
