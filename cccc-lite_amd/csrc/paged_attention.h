@@ -508,14 +508,21 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
 #pragma unroll
     for (int d = 0; d < DIM / 16; d++) { out[d] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f }; }
 
+    // which 16 rows of block n have no page
+    auto lacks_of = [&](int n) {
+        int lacks = 0;
+#pragma unroll
+        for (int part = 0; part < TILES; part++) { lacks |= (int)((uint32_t)__builtin_amdgcn_readlane((int)(rows_from >> 32), n % BATCH * TILES + part) >> 31) << part; }
+        return lacks;
+    };
+    int kept = 0;
+
     auto block = [&](int n) {
         const uint8_t* const kb = my_lds + n % STAGES * SIDE;
         const uint8_t* const vb = my_lds + VALUES + n % STAGES * SIDE;
         const uint8_t* const exponents = my_lds + EXPONENTS + n % STAGES * F::EXPONENTS;
         const int entry = begin + wave + 4 * n;
-        int lacks = 0;
-#pragma unroll
-        for (int part = 0; part < TILES; part++) { lacks |= (int)((uint32_t)__builtin_amdgcn_readlane((int)(rows_from >> 32), n % BATCH * TILES + part) >> 31) << part; }
+        const int lacks = STAGES == 2 && n % BATCH == BATCH - 1 && n + 1 < n_mine ? kept : lacks_of(n);
         // what was asked for behind the keys of n may still be on its way
         if (STAGES == 2 && n + 1 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(2 * LOADS + KEY_LOADS) : "memory"); }
         else { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS) : "memory"); }
@@ -549,7 +556,11 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         if (n + STAGES < n_mine)
         {
             asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");           // the keys have been read
-            if ((n + STAGES) % BATCH == 0) { look_up(n + STAGES); }
+            if ((n + STAGES) % BATCH == 0)
+            {
+                if (STAGES == 2) { kept = lacks_of(n + 1); }               // the one block whose place in the list is overwritten before its turn
+                look_up(n + STAGES);
+            }
             stage(n + STAGES, false);
         }
         if (STAGES == 2 && n + 2 < n_mine) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS + 2 * KEY_LOADS) : "memory"); }

@@ -373,3 +373,37 @@ def test_hundreds_of_sequences(gpu, pkg, n_seqs, kind, long, chunk):
     for t, s, pos in e.slots():
         for i, name in enumerate(("k", "v")): want[name][e.table[s, pos // 16], :, pos % 16] = x[t, i]
     for name in ("k", "v"): assert np.array_equal(got[name].reshape(want[name].shape), want[name])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_that_are_missing_far_down_a_sequence(gpu, pkg, kind, dim, new):
+    """Runs of missing pages around every place where a wave or a tile looks up the next pages of its list (32, 64 and 128 blocks of a wave, 64 of a tile), keys in one piece and in parts."""
+    torch, dev, lib = gpu
+    ctx, n_q, n_kv = 9000, 2, 1
+    b = Batch(dim + kind + new, kind, dim, n_kv, 16, [new], [ctx])
+    rows = {name: b.rows(name, 0) for name in ("k", "v")}
+    lost = np.zeros(ctx, dtype=bool)
+    # the four waves' blocks n of 32 or 64 keys: keys 128 n or 256 n on
+    for n in (7, 8, 15, 16, 31, 32, 63):
+        for first in (128 * n, 256 * n):
+            if first + 256 <= ctx - 100: lost[first:first + 128] = True
+    b.table[0, np.flatnonzero(lost[::16])] = -1
+    b.upload(torch, dev)
+    q = from_bf16(to_bf16(b.rng.standard_normal((new, n_q, dim))))
+    dq = put(torch, dev, to_bf16(q))
+    need = lib.attention_paged_workspace_bytes(b.descriptor(pkg), n_q, new, new, ctx)
+    ws = torch.full((need + 16,), 0x5A, dtype=torch.uint8, device=dev)
+    for given in (0, need):
+        y = torch.zeros(new, n_q, dim, dtype=torch.int16, device=dev)
+        assert lib.attention_paged(b.descriptor(pkg), ptr(dq), ptr(y), ptr(ws) if given else None, given, n_q, new, new, ctx, 0, 0, n_q * dim, n_q * dim) == 0
+        got = from_bf16(y.cpu().numpy().view(np.uint16))
+        for t in (0, new // 2, new - 1):
+            seen = ~lost[:ctx - new + t + 1]
+            k, v = rows["k"][0, :len(seen)][seen], rows["v"][0, :len(seen)][seen]
+            for h in range(n_q):
+                w = np.exp(k @ q[t, h] / np.sqrt(dim) - (k @ q[t, h] / np.sqrt(dim)).max())
+                w /= w.sum()
+                # a probability's and the result's rounding, 2^-8 each, and room for FP32
+                assert (np.abs(got[t, h] - w @ v) <= 2.0 ** -7 * w @ np.abs(v) + 2.0 ** -8 * np.abs(w @ v)).all(), (given, t, h)
