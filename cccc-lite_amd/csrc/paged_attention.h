@@ -391,11 +391,14 @@ __device__ __forceinline__ void add_parts(int n, uint16_t* y, Part part)
         for (int r = 0; r < AT_ONCE; r++)
         {
             const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
-            if (r0 + r < n && w != 0.0f)                                    // a part without a key has weight 0
+            if (r0 + r < n)
             {
-                l += w * stat[r].y;
+                l += w * stat[r].y;                                         // NaN where a score is, also if all are: the maximum is then minus infinity, the weight 0
+                if (w != 0.0f)                                              // a part without a key has weight 0
+                {
 #pragma unroll
-                for (int d = 0; d < PER; d++) { sum[d] += w * (d % 2 ? v[r][d / 2].y : v[r][d / 2].x); }
+                    for (int d = 0; d < PER; d++) { sum[d] += w * (d % 2 ? v[r][d / 2].y : v[r][d / 2].x); }
+                }
             }
         }
     }
