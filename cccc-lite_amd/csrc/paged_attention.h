@@ -391,14 +391,11 @@ __device__ __forceinline__ void add_parts(int n, uint16_t* y, Part part)
         for (int r = 0; r < AT_ONCE; r++)
         {
             const float w = __builtin_amdgcn_exp2f(stat[r].x - base);
-            if (r0 + r < n)
+            if (r0 + r < n)                                                 // also with weight 0: a part without a key has sums of 0, one with infinities or NaN makes them NaN
             {
                 l += w * stat[r].y;                                         // NaN where a score is, also if all are: the maximum is then minus infinity, the weight 0
-                if (w != 0.0f)                                              // a part without a key has weight 0
-                {
 #pragma unroll
-                    for (int d = 0; d < PER; d++) { sum[d] += w * (d % 2 ? v[r][d / 2].y : v[r][d / 2].x); }
-                }
+                for (int d = 0; d < PER; d++) { sum[d] += w * (d % 2 ? v[r][d / 2].y : v[r][d / 2].x); }
             }
         }
     }
@@ -730,7 +727,7 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         {
             sum[d] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; w++) { sum[d] += weight[w] != 0.0f ? weight[w] * sums[(w * 16 + r) * SUM + d0 + d] : 0.0f; }
+            for (int w = 0; w < 4; w++) { sum[d] += weight[w] * sums[(w * 16 + r) * SUM + d0 + d]; }      // also with weight 0, as in add_parts
         }
         if (n_parts > 1)
         {

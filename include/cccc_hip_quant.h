@@ -410,7 +410,8 @@ C_EXPORT int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void
  * positions 0 .. p, with window > 0 only p - window + 1 .. p and the first n_sink ones.  q [n_tokens] rows of n_q_heads heads with row pitch ldq, y likewise
  * with ldy (multiples of 8); scale 1 / sqrt(head_dim).  FP32 scores, softmax and sums, probabilities rounded to BF16 for the product with V, one rounding
  * of the result; sums are divided last: they stay finite for |v| up to 2^90.  What a token does not see does not reach it, whatever it holds; a token that sees nothing, or whose scores are all minus infinity,
- * gives 0.  Any number of query heads per kv head up to 64.
+ * gives 0.  Otherwise a NaN score, or one of plus infinity, makes a token's head NaN, and an infinite or NaN value that a token sees leaves its dim not finite, however small the
+ * weight.  Any number of query heads per kv head up to 64.
  * max_new and max_ctx are the most new tokens and the most rows that any sequence may have (a graph: over all its replays): grids and workspace follow from
  * them, and a sequence with more new tokens than max_new is left out.  workspace: hip_attention_paged_workspace_bytes(the same arguments) bytes, 16-byte
  * aligned, content between calls of no matter; calls that share one must be ordered.  With fewer bytes, or NULL and 0, the keys are split over fewer workgroups.

@@ -76,3 +76,56 @@ def test_a_query_that_is_not_a_number_beside_others(gpu, pkg, kind, dim):
         got = from_bf16(run_attend(gpu, pkg, b, q, 8, workspace=workspace))
         odd = np.isnan(q).any(-1)
         assert np.isnan(got[odd]).all() and (np.abs(got - want) <= bound)[~odd].all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [1, 5])
+def test_splits_of_which_every_key_is_not_a_number(gpu, pkg, kind, new):
+    """The first 64, 128, ... rows of keys are NaN: for some of them whole parts and ranges are, and no key beside them.  Every token sees them."""
+    torch, dev, lib = gpu
+    n_q, dim, ctx = 4, 128, 2000
+    b = Batch(kind + new, kind, dim, 1, 16, [new], [ctx]).upload(torch, dev)
+    assert split(gpu, pkg, b, n_q)
+    q = from_bf16(to_bf16(b.rng.standard_normal((b.tokens, n_q, dim))))
+    assert np.isfinite(from_bf16(run_attend(gpu, pkg, b, q, n_q))).all()
+    wild = 0x7FC0 if kind == BF16 else 0x7F
+    for upto in range(64, ctx - 64, 64):
+        pos = np.arange(upto - 64, upto)
+        b.dev["k"][torch.from_numpy(b.table[0, pos // 16]).long(), 0, torch.from_numpy(pos % 16), 9] = wild
+        assert np.isnan(from_bf16(run_attend(gpu, pkg, b, q, n_q))).all(), upto
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", NEW)
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("first,last", [(1024, 1088), (1024, 1536), (896, 2048)])
+def test_values_that_are_infinite_where_weights_vanish(gpu, pkg, kind, dim, new, workspace, first, last):
+    """A block, a part or more whose scores lie so far below the rest that their weights are 0 in 32 bits, with values that are infinite or NaN in a few dims: those dims are not finite, whether
+    or not the keys are split, and the others are as the formula."""
+    n_q, n_kv = 4, 2
+    b = Batch(dim + kind + new + first, kind, dim, n_kv, 16, [new], [4000])
+    rows = {name: [b.rows(name, 0)] for name in ("k", "v")}
+    pos = np.arange(first, last)
+    page, row = b.table[0, pos // 16], pos % 16
+    # 8 times the key's first element over 8 or 11: a score under -600, all others within some 10
+    if kind == BF16: b.pool["k"][page, 1, row, 0] = to_bf16(np.float32(-1024.0))
+    else:
+        b.pool["k"][page, 1, row] = 0
+        b.pool["k"][page, 1, row, 0] = 0xB8 if kind == E4M3 else 0xBC           # -1
+        b.scale["k"][page, 1, row] = 127 + 10
+    b.pool["v"][page, 1, row, 3::17] = {BF16: 0x7F80, E4M3: 0x7F, E5M2: 0x7C}[kind]
+    # the reference: scores of -100 or so, e^-100 of the sum, which the bound does not notice
+    rows["k"][0][1, pos] = 0.0
+    rows["k"][0][1, pos, 0] = -100.0 * np.sqrt(dim) / 8.0
+    b.upload(*gpu[:2])
+    assert split(gpu, pkg, b, n_q)
+    q = np.zeros((b.tokens, n_q, dim))
+    q[:, :, 0] = 8.0
+    q[:, :, 1:] = from_bf16(to_bf16(b.rng.standard_normal((b.tokens, n_q, dim - 1)) * 0.25))
+    got = from_bf16(run_attend(gpu, pkg, b, q, n_q, workspace=workspace))
+    want, bound = attend(b, q, n_q, rows=rows)
+    reached = np.zeros(got.shape, dtype=bool)
+    reached[:, 2:, 3::17] = True
+    assert not np.isfinite(got[reached]).any()
+    assert (np.abs(got - want) <= bound)[~reached].all()
