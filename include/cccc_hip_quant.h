@@ -358,11 +358,12 @@ C_EXPORT int hip_argmax_pick_embed_bf16(const void* workspace, unsigned int n, v
  * or a whole chunk; rows held as BF16 or, quantised as they are written, as FP8.  Activations are token-major BF16.
  *
  * What a call is told about the batch lies in device memory, so that a captured graph can be replayed with other lengths and pages:
- *   seq_start int32 [n_seqs + 1]: rows seq_start[s] .. seq_start[s + 1] - 1 of the activations are the new tokens of sequence s (none: an empty range).
- *                   Rows before the first or behind the last sequence, up to n_tokens, are left as they were.
+ *   seq_start int32 [n_seqs + 1], ascending: rows seq_start[s] .. seq_start[s + 1] - 1 of the activations are the new tokens of sequence s (none: an empty range).
+ *                   Rows before the first or behind the last sequence, up to n_tokens, are left as they were.  (Where the array does not ascend, rows that no range holds are
+ *                   left as they were too, and which of the others are computed is not said.)
  *   ctx_len   int32 [n_seqs]: rows of the sequence in the cache, its new tokens included; those are the last positions.
  *   page_table int32 [n_seqs][table_stride]: position `pos` lies in page page_table[s][pos / page_size], at row pos % page_size.  Sequences may share pages.
- * A length beyond table_stride * page_size (for the attention also max_ctx) is cut to it.  A page outside 0 .. n_pages - 1 is never touched: its rows are not
+ * A length beyond table_stride * page_size or 2^30 (for the attention also max_ctx) is cut to it.  A page outside 0 .. n_pages - 1 is never touched: its rows are not
  * written, read back as 0 and seen by no token; likewise new tokens at negative positions (more new tokens than ctx_len).
  *
  * FP8 rows: codes c = fp8(x / 2^e), nearest even, one exponent byte e + 127 per row and kv head, 2^e the smallest power of two >= 2^-100 for which the row's
@@ -415,7 +416,10 @@ C_EXPORT int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void
  * max_new and max_ctx are the most new tokens and the most rows that any sequence may have (a graph: over all its replays): grids and workspace follow from
  * them, and a sequence with more new tokens than max_new is left out.  workspace: hip_attention_paged_workspace_bytes(the same arguments) bytes, 16-byte
  * aligned, content between calls of no matter; calls that share one must be ordered.  With fewer bytes, or NULL and 0, the keys are split over fewer workgroups.
- * y must not overlap q.  0 for n_tokens 0. */
+ * Up to 256 sequences the keys of short ones (16 rows of new tokens x query heads per kv head, at most) are split by the lengths of all; more sequences are a workgroup each and kv head, so that
+ * one that is much longer than the rest sets the time of the call: it is better called apart.
+ * y must not overlap q.  0 for n_tokens 0.  -1 also where the grid would pass what a launch can have: n_tokens * n_q_heads of 2^24 and more, n_seqs * n_kv_heads from 2^23 on (2^17
+ * where max_new lets sequences have more than 16 rows per kv head), n_seqs * max_ctx (with a window: * what it leaves) from 2^37 on. */
 C_EXPORT unsigned long long hip_attention_paged_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink);
 C_EXPORT int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, void* workspace, unsigned long long workspace_bytes,
                                       int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink, int ldq, int ldy);
