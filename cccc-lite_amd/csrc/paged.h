@@ -21,6 +21,9 @@ struct PagedArgs
     int max_ctx;                    // rows a sequence may have: the table's, and the caller's limit
 };
 
+// Rows of a sequence in the cache, of its length as it is stored.
+__device__ __forceinline__ int paged_rows(const PagedArgs& a, int ctx_len) { return max(min(ctx_len, a.max_ctx), 0); }
+
 // Where activation rows t0 .. t0 + N - 1 belong: sequence (-1: to none), position, page (-1: none).  Called by whole waves with one t0: a lane per sequence,
 // so one trip to memory for the first 64 and for each 256 more, then one each for the N rows' lengths and pages.  Ranges that are not in order name no sequence, or one whose
 // range has t: a row index never leaves the range that was looked at.
@@ -60,16 +63,13 @@ struct PagedPlaces
         for (int n = 0; n < N; n++)
         {
             if (at[n] != s[n] || begin[n] > t0 + n || end[n] <= t0 + n) { s[n] = -1; }
-            pos[n] = max(min(rows[n], a.max_ctx), 0) - (end[n] - (t0 + n));
+            pos[n] = paged_rows(a, rows[n]) - (end[n] - (t0 + n));
             page[n] = s[n] < 0 || pos[n] < 0 ? -1 : a.table[(size_t)at[n] * a.table_stride + (pos[n] >> a.shift)];
         }
 #pragma unroll
         for (int n = 0; n < N; n++) { page[n] = page[n] < a.n_pages ? max(page[n], -1) : -1; }
     }
 };
-
-// Rows of a sequence in the cache.
-__device__ __forceinline__ int paged_rows(const PagedArgs& a, int s) { return max(min(a.ctx_len[s], a.max_ctx), 0); }
 
 // Page of position pos >= 0, or -1.
 __device__ __forceinline__ int paged_page(const PagedArgs& a, int s, int pos)

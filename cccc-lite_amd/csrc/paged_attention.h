@@ -75,7 +75,7 @@ struct SeqWords
         const int first = max(begin, 0), last = min(end, p.n_tokens);
         // (compared and not subtracted: ranges may hold anything)
         if (s >= a.n_seqs || last <= first || (long long)end - begin > p.max_new) { return { 0, 0, 0 }; }
-        return { first, last - first, max(min(rows, a.max_ctx), 0) - (end - first) };
+        return { first, last - first, paged_rows(a, rows) - (end - first) };
     }
 };
 
