@@ -2,8 +2,8 @@
 //   y = sum_k p_k v_k / sum_k p_k,  p_k = exp(scale q k - m),  over the keys that the token sees, m a running maximum.
 // The rows of a kv head are those of the sequence's new tokens and of the query heads that share it: row r is token r / group, head r % group.
 // One kernel with two forms: sequences of up to 16 rows per kv head (RowsForm), their keys in parts that the last workgroup of a sequence adds up, and tiles of
-// 128 rows of longer ones (TileForm), with ranges of keys where tiles are few, which a second launch adds.  The same sequences in tiles alone, MI355X us: 64 of one
-// token on 1000 to 8000 E4M3 rows 219 for 111, 16 with a window of 4096 48 for 32, one on 4096 BF16 rows 16.7 for 15.1, 8 of five tokens on 500 to 3000 16.9 for 16.9.
+// 128 rows of longer ones (TileForm), with ranges of keys where tiles are few, which a second launch adds.  The same sequences in tiles alone, MI355X us, 32 / 8 heads: 64 of
+// one token on 1000 to 8000 E4M3 rows 216 for 108, 16 with a window of 4096 46 for 31, one on 4096 BF16 rows 16.0 for 13.4, 8 of four tokens on 500 to 3000 E4M3 rows 22 for 15.
 #pragma once
 #include "paged.h"
 
@@ -103,15 +103,18 @@ constexpr int PA_ROWS = 16, PA_TILE = 128, PA_TILE_KEYS = 64;
 
 // Sequences of up to 16 rows per kv head: the keys of each in shares of four blocks (a block per wave), cut into parts of about the same number of shares, a
 // workgroup each.  How many shares a part has follows from those of all sequences, so that long and short ones leave no workgroup with much more than
-// another: about two workgroups' worth of an even split, since a part costs some 5 us besides its keys, but not over PA_PART, which evens out what is
-// left over at the end.  (MI355X, 32 / 8 heads, E4M3, parts of a sequence: 64 sequences of 1000 to 8000 keys 1 113 us, 3 111, 6 123; 16 of 4100 keys 1 35, 2 31,
-// 4 32; 8 of 4000 keys 1 32, 2 24, 4 20.3, 8 20.5.  PA_PART 9 / 14 / 20 / 32: 64 sequences of 1000 to 8000 keys 111.5 / 109.7 / 109.3 / 114.7 us, 64 of 4500
-// 105.2 / 105.2 / 97.3 / 96.9, 16 of 500 to 16000 46.8 / 54.2 / 54.3 / 54.2, 4 of 32000 BF16 97.8 / 99.2 / 91.9 / 86.0, 64 BF16 191.9 / 189.8 / 193.6 / 197.3.)
+// another: about two workgroups' worth of an even split, since a part costs some 5 us besides its keys, but of that not over PA_PART, which evens out what is
+// left over at the end.  At least what three rounds of parts leave, and what fits the parts that there is room for: with very many keys a part has more than PA_PART shares.
+// (MI355X, 32 / 8 heads, E4M3, us.  Parts of a sequence 1 / 2 / 4, this rule: 16 of 4100 keys 34.9 / 30.2 / 31.2, 30.1; 8 of 4000 31.4 / 22.8 / 18.7, 18.7; 64 of 1000 to 8000
+// with 1 / 3 / 6 on average 110.0 / 108.9 / 108.9, 107.2.  PA_PART 9 / 14 / 20 / 32: 64 of 1000 to 8000 110.2 / 106.8 / 107.4 / 112.4, 64 of 4500 103.2 / 103.0 / 94.8 / 94.9,
+// 32 of 2000 to 4000 40.7 / 42.8 / 42.5 / 42.6, 16 of 500 to 16000 45.3 / 52.9 / 52.7 / 52.7, 4 of 32000 BF16 94.7 / 97.0 / 89.2 / 83.7, 64 BF16 190.7 / 188.3 / 191.4 / 194.3.
+// 20 is right for a full batch; a few sequences of uneven lengths would like 9, a few of long ones 32: up to 16 % that one number does not give.)
 constexpr int PA_PART = 20;
 
 // The most sequences whose keys are cut into parts: more are a workgroup each, enough of them to fill the GPU, and nobody has to look at all of them.
-// MI355X, 32 / 8 heads E4M3 us, cut / one each: 64 of 100 to 8000 105 / 107, 256 355 / 363, 256 of 200 to 2000 109 / 106; 8 / 1 heads, 100
-// to 8000: 64 24 / 52, 128 35 / 54, 256 64 / 60.  Beyond, with a trip to memory for each 64 sequences: 512 of 200 to 2000 257 / 199, 1024 606 / 381.
+// MI355X, 32 / 8 heads E4M3 us, cut / one each: 64 of 100 to 8000 103 / 105, 256 352 / 358, 256 of 200 to 2000 107 / 103; 8 / 1 heads, 100
+// to 8000: 64 24 / 51, 128 35 / 52, 256 64 / 61.  Beyond, with a trip to memory for each 64 sequences: 512 of 200 to 2000 257 / 199, 1024 606 / 381.  A sequence much longer
+// than the rest sets the time beyond: by itself 8000 / 32000 / 100000 rows take 48 / 180 / 545 us as a workgroup per kv head, 15 / 22 / 43 cut.
 constexpr int PA_CUT_SEQS = 256;
 
 template <int KEYS>
@@ -405,8 +408,8 @@ __device__ __forceinline__ void add_parts(int n, uint16_t* y, Part part)
     for (int d = 0; d < PER; d += 4) { *(u32x2*)(y + d) = pack4(sum + d); }
 }
 
-// Up to 16 rows of a kv head: single tokens, or a few.  Bound by the cached rows' way from memory: 64 sequences of 1000 to 8000 E4M3 rows 110 us, 5.3 TB/s (a large
-// copy: 5.1); few or short ones by the chain of launch, place, page, row, flags and parts: one sequence of 4096 BF16 rows 15 us, of which the rows' way takes 3.
+// Up to 16 rows of a kv head: single tokens, or a few.  Bound by the cached rows' way from memory: 64 sequences of 1000 to 8000 E4M3 rows 108 us, 5.4 TB/s (a large
+// copy: 5.1); few or short ones by the chain of launch, place, page, row, flags and parts: one sequence of 4096 BF16 rows 13 us, of which the rows' way takes 3.
 //   A workgroup of four waves takes a range of the sequence's blocks of KEYS keys, a wave every fourth block, each with a pipeline of its own: rows go by
 // direct loads to the wave's part of LDS, keys and values STAGES blocks ahead each, and nothing but the wave's own count of loads in flight is waited for.
 //   scores: v_mfma_f32_16x16x32_bf16, key rows as row operand, the 16 queries as columns: D lane (row j = lane % 16, g = lane / 16) holds keys 4 g .. + 3
@@ -783,7 +786,7 @@ __device__ __forceinline__ void attend_part(const PagedArgs& a, const PagedAtten
 
 // 128 rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions: for a block of 64 keys of 128 dims a wave
 // has 1024 cycles of products, about as many of weights, masks' tests and addresses, and 4 x 254 on the way from LDS that its workgroup shares.  Two workgroups on a
-// CU fill each other's gaps (a block of both 2.15 us, a lone one 1.35): 2048 tokens behind 6000 E4M3 rows 236 us, 1000 TFLOP/s of the 1413 that a
+// CU fill each other's gaps (a block of both 2.15 us, a lone one 1.35): 2048 tokens behind 6000 E4M3 rows 226 to 244 us by the card, 965 to 1040 TFLOP/s of the 1413 that a
 // large product reaches.  (64 rows per wave, half the way from LDS, do not fit a wave's registers: three times as long.)
 //   A workgroup of four waves takes 128 rows, a wave 32 of them and every key of each block of 64; keys and values reach LDS as BF16, shared by
 // the waves: from a BF16 cache by direct loads, from FP8 through registers, times their powers of two (exact, once per workgroup).
