@@ -203,3 +203,27 @@ def test_large_and_small_values(gpu, pkg, kind, new, power, workspace):
     b.upload(*gpu[:2])
     assert np.abs(b.values("v")).max() < 2.0 ** 90
     check_attend(gpu, pkg, b, 4, workspace=workspace)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_calls_repeat_themselves(gpu, pkg, kind):
+    """A thousand calls of either kind, one behind the other on one workspace, whose parts pass between workgroups of the whole GPU: the same bits each time."""
+    torch, dev, lib = gpu
+    calls, want = two_calls(gpu, pkg, kind)
+    ws = torch.empty(max(c.need for c in calls), dtype=torch.uint8, device=dev)
+    stream, differs = torch.cuda.Stream(device=dev), torch.zeros((), dtype=torch.int64, device=dev)
+    torch.cuda.synchronize()
+    lib.set_sync(False)
+    try:
+        lib.set_stream(stream.cuda_stream)
+        with torch.cuda.stream(stream):
+            for _ in range(1000):
+                for c, w in zip(calls, want):
+                    c.y.fill_(0x1234)
+                    c(ws)
+                    differs += (c.y != w).sum()
+        torch.cuda.synchronize()
+    finally:
+        lib.set_stream(None)
+        lib.set_sync(True)
+    assert int(differs) == 0
