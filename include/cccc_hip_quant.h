@@ -418,8 +418,8 @@ C_EXPORT int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void
  * aligned, content between calls of no matter; calls that share one must be ordered.  With fewer bytes, or NULL and 0, the keys are split over fewer workgroups.
  * Up to 256 sequences the keys of short ones (16 rows of new tokens x query heads per kv head, at most) are split by the lengths of all; more sequences are a workgroup each and kv head, so that
  * one that is much longer than the rest sets the time of the call: it is better called apart.
- * y must not overlap q.  0 for n_tokens 0.  -1 also where the grid would pass what a launch can have: n_tokens * n_q_heads of 2^24 and more, n_seqs * n_kv_heads from 2^23 on (2^17
- * where max_new lets sequences have more than 16 rows per kv head), n_seqs * max_ctx (with a window: * what it leaves) from 2^37 on. */
+ * y must not overlap q.  0 for n_tokens 0.  -1 also where the grid would pass what a launch can have: n_tokens * n_q_heads of 2^24 and more, n_seqs * n_kv_heads from about 2^23 on
+ * (2^17 where max_new lets sequences have more than 16 rows per kv head), n_seqs * max_ctx (with a window: * what it leaves) from about 2^37 on. */
 C_EXPORT unsigned long long hip_attention_paged_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink);
 C_EXPORT int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, void* workspace, unsigned long long workspace_bytes,
                                       int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink, int ldq, int ldy);
