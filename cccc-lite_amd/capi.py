@@ -59,6 +59,12 @@ def make_paged_kv(type, head_dim, n_kv_heads, page_size, n_pages, k, v, page_tab
     return PagedKV(type, head_dim, n_kv_heads, page_size, n_pages, n_seqs, table_stride, k, v, k_scale, v_scale,
                    page_stride, scale_stride, page_table, ctx_len, seq_start)
 
+
+def paged_layers(caches) -> ctypes.Array:
+    """The caches of a model's layers side by side, for the entries that take all of them."""
+    return (PagedKV * len(caches))(*caches)
+
+
 EXPORTS = (
     "hip_convert",
     "hip_fp4_blockscale_to_bf16",
@@ -89,6 +95,13 @@ EXPORTS = (
     "hip_kv_paged_read_bf16",
     "hip_attention_paged_workspace_bytes",
     "hip_attention_paged_bf16",
+    "hip_qk_norm_rope_kv_paged_at_bf16",
+    "hip_attention_paged_tree_bf16",
+    "hip_kv_paged_keep",
+    "hip_kv_paged_fork_workspace_bytes",
+    "hip_kv_paged_fork",
+    "hip_beam_select_workspace_bytes",
+    "hip_beam_select_bf16",
     "hip_add_bf16",
     "hip_swiglu_bf16",
     "hip_add_rms_norm_bf16",
@@ -183,6 +196,20 @@ class QuantLibrary:
         L.hip_attention_paged_workspace_bytes.argtypes = [kv, i32, i32, i32, i32, i32, i32]
         L.hip_attention_paged_bf16.restype = i32
         L.hip_attention_paged_bf16.argtypes = [kv, vp, vp, vp, u64] + [i32] * 8
+        L.hip_qk_norm_rope_kv_paged_at_bf16.restype = i32
+        L.hip_qk_norm_rope_kv_paged_at_bf16.argtypes = [kv] + [vp] * 7 + [i32, vp, i32, i64, vp, vp, i32, i32, i32, i32, i32, f32]
+        L.hip_attention_paged_tree_bf16.restype = i32
+        L.hip_attention_paged_tree_bf16.argtypes = [kv, vp, vp, vp, i64, vp, u64] + [i32] * 8
+        L.hip_kv_paged_keep.restype = i32
+        L.hip_kv_paged_keep.argtypes = [kv, i32, vp, vp, i32, i32, vp]
+        L.hip_kv_paged_fork_workspace_bytes.restype = u64
+        L.hip_kv_paged_fork_workspace_bytes.argtypes = [kv, i32, i32]
+        L.hip_kv_paged_fork.restype = i32
+        L.hip_kv_paged_fork.argtypes = [kv, i32, i32] + [vp] * 8 + [u64]
+        L.hip_beam_select_workspace_bytes.restype = u64
+        L.hip_beam_select_workspace_bytes.argtypes = [i32] * 4
+        L.hip_beam_select_bf16.restype = i32
+        L.hip_beam_select_bf16.argtypes = [vp, i64, vp, vp] + [i32] * 5 + [vp] * 4 + [u64]
         L.hip_add_bf16.restype = i32
         L.hip_add_bf16.argtypes = [vp, vp, vp, ctypes.c_ulonglong]
         L.hip_swiglu_bf16.restype = i32
@@ -263,6 +290,29 @@ class QuantLibrary:
 
     def attention_paged(self, cache: PagedKV, q, y, workspace, workspace_bytes, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, ldq, ldy) -> int:
         return self.c.hip_attention_paged_bf16(cache, q, y, workspace, workspace_bytes, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, ldq, ldy)
+
+    def qk_norm_rope_kv_paged_at(self, cache: PagedKV, q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, n_positions, positions, n_axes, position_stride, axis, q_out,
+                                 n_q_heads, n_tokens, ldq, ldk, ldv, eps=1e-6) -> int:
+        return self.c.hip_qk_norm_rope_kv_paged_at_bf16(cache, q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, n_positions, positions, n_axes, position_stride, axis, q_out, n_q_heads, n_tokens,
+                                                        ldq, ldk, ldv, eps)
+
+    def attention_paged_tree(self, cache: PagedKV, q, y, seen, seen_stride, workspace, workspace_bytes, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, ldq, ldy) -> int:
+        return self.c.hip_attention_paged_tree_bf16(cache, q, y, seen, seen_stride, workspace, workspace_bytes, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, ldq, ldy)
+
+    def kv_paged_keep(self, caches, n_layers, keep, n_keep, n_tokens, max_new, ctx_out) -> int:
+        return self.c.hip_kv_paged_keep(caches, n_layers, keep, n_keep, n_tokens, max_new, ctx_out)
+
+    def kv_paged_fork_workspace_bytes(self, caches, n_layers, n_out) -> int:
+        return int(self.c.hip_kv_paged_fork_workspace_bytes(caches, n_layers, n_out))
+
+    def kv_paged_fork(self, caches, n_layers, n_out, parent, rows, grow, reserved, table_out, ctx_out, missing, workspace, workspace_bytes) -> int:
+        return self.c.hip_kv_paged_fork(caches, n_layers, n_out, parent, rows, grow, reserved, table_out, ctx_out, missing, workspace, workspace_bytes)
+
+    def beam_select_workspace_bytes(self, n_groups, n_beams, vocab, n_out) -> int:
+        return int(self.c.hip_beam_select_workspace_bytes(n_groups, n_beams, vocab, n_out))
+
+    def beam_select(self, logits, ld, score, last, eos, n_groups, n_beams, vocab, n_out, parent_out, token_out, score_out, workspace, workspace_bytes) -> int:
+        return self.c.hip_beam_select_bf16(logits, ld, score, last, eos, n_groups, n_beams, vocab, n_out, parent_out, token_out, score_out, workspace, workspace_bytes)
 
     def set_sync(self, enabled: bool) -> int:
         return self.c.hip_quant_set_sync(1 if enabled else 0)

@@ -131,6 +131,10 @@ struct PagedAppend
     int n_q, n_tokens, n_positions;
     size_t ldq, ldk, ldv;
     float eps;
+    const int* positions;           // given positions: [n_axes] rows of one per token
+    const uint8_t* axis;            // of each pair of a head; nullptr: 0
+    int n_axes;
+    size_t position_stride;
 };
 
 __device__ __forceinline__ void unpack4(const u32x2 raw, float* f)
@@ -150,9 +154,10 @@ __device__ __forceinline__ u32x2 pack4(const float* f)
 
 // Norm, rotation and append of a head by DIM / 8 lanes: lane i holds elements 4 i .. + 3 of both halves of the head, so that the rotation needs no
 // neighbour.  A lane takes the same head of TOKENS tokens: rows that do not hang on where their token belongs are asked for first, and the trips that tell
-// it are shared.  Bound by memory where tokens are many (4 prompts of 1500 to 2600 tokens, 32 / 8 heads, E5M2: 38 us, 4.6 TB/s), by the launch where they are few
+// it are shared.  AT: the positions of the rotation are given, on up to four axes; a lane's four pairs may lie on any of them.
+// Bound by memory where tokens are many (4 prompts of 1500 to 2600 tokens, 32 / 8 heads, E5M2: 38 us, 4.6 TB/s), by the launch where they are few
 // (16 tokens 4.1 us).  Grid: tokens / TOKENS x workgroups of 256 lanes over the n_q + 2 n_kv heads.
-template <int TYPE, int DIM, int TOKENS>
+template <int TYPE, int DIM, int TOKENS, bool AT>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedArgs a, const PagedAppend p)
 {
     constexpr int LANES = DIM / 8, PER_WG = 256 / LANES, TOP = TYPE == DT_E4M3 ? 8 : 15;
@@ -179,10 +184,43 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedArgs a, co
         unpack4(*(const u32x2*)(nw + i * 4), w);
         unpack4(*(const u32x2*)(nw + i * 4 + DIM / 2), w + 4);
     }
-    const PagedPlaces<TOKENS> at(a, t0);
     u32x2 cs[TOKENS], sn[TOKENS];
+    bool out[TOKENS] = {};                                                  // AT: a position that no row of the tables has
+    uint32_t on_axis[2] = {};                                               // AT: the lane's pairs that lie on any axis
+    if constexpr (AT)
+    {
+        const uint32_t axes = p.axis ? *(const uint32_t*)(p.axis + i * 4) : 0;
+#pragma unroll
+        for (int n = 0; n < TOKENS; n++) { cs[n] = sn[n] = u32x2{ 0, 0 }; }
+        for (int x = 0; x < p.n_axes; x++)
+        {
+            // which of the lane's pairs lie on axis x
+            uint32_t mine[2] = {};
+#pragma unroll
+            for (int e = 0; e < 4; e++) { mine[e / 2] |= (axes >> (8 * e) & 255u) == (uint32_t)x ? 0xFFFFu << (16 * (e & 1)) : 0u; }
+            on_axis[0] |= mine[0];
+            on_axis[1] |= mine[1];
+            int pos[TOKENS];
+#pragma unroll
+            for (int n = 0; n < TOKENS; n++) { pos[n] = p.positions[(size_t)x * p.position_stride + min(t0 + n, p.n_tokens - 1)]; }
+#pragma unroll
+            for (int n = 0; n < TOKENS; n++)
+            {
+                out[n] = out[n] || pos[n] < 0 || pos[n] >= p.n_positions;
+                const size_t from = (size_t)min(max(pos[n], 0), p.n_positions - 1) * (DIM / 2) + i * 4;
+                const u32x2 c = *(const u32x2*)(p.cos_tab + from), s = *(const u32x2*)(p.sin_tab + from);
+#pragma unroll
+                for (int d = 0; d < 2; d++)
+                {
+                    cs[n][d] |= c[d] & mine[d];
+                    sn[n][d] |= s[d] & mine[d];
+                }
+            }
+        }
+    }
+    const PagedPlaces<TOKENS> at(a, t0);
     const bool turns = p.cos_tab && !is_v;
-    if (turns)
+    if (turns && !AT)
     {
 #pragma unroll
         for (int n = 0; n < TOKENS; n++)
@@ -196,7 +234,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedArgs a, co
     for (int n = 0; n < TOKENS; n++)
     {
         const int t = t0 + n, pos = at.pos[n];
-        if (at.s[n] < 0 || t >= p.n_tokens || pos < 0 || (p.cos_tab && pos >= p.n_positions) || spare) { continue; }
+        if (at.s[n] < 0 || t >= p.n_tokens || pos < 0 || (AT ? out[n] : p.cos_tab && pos >= p.n_positions) || spare) { continue; }
         float x[8];
         unpack4(raw[n][0], x);
         unpack4(raw[n][1], x + 4);
@@ -219,6 +257,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedArgs a, co
             for (int e = 0; e < 4; e++)
             {
                 const float lo = x[e], hi = x[e + 4];
+                if (AT && (on_axis[e / 2] >> (16 * (e & 1)) & 1) == 0) { continue; }
                 x[e] = lo * c[e] - hi * s[e];
                 x[e + 4] = hi * c[e] + lo * s[e];
             }

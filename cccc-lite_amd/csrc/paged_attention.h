@@ -1,4 +1,4 @@
-// Causal attention of the new tokens of a batch of sequences over their pages.
+// Attention of the new tokens of a batch of sequences over their pages, causal or (TREE) with bits that say which new tokens each sees.
 //   y = sum_k p_k v_k / sum_k p_k,  p_k = exp(scale q k - m),  over the keys that the token sees, m a running maximum.
 // The rows of a kv head are those of the sequence's new tokens and of the query heads that share it: row r is token r / group, head r % group.
 // One kernel with two forms: sequences of up to 16 rows per kv head (RowsForm), their keys in parts that the last workgroup of a sequence adds up, and tiles of
@@ -26,6 +26,8 @@ struct PagedAttention
     int min_rows;                   // sequences of at most so many rows per kv head are not cut into tiles
     int snake;                      // the second half of the tiles in the other order
     float scale;                    // log2 e / sqrt(dim)
+    const unsigned long long* seen; // trees: bits of the new tokens that a token sees, seen_stride words each
+    size_t seen_stride;
 
     __device__ __forceinline__ float* row_sums(int slot, int kvh, int n_kv, int row, int dim) const { return row_partial + (((size_t)slot * n_kv + kvh) * 16 + row) * dim; }
     __device__ __forceinline__ float* row_stats(int slot, int kvh, int n_kv, int row, int dim) const
@@ -98,6 +100,36 @@ struct KeyBlocks
 };
 
 __device__ __forceinline__ bool sees(const PagedAttention& p, int pos, int key) { return key <= pos && (p.window == 0 || key > pos - p.window || key < p.n_sink); }
+
+// Trees: a token sees the rows in front of its sequence's new tokens (within its window) and the new tokens whose bits are set.
+// Which of keys key0 .. + 63 that is: `first` is the position of the first new token, pos the one that the token's window counts from, word(i) bits 64 i .. + 63 of
+// the new tokens (any i from 0 on).
+template <class Word>
+__device__ __forceinline__ unsigned long long named_keys(const PagedAttention& p, int first, int pos, int key0, Word word)
+{
+    const int from = key0 - first;                                          // of the new tokens
+    unsigned long long r = ~0ull;
+    if (from >= 0)
+    {
+        r = word(from >> 6) >> (from & 63);
+        if (from & 63) { r |= word((from >> 6) + 1) << (64 - (from & 63)); }
+    }
+    else if (from > -64) { r = word(0) << -from | ((1ull << -from) - 1); }
+    if (p.window != 0)
+    {
+        // hidden: rows in front, from n_sink to pos - window
+        const int lo = max(p.n_sink - key0, 0), hi = min(min(pos - p.window, first - 1) - key0, 63);
+        if (lo <= hi) { r &= ~(~0ull >> (63 - hi) & ~0ull << lo); }
+    }
+    return r;
+}
+
+// Bits 64 i .. + 63 of a row of bits for n new tokens.
+__device__ __forceinline__ unsigned long long seen_word(const unsigned long long* row, int n, int i)
+{
+    const int left = n - 64 * i;
+    return left <= 0 ? 0ull : row[i] & (left >= 64 ? ~0ull : (1ull << left) - 1);
+}
 
 constexpr int PA_ROWS = 16, PA_TILE = 128, PA_TILE_KEYS = 64;
 
@@ -188,6 +220,7 @@ struct Tile
 // the tiles comes in the other order, so that a long one has a short one beside it (MI355X, 512 tiles of 2048 tokens behind 6000: 249 us for 256; with more
 // tiles than that a CU takes the next one when it is done, and the order from long to short is the better one: 2000 tiles of four prompts 142 us for 146).  Called by whole waves: a lane per
 // sequence, 256 of them per trip to memory, their tiles added up.
+template <bool TREE>
 __device__ __forceinline__ Tile find_tile(const PagedArgs& a, const PagedAttention& p, int tile)
 {
     Tile r;
@@ -224,8 +257,8 @@ __device__ __forceinline__ Tile find_tile(const PagedArgs& a, const PagedAttenti
     }
     if (r.s < 0) { return r; }
     r.n_rows = uniform(r.mine.n * p.group);
-    r.lo = uniform(r.mine.pos + r.row0 / p.group);
-    r.hi = uniform(r.mine.pos + min(r.row0 + PA_TILE - 1, r.n_rows - 1) / p.group);
+    r.lo = uniform(TREE ? r.mine.pos : r.mine.pos + r.row0 / p.group);
+    r.hi = uniform(TREE ? r.mine.pos + r.mine.n - 1 : r.mine.pos + min(r.row0 + PA_TILE - 1, r.n_rows - 1) / p.group);
     r.blocks = KeyBlocks<PA_TILE_KEYS>(p, r.lo, r.hi);
     r.blocks.n = uniform(r.blocks.n);
     r.blocks.sinks = uniform(r.blocks.sinks);
@@ -427,7 +460,7 @@ struct RowsForm
     static constexpr int STAT = 4 * (WAVE > PA_ROWS * SUM * 4 ? WAVE : PA_ROWS * SUM * 4), LDS = STAT + 4 * PA_ROWS * 8;
 };
 
-template <int TYPE, int DIM>
+template <int TYPE, int DIM, bool TREE>
 __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int s, const NewTokens& mine, int kvh, int from_share, int to_share, int slot, int part, int n_parts)
 {
     typedef RowsForm<TYPE, DIM> F;
@@ -442,6 +475,10 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
 
     const int row = min(j, n_rows - 1), token = row / p.group, head = kvh * p.group + row % p.group;
     const int my_pos = mine.pos + token;
+    // trees: what the row's token sees of the new ones, 16 at most; asked for here, there with the first pages, before the counted loads
+    int seen_pos = 0;
+    uint32_t new_seen = 0;
+    if constexpr (TREE) { new_seen = (uint32_t)p.seen[(size_t)(mine.first + token) * p.seen_stride] & ((1u << mine.n) - 1); }
     u32x4 qf[DIM / 32];                                                     // elements 32 c + 8 g .. + 7
 #pragma unroll
     for (int c = 0; c < DIM / 32; c++) { qf[c] = *(const u32x4*)(p.q + (size_t)(mine.first + token) * p.ldq + (size_t)head * DIM + c * 32 + g * 8); }
@@ -501,7 +538,7 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         }
     };
     // list entries plain_from .. plain_to - 1: every row sees every key
-    int plain_from = 0, plain_to = (lo + 1) / KEYS;
+    int plain_from = 0, plain_to = (TREE ? max(lo, 0) : lo + 1) / KEYS;
     if (p.window != 0) { plain_from = (hi - p.window + KEYS) / KEYS; }
     plain_from = uniform(max(plain_from - blocks.skip, hi < p.window || p.window == 0 ? 0 : blocks.sinks));
     plain_to = uniform(plain_to - blocks.skip);
@@ -519,6 +556,8 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         return lacks;
     };
     int kept = 0;
+    // trees: which keys of a block the row sees
+    auto keys_seen = [&](int key0) { return named_keys(p, mine.pos, seen_pos, key0, [&](int i) { return i == 0 ? (unsigned long long)new_seen : 0ull; }); };
 
     auto block = [&](int n) {
         const uint8_t* const kb = my_lds + n % STAGES * SIDE;
@@ -604,10 +643,13 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
         if (!plain)
         {
             const int b = blocks.block(entry);
+            unsigned long long bits = 0;
+            if constexpr (TREE) { bits = keys_seen(b * KEYS); }
 #pragma unroll
             for (int e = 0; e < 4 * TILES; e++)
             {
-                const bool see = sees(p, my_pos, b * KEYS + 16 * (e >> 2) + 4 * g + (e & 3)) && !(lacks >> (e >> 2) & 1);
+                const int at = 16 * (e >> 2) + 4 * g + (e & 3);
+                const bool see = (TREE ? (bits >> at & 1) != 0 : sees(p, my_pos, b * KEYS + at)) && !(lacks >> (e >> 2) & 1);
                 acc[e >> 2][e & 3] = see ? acc[e >> 2][e & 3] : -INFINITY;
                 if constexpr (TYPE != DT_BF16) { value_exponents[e >> 2][e & 3] = see ? value_exponents[e >> 2][e & 3] : 0; }     // one that nobody wrote may be an infinity's
             }
@@ -624,7 +666,7 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
 #pragma unroll 1
                 for (int key = 0; key < KEYS; key++)
                 {
-                    const bool see = sees(p, my_pos, b * KEYS + key) && !(lacks >> (key / 16) & 1);
+                    const bool see = (TREE ? (bits >> key & 1) != 0 : sees(p, my_pos, b * KEYS + key)) && !(lacks >> (key / 16) & 1);
 #pragma unroll
                     for (int d = 0; d < DIM / 16; d++)
                     {
@@ -692,6 +734,11 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
     if (n_mine > 0)
     {
         look_up(0);
+        if constexpr (TREE)
+        {
+            asm volatile("" : "+v"(new_seen));
+            seen_pos = mine.pos + max(__builtin_popcount(new_seen) - 1, 0);
+        }
         stage(0, false);
         stage(0, true);
     }
@@ -769,7 +816,7 @@ __device__ __forceinline__ void attend_rows(const PagedArgs& a, const PagedAtten
 }
 
 // Part c of a kv head's, or with row_parts 0 all of sequence c.
-template <int TYPE, int DIM>
+template <int TYPE, int DIM, bool TREE>
 __device__ __forceinline__ void attend_part(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int c, int kvh)
 {
     typedef Parts<RowsForm<TYPE, DIM>::KEYS> P;
@@ -777,11 +824,11 @@ __device__ __forceinline__ void attend_part(const PagedArgs& a, const PagedAtten
     {
         const NewTokens mine = SeqWords(a, c).tokens(a, p, c);
         const int shares = uniform(P::shares_of(p, mine));
-        if (shares > 0) { attend_rows<TYPE, DIM>(a, p, lds, c, mine, kvh, 0, shares, 0, 0, 1); }
+        if (shares > 0) { attend_rows<TYPE, DIM, TREE>(a, p, lds, c, mine, kvh, 0, shares, 0, 0, 1); }
         return;
     }
     const P of(a, p, c);
-    if (of.s >= 0) { attend_rows<TYPE, DIM>(a, p, lds, of.s, of.mine, kvh, (int)((long long)of.shares * of.part / of.parts), (int)((long long)of.shares * (of.part + 1) / of.parts), c, of.part, of.parts); }
+    if (of.s >= 0) { attend_rows<TYPE, DIM, TREE>(a, p, lds, of.s, of.mine, kvh, (int)((long long)of.shares * of.part / of.parts), (int)((long long)of.shares * (of.part + 1) / of.parts), c, of.part, of.parts); }
 }
 
 // 128 rows of a kv head: chunks and prompts.  Bound by the matrix cores and what a wave issues between their instructions: for a block of 64 keys of 128 dims a wave
@@ -802,7 +849,7 @@ struct TileForm
     static constexpr int ODD = 4 * BLOCK, LDS = ODD + 32;                   // two blocks of keys, two of values
 };
 
-template <int TYPE, int DIM>
+template <int TYPE, int DIM, bool TREE>
 __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAttention& p, uint8_t* lds, int tile, int kvh, int range)
 {
     typedef TileForm<TYPE, DIM> F;
@@ -811,7 +858,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     uint32_t* const odd_rows = (uint32_t*)(lds + F::ODD);                   // per buffer of values and wave that staged: something infinite or NaN
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 31, h = lane >> 5;
-    const Tile rows = find_tile(a, p, tile);
+    const Tile rows = find_tile<TREE>(a, p, tile);
     if (rows.s < 0 || range >= rows.n_ranges) { return; }
     const NewTokens mine = rows.mine;
     const auto& blocks = rows.blocks;
@@ -822,6 +869,15 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     const int r = row0 + wave * 32 + j, row = min(r, n_rows - 1);
     const bool real = r < n_rows;
     const int token = mine.first + row / p.group, head = kvh * p.group + row % p.group, my_pos = mine.pos + row / p.group;
+    // trees: the bits of the row's token, and as many positions behind the first new token as it descends from tokens
+    const unsigned long long* const seen_row = p.seen + (TREE ? (size_t)token * p.seen_stride : 0);
+    int seen_pos = 0;
+    if (TREE && p.window != 0)
+    {
+        for (int i = 0; 64 * i < mine.n; i++) { seen_pos += __builtin_popcountll(seen_word(seen_row, mine.n, i)); }
+        seen_pos = mine.pos + max(seen_pos - 1, 0);
+    }
+    auto keys_seen = [&](int key0) { return named_keys(p, mine.pos, seen_pos, key0, [&](int i) { return seen_word(seen_row, mine.n, i); }); };
     u32x4 qf[DIM / 16];
 #pragma unroll
     for (int c = 0; c < DIM / 16; c++) { qf[c] = *(const u32x4*)(p.q + (size_t)token * p.ldq + (size_t)head * DIM + c * 16 + h * 8); }
@@ -911,7 +967,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     auto values_at = [&](int i) { return (uint32_t)(2 + ((i - begin) & 1)) * BLOCK; };
     const uint32_t part = wave * (BLOCK / 4);                               // the wave's rows of a block
     // entries plain_from .. plain_to - 1: every row of the tile sees every key
-    int plain_from = 0, plain_to = (tile_lo + 1) / KEYS;
+    int plain_from = 0, plain_to = (TREE ? max(tile_lo, 0) : tile_lo + 1) / KEYS;
     if (p.window != 0) { plain_from = (tile_hi - p.window + KEYS) / KEYS; }
     plain_from = max(plain_from - blocks.skip, tile_hi < p.window || p.window == 0 ? 0 : blocks.sinks);
     plain_to -= blocks.skip;
@@ -952,6 +1008,17 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
 
     // scores of keys that a row does not see
     auto mask = [&](f32x16 (&acc)[2], int b, int lacks) {
+        if constexpr (TREE)
+        {
+            const unsigned long long bits = keys_seen(b * KEYS) >> (4 * h);
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+            {
+                const bool see = (bits >> (8 * (e / 4) + e % 4) & 1) != 0 && !(lacks >> (e / 8) & 1);
+                acc[e / 16][e % 16] = see ? acc[e / 16][e % 16] : -INFINITY;
+            }
+            return;
+        }
         // element e: key 8 (e / 4) + 4 h + e % 4 of the block
         const int last = my_pos - b * KEYS - 4 * h, from = p.window == 0 ? -0x40000000 : last - p.window, sinks = p.n_sink - b * KEYS - 4 * h;
 #pragma unroll
@@ -1058,11 +1125,12 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
         if (__builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]) == 0) { return; }
         uint8_t* const vb = lds + values_at(i);
         const int b = blocks.block(i);
+        const unsigned long long bits = TREE ? keys_seen(b * KEYS) : 0;
 #pragma unroll 1
         for (int key = 0; key < KEYS; key++)
         {
             if (lacks >> (key / 16) & 1) { continue; }
-            const bool see = sees(p, my_pos, b * KEYS + key);
+            const bool see = TREE ? (bits >> key & 1) != 0 : sees(p, my_pos, b * KEYS + key);
 #pragma unroll
             for (int n = 0; n < DIM / 8; n++)
             {
@@ -1202,7 +1270,7 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
 }
 
 // Both forms in one launch, tiles first: single tokens beside a chunk run beside it.  Grid: ranges x tiles x kv heads, then parts x kv heads.
-template <int TYPE, int DIM>
+template <int TYPE, int DIM, bool TREE>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs a, const PagedAttention p)
 {
     typedef RowsForm<TYPE, DIM> R;
@@ -1210,16 +1278,16 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedArgs
     __shared__ __attribute__((aligned(1024))) uint8_t lds[R::LDS > T::LDS ? R::LDS : T::LDS];
     static_assert(sizeof(lds) <= 80 * 1024, "two workgroups on a CU");
     const int tiles = p.tiles * a.n_kv, n_tiles = tiles * p.tile_split;
-    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
-    else { attend_part<TYPE, DIM>(a, p, lds, (blockIdx.x - n_tiles) / a.n_kv, (blockIdx.x - n_tiles) % a.n_kv); }
+    if ((int)blockIdx.x < n_tiles) { attend_tile<TYPE, DIM, TREE>(a, p, lds, blockIdx.x % tiles / a.n_kv, blockIdx.x % a.n_kv, blockIdx.x / tiles); }
+    else { attend_part<TYPE, DIM, TREE>(a, p, lds, (blockIdx.x - n_tiles) / a.n_kv, (blockIdx.x - n_tiles) % a.n_kv); }
 }
 
 // The tiles' ranges added, 16 rows per workgroup and DIM / 16 dims of a row per thread.  Rows in one piece are written already.  Grid: eighths of tiles x kv heads.
-template <int DIM>
+template <int DIM, bool TREE>
 __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
 {
     const int kvh = blockIdx.x % a.n_kv, at = blockIdx.x / a.n_kv;
-    const Tile rows = find_tile(a, p, at / 8);
+    const Tile rows = find_tile<TREE>(a, p, at / 8);
     const int row = rows.row0 + at % 8 * 16 + (threadIdx.x >> 4);
     if (rows.s < 0 || row >= rows.n_rows || rows.n_ranges <= 1) { return; }
     const size_t token = rows.mine.first + row / p.group, head = kvh * p.group + row % p.group, at_row = token * p.n_q + head;

@@ -1,0 +1,259 @@
+// Rows and pages of a paged key / value cache moved about, in all layers at once: what is kept of a sequence's new tokens, and batches that fork.
+#pragma once
+#include "paged.h"
+
+namespace ccq
+{
+
+// The pools of up to this many layers travel with a launch.
+constexpr int MOVE_LAYERS = 64;
+
+struct PagedLayers
+{
+    uint8_t *k[MOVE_LAYERS], *v[MOVE_LAYERS], *k_scale[MOVE_LAYERS], *v_scale[MOVE_LAYERS];
+    int n;
+    int row;                        // bytes of a row of one kv head: 64, 128 or 256
+};
+
+struct PagedKeep
+{
+    const int *keep, *n_keep;
+    int* ctx_out;
+    int n_tokens, max_new;
+};
+
+// Rows of a sequence's kept tokens, KEEP_ROWS at a time and KEEP_UNITS times 256 pieces of 16 bytes, through registers.
+// Kept indices ascend and none is below its place, so that a place is never a source of later rows: what a chunk reads is read before it writes, and nothing else has to
+// wait.  Bound by the launch and four trips to memory in a row (places, pages, rows, and the way back).
+// Grid: sequences x layers x (keys, values).
+constexpr int KEEP_ROWS = 16, KEEP_UNITS = 8;
+
+__global__ __launch_bounds__(256) void paged_keep_kernel(const PagedArgs a, const PagedLayers layers, const PagedKeep p)
+{
+    // where the chunk's rows come from and go to: page (-1: no move) and row of kv head 0
+    __shared__ int from_page[KEEP_ROWS], from_row[KEEP_ROWS], to_page[KEEP_ROWS], to_row[KEEP_ROWS];
+    const int s = blockIdx.x % a.n_seqs, side = blockIdx.x / a.n_seqs % 2, layer = blockIdx.x / a.n_seqs / 2;
+    const int begin = a.seq_start[s], end = a.seq_start[s + 1], rows = paged_rows(a, a.ctx_len[s]);
+    int kept = p.n_keep[s];
+    const bool mine = begin >= 0 && end <= p.n_tokens && begin < end && (long long)end - begin <= p.max_new;
+    const int n = mine ? end - begin : 0, first = rows - n;
+    kept = min(max(kept, 0), n);
+    if (p.ctx_out && threadIdx.x == 0 && blockIdx.x < a.n_seqs) { p.ctx_out[s] = max(first + kept, 0); }
+    uint8_t* const pool = side ? layers.v[layer] : layers.k[layer];
+    uint8_t* const scale = side ? layers.v_scale[layer] : layers.k_scale[layer];
+    const int pieces = layers.row / 16, i = threadIdx.x / pieces % KEEP_ROWS, heads_at_once = 256 / pieces / KEEP_ROWS, h0 = threadIdx.x / pieces / KEEP_ROWS;
+    const size_t piece = threadIdx.x % pieces * 16;
+    for (int i0 = 0; i0 < kept; i0 += KEEP_ROWS)
+    {
+        if (threadIdx.x < KEEP_ROWS)
+        {
+            const int at = i0 + threadIdx.x, of = at < kept ? p.keep[begin + at] : 0;
+            const int src = first + of, dst = first + at;
+            int page = -1, place = -1;
+            if (at < kept && of > at && of < n && dst >= 0)
+            {
+                page = paged_page(a, s, src);
+                place = paged_page(a, s, dst);
+            }
+            from_page[threadIdx.x] = place < 0 ? -1 : page;
+            to_page[threadIdx.x] = place;
+            from_row[threadIdx.x] = paged_row(a, 0, max(src, 0));
+            to_row[threadIdx.x] = paged_row(a, 0, max(dst, 0));
+        }
+        __syncthreads();
+        const bool moves = from_page[i] >= 0;
+        for (int h1 = 0; h1 < a.n_kv; h1 += KEEP_UNITS * heads_at_once)
+        {
+            u32x4 unit[KEEP_UNITS];
+#pragma unroll
+            for (int u = 0; u < KEEP_UNITS; u++)
+            {
+                const int h = h1 + u * heads_at_once + h0;
+                if (moves && h < a.n_kv) { unit[u] = *(const u32x4*)(pool + from_page[i] * a.page_stride + (((size_t)h << a.shift) + from_row[i]) * layers.row + piece); }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < KEEP_UNITS; u++)
+            {
+                const int h = h1 + u * heads_at_once + h0;
+                if (moves && h < a.n_kv) { *(u32x4*)(pool + to_page[i] * a.page_stride + (((size_t)h << a.shift) + to_row[i]) * layers.row + piece) = unit[u]; }
+            }
+        }
+        if (scale)
+        {
+            const int row = threadIdx.x % KEEP_ROWS;
+            for (int h1 = 0; h1 < a.n_kv; h1 += 256 / KEEP_ROWS)
+            {
+                const int h = h1 + threadIdx.x / KEEP_ROWS;
+                const bool moves = from_page[row] >= 0 && h < a.n_kv;
+                uint8_t unit = 0;
+                if (moves) { unit = scale[from_page[row] * a.scale_stride + ((size_t)h << a.shift) + from_row[row]]; }
+                __syncthreads();
+                if (moves) { scale[to_page[row] * a.scale_stride + ((size_t)h << a.shift) + to_row[row]] = unit; }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+struct PagedFork
+{
+    const int *parent, *rows, *grow;
+    const uint8_t* reserved;
+    int *table_out, *ctx_out, *missing;
+    int n_out;
+    int* holder;                    // [n_pages] who holds a page: NOBODY, a sequence's number + 1 (as its last one, the lowest such), 0 (as a whole one, or reserved)
+    int* free_pages;                // [n_pages] pages of nobody, lowest first
+    int* base;                      // [n_out] new pages handed out to the sequences in front
+    int* copies;                    // [n_out][4] page, new page (-1: none), rows
+};
+
+constexpr int FORK_NOBODY = 0x7FFFFFFF, FORK_THREADS = 1024;
+
+// What sequence s of the new batch is to hold.
+struct Forked
+{
+    const int* old;                 // its parent's pages
+    int rows, total;                // rows taken over, and with those to come
+    int whole, taken, all;          // pages taken over as whole ones, with a last one, and with new ones
+
+    __device__ __forceinline__ Forked(const PagedArgs& a, const PagedFork& f, int s)
+    {
+        const int parent = f.parent[s];
+        const bool has = parent >= 0 && parent < a.n_seqs;
+        const int have = has ? paged_rows(a, a.ctx_len[parent]) : 0;
+        rows = f.rows ? min(max(f.rows[s], 0), have) : have;
+        total = (int)min((long long)rows + max(f.grow[s], 0), (long long)a.max_ctx);
+        old = a.table + (size_t)(has ? parent : 0) * a.table_stride;
+        whole = rows >> a.shift;
+        const int more = (1 << a.shift) - 1;
+        taken = (rows + more) >> a.shift;
+        all = (total + more) >> a.shift;
+    }
+    __device__ __forceinline__ int page(const PagedArgs& a, int i) const { const int page = old[i]; return page >= 0 && page < a.n_pages ? page : -1; }
+};
+
+// Sum of v over the threads in front of this one, and over all (1024 threads).
+__device__ __forceinline__ int fork_scan(int v, int& all, int* lds)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int upto = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2)
+    {
+        const int other = __shfl_up(upto, d);
+        upto += lane >= d ? other : 0;
+    }
+    __syncthreads();
+    if (lane == 63) { lds[wave] = upto; }
+    __syncthreads();
+    int before = 0;
+    all = 0;
+    for (int w = 0; w < FORK_THREADS / 64; w++)
+    {
+        before += w < wave ? lds[w] : 0;
+        all += lds[w];
+    }
+    return before + upto - v;
+}
+
+// The tables of a forked batch, by one workgroup: who holds each page, which are free, who gets which.
+__global__ __launch_bounds__(FORK_THREADS) void paged_fork_kernel(const PagedArgs a, const PagedFork f)
+{
+    __shared__ int lds[FORK_THREADS / 64];
+    for (int i = threadIdx.x; i < a.n_pages; i += FORK_THREADS) { f.holder[i] = f.reserved && f.reserved[i] ? 0 : FORK_NOBODY; }
+    __threadfence();
+    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int s = wave; s < f.n_out; s += FORK_THREADS / 64)
+    {
+        const Forked mine(a, f, s);
+        for (int i = lane; i < mine.taken; i += 64)
+        {
+            const int page = mine.page(a, i);
+            if (page >= 0) { atomicMin(f.holder + page, i < mine.whole ? 0 : s + 1); }
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    int needed = 0;
+    for (int s0 = 0; s0 < f.n_out; s0 += FORK_THREADS)
+    {
+        const int s = s0 + threadIdx.x;
+        int need = 0;
+        if (s < f.n_out)
+        {
+            const Forked mine(a, f, s);
+            const int last = mine.taken > mine.whole ? mine.page(a, mine.whole) : -1;
+            const bool copied = last >= 0 && __hip_atomic_load(f.holder + last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != s + 1;
+            need = mine.all - mine.taken + (copied ? 1 : 0);
+            f.copies[4 * s] = copied ? last : -1;
+            f.copies[4 * s + 2] = mine.rows - (mine.whole << a.shift);
+            f.ctx_out[s] = mine.total;
+        }
+        int all;
+        const int before = fork_scan(need, all, lds);
+        if (s < f.n_out) { f.base[s] = needed + before; }
+        needed += all;
+    }
+    int n_free = 0;
+    for (int i0 = 0; i0 < a.n_pages && n_free < needed; i0 += FORK_THREADS)
+    {
+        const int i = i0 + threadIdx.x;
+        const bool free = i < a.n_pages && __hip_atomic_load(f.holder + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == FORK_NOBODY;
+        int all;
+        const int before = fork_scan(free ? 1 : 0, all, lds);
+        if (free) { f.free_pages[n_free + before] = i; }
+        n_free += all;
+    }
+    if (threadIdx.x == 0) { *f.missing = max(needed - n_free, 0); }
+    __threadfence();
+    __syncthreads();
+    for (int s = wave; s < f.n_out; s += FORK_THREADS / 64)
+    {
+        const Forked mine(a, f, s);
+        const bool copied = f.copies[4 * s] >= 0;
+        const int base = f.base[s];
+        for (int i = lane; i < a.table_stride; i += 64)
+        {
+            int page = -1;
+            const bool last = i == mine.whole && mine.taken > mine.whole;
+            if (i >= mine.taken ? i < mine.all : last && copied)
+            {
+                const int at = base + (i >= mine.taken ? i - mine.taken + (copied ? 1 : 0) : 0);
+                page = at < n_free ? f.free_pages[at] : -1;
+                if (last) { f.copies[4 * s + 1] = page; }
+            }
+            else if (i < mine.taken) { page = mine.page(a, i); }
+            f.table_out[(size_t)s * a.table_stride + i] = page;
+        }
+    }
+}
+
+// The rows of last pages that became a sequence's own.  Grid: sequences x layers x (keys, values).
+__global__ __launch_bounds__(256) void paged_fork_copy_kernel(const PagedArgs a, const PagedLayers layers, const int* copies, int n_out)
+{
+    const int s = blockIdx.x % n_out, side = blockIdx.x / n_out % 2, layer = blockIdx.x / n_out / 2;
+    const int from = copies[4 * s], to = copies[4 * s + 1], rows = copies[4 * s + 2];
+    if (from < 0 || to < 0) { return; }
+    uint8_t* const pool = side ? layers.v[layer] : layers.k[layer];
+    uint8_t* const scale = side ? layers.v_scale[layer] : layers.k_scale[layer];
+    const int per_head = rows * (layers.row / 16);                          // pieces of 16 bytes
+    const size_t head = (size_t)layers.row << a.shift;
+    const uint8_t* const src = pool + from * a.page_stride;
+    uint8_t* const dst = pool + to * a.page_stride;
+    for (int h = 0; h < a.n_kv; h++)
+    {
+        for (int i = threadIdx.x; i < per_head; i += 256) { *(u32x4*)(dst + h * head + i * 16) = *(const u32x4*)(src + h * head + i * 16); }
+    }
+    if (scale)
+    {
+        for (int i = threadIdx.x; i < rows * a.n_kv; i += 256)
+        {
+            const size_t at = ((size_t)(i / rows) << a.shift) + i % rows;
+            scale[to * a.scale_stride + at] = scale[from * a.scale_stride + at];
+        }
+    }
+}
+
+}    // namespace ccq

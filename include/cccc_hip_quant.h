@@ -425,6 +425,63 @@ C_EXPORT int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, 
                                       int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink, int ldq, int ldy);
 
 /*
+ * Sequences that branch: drafted tokens that form trees, and beams (no counterpart in the reference).
+ *
+ * A tree of drafted tokens is a sequence's new tokens as any others, in the cache one behind the other in the order of the activations; what makes them a tree is the
+ * positions that they are rotated by (a token's depth behind the rows in front of the tree) and the tokens that each sees.  A step: hip_qk_norm_rope_kv_paged_at_bf16 and
+ * hip_attention_paged_tree_bf16 in every layer, the picks of all tokens, then one hip_kv_paged_keep for the path that the picks confirm.
+ */
+
+/* hip_qk_norm_rope_kv_paged_bf16 with the positions of the rotation given: positions int32 [n_axes][n_tokens], row a at positions + a * position_stride (n_axes 1 to 4).  Pair i
+ * of a head (elements i and head_dim / 2 + i) turns by row positions[axis[i]][token] of cos_tab and sin_tab; axis: head_dim / 2 bytes, 4-byte aligned, NULL: all pairs on axis 0.  A pair whose byte is
+ * n_axes or more is not turned.  Where in the cache a token goes follows from seq_start and ctx_len, as there.  A token with a position outside 0 .. n_positions - 1 on any axis is left out.
+ * cos_tab, sin_tab and positions are needed. */
+C_EXPORT int hip_qk_norm_rope_kv_paged_at_bf16(const hip_paged_kv* cache, const void* q, const void* k, const void* v,
+                                               const void* q_norm_w, const void* k_norm_w, const void* cos_tab, const void* sin_tab, int n_positions,
+                                               const void* positions, int n_axes, long long position_stride, const void* axis,
+                                               void* q_out, int n_q_heads, int n_tokens, int ldq, int ldk, int ldv, float epsilon);
+
+/* hip_attention_paged_bf16 for tokens that do not see all new tokens in front of them: token t sees every row in front of its sequence's first new token, and new token j of its sequence
+ * where bit j % 64 of word seen[t * seen_stride + j / 64] is set (uint64, 8-byte aligned; its own bit too if it is to see itself; bits from the sequence's number of new tokens on are not looked at).  seen_stride * 64 is max_new at least.
+ * With window > 0 a token that sees n new tokens, itself among them, is taken to be n - 1 positions behind the first one (its depth, where it sees the tokens that it descends from), and
+ * of the rows in front sees those less than `window` behind that position and the first n_sink ones; new tokens go by their bits alone.  Everything else as there, the workspace too
+ * (hip_attention_paged_workspace_bytes). */
+C_EXPORT int hip_attention_paged_tree_bf16(const hip_paged_kv* cache, const void* q, void* y, const void* seen, long long seen_stride, void* workspace, unsigned long long workspace_bytes,
+                                           int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink, int ldq, int ldy);
+
+/* The entries below take the caches of all layers of a model, `caches` in host memory, n_layers of them: alike but for k, v, k_scale and v_scale (else -1). */
+
+/* Of the new tokens of sequence s those at keep[seq_start[s] + i], i < n_keep[s] (int32, counted from its first new token, ascending), stay: the i-th one's row moves to where new token i is, in
+ * all layers.  An index below its place i, or not below the sequence's number of new tokens, moves nothing; n_keep beyond that number is cut to it.  ctx_out int32 [n_seqs], not ctx_len itself (NULL: none):
+ * the rows left, ctx_len less the tokens that do not stay.  A sequence with more new tokens than max_new is left as it is, its ctx_len too.  Rows behind the
+ * kept ones hold anything afterwards.  Pages that new tokens lie in belong to one sequence; rows whose source or place has no page do not move.  0 for n_tokens 0 without ctx_out. */
+C_EXPORT int hip_kv_paged_keep(const hip_paged_kv* caches, int n_layers, const void* keep, const void* n_keep, int n_tokens, int max_new, void* ctx_out);
+
+/* A batch of n_out sequences from the n_seqs of the caches (whose seq_start is not looked at): sequence s takes over the first rows[s] rows of sequence parent[s] (rows NULL: all; a parent outside 0 .. n_seqs - 1: none), and
+ * has pages for grow[s] rows more.  All int32, as table_out [n_out][table_stride], ctx_out [n_out] (rows taken over + grow, cut to what the table can hold) and missing [1].
+ *   Whole pages are shared.  A last page that is partly filled is a sequence's own: where others have the page too, as a whole one, or as their last one with a lower number, or
+ * it is reserved, the sequence gets a new page with its rows copied in all layers (the others' rows, and those behind, stay as they are).  Pages for the rows to come are new ones.
+ *   New pages are those that no sequence of the new batch has taken over and that are not reserved (bytes [n_pages], not 0: reserved; NULL: none), lowest first, handed out in the order
+ * of the sequences, to each its last page first.  So a sequence that nobody takes over is freed, and pages that the caller holds for other ends are to be reserved.
+ *   Where pages run out, entries of table_out are -1 and counted in `missing` (0 otherwise).  Entries taken over that are no page are -1, those behind a sequence's pages too.
+ * table_out and ctx_out are buffers of their own, not those of the caches.  workspace: hip_kv_paged_fork_workspace_bytes bytes, 16-byte aligned, content between calls of no matter; calls that
+ * share one must be ordered.  n_out up to 65536, n_out * table_stride below 2^31.  The new batch in place of the old one, a descriptor per layer with table_out and ctx_out serves the next step. */
+C_EXPORT unsigned long long hip_kv_paged_fork_workspace_bytes(const hip_paged_kv* caches, int n_layers, int n_out);
+C_EXPORT int hip_kv_paged_fork(const hip_paged_kv* caches, int n_layers, int n_out, const void* parent, const void* rows, const void* grow, const void* reserved,
+                               void* table_out, void* ctx_out, void* missing, void* workspace, unsigned long long workspace_bytes);
+
+/* The n_out best continuations of each of n_groups groups of n_beams beams: of beam b by token v with score[b] + log softmax(logits[b])[v], v < vocab.  logits BF16 [n_groups * n_beams] rows
+ * with pitch ld (a multiple of 8), score FP32 [n_groups * n_beams] (NULL: zeros).  Per group, best first: parent_out int32 (the row, counted through all groups, so that hip_kv_paged_fork
+ * takes it as it is), token_out int32 and score_out FP32, [n_groups][n_out] each.  Sums are compared in 64 bits, within a beam the logits themselves; equal ones go to the lower beam, then the lower token.
+ *   last int32 [n_groups * n_beams] (NULL: none): a beam whose last token is `eos` has ended and goes on with eos at its score alone.  A beam whose score is not finite has not begun.  Continuations that cannot be (other
+ * tokens of an ended beam, all of one that has not begun, logits of minus infinity or NaN) have minus infinity and come last, by beam and token; a logit of plus infinity leaves its beam's finite ones no weight.
+ * n_beams up to 64, n_out up to 128 and n_beams * vocab, vocab up to 1048576.  score_out may be score and token_out last if n_out is n_beams; other overlaps are not allowed.
+ * workspace: hip_beam_select_workspace_bytes bytes, 16-byte aligned, content of no matter; calls that share one must be ordered.  logits 16-byte aligned.  0 for n_groups 0. */
+C_EXPORT unsigned long long hip_beam_select_workspace_bytes(int n_groups, int n_beams, int vocab, int n_out);
+C_EXPORT int hip_beam_select_bf16(const void* logits, long long ld, const void* score, const void* last, int eos, int n_groups, int n_beams, int vocab, int n_out,
+                                  void* parent_out, void* token_out, void* score_out, void* workspace, unsigned long long workspace_bytes);
+
+/*
  * Library controls (no counterpart in the reference, which always uses the null stream and always
  * synchronises: cccc-hip/hip_functions.cpp:32-42).
  * Both switches are per host thread, like the reference's current-device pointer (cccc/GpuControl.cpp:18);
