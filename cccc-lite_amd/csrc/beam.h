@@ -7,6 +7,7 @@
 // can have more.
 #pragma once
 #include "quant_device.h"
+#include <type_traits>
 
 namespace ccq
 {
@@ -25,15 +26,24 @@ struct BeamSelect
 };
 
 constexpr int BEAM_THREADS = 256, BEAM_PICK_THREADS = 1024;
-constexpr uint32_t BEAM_LEAST = 0x007Fu, BEAM_MOST = 0xFF80u;              // orders of minus and of plus infinity
 
-// BF16 bits -> 16 bits in the order of the numbers; NaN as minus infinity, -0 as 0.
-__device__ __forceinline__ uint32_t beam_order(uint32_t b)
+// The order of a logit: 16 bits that compare as the numbers do, -0 as 0 (sign and magnitude as a whole number, from 0x8000 on).
+constexpr uint32_t BEAM_LEAST = 0x8000u - 0x7F80u, BEAM_MOST = 0x8000u + 0x7F80u;              // of minus and of plus infinity
+__device__ __forceinline__ float beam_logit(uint32_t order) { return bits_to_f32((order >= 0x8000u ? order - 0x8000u : 0x8000u | (0x8000u - order)) << 16); }
+
+// The same of two logits, not yet from 0x8000 on.
+typedef short beam_i16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t beam_signed(uint32_t two)
 {
-    b = (b & 0x7FFFu) > 0x7F80u ? 0xFF80u : b == 0x8000u ? 0u : b;
-    return b & 0x8000u ? b ^ 0xFFFFu : b | 0x8000u;
+    const beam_i16x2 x = __builtin_bit_cast(beam_i16x2, two), sign = x >> 15;
+    return __builtin_bit_cast(uint32_t, (beam_i16x2)((x ^ (sign & (short)0x7FFF)) - sign));
 }
-__device__ __forceinline__ float beam_logit(uint32_t order) { return bits_to_f32((order & 0x8000u ? order ^ 0x8000u : order ^ 0xFFFFu) << 16); }
+// Order of a logit's bits, NaN as minus infinity.
+__device__ __forceinline__ uint32_t beam_order(uint32_t bits)
+{
+    const uint32_t size = bits & 0x7FFFu;
+    return size > 0x7F80u ? BEAM_LEAST : bits & 0x8000u ? 0x8000u - size : 0x8000u + size;
+}
 
 enum class Beam { ALIVE, ENDED, UNBORN };
 __device__ __forceinline__ Beam beam_state(const BeamSelect& p, int row)
@@ -42,31 +52,28 @@ __device__ __forceinline__ Beam beam_state(const BeamSelect& p, int row)
     return p.last && p.last[row] == p.eos ? Beam::ENDED : Beam::ALIVE;
 }
 
-// e^d for d <= 0 in 64 bits, to 1e-11 of it: 2^n 2^f, |f| <= 1/2, the series of 2^f = e^(f ln 2) to the ninth power.  Scores that are next to each other decide, so
-// that the sum's error has to be well below what separates two of them.
-__device__ __forceinline__ double beam_exp(double d)
+template <class F>
+__device__ __forceinline__ uint32_t beam_reduce(uint32_t v, F f)
 {
-    const double t = fmax(d, -700.0) * 1.4426950408889634074, n = rint(t), x = (t - n) * 0.69314718055994530942;
-    double r = 1.0 / 362880.0;
-    r = fma(r, x, 1.0 / 40320.0);
-    r = fma(r, x, 1.0 / 5040.0);
-    r = fma(r, x, 1.0 / 720.0);
-    r = fma(r, x, 1.0 / 120.0);
-    r = fma(r, x, 1.0 / 24.0);
-    r = fma(r, x, 1.0 / 6.0);
-    r = fma(r, x, 0.5);
-    r = fma(r, x, 1.0);
-    r = fma(r, x, 1.0);
-    return __builtin_bit_cast(double, __builtin_bit_cast(long long, r) + ((long long)(int)n << 52));
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));          // quad_perm [1,0,3,2]
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));          // quad_perm [2,3,0,1]
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));         // row_half_mirror
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));         // row_mirror
+    const uint32_t a = f((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
+    return f(a, f((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
 }
 
-// The largest number that at least k of the 256 at `of` reach, or one between it and the next smaller of them; 1 if fewer than k are above 0.  Bit by bit, by each wave for itself.
-__device__ __forceinline__ uint32_t beam_kth(const uint32_t* of, int k)
+// A number that k of the 256 at `of` reach, or more only if the k-th largest is there several times; the largest of them all in `top`.  Bit by bit behind those that all have in common, by each
+// wave for itself.
+__device__ __forceinline__ uint32_t beam_kth(const uint32_t* of, int k, uint32_t& top)
 {
     const int lane = threadIdx.x & 63;
     const uint32_t v[4] = { of[lane], of[64 + lane], of[128 + lane], of[192 + lane] };
-    uint32_t kth = 0;
-    for (int bit = 31; bit >= 0; bit--)
+    top = beam_reduce(max(max(v[0], v[1]), max(v[2], v[3])), [](uint32_t a, uint32_t b) { return max(a, b); });
+    const uint32_t bottom = beam_reduce(min(min(v[0], v[1]), min(v[2], v[3])), [](uint32_t a, uint32_t b) { return min(a, b); });
+    int bit = 31 - __builtin_clz(top ^ bottom | 1u);
+    uint32_t kth = top >> bit >> 1 << bit << 1;
+    for (; bit >= 0; bit--)
     {
         const uint32_t next = kth | 1u << bit;
         int reach = 0;
@@ -75,84 +82,124 @@ __device__ __forceinline__ uint32_t beam_kth(const uint32_t* of, int k)
         if (reach >= k) { kth = next; }
         if (reach == k) { break; }
     }
-    return max(kth, 1u);
+    return kth;
 }
 
-// A chunk of 256 PER logits of a row, PER of them per thread, eight side by side.  Grid: rows x chunks.  LDS: two lists of numbers.
+// e^d, d <= 0, without the error that log2 e in 24 bits would give all of them alike.
+__device__ __forceinline__ float beam_exp(float d) { return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933349609f, d * 1.92596299112661746887e-8f)); }
+
+// A chunk of 256 PER logits of a row, PER of them per thread, eight side by side; PER <= 64.  Each logit is seen once, as it arrives: the thread's largest number, and its sum
+// beside its largest logit so far (FP32 exponentials of exact differences, errors of both signs: the logarithm of a row's sum is right to some 1e-8).  The few threads that reach the
+// bound have their logits read once more, from the L2.  Grid: rows x chunks.  LDS: two lists of numbers.
 template <int PER>
 __global__ __launch_bounds__(BEAM_THREADS) void beam_chunk_kernel(const BeamSelect p)
 {
     constexpr int CHUNK = BEAM_THREADS * PER, VECTORS = PER / 8;
+    constexpr uint32_t BARRED = 0xFF80FF80u;                                // minus infinity, twice
     extern __shared__ __attribute__((aligned(16))) uint32_t lists[];
-    __shared__ __attribute__((aligned(16))) uint32_t best[BEAM_THREADS];
+    __shared__ uint32_t best[BEAM_THREADS];
     __shared__ double sums[BEAM_THREADS / 64];
-    __shared__ int counts[2];
-    const int row = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks, first = chunk * CHUNK, left = p.vocab - first;
-    const Beam state = beam_state(p, row);
+    __shared__ int winners[128];
+    __shared__ int counts[3];
+    const int row = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks, first = chunk * CHUNK, left = p.vocab - first, lane = threadIdx.x & 63;
     const uint16_t* const src = p.logits + (size_t)row * p.ld + first;
-    u32x4 raw[VECTORS];
-#pragma unroll
-    for (int v = 0; v < VECTORS; v++)
-    {
-        const int at = (v * BEAM_THREADS + (int)threadIdx.x) * 8;
-        raw[v] = state == Beam::ALIVE && at < left ? *(const u32x4*)(src + at) : u32x4{ 0, 0, 0, 0 };
-    }
-    // element e of vector v as a number
-    auto number = [&](int v, int e) {
-        const int at = (v * BEAM_THREADS + (int)threadIdx.x) * 8 + e;
-        uint32_t order = beam_order(raw[v][e / 2] >> (16 * (e & 1)) & 0xFFFFu);
-        if (state != Beam::ALIVE) { order = state == Beam::ENDED && first + at == p.eos ? BEAM_MOST : BEAM_LEAST; }
-        return at < left ? order << 16 | (uint32_t)(0xFFFF - at) : 0u;
-    };
-    uint32_t mine = 0;
-#pragma unroll
-    for (int v = 0; v < VECTORS; v++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) { mine = max(mine, number(v, e)); }
-    best[threadIdx.x] = mine;
-    if (threadIdx.x < 2) { counts[threadIdx.x] = 0; }
-    __syncthreads();
-    uint32_t from = beam_kth(best, p.n_out), top = max(max(best[threadIdx.x & 63], best[64 + (threadIdx.x & 63)]), max(best[128 + (threadIdx.x & 63)], best[192 + (threadIdx.x & 63)]));
-#pragma unroll
-    for (int d = 32; d >= 1; d /= 2) { top = max(top, (uint32_t)__shfl_xor((int)top, d)); }
-    // the sum, of rows that go on
-    const float m = beam_logit(top >> 16);
-    double sum = 0.0;
-    if (state == Beam::ALIVE)
-    {
+    auto place = [&](int thread, int n) { return (n / 8 * BEAM_THREADS + thread) * 8 + n % 8; };                   // of a thread's n-th
+    int largest = -0x7FFFFFFF - 1;                                          // order, then 63 - n
+    float m = -3.402823466e38f, sum = 0.0f;
+    auto take = [&](auto partial) {
+        // a last chunk: behind the vocabulary barred, and left out at the end
+        u32x4 raw[VECTORS];
 #pragma unroll
         for (int v = 0; v < VECTORS; v++)
+        {
+            const int at = place(threadIdx.x, 8 * v);
+            raw[v] = *(const u32x4*)(src + (partial && at >= left ? 0 : at));
+        }
 #pragma unroll
-            for (int e = 0; e < 8; e++)
+        for (int v = 0; v < VECTORS; v++)
+        {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
             {
-                const uint32_t of = number(v, e);
-                const float x = beam_logit(of >> 16);
-                if (of != 0 && x > -INFINITY) { sum += x == m ? 1.0 : m == INFINITY ? 0.0 : beam_exp((double)x - (double)m); }
+                const int n = 8 * v + e;
+                uint32_t two = raw[v][e / 2];
+                if constexpr (partial)
+                {
+                    two = place(threadIdx.x, n) < left ? two : BARRED;
+                    two = place(threadIdx.x, n + 1) < left ? two : (two & 0xFFFFu) | (BARRED & 0xFFFF0000u);
+                }
+                const uint32_t order = beam_signed(two);
+                largest = max(largest, max((int)(order << 16 | (uint32_t)(63 - n)), (int)((order & 0xFFFF0000u) | (uint32_t)(62 - n))));
+                x[e] = bits_to_f32(two << 16);
+                x[e + 1] = bits_to_f32(two & 0xFFFF0000u);
             }
-    }
+            const float next = fmaxf(fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))), m);
+            float part[2] = { sum * beam_exp(m - next), 0.0f };
 #pragma unroll
-    for (int d = 32; d >= 1; d /= 2) { sum += __shfl_xor(sum, d); }
-    if ((threadIdx.x & 63) == 0) { sums[threadIdx.x >> 6] = sum; }
-    __syncthreads();
-    if (threadIdx.x == 0)
+            for (int e = 0; e < 8; e++) { part[e & 1] += beam_exp(x[e] - next); }
+            sum = part[0] + part[1];
+            m = next;
+        }
+    };
+    if (left >= CHUNK) { take(std::false_type()); }
+    else { take(std::true_type()); }
+    const Beam state = beam_state(p, row);
+    const int eos = state == Beam::ENDED ? p.eos - first : -1;
+    auto number = [](uint32_t order, int at) { return order << 16 | (uint32_t)(0xFFFF - at); };
+    auto number_of = [&](uint32_t bits, int at) { return number(state == Beam::ALIVE ? beam_order(bits) : at == eos ? BEAM_MOST : BEAM_LEAST, at); };
+    uint32_t mine = number((uint32_t)((largest >> 16) + 0x8000), place(threadIdx.x, 63 - (largest & 0xFFFF)));
+    if (state != Beam::ALIVE)
     {
-        double all = 0.0;
-#pragma unroll
-        for (int w = 0; w < BEAM_THREADS / 64; w++) { all += sums[w]; }
-        p.stats[(size_t)row * p.chunks + chunk] = make_double2(m, all);
+        const bool owns = eos >= 0 && eos < CHUNK && eos / 8 % BEAM_THREADS == (int)threadIdx.x;
+        mine = number_of(0, owns ? eos : place(threadIdx.x, 0));
+        sum = 0.0f;
     }
+    else if (!(sum == sum))
+    {
+        // NaN or plus infinity among them: one by one
+        mine = 0;
+        for (int n = 0; n < PER; n++)
+        {
+            const int at = place(threadIdx.x, n);
+            mine = max(mine, number_of(at < left ? src[at] : 0xFF80u, at));
+        }
+        m = beam_logit(mine >> 16);
+        sum = 0.0f;
+        for (int n = 0; n < PER && m > -INFINITY; n++)
+        {
+            const int at = place(threadIdx.x, n);
+            const float x = beam_logit(number_of(at < left ? src[at] : 0xFF80u, at) >> 16);
+            sum += x == m ? 1.0f : m < INFINITY ? beam_exp(x - m) : 0.0f;
+        }
+    }
+    best[threadIdx.x] = mine;
+    if (threadIdx.x < 3) { counts[threadIdx.x] = 0; }
+    __syncthreads();
+    uint32_t top;
+    uint32_t from = beam_kth(best, p.n_out, top);
+    const float all_m = beam_logit(top >> 16);
+    double all = m == all_m ? (double)sum : all_m < INFINITY && sum > 0.0f ? (double)(sum * beam_exp(m - all_m)) : 0.0;
+#pragma unroll
+    for (int d = 32; d >= 1; d /= 2) { all += __shfl_xor(all, d); }
+    if (lane == 0) { sums[threadIdx.x >> 6] = all; }
+    if (mine >= from) { winners[atomicAdd(counts + 2, 1)] = threadIdx.x; }
+    __syncthreads();
+    if (threadIdx.x == 0) { p.stats[(size_t)row * p.chunks + chunk] = make_double2(all_m, (sums[0] + sums[1]) + (sums[2] + sums[3])); }
     // what reaches the K-th largest of the threads' largest
     uint32_t *list = lists, *next = lists + p.n_out * PER;
-    if (mine >= from)
+    const int n_winners = counts[2];
+    for (int i = threadIdx.x; i < n_winners * VECTORS; i += BEAM_THREADS)
     {
+        const int at = place(winners[i / VECTORS], i % VECTORS * 8);
+        if (at >= left) { continue; }
+        const u32x4 eight = *(const u32x4*)(src + at);
 #pragma unroll
-        for (int v = 0; v < VECTORS; v++)
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-            {
-                const uint32_t of = number(v, e);
-                if (of >= from) { list[atomicAdd(counts, 1)] = of; }
-            }
+        for (int e = 0; e < 8; e++)
+        {
+            const uint32_t of = number_of(eight[e / 2] >> (16 * (e & 1)) & 0xFFFFu, at + e);
+            if (of >= from && at + e < left) { list[atomicAdd(counts, 1)] = of; }
+        }
     }
     __syncthreads();
     int n = counts[0];
@@ -164,7 +211,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_chunk_kernel(const BeamSele
         best[threadIdx.x] = mine;
         if (threadIdx.x == 0) { counts[round & 1] = 0; }
         __syncthreads();
-        from = beam_kth(best, p.n_out);
+        from = beam_kth(best, p.n_out, top);
         for (int i = threadIdx.x; i < n; i += BEAM_THREADS)
         {
             const uint32_t of = list[i];
@@ -181,9 +228,9 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_chunk_kernel(const BeamSele
     for (int i = threadIdx.x; i < n; i += BEAM_THREADS)
     {
         const uint32_t of = list[i];
-        int place = 0;
-        for (int j = 0; j < n; j++) { place += list[j] > of; }
-        if (place < p.n_out) { found[place] = of; }
+        int rank = 0;
+        for (int j = 0; j < n; j++) { rank += list[j] > of; }
+        if (rank < p.n_out) { found[rank] = of; }
     }
 }
 
@@ -194,7 +241,11 @@ struct BeamRank
     __device__ __forceinline__ bool operator>(const BeamRank& o) const { return total > o.total || (total == o.total && then > o.then); }
 };
 
-// The n_out best of what the chunks of a group's rows left: byte by byte of their ranks, by how many have each value, until just n_out reach the bytes found.  Grid: groups.
+// The n_out best of what the chunks of a group's rows left, whose lists are in order.  With j + 1 of each list at least as large as its j-th, as many lists as n_out needs give a bound
+// that n_out continuations reach, and few more do: those are ranked by counting.  Where more reach it than there is room for (equal totals, such as minus infinity), the ranks are gone
+// through byte by byte, by how many have each value, until just n_out reach the bytes found.  Grid: groups.
+constexpr int BEAM_ROOM = 512;
+
 template <int PER>
 __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const BeamSelect p)
 {
@@ -203,21 +254,37 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
     __shared__ Beam states[64];
     __shared__ int bins[256];
     __shared__ int chosen[3];                                               // the byte, how many are above it, and with it
-    __shared__ BeamRank picked[128];
-    __shared__ int from[128];
+    __shared__ BeamRank picked[BEAM_ROOM];
+    __shared__ int from[BEAM_ROOM];
+    __shared__ uint32_t heads[256];
     __shared__ int count;
     const int group = blockIdx.x, row0 = group * p.n_beams, per_row = p.chunks * p.n_out, n_all = p.n_beams * per_row;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // asked for beside the statistics: what the thread keeps, and its list's entry for the bound, to which the first 256 lists go
+    const uint32_t* const found = p.found + (size_t)row0 * per_row;
+    const int n_lists = min(p.n_beams * p.chunks, 256), deep = (p.n_out + n_lists - 1) / n_lists - 1, head = threadIdx.x * p.n_out + deep;
+    const bool holds = n_all <= HELD * BEAM_PICK_THREADS;
+    uint32_t words[HELD], head_word = (int)threadIdx.x < n_lists ? found[head] : 0u;
+#pragma unroll
+    for (int n = 0; n < HELD; n++)
+    {
+        const int i = n * BEAM_PICK_THREADS + threadIdx.x;
+        words[n] = holds && i < n_all ? found[i] : 0u;
+    }
     for (int b = wave; b < p.n_beams; b += BEAM_PICK_THREADS / 64)
     {
         const double2* const of = p.stats + (size_t)(row0 + b) * p.chunks;
-        double m = -INFINITY, sum = 0.0;
-        for (int c = lane; c < p.chunks; c += 64) { m = fmax(m, of[c].x); }
-#pragma unroll
-        for (int d = 32; d >= 1; d /= 2) { m = fmax(m, __shfl_xor(m, d)); }
-        for (int c = lane; c < p.chunks; c += 64) { sum += of[c].x == m ? of[c].y : m < INFINITY ? of[c].y * exp(of[c].x - m) : 0.0; }
-#pragma unroll
-        for (int d = 32; d >= 1; d /= 2) { sum += __shfl_xor(sum, d); }
+        double m, sum;
+        const double2 mine = lane < p.chunks ? of[lane] : make_double2(-INFINITY, 0.0);
+        m = mine.x;
+        for (int c = lane + 64; c < p.chunks; c += 64) { m = fmax(m, of[c].x); }
+        const int span = min(p.chunks, 64);
+        for (int d = 1; d < span; d *= 2) { m = fmax(m, __shfl_xor(m, d)); }
+        m = __shfl(m, 0);
+        auto part = [&](const double2& c) { return c.x == m ? c.y : m < INFINITY && c.y > 0.0 ? c.y * exp(c.x - m) : 0.0; };
+        sum = part(mine);
+        for (int c = lane + 64; c < p.chunks; c += 64) { sum += part(of[c]); }
+        for (int d = 1; d < span; d *= 2) { sum += __shfl_xor(sum, d); }
         if (lane == 0)
         {
             states[b] = beam_state(p, row0 + b);
@@ -228,10 +295,8 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
     }
     if (threadIdx.x == 0) { count = 0; }
     __syncthreads();
-    const uint32_t* const found = p.found + (size_t)row0 * per_row;
     auto token_of = [&](int i, uint32_t of) { return i % per_row / p.n_out * CHUNK + (0xFFFF - (int)(of & 0xFFFFu)); };
-    auto rank_of = [&](int i) {
-        const uint32_t of = i < n_all ? found[i] : 0u;
+    auto rank_of = [&](int i, uint32_t of) {
         if (of == 0) { return BeamRank{ 0, 0 }; }
         const int b = i / per_row;
         const uint32_t order = of >> 16;
@@ -246,12 +311,8 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
         return BeamRank{ bits >> 63 ? ~bits : bits | 1ull << 63, (unsigned long long)(0xFFFF - b) << 48 | (unsigned long long)order << 32 | (0xFFFFFFFFu - (uint32_t)token_of(i, of)) };
     };
     BeamRank held[HELD];
-    const bool holds = n_all <= HELD * BEAM_PICK_THREADS;
-    if (holds)
-    {
 #pragma unroll
-        for (int n = 0; n < HELD; n++) { held[n] = rank_of(n * BEAM_PICK_THREADS + threadIdx.x); }
-    }
+    for (int n = 0; n < HELD; n++) { held[n] = rank_of(n * BEAM_PICK_THREADS + threadIdx.x, words[n]); }
     auto each = [&](auto f) {
         if (holds)
         {
@@ -260,77 +321,104 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
         }
         else
         {
-            for (int i = threadIdx.x; i < n_all; i += BEAM_PICK_THREADS) { f(i, rank_of(i)); }
+            for (int i = threadIdx.x; i < n_all; i += BEAM_PICK_THREADS) { f(i, rank_of(i, found[i])); }
         }
     };
-    // ranks that agree with `least` in the bytes found so far are open, larger ones are in: `need` more
-    BeamRank least = { 0, 0 };
-    int need = p.n_out;
-    for (int byte = 0; byte < 16; byte++)
-    {
-        const int shift = 56 - byte % 8 * 8;
-        if (threadIdx.x < 256) { bins[threadIdx.x] = 0; }
-        __syncthreads();
-        each([&](int, const BeamRank& r) {
-            const unsigned long long word = byte < 8 ? r.total : r.then, known = byte < 8 ? least.total : least.then;
-            const bool open = (byte < 8 || r.total == least.total) && (shift == 56 || word >> (shift + 8) == known >> (shift + 8));
-            if (open && (r.total | r.then) != 0) { atomicAdd(bins + (word >> shift & 255), 1); }
-        });
-        __syncthreads();
-        if (wave == 0)
-        {
-            // lane l: bins 255 - 4 l down to 252 - 4 l
-            int n[4], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-            {
-                n[i] = bins[255 - 4 * lane - i];
-                sum += n[i];
-            }
-            int above = sum;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2)
-            {
-                const int other = __shfl_up(above, d);
-                above += lane >= d ? other : 0;
-            }
-            above -= sum;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-            {
-                if (above < need && above + n[i] >= need)
-                {
-                    chosen[0] = 255 - 4 * lane - i;
-                    chosen[1] = above;
-                    chosen[2] = n[i];
-                }
-                above += n[i];
-            }
-        }
-        __syncthreads();
-        (byte < 8 ? least.total : least.then) |= (unsigned long long)chosen[0] << shift;
-        need -= chosen[1];
-        if (chosen[2] == need) { break; }
-    }
-    // all from `least` on, n_out of them, each to its place
+    // the bound, of the totals' upper halves
+    if (threadIdx.x < 256) { heads[threadIdx.x] = (uint32_t)(rank_of(head, head_word).total >> 32); }
+    __syncthreads();
+    uint32_t top;
+    const uint32_t bound = beam_kth(heads, (p.n_out + deep) / (deep + 1), top);
     each([&](int i, const BeamRank& r) {
-        if (!(least > r) && (r.total | r.then) != 0)
+        if ((uint32_t)(r.total >> 32) >= bound && (r.total | r.then) != 0)
         {
             const int at = atomicAdd(&count, 1);
-            picked[at] = r;
-            from[at] = i;
+            if (at < BEAM_ROOM)
+            {
+                picked[at] = r;
+                from[at] = i;
+            }
         }
     });
     __syncthreads();
-    if ((int)threadIdx.x < p.n_out)
+    int n_picked = count;
+    if (n_picked > BEAM_ROOM)
+    {
+        __syncthreads();
+        if (threadIdx.x == 0) { count = 0; }
+        // ranks that agree with `least` in the bytes found so far are open, larger ones are in: `need` more
+        BeamRank least = { 0, 0 };
+        int need = p.n_out;
+        for (int byte = 0; byte < 16; byte++)
+        {
+            const int shift = 56 - byte % 8 * 8;
+            if (threadIdx.x < 256) { bins[threadIdx.x] = 0; }
+            __syncthreads();
+            each([&](int, const BeamRank& r) {
+                const unsigned long long word = byte < 8 ? r.total : r.then, known = byte < 8 ? least.total : least.then;
+                const bool open = (byte < 8 || r.total == least.total) && (shift == 56 || word >> (shift + 8) == known >> (shift + 8));
+                if (open && (r.total | r.then) != 0) { atomicAdd(bins + (word >> shift & 255), 1); }
+            });
+            __syncthreads();
+            if (wave == 0)
+            {
+                // lane l: bins 255 - 4 l down to 252 - 4 l
+                int n[4], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                {
+                    n[i] = bins[255 - 4 * lane - i];
+                    sum += n[i];
+                }
+                int above = sum;
+#pragma unroll
+                for (int d = 1; d < 64; d *= 2)
+                {
+                    const int other = __shfl_up(above, d);
+                    above += lane >= d ? other : 0;
+                }
+                above -= sum;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                {
+                    if (above < need && above + n[i] >= need)
+                    {
+                        chosen[0] = 255 - 4 * lane - i;
+                        chosen[1] = above;
+                        chosen[2] = n[i];
+                    }
+                    above += n[i];
+                }
+            }
+            __syncthreads();
+            (byte < 8 ? least.total : least.then) |= (unsigned long long)chosen[0] << shift;
+            need -= chosen[1];
+            if (chosen[2] == need) { break; }
+        }
+        // all from `least` on, n_out of them
+        each([&](int i, const BeamRank& r) {
+            if (!(least > r) && (r.total | r.then) != 0)
+            {
+                const int at = atomicAdd(&count, 1);
+                picked[at] = r;
+                from[at] = i;
+            }
+        });
+        __syncthreads();
+        n_picked = p.n_out;
+    }
+    if ((int)threadIdx.x < n_picked)
     {
         const BeamRank mine = picked[threadIdx.x];
         int place = 0;
-        for (int j = 0; j < p.n_out; j++) { place += picked[j] > mine; }
-        const int i = from[threadIdx.x], to = group * p.n_out + place;
-        p.parent_out[to] = row0 + i / per_row;
-        p.token_out[to] = token_of(i, found[i]);
-        p.score_out[to] = (float)__builtin_bit_cast(double, mine.total >> 63 ? mine.total & ~(1ull << 63) : ~mine.total);
+        for (int j = 0; j < n_picked; j++) { place += picked[j] > mine; }
+        if (place < p.n_out)
+        {
+            const int i = from[threadIdx.x], to = group * p.n_out + place;
+            p.parent_out[to] = row0 + i / per_row;
+            p.token_out[to] = token_of(i, found[i]);
+            p.score_out[to] = (float)__builtin_bit_cast(double, mine.total >> 63 ? mine.total & ~(1ull << 63) : ~mine.total);
+        }
     }
 }
 
