@@ -24,11 +24,11 @@ bool layers_args(const hip_paged_kv* caches, int n_layers, PagedArgs& a)
     return true;
 }
 
-// Layers from `first` on that one launch takes with `per_layer` workgroups each.
-PagedLayers some_layers(const hip_paged_kv* caches, int first, int n_layers, long long per_layer)
+// Layers from `first` on that one launch takes: 64 of up to 2 * 65536 workgroups each are half of what a grid can have.
+PagedLayers some_layers(const hip_paged_kv* caches, int first, int n_layers)
 {
     PagedLayers l = {};
-    l.n = (int)std::max(1LL, std::min<long long>(std::min(n_layers - first, MOVE_LAYERS), MOST_BLOCKS / per_layer));
+    l.n = std::min(n_layers - first, MOVE_LAYERS);
     l.row = caches->head_dim * (caches->type == CCCC_BFLOAT16 ? 2 : 1);
     for (int i = 0; i < l.n; i++)
     {
@@ -53,7 +53,7 @@ int hip_kv_paged_keep(const hip_paged_kv* caches, int n_layers, const void* keep
     const long long per_layer = 2LL * a.n_seqs;
     for (int first = 0; first < n_layers;)
     {
-        const PagedLayers layers = some_layers(caches, first, n_layers, per_layer);
+        const PagedLayers layers = some_layers(caches, first, n_layers);
         const PagedKeep p = { (const int*)keep, (const int*)n_keep, first == 0 ? (int*)ctx_out : nullptr, n_tokens, max_new };
         paged_keep_kernel<<<(unsigned)(per_layer * layers.n), 256, 0, stream()>>>(a, layers, p);
         first += layers.n;
@@ -64,8 +64,8 @@ int hip_kv_paged_keep(const hip_paged_kv* caches, int n_layers, const void* keep
 unsigned long long hip_kv_paged_fork_workspace_bytes(const hip_paged_kv* caches, int n_layers, int n_out)
 {
     PagedArgs a;
-    if (!layers_args(caches, n_layers, a) || n_out <= 0 || n_out > 65536 || (long long)n_out * a.table_stride > 0x7FFFFFFFLL) { return 0; }
-    return padded((size_t)n_out * 16) + padded((size_t)n_out * 4) + 2 * padded((size_t)a.n_pages * 4);
+    if (!layers_args(caches, n_layers, a) || n_out <= 0 || n_out > 65536 || (long long)n_out * a.table_stride > 0x3FFFFFFFLL) { return 0; }
+    return 16 + padded((size_t)n_out * 8) + 2 * padded((size_t)a.n_pages * 4);
 }
 
 int hip_kv_paged_fork(const hip_paged_kv* caches, int n_layers, int n_out, const void* parent, const void* rows, const void* grow, const void* reserved, void* table_out, void* ctx_out, void* missing,
@@ -77,22 +77,24 @@ int hip_kv_paged_fork(const hip_paged_kv* caches, int n_layers, int n_out, const
     {
         if (!aligned(p, 4)) { return -1; }
     }
-    if ((long long)n_out * a.table_stride > 0x7FFFFFFFLL || !aligned(workspace, 16) || table_out == caches->page_table || ctx_out == caches->ctx_len || workspace_bytes < hip_kv_paged_fork_workspace_bytes(caches, n_layers, n_out)) { return -1; }
+    if ((long long)n_out * a.table_stride > 0x3FFFFFFFLL || !aligned(workspace, 16) || table_out == caches->page_table || ctx_out == caches->ctx_len || workspace_bytes < hip_kv_paged_fork_workspace_bytes(caches, n_layers, n_out)) { return -1; }
     char* at = (char*)workspace;
     PagedFork f = { (const int*)parent, (const int*)rows, (const int*)grow, (const uint8_t*)reserved, (int*)table_out, (int*)ctx_out, (int*)missing, n_out };
-    f.copies = (int*)at;
-    at += padded((size_t)n_out * 16);
+    f.n_free = (int*)at;
+    at += 16;
     f.base = (int*)at;
-    at += padded((size_t)n_out * 4);
+    at += padded((size_t)n_out * 8);
     f.holder = (int*)at;
     at += padded((size_t)a.n_pages * 4);
     f.free_pages = (int*)at;
-    paged_fork_kernel<<<1, FORK_THREADS, 0, stream()>>>(a, f);
-    const long long per_layer = 2LL * n_out;
+    if (a.n_pages <= FORK_LDS_PAGES) { paged_fork_kernel<true><<<1, FORK_THREADS, 0, stream()>>>(a, f); }
+    else { paged_fork_kernel<false><<<1, FORK_THREADS, 0, stream()>>>(a, f); }
+    const long long per_layer = 2LL * n_out, tables = (long long)n_out * ((a.table_stride + 255) / 256);
     for (int first = 0; first < n_layers;)
     {
-        const PagedLayers layers = some_layers(caches, first, n_layers, per_layer);
-        paged_fork_copy_kernel<<<(unsigned)(per_layer * layers.n), 256, 0, stream()>>>(a, layers, f.copies, n_out);
+        const PagedLayers layers = some_layers(caches, first, n_layers);
+        const unsigned n_copies = (unsigned)(per_layer * layers.n);
+        paged_fork_copy_kernel<<<n_copies + (first == 0 ? (unsigned)tables : 0), 256, 0, stream()>>>(a, layers, f, (int)n_copies);
         first += layers.n;
     }
     return finish("kv_paged_fork");

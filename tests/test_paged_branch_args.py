@@ -96,8 +96,8 @@ def test_fork_arguments(setup):
                 dict(missing=p + 8195), dict(ws=p + 16392), dict(nb=need - 1), dict(nb=0), dict(n_out=0), dict(n_out=-1), dict(n_out=65537), dict(table=p), dict(ctx=p + 64)):
         assert fork(lib, c, p, **bad) == -1, bad
     wide = capi.paged_layers([capi.make_paged_kv(**(good | dict(table_stride=2 ** 20)))])
-    assert lib.kv_paged_fork_workspace_bytes(wide, 1, 2048) == 0 and fork(lib, wide, p, n_out=2048, nb=1 << 40) == -1
-    assert lib.kv_paged_fork_workspace_bytes(wide, 1, 2047) > 0
+    assert lib.kv_paged_fork_workspace_bytes(wide, 1, 1024) == 0 and fork(lib, wide, p, n_out=1024, nb=1 << 40) == -1
+    assert lib.kv_paged_fork_workspace_bytes(wide, 1, 1023) > 0
     assert lib.kv_paged_fork_workspace_bytes(c, 1, 0) == 0
     assert not raw.any()
 
