@@ -96,6 +96,7 @@ EXPORTS = (
     "hip_attention_paged_workspace_bytes",
     "hip_attention_paged_bf16",
     "hip_qk_norm_rope_kv_paged_at_bf16",
+    "hip_attention_paged_tree_workspace_bytes",
     "hip_attention_paged_tree_bf16",
     "hip_kv_paged_keep",
     "hip_kv_paged_fork_workspace_bytes",
@@ -198,6 +199,8 @@ class QuantLibrary:
         L.hip_attention_paged_bf16.argtypes = [kv, vp, vp, vp, u64] + [i32] * 8
         L.hip_qk_norm_rope_kv_paged_at_bf16.restype = i32
         L.hip_qk_norm_rope_kv_paged_at_bf16.argtypes = [kv] + [vp] * 7 + [i32, vp, i32, i64, vp, vp, i32, i32, i32, i32, i32, f32]
+        L.hip_attention_paged_tree_workspace_bytes.restype = u64
+        L.hip_attention_paged_tree_workspace_bytes.argtypes = L.hip_attention_paged_workspace_bytes.argtypes
         L.hip_attention_paged_tree_bf16.restype = i32
         L.hip_attention_paged_tree_bf16.argtypes = [kv, vp, vp, vp, i64, vp, u64] + [i32] * 8
         L.hip_kv_paged_keep.restype = i32
@@ -295,6 +298,9 @@ class QuantLibrary:
                                  n_q_heads, n_tokens, ldq, ldk, ldv, eps=1e-6) -> int:
         return self.c.hip_qk_norm_rope_kv_paged_at_bf16(cache, q, k, v, q_norm_w, k_norm_w, cos_tab, sin_tab, n_positions, positions, n_axes, position_stride, axis, q_out, n_q_heads, n_tokens,
                                                         ldq, ldk, ldv, eps)
+
+    def attention_paged_tree_workspace_bytes(self, cache: PagedKV, n_q_heads, n_tokens, max_new, max_ctx, window=0, n_sink=0) -> int:
+        return int(self.c.hip_attention_paged_tree_workspace_bytes(cache, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink))
 
     def attention_paged_tree(self, cache: PagedKV, q, y, seen, seen_stride, workspace, workspace_bytes, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, ldq, ldy) -> int:
         return self.c.hip_attention_paged_tree_bf16(cache, q, y, seen, seen_stride, workspace, workspace_bytes, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, ldq, ldy)

@@ -41,10 +41,7 @@ int hip_kv_paged_read_bf16(const hip_paged_kv* cache, void* k_out, void* v_out, 
 
 unsigned long long hip_attention_paged_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink)
 {
-    PagedArgs a;
-    if (!attention_args(cache, a, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink) || n_tokens == 0) { return 0; }
-    Plan plan;
-    return plan_attention(a, keys_per_block(cache), n_q_heads, cache->head_dim, n_tokens, max_new, window, n_sink, plan) ? plan.tile_bytes + plan.row_bytes : 0;
+    return attention_workspace_bytes(cache, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, false);
 }
 
 int hip_attention_paged_bf16(const hip_paged_kv* cache, const void* q, void* y, void* workspace, unsigned long long workspace_bytes, int n_q_heads, int n_tokens, int max_new, int max_ctx,

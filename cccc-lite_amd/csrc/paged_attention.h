@@ -28,12 +28,20 @@ struct PagedAttention
     float scale;                    // log2 e / sqrt(dim)
     const unsigned long long* seen; // trees: bits of the new tokens that a token sees, seen_stride words each
     size_t seen_stride;
+    int piece_slots;                // trees: `tiles` counts pieces of tiles (find_piece), about so many of them per kv head besides one for each tile; 0: whole tiles
 
     __device__ __forceinline__ float* row_sums(int slot, int kvh, int n_kv, int row, int dim) const { return row_partial + (((size_t)slot * n_kv + kvh) * 16 + row) * dim; }
     __device__ __forceinline__ float* row_stats(int slot, int kvh, int n_kv, int row, int dim) const
     {
         return row_partial + (size_t)row_parts * n_kv * 16 * dim + (((size_t)slot * n_kv + kvh) * 16 + row) * 2;
     }
+    // of a piece of a tile that is in several, 2 piece_slots of them at most, by its row in the tile
+    __device__ __forceinline__ float* piece_sums(int piece, int kvh, int n_kv, int row, int dim) const { return partial + (((size_t)piece * n_kv + kvh) * 128 + row) * dim; }
+    __device__ __forceinline__ float2* piece_stats(int piece, int kvh, int n_kv, int row, int dim) const
+    {
+        return (float2*)(partial + (size_t)2 * piece_slots * n_kv * 128 * dim) + ((size_t)piece * n_kv + kvh) * 128 + row;
+    }
+    __device__ __forceinline__ float* piece_length() const { return partial - 4; }       // 1 / blocks of a range
     __device__ __forceinline__ size_t outputs() const { return (size_t)n_tokens * n_q; }
     __device__ __forceinline__ float* sums(int range, size_t row, int dim) const { return partial + ((size_t)range * outputs() + row) * dim; }
     __device__ __forceinline__ float2* stats(int range, size_t row, int dim) const { return (float2*)(partial + (size_t)tile_split * outputs() * dim) + (size_t)range * outputs() + row; }
@@ -209,9 +217,10 @@ struct Parts
 };
 
 // A tile: rows row0 .. + 127 of sequence s (< 0: none), the positions of their tokens and the keys they see, in n_ranges ranges of `per` blocks.
+// Of trees: the range that workgroup `tile` has of it, and where the sums of its first range go.
 struct Tile
 {
-    int s = -1, row0 = 0, n_rows = 0, lo = 0, hi = 0, per = 1, n_ranges = 1;
+    int s = -1, row0 = 0, n_rows = 0, lo = 0, hi = 0, per = 1, n_ranges = 1, range = 0, piece0 = 0;
     NewTokens mine = { 0, 0, 0 };
     KeyBlocks<PA_TILE_KEYS> blocks;
 };
@@ -220,7 +229,6 @@ struct Tile
 // the tiles comes in the other order, so that a long one has a short one beside it (MI355X, 512 tiles of 2048 tokens behind 6000: 249 us for 256; with more
 // tiles than that a CU takes the next one when it is done, and the order from long to short is the better one: 2000 tiles of four prompts 142 us for 146).  Called by whole waves: a lane per
 // sequence, 256 of them per trip to memory, their tiles added up.
-template <bool TREE>
 __device__ __forceinline__ Tile find_tile(const PagedArgs& a, const PagedAttention& p, int tile)
 {
     Tile r;
@@ -257,14 +265,131 @@ __device__ __forceinline__ Tile find_tile(const PagedArgs& a, const PagedAttenti
     }
     if (r.s < 0) { return r; }
     r.n_rows = uniform(r.mine.n * p.group);
-    r.lo = uniform(TREE ? r.mine.pos : r.mine.pos + r.row0 / p.group);
-    r.hi = uniform(TREE ? r.mine.pos + r.mine.n - 1 : r.mine.pos + min(r.row0 + PA_TILE - 1, r.n_rows - 1) / p.group);
+    r.lo = uniform(r.mine.pos + r.row0 / p.group);
+    r.hi = uniform(r.mine.pos + min(r.row0 + PA_TILE - 1, r.n_rows - 1) / p.group);
     r.blocks = KeyBlocks<PA_TILE_KEYS>(p, r.lo, r.hi);
     r.blocks.n = uniform(r.blocks.n);
     r.blocks.sinks = uniform(r.blocks.sinks);
     r.blocks.skip = uniform(r.blocks.skip);
     r.per = max((r.blocks.n + p.tile_split - 1) / p.tile_split, 4);
     r.n_ranges = max((r.blocks.n + r.per - 1) / r.per, 1);
+    return r;
+}
+
+// Trees: piece `piece` of all tiles' ranges of keys.  All of a sequence's tiles see the same blocks, so that lengths alone say how many pieces there are.  Every range is of about the same length, which follows from
+// all sequences: the shortest, from an even split over the workgroups that run at once, with which there are no more pieces than those (a piece costs 5 us besides its 2.15 per block, and its sums are written and read), but
+// at least PIECE_LEAST blocks.  With more than 256 sequences, or tiles enough, it is the even split.  MI355X us, attention + the launch that adds, 32 / 8 heads of 128 E4M3, 32 sequences of 17 to 33 tokens on 1000 to 8000
+// rows: as many ranges for short ones as for long ones 150 + 10, these 120 + 11.
+// ADDED: tile `piece` of those in several ranges, with the length that the attention's first workgroup left.
+constexpr int PIECE_LEAST = 4;
+
+template <bool ADDED>
+__device__ __forceinline__ Tile find_piece(const PagedArgs& a, const PagedAttention& p, int piece)
+{
+    Tile r;
+    const int lane = threadIdx.x & 63;
+    SeqWords words[4];
+    NewTokens mine[4];
+    int tiles[4], blocks[4];
+    auto read = [&](int base) {                                             // 256 sequences
+        words[0] = SeqWords(a, base + lane);
+        if (base + 64 < a.n_seqs)
+        {
+#pragma unroll
+            for (int b = 1; b < 4; b++) { words[b] = SeqWords(a, base + 64 * b + lane); }
+        }
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+        {
+            if (b != 0 && base + 64 * b >= a.n_seqs)
+            {
+                tiles[b] = blocks[b] = 0;
+                continue;
+            }
+            mine[b] = words[b].tokens(a, p, base + 64 * b + lane);
+            const int rows = mine[b].n * p.group;
+            tiles[b] = rows > p.min_rows ? (rows + PA_TILE - 1) / PA_TILE : 0;
+            blocks[b] = tiles[b] > 0 ? KeyBlocks<PA_TILE_KEYS>(p, mine[b].pos, mine[b].pos + mine[b].n - 1).n : 0;
+        }
+    };
+    // ranges of `per` blocks, or so (the same for whoever asks)
+    auto ranges_of = [](int n, float by) { return max((int)ceilf((float)n * by - 0.001f), 1); };
+    float by = 0.0f;                                                        // 1 / per
+    const float left = ADDED ? *p.piece_length() : 0.0f;
+    read(0);
+    if (ADDED) { by = left; }
+    else if (p.piece_slots > 0)
+    {
+        float all = 0.0f;
+        int n_tiles = 0;
+        for (int base = 0; base < a.n_seqs; base += 256)
+        {
+            if (base != 0) { read(base); }
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+            {
+                all += (float)tiles[b] * (float)blocks[b];
+                n_tiles += tiles[b];
+            }
+        }
+        if (a.n_seqs > 256) { read(0); }
+        all = reduce_lanes<16>(all, [](float u, float v) { return u + v; });
+        all = (__shfl(all, 0) + __shfl(all, 16)) + (__shfl(all, 32) + __shfl(all, 48));
+        n_tiles = __builtin_amdgcn_readlane(add_up_lanes(n_tiles), 63);
+        // (the sum's rounding counts upwards)
+        float per = fmaxf(all * 1.001f / (float)p.piece_slots, (float)PIECE_LEAST);
+        if (a.n_seqs <= 256 && n_tiles <= p.piece_slots)
+        {
+            auto fits = [&](float per) {
+                int pieces = 0;
+#pragma unroll
+                for (int b = 0; b < 4; b++) { pieces += tiles[b] * ranges_of(blocks[b], __builtin_amdgcn_rcpf(per)); }
+                return __builtin_amdgcn_readlane(add_up_lanes(pieces), 63) <= p.piece_slots;
+            };
+            for (int n = 0; n < 40 && !fits(per); n++) { per *= n < 10 ? 1.06f : 1.3f; }
+        }
+        by = __builtin_amdgcn_rcpf(per);
+        if (blockIdx.x == 0 && threadIdx.x == 0) { *p.piece_length() = by; }
+    }
+    int before = 0, split_before = 0;
+    for (int base = 0; base < a.n_seqs; base += 256)
+    {
+        if (base != 0) { read(base); }
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+        {
+            if (base + 64 * b >= a.n_seqs) { break; }
+            const int ranges = ranges_of(blocks[b], by), split_upto = split_before + add_up_lanes(ranges > 1 ? tiles[b] * ranges : 0);
+            const int upto = before + add_up_lanes(!ADDED ? tiles[b] * ranges : ranges > 1 ? tiles[b] : 0);
+            const unsigned long long past = __ballot(upto > piece);
+            if (past != 0)
+            {
+                const int at = __builtin_ctzll(past);
+                r.s = uniform(base + 64 * b + at);
+                r.mine = { __builtin_amdgcn_readlane(mine[b].first, at), __builtin_amdgcn_readlane(mine[b].n, at), __builtin_amdgcn_readlane(mine[b].pos, at) };
+                r.n_ranges = __builtin_amdgcn_readlane(ranges, at);
+                const int back = __builtin_amdgcn_readlane(upto, at) - 1 - piece, tile = ADDED ? back : back / r.n_ranges;
+                r.range = ADDED ? 0 : r.n_ranges - 1 - back % r.n_ranges;
+                r.piece0 = uniform(__builtin_amdgcn_readlane(split_upto, at) - (tile + 1) * r.n_ranges);
+                r.row0 = uniform(tile) * PA_TILE;
+                break;
+            }
+            before = __builtin_amdgcn_readlane(upto, 63);
+            split_before = __builtin_amdgcn_readlane(split_upto, 63);
+        }
+        if (r.s >= 0) { break; }
+    }
+    if (r.s < 0) { return r; }
+    r.n_rows = uniform(r.mine.n * p.group);
+    r.lo = uniform(r.mine.pos);
+    r.hi = uniform(r.mine.pos + r.mine.n - 1);
+    r.blocks = KeyBlocks<PA_TILE_KEYS>(p, r.lo, r.hi);
+    r.blocks.n = uniform(r.blocks.n);
+    r.blocks.sinks = uniform(r.blocks.sinks);
+    r.blocks.skip = uniform(r.blocks.skip);
+    r.n_ranges = uniform(r.n_ranges);
+    r.range = uniform(r.range);
+    r.per = (r.blocks.n + r.n_ranges - 1) / r.n_ranges;
     return r;
 }
 
@@ -858,7 +983,13 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     uint32_t* const odd_rows = (uint32_t*)(lds + F::ODD);                   // per buffer of values and wave that staged: something infinite or NaN
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int j = lane & 31, h = lane >> 5;
-    const Tile rows = find_tile<TREE>(a, p, tile);
+    Tile rows;
+    if constexpr (TREE)
+    {
+        rows = find_piece<false>(a, p, tile);
+        range = rows.range;
+    }
+    else { rows = find_tile(a, p, tile); }
     if (rows.s < 0 || range >= rows.n_ranges) { return; }
     const NewTokens mine = rows.mine;
     const auto& blocks = rows.blocks;
@@ -1247,12 +1378,12 @@ __device__ __forceinline__ void attend_tile(const PagedArgs& a, const PagedAtten
     const size_t at_row = (size_t)token * p.n_q + head;
     if (rows.n_ranges > 1)
     {
-        float* const dst = p.sums(range, at_row, DIM) + 4 * h;
+        float* const dst = (TREE ? p.piece_sums(rows.piece0 + range, kvh, a.n_kv, wave * 32 + j, DIM) : p.sums(range, at_row, DIM)) + 4 * h;
 #pragma unroll
         for (int d = 0; d < DIM / 32; d++)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) { *(f32x4*)(dst + 32 * d + 2 * e) = f32x4{ out[d][e], out[d][e + 1], out[d][e + 2], out[d][e + 3] }; }
-        if (h == 0) { *p.stats(range, at_row, DIM) = make_float2(m, total); }
+        if (h == 0) { *(TREE ? p.piece_stats(rows.piece0 + range, kvh, a.n_kv, wave * 32 + j, DIM) : p.stats(range, at_row, DIM)) = make_float2(m, total); }
         return;
     }
     uint16_t* const dst = p.y + (size_t)token * p.ldy + (size_t)head * DIM + 4 * h;
@@ -1287,14 +1418,14 @@ template <int DIM, bool TREE>
 __global__ __launch_bounds__(256) void paged_attention_combine_kernel(const PagedArgs a, const PagedAttention p)
 {
     const int kvh = blockIdx.x % a.n_kv, at = blockIdx.x / a.n_kv;
-    const Tile rows = find_tile<TREE>(a, p, at / 8);
+    const Tile rows = TREE ? find_piece<true>(a, p, at / 8) : find_tile(a, p, at / 8);
     const int row = rows.row0 + at % 8 * 16 + (threadIdx.x >> 4);
     if (rows.s < 0 || row >= rows.n_rows || rows.n_ranges <= 1) { return; }
     const size_t token = rows.mine.first + row / p.group, head = kvh * p.group + row % p.group, at_row = token * p.n_q + head;
     const int d0 = (threadIdx.x & 15) * (DIM / 16);
     add_parts<DIM, true>(rows.n_ranges, p.y + token * p.ldy + head * DIM + d0, [&](int i, const float*& from, const float*& stat) {
-        from = p.sums(i, at_row, DIM) + d0;
-        stat = (const float*)p.stats(i, at_row, DIM);
+        from = (TREE ? p.piece_sums(rows.piece0 + i, kvh, a.n_kv, row - rows.row0, DIM) : p.sums(i, at_row, DIM)) + d0;
+        stat = (const float*)(TREE ? p.piece_stats(rows.piece0 + i, kvh, a.n_kv, row - rows.row0, DIM) : p.stats(i, at_row, DIM));
     });
 }
 

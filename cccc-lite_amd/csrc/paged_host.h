@@ -114,6 +114,7 @@ struct Plan
     bool rows;
     int min_rows, row_slots, row_parts;
     size_t tile_bytes, row_bytes;   // of partial sums
+    int piece_slots;                 // trees (find_piece): tiles counts their pieces, at most, and how many run at once per kv head
 };
 
 // Ranges of keys for tiles that are few workgroups.  A tile takes 5 us and 1.35 per block of 64 keys where a CU has one workgroup, 2.15 for two side by side (heads of
@@ -138,14 +139,17 @@ inline int tile_ranges(long long workgroups, int blocks, size_t outputs, int dim
     return best;
 }
 
+// Workspace for each of the pieces per kv head that run at once.
+inline size_t piece_bytes(const PagedArgs& a, int dim) { return (size_t)2 * a.n_kv * 128 * (dim + 2) * 4; }
+
 // False: more than a launch can have.
-inline bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, int n_tokens, int max_new, int window, int n_sink, Plan& plan)
+inline bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int dim, int n_tokens, int max_new, int window, int n_sink, bool tree, Plan& plan)
 {
     const int group = n_q / a.n_kv;
     const long long rows = (long long)n_tokens * group, slots = 2LL * cu_count();
     // Sequences of up to 16 rows per kv head have a form of their own, also beside longer ones -- unless every sequence has max_new tokens, as far as
     // their number tells.
-    plan = { 0, 1, true, 0, 0, 0, 0, 0 };
+    plan = { 0, 1, true, 0, 0, 0, 0, 0, 0 };
     const long long keys = window == 0 ? a.max_ctx : std::min<long long>(a.max_ctx, (long long)window + n_sink + max_new);
     if ((long long)std::min(max_new, n_tokens) * group > PA_ROWS)
     {
@@ -155,8 +159,17 @@ inline bool plan_attention(const PagedArgs& a, int keys_per_block, int n_q, int 
         const long long tiles = (rows - cut) / 128 + cut;
         if (tiles * a.n_kv * 64 > MOST_BLOCKS) { return false; }
         plan.tiles = (int)tiles;
-        plan.tile_split = tile_ranges(tiles * a.n_kv, (int)((keys + PA_TILE_KEYS - 1) / PA_TILE_KEYS), (size_t)n_tokens * n_q, dim);
-        plan.tile_bytes = plan.tile_split > 1 ? ((size_t)n_tokens * n_q * plan.tile_split * (dim + 2) * 4 + 15) & ~(size_t)15 : 0;
+        if (tree)
+        {
+            plan.piece_slots = (int)std::max<long long>(1, slots / a.n_kv);
+            if ((tiles + plan.piece_slots) * a.n_kv * 64 > MOST_BLOCKS) { return false; }
+            plan.tile_bytes = 16 + plan.piece_slots * piece_bytes(a, dim);
+        }
+        else
+        {
+            plan.tile_split = tile_ranges(tiles * a.n_kv, (int)((keys + PA_TILE_KEYS - 1) / PA_TILE_KEYS), (size_t)n_tokens * n_q, dim);
+            plan.tile_bytes = plan.tile_split > 1 ? ((size_t)n_tokens * n_q * plan.tile_split * (dim + 2) * 4 + 15) & ~(size_t)15 : 0;
+        }
     }
     if (plan.rows)
     {
@@ -181,6 +194,14 @@ inline unsigned long long name_call()
     return name;
 }
 
+inline unsigned long long attention_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink, bool tree)
+{
+    PagedArgs a;
+    if (!attention_args(cache, a, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink) || n_tokens == 0) { return 0; }
+    Plan plan;
+    return plan_attention(a, keys_per_block(cache), n_q_heads, cache->head_dim, n_tokens, max_new, window, n_sink, tree, plan) ? plan.tile_bytes + plan.row_bytes : 0;
+}
+
 template <bool TREE>
 int launch_attention(const char* name, const hip_paged_kv* cache, const void* q, void* y, const unsigned long long* seen, long long seen_stride, void* workspace, unsigned long long workspace_bytes,
                      int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink, int ldq, int ldy)
@@ -195,26 +216,30 @@ int launch_attention(const char* name, const hip_paged_kv* cache, const void* q,
     if (n_tokens == 0) { return 0; }
     if (y == q) { return -1; }
     Plan plan;
-    if (!plan_attention(a, keys_per_block(cache), n_q_heads, dim, n_tokens, max_new, window, n_sink, plan)) { return -1; }
-    // too little workspace: tiles and sequences in one piece each
+    if (!plan_attention(a, keys_per_block(cache), n_q_heads, dim, n_tokens, max_new, window, n_sink, TREE, plan)) { return -1; }
+    // too little workspace: tiles and sequences in one piece each, tiles of trees in fewer
     if (workspace_bytes < plan.tile_bytes + plan.row_bytes)
     {
         plan.tile_split = 1;
         plan.tile_bytes = 0;
         if (workspace_bytes < plan.row_bytes) { plan.row_parts = 0; }
+        const size_t rest = workspace_bytes - (plan.row_parts ? plan.row_bytes : 0);
+        plan.piece_slots = plan.piece_slots == 0 || rest < 16 ? 0 : (int)((rest - 16) / piece_bytes(a, dim));
     }
+    const int most_added = TREE ? std::min(plan.tiles, plan.piece_slots) : plan.tiles;         // tiles in several ranges
+    plan.tiles += plan.piece_slots;
     const long long tiles = (long long)plan.tiles * a.n_kv * plan.tile_split, parts = plan.rows ? (long long)(plan.row_parts ? plan.row_parts : a.n_seqs) * a.n_kv : 0;
     // the workspace: the parts' words, sums and statistics, then the tiles'
     const size_t words = (size_t)plan.row_parts * a.n_kv;
     char* const part_sums = (char*)workspace + words * 8;
-    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)((char*)workspace + (plan.row_parts ? plan.row_bytes : 0)), (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv,
+    const PagedAttention p = { (const uint16_t*)q, (uint16_t*)y, (float*)((char*)workspace + (plan.row_parts ? plan.row_bytes : 0) + (TREE ? 16 : 0)), (size_t)ldq, (size_t)ldy, n_q_heads, n_q_heads / a.n_kv,
                                n_tokens, max_new, window, n_sink, plan.tiles, plan.tile_split, plan.row_slots, plan.row_parts, (float*)part_sums, (unsigned long long*)workspace,
-                               plan.row_parts ? name_call() : 0, plan.min_rows, tiles <= 2LL * cu_count() ? 1 : 0, 1.4426950408889634f / sqrtf((float)dim), seen, (size_t)seen_stride };
+                               plan.row_parts ? name_call() : 0, plan.min_rows, tiles <= 2LL * cu_count() ? 1 : 0, 1.4426950408889634f / sqrtf((float)dim), seen, (size_t)seen_stride, plan.piece_slots };
     const auto kernel = CCQ_PAGED_KERNEL(paged_attention_kernel, cache, TREE);
     kernel<<<(unsigned)(tiles + parts), 256, 0, stream()>>>(a, p);
-    if (plan.tile_split > 1)
+    if (plan.tile_split > 1 || plan.piece_slots > 0)
     {
-        const unsigned blocks = (unsigned)(plan.tiles * a.n_kv * 8);
+        const unsigned blocks = (unsigned)(most_added * a.n_kv * 8);
         if (dim == 64) { paged_attention_combine_kernel<64, TREE><<<blocks, 256, 0, stream()>>>(a, p); }
         else { paged_attention_combine_kernel<128, TREE><<<blocks, 256, 0, stream()>>>(a, p); }
     }

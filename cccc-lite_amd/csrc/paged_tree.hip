@@ -11,6 +11,11 @@ int hip_qk_norm_rope_kv_paged_at_bf16(const hip_paged_kv* cache, const void* q, 
                                ldk, ldv, epsilon);
 }
 
+unsigned long long hip_attention_paged_tree_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink)
+{
+    return attention_workspace_bytes(cache, n_q_heads, n_tokens, max_new, max_ctx, window, n_sink, true);
+}
+
 int hip_attention_paged_tree_bf16(const hip_paged_kv* cache, const void* q, void* y, const void* seen, long long seen_stride, void* workspace, unsigned long long workspace_bytes, int n_q_heads,
                                   int n_tokens, int max_new, int max_ctx, int window, int n_sink, int ldq, int ldy)
 {

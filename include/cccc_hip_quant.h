@@ -444,8 +444,9 @@ C_EXPORT int hip_qk_norm_rope_kv_paged_at_bf16(const hip_paged_kv* cache, const 
 /* hip_attention_paged_bf16 for tokens that do not see all new tokens in front of them: token t sees every row in front of its sequence's first new token, and new token j of its sequence
  * where bit j % 64 of word seen[t * seen_stride + j / 64] is set (uint64, 8-byte aligned; its own bit too if it is to see itself; bits from the sequence's number of new tokens on are not looked at).  seen_stride * 64 is max_new at least.
  * With window > 0 a token that sees n new tokens, itself among them, is taken to be n - 1 positions behind the first one (its depth, where it sees the tokens that it descends from), and
- * of the rows in front sees those less than `window` behind that position and the first n_sink ones; new tokens go by their bits alone.  Everything else as there, the workspace too
- * (hip_attention_paged_workspace_bytes). */
+ * of the rows in front sees those less than `window` behind that position and the first n_sink ones; new tokens go by their bits alone.  Everything else as there, but for the workspace: hip_attention_paged_tree_workspace_bytes;
+ * with less the keys are split over fewer workgroups. */
+C_EXPORT unsigned long long hip_attention_paged_tree_workspace_bytes(const hip_paged_kv* cache, int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink);
 C_EXPORT int hip_attention_paged_tree_bf16(const hip_paged_kv* cache, const void* q, void* y, const void* seen, long long seen_stride, void* workspace, unsigned long long workspace_bytes,
                                            int n_q_heads, int n_tokens, int max_new, int max_ctx, int window, int n_sink, int ldq, int ldy);
 

@@ -10,7 +10,7 @@ from test_gpu_paged_edges import odd_codes
 pytestmark = pytest.mark.gpu
 
 
-def run_tree(gpu, pkg, b, q, n_q, seen, window=0, n_sink=0, workspace=True, max_new=None, max_ctx=None, pad=0, extra=1, more=0, **other):
+def run_tree(gpu, pkg, b, q, n_q, seen, window=0, n_sink=0, workspace=1.0, max_new=None, max_ctx=None, pad=0, extra=1, more=0, **other):
     """Rows of y (one more than there are tokens, ending as they began).  seen: per sequence [n][n], or the words; bits behind hold anything, rows are `more` words longer."""
     torch, dev, lib = gpu
     tokens, dim = b.tokens, b.dim
@@ -24,8 +24,9 @@ def run_tree(gpu, pkg, b, q, n_q, seen, window=0, n_sink=0, workspace=True, max_
     qd[:tokens, :n_q * dim] = put(torch, dev, to_bf16(q).reshape(tokens, -1))
     y = torch.full((tokens + extra, ld), 0x1234, dtype=torch.int16, device=dev)
     cache = b.descriptor(pkg, **other)
-    need = lib.attention_paged_workspace_bytes(cache, n_q, tokens + extra, max_new, max_ctx, window, n_sink)
-    ws = torch.full((need + 16,), 0x7F, dtype=torch.uint8, device=dev) if workspace and need else None
+    need = lib.attention_paged_tree_workspace_bytes(cache, n_q, tokens + extra, max_new, max_ctx, window, n_sink)
+    need = int(need * workspace) & ~15
+    ws = torch.full((need + 16,), 0x7F, dtype=torch.uint8, device=dev) if need else None
     assert lib.attention_paged_tree(cache, ptr(qd), ptr(y), ptr(wd), stride, ptr(ws), need if ws is not None else 0, n_q, tokens + extra, max_new, max_ctx, window, n_sink, ld, ld) == 0
     torch.cuda.synchronize()
     if ws is not None: assert (ws[need:] == 0x7F).all()
@@ -46,7 +47,7 @@ def check_tree(gpu, pkg, b, n_q, seen, window=0, n_sink=0, q=None, rows=None, lo
 SHAPES = [  # dim, n_q, n_kv, page, new, ctx
     (128, 4, 1, 16, [1], [1]), (128, 4, 1, 16, [4], [4]), (64, 8, 1, 16, [2, 1, 0, 2], [64, 300, 20, 7]), (128, 8, 8, 32, [16, 3], [127, 513]), (128, 3, 1, 64, [5, 2], [33, 129]), (64, 10, 2, 16, [3, 1, 3], [3, 200, 70]),
     (128, 8, 2, 16, [13], [4108]), (128, 4, 1, 32, [129], [129]), (64, 4, 2, 64, [65, 1, 30], [465, 400, 90]), (128, 16, 1, 128, [9, 70], [500, 71]), (128, 2, 2, 16, [64, 3], [700, 64]), (64, 64, 1, 16, [1, 5], [90, 1030]),
-    (128, 4, 1, 16, [4, 60, 4], [64, 1500, 68])]
+    (128, 4, 1, 16, [4, 60, 4], [64, 1500, 68]), (64, 8, 2, 16, [33, 5, 70, 17], [2100, 1300, 70, 3000]), (128, 16, 4, 32, [26] * 5, [1700, 26, 130, 900, 2500])]
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -173,9 +174,9 @@ def test_workspaces(gpu, pkg, kind, dim, n_q, n_kv, page, new, ctx):
     b = Batch(sum(ctx) + kind, kind, dim, n_kv, page, new, ctx).upload(torch, dev)
     q, seen = from_bf16(to_bf16(b.rng.standard_normal((b.tokens, n_q, dim)))), trees(b.rng, new)
     want = check_tree(gpu, pkg, b, n_q, seen, q=q)
-    check_tree(gpu, pkg, b, n_q, seen, q=q, workspace=False)
+    for part in (0, 0.1, 0.5, 0.9): check_tree(gpu, pkg, b, n_q, seen, q=q, workspace=part)
     cache, stride = b.descriptor(pkg), -(-max(new) // 64)
-    need = lib.attention_paged_workspace_bytes(cache, n_q, b.tokens, max(new), max(ctx))
+    need = lib.attention_paged_tree_workspace_bytes(cache, n_q, b.tokens, max(new), max(ctx))
     qd, wd, y = put(torch, dev, to_bf16(q)), torch.from_numpy(bits(seen, stride)).to(dev), torch.zeros(b.tokens, n_q * dim, dtype=torch.int16, device=dev)
     first = None
     for i in range(100):
@@ -198,7 +199,7 @@ def test_a_captured_call_with_other_trees(gpu, pkg, kind):
     y = [torch.zeros(tokens, n_q * dim, dtype=torch.int16, device=dev) for _ in range(2)]
     words = torch.zeros(tokens, 1, dtype=torch.int64, device=dev)
     cache = b.descriptor(pkg)
-    need = lib.attention_paged_workspace_bytes(cache, n_q, tokens, tokens, most)
+    need = lib.attention_paged_tree_workspace_bytes(cache, n_q, tokens, tokens, most)
     spaces = [torch.full((need,), 0x55, dtype=torch.uint8, device=dev) for _ in range(2)]
     call = lambda i, ws: lib.attention_paged_tree(cache, ptr(q[i]), ptr(y[i]), ptr(words), 1, ptr(ws), need, n_q, tokens, tokens, most, 0, 0, n_q * dim, n_q * dim)  # noqa: E731
     stream = torch.cuda.Stream(device=dev)

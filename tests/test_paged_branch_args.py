@@ -38,6 +38,7 @@ def test_descriptors(setup, change):
     lib, capi, good, p, raw = setup
     c = capi.make_paged_kv(**(good | change))
     one = capi.paged_layers([c])
+    assert lib.attention_paged_tree_workspace_bytes(c, 4, 1, 1, 16) == 0
     assert at(lib, c, p) == tree(lib, c, p) == keep(lib, one, p) == fork(lib, one, p) == -1
     assert lib.kv_paged_fork_workspace_bytes(one, 1, 2) == 0
     assert not raw.any()
