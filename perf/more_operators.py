@@ -553,7 +553,7 @@ def _bound(s):
         ld, at = (n_q + 2 * n_kv) * dim, s["qkv"].data_ptr()
         return lib.qk_norm_rope_kv_paged_at, (cache, at, at + 2 * n_q * dim, at + 2 * (n_q + n_kv) * dim, ptr(s["norm_w"][0]), ptr(s["norm_w"][1]), ptr(s["cos"]), ptr(s["sin"]), s["cos"].shape[0],
                                               ptr(s["positions"]), c["axes"], s["positions"].stride(0), ptr(s["axis"]), ptr(s["q_out"]), n_q, s["tokens"], ld, ld, ld, EPS), (s["q_out"],) + _pool_values(s)
-    need = lib.attention_paged_workspace_bytes(cache, n_q, s["tokens"], s["max_new"], s["max_ctx"], c["window"], c["sinks"])
+    need = lib.attention_paged_tree_workspace_bytes(cache, n_q, s["tokens"], s["max_new"], s["max_ctx"], c["window"], c["sinks"])
     s["workspace"] = space(need)
     ld = n_q * dim
     return lib.attention_paged_tree, (cache, ptr(s["q"]), ptr(s["y"]), ptr(s["seen"]), s["seen"].shape[1], ptr(s["workspace"]), need, n_q, s["tokens"], s["max_new"], s["max_ctx"],
