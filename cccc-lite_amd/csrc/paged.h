@@ -185,41 +185,47 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedArgs a, co
         unpack4(*(const u32x2*)(nw + i * 4 + DIM / 2), w + 4);
     }
     u32x2 cs[TOKENS], sn[TOKENS];
-    bool out[TOKENS] = {};                                                  // AT: a position that no row of the tables has
-    uint32_t on_axis[2] = {};                                               // AT: the lane's pairs that lie on any axis
+    // AT: the tokens' positions, asked for in front of where they belong
+    int given[TOKENS][AT ? 4 : 1];
+    uint32_t axes = 0;
     if constexpr (AT)
     {
-        const uint32_t axes = p.axis ? *(const uint32_t*)(p.axis + i * 4) : 0;
+        axes = p.axis ? *(const uint32_t*)(p.axis + i * 4) : 0;             // of the lane's four pairs
 #pragma unroll
-        for (int n = 0; n < TOKENS; n++) { cs[n] = sn[n] = u32x2{ 0, 0 }; }
-        for (int x = 0; x < p.n_axes; x++)
+        for (int n = 0; n < TOKENS; n++)
         {
-            // which of the lane's pairs lie on axis x
-            uint32_t mine[2] = {};
 #pragma unroll
-            for (int e = 0; e < 4; e++) { mine[e / 2] |= (axes >> (8 * e) & 255u) == (uint32_t)x ? 0xFFFFu << (16 * (e & 1)) : 0u; }
-            on_axis[0] |= mine[0];
-            on_axis[1] |= mine[1];
-            int pos[TOKENS];
-#pragma unroll
-            for (int n = 0; n < TOKENS; n++) { pos[n] = p.positions[(size_t)x * p.position_stride + min(t0 + n, p.n_tokens - 1)]; }
-#pragma unroll
-            for (int n = 0; n < TOKENS; n++)
-            {
-                out[n] = out[n] || pos[n] < 0 || pos[n] >= p.n_positions;
-                const size_t from = (size_t)min(max(pos[n], 0), p.n_positions - 1) * (DIM / 2) + i * 4;
-                const u32x2 c = *(const u32x2*)(p.cos_tab + from), s = *(const u32x2*)(p.sin_tab + from);
-#pragma unroll
-                for (int d = 0; d < 2; d++)
-                {
-                    cs[n][d] |= c[d] & mine[d];
-                    sn[n][d] |= s[d] & mine[d];
-                }
-            }
+            for (int x = 0; x < 4; x++) { given[n][x] = x < p.n_axes ? p.positions[(size_t)x * p.position_stride + min(t0 + n, p.n_tokens - 1)] : 0; }
         }
     }
     const PagedPlaces<TOKENS> at(a, t0);
     const bool turns = p.cos_tab && !is_v;
+    if (AT && turns)
+    {
+        const bool alike = axes == (axes & 255u) * 0x01010101u;             // all four on one axis: 8 bytes of a row each of cosines and sines, else 2 bytes of four rows
+        auto row = [&](int n, uint32_t axis) {
+            const int pos = axis == 0 ? given[n][0] : axis == 1 ? given[n][AT ? 1 : 0] : axis == 2 ? given[n][AT ? 2 : 0] : given[n][AT ? 3 : 0];
+            return (size_t)min(max(pos, 0), p.n_positions - 1) * (DIM / 2) + i * 4;
+        };
+#pragma unroll
+        for (int n = 0; n < TOKENS; n++)
+        {
+            if (alike)
+            {
+                const size_t from = row(n, axes & 255u);
+                cs[n] = *(const u32x2*)(p.cos_tab + from);
+                sn[n] = *(const u32x2*)(p.sin_tab + from);
+                continue;
+            }
+#pragma unroll
+            for (int d = 0; d < 2; d++)
+            {
+                const size_t lo = row(n, axes >> (16 * d) & 255u) + 2 * d, hi = row(n, axes >> (16 * d + 8) & 255u) + 2 * d + 1;
+                cs[n][d] = p.cos_tab[lo] | (uint32_t)p.cos_tab[hi] << 16;
+                sn[n][d] = p.sin_tab[lo] | (uint32_t)p.sin_tab[hi] << 16;
+            }
+        }
+    }
     if (turns && !AT)
     {
 #pragma unroll
@@ -234,7 +240,13 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedArgs a, co
     for (int n = 0; n < TOKENS; n++)
     {
         const int t = t0 + n, pos = at.pos[n];
-        if (at.s[n] < 0 || t >= p.n_tokens || pos < 0 || (AT ? out[n] : p.cos_tab && pos >= p.n_positions) || spare) { continue; }
+        bool out = !AT && p.cos_tab && pos >= p.n_positions;                // a position that no row of the tables has
+        if constexpr (AT)
+        {
+#pragma unroll
+            for (int x = 0; x < 4; x++) { out = out || given[n][x] < 0 || given[n][x] >= p.n_positions; }
+        }
+        if (at.s[n] < 0 || t >= p.n_tokens || pos < 0 || out || spare) { continue; }
         float x[8];
         unpack4(raw[n][0], x);
         unpack4(raw[n][1], x + 4);
@@ -257,7 +269,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedArgs a, co
             for (int e = 0; e < 4; e++)
             {
                 const float lo = x[e], hi = x[e + 4];
-                if (AT && (on_axis[e / 2] >> (16 * (e & 1)) & 1) == 0) { continue; }
+                if (AT && (axes >> (8 * e) & 255u) >= (uint32_t)p.n_axes) { continue; }
                 x[e] = lo * c[e] - hi * s[e];
                 x[e + 4] = hi * c[e] + lo * s[e];
             }
