@@ -52,6 +52,15 @@ __device__ __forceinline__ Beam beam_state(const BeamSelect& p, int row)
     return p.last && p.last[row] == p.eos ? Beam::ENDED : Beam::ALIVE;
 }
 
+// Sum over 16 lanes.
+__device__ __forceinline__ int beam_sum16(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);           // quad_perm [1,0,3,2]
+    v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);           // quad_perm [2,3,0,1]
+    v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, true);          // row_half_mirror
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, true);    // row_mirror
+}
+
 template <class F>
 __device__ __forceinline__ uint32_t beam_reduce(uint32_t v, F f)
 {
@@ -225,12 +234,15 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_chunk_kernel(const BeamSele
     }
     uint32_t* const found = p.found + ((size_t)row * p.chunks + chunk) * p.n_out;
     for (int i = n + threadIdx.x; i < p.n_out; i += BEAM_THREADS) { found[i] = 0; }
-    for (int i = threadIdx.x; i < n; i += BEAM_THREADS)
+    // places by counting, 16 lanes for each
+    for (int i0 = 0; i0 < n; i0 += BEAM_THREADS / 16)
     {
-        const uint32_t of = list[i];
+        const int i = i0 + threadIdx.x / 16;
+        const uint32_t of = i < n ? list[i] : 0u;
         int rank = 0;
-        for (int j = 0; j < n; j++) { rank += list[j] > of; }
-        if (rank < p.n_out) { found[rank] = of; }
+        for (int j = threadIdx.x % 16; j < n; j += 16) { rank += list[j] > of; }
+        rank = beam_sum16(rank);
+        if (i < n && threadIdx.x % 16 == 0 && rank < p.n_out) { found[rank] = of; }
     }
 }
 
@@ -245,6 +257,13 @@ struct BeamRank
 // that n_out continuations reach, and few more do: those are ranked by counting.  Where more reach it than there is room for (equal totals, such as minus infinity), the ranks are gone
 // through byte by byte, by how many have each value, until just n_out reach the bytes found.  Grid: groups.
 constexpr int BEAM_ROOM = 512;
+
+// i / d for 0 <= i < 2^24, `by` next to 1 / d.
+__device__ __forceinline__ int beam_divided(int i, int d, float by)
+{
+    const int q = (int)((float)i * by), left = i - q * d;
+    return q + (left >= d ? 1 : 0) - (left < 0 ? 1 : 0);
+}
 
 template <int PER>
 __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const BeamSelect p)
@@ -295,10 +314,12 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
     }
     if (threadIdx.x == 0) { count = 0; }
     __syncthreads();
-    auto token_of = [&](int i, uint32_t of) { return i % per_row / p.n_out * CHUNK + (0xFFFF - (int)(of & 0xFFFFu)); };
+    const float by_row = 1.0f / (float)per_row, by_out = 1.0f / (float)p.n_out;
+    auto beam_of = [&](int i) { return beam_divided(i, per_row, by_row); };
+    auto token_of = [&](int i, int b, uint32_t of) { return beam_divided(i - b * per_row, p.n_out, by_out) * CHUNK + (0xFFFF - (int)(of & 0xFFFFu)); };
     auto rank_of = [&](int i, uint32_t of) {
         if (of == 0) { return BeamRank{ 0, 0 }; }
-        const int b = i / per_row;
+        const int b = beam_of(i);
         const uint32_t order = of >> 16;
         double total = -INFINITY;
         if (states[b] == Beam::ENDED && order == BEAM_MOST) { total = scores[b]; }
@@ -308,7 +329,7 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
             total = scores[b] + ((x == largest[b] ? 0.0 : x - largest[b]) - log_sum[b]);
         }
         const unsigned long long bits = __builtin_bit_cast(unsigned long long, total + 0.0);       // -0 is 0
-        return BeamRank{ bits >> 63 ? ~bits : bits | 1ull << 63, (unsigned long long)(0xFFFF - b) << 48 | (unsigned long long)order << 32 | (0xFFFFFFFFu - (uint32_t)token_of(i, of)) };
+        return BeamRank{ bits >> 63 ? ~bits : bits | 1ull << 63, (unsigned long long)(0xFFFF - b) << 48 | (unsigned long long)order << 32 | (0xFFFFFFFFu - (uint32_t)token_of(i, b, of)) };
     };
     BeamRank held[HELD];
 #pragma unroll
@@ -407,16 +428,18 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
         __syncthreads();
         n_picked = p.n_out;
     }
-    if ((int)threadIdx.x < n_picked)
+    for (int i0 = 0; i0 < n_picked; i0 += BEAM_PICK_THREADS / 16)
     {
-        const BeamRank mine = picked[threadIdx.x];
+        const int n = i0 + threadIdx.x / 16;
+        const BeamRank mine = picked[min(n, n_picked - 1)];
         int place = 0;
-        for (int j = 0; j < n_picked; j++) { place += picked[j] > mine; }
-        if (place < p.n_out)
+        for (int j = threadIdx.x % 16; j < n_picked; j += 16) { place += picked[j] > mine; }
+        place = beam_sum16(place);
+        if (n < n_picked && threadIdx.x % 16 == 0 && place < p.n_out)
         {
-            const int i = from[threadIdx.x], to = group * p.n_out + place;
-            p.parent_out[to] = row0 + i / per_row;
-            p.token_out[to] = token_of(i, found[i]);
+            const int i = from[n], to = group * p.n_out + place, b = beam_of(i);
+            p.parent_out[to] = row0 + b;
+            p.token_out[to] = token_of(i, b, found[i]);
             p.score_out[to] = (float)__builtin_bit_cast(double, mine.total >> 63 ? mine.total & ~(1ull << 63) : ~mine.total);
         }
     }
