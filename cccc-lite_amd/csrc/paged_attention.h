@@ -313,7 +313,7 @@ __device__ __forceinline__ Tile find_piece(const PagedArgs& a, const PagedAttent
         }
     };
     // ranges of `per` blocks, or so (the same for whoever asks)
-    auto ranges_of = [](int n, float by) { return max((int)ceilf((float)n * by - 0.001f), 1); };
+    auto ranges_of = [](int n, float by) { return max((int)ceilf(fmaf((float)n, by, -0.001f)), 1); };
     float by = 0.0f;                                                        // 1 / per
     const float left = ADDED ? *p.piece_length() : 0.0f;
     read(0);

@@ -127,7 +127,7 @@ def shared(b, rng, groups, prefix):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("dim,n_kv,page,ctx,n_layers", [(128, 1, 16, [1], 1), (64, 2, 16, [37, 33, 48, 64], 2), (128, 8, 32, [200, 200, 200, 200, 31, 32], 2), (64, 16, 64, [1000, 70, 5, 0, 64, 128, 129], 2), (128, 2, 4096, [5000, 4096], 1)])
+@pytest.mark.parametrize("dim,n_kv,page,ctx,n_layers", [(128, 1, 16, [1], 1), (64, 2, 16, [37, 33, 48, 64], 2), (128, 8, 32, [200, 200, 200, 200, 31, 32], 2), (64, 16, 64, [1000, 70, 5, 0, 64, 128, 129], 2), (64, 1, 4096, [5000, 4096], 1)])
 @pytest.mark.parametrize("case", ["beams", "same", "all of one", "parts", "fresh", "fewer", "more"])
 def test_fork(gpu, pkg, kind, dim, n_kv, page, ctx, n_layers, case):
     n = len(ctx)

@@ -263,3 +263,62 @@ def test_far_positions(gpu, pkg, kind):
             w /= w.sum()
             # a probability's and the result's rounding, 2^-8 each, and room for FP32
             assert (np.abs(got[t, h] - w @ v[see]) <= 2.0 ** -7 * (w @ np.abs(v[see])) + 2.0 ** -8 * np.abs(w @ v[see])).all()
+
+
+@pytest.mark.parametrize("kind", [BF16, E5M2])
+@pytest.mark.parametrize("n_seqs,big,n_q,n_kv", [(300, 3, 2, 1), (520, 7, 4, 1), (90, 1, 32, 8), (257, 1, 4, 4)])
+def test_many_sequences(gpu, pkg, kind, n_seqs, big, n_q, n_kv):
+    """More sequences than are looked up at once, every `big`-th one in tiles, and more tiles than run at once."""
+    rng = np.random.default_rng(n_seqs)
+    new = [int(rng.integers(34, 50)) if s % big == 0 else int(rng.integers(0, 5)) for s in range(n_seqs)] if n_seqs != 257 else [int(rng.integers(0, 17)) for _ in range(n_seqs)]
+    ctx = [n + int(rng.integers(0, 300)) for n in new]
+    ctx[n_seqs // 2] = new[n_seqs // 2] + 2000
+    b = Batch(n_seqs + kind, kind, 64, n_kv, 16, new, ctx).upload(*gpu[:2])
+    seen = trees(rng, new)
+    q = from_bf16(to_bf16(rng.standard_normal((b.tokens, n_q, 64))))
+    values = {name: b.values(name) for name in ("k", "v")}
+    rows = {name: [values[name][b.table[s, np.arange(c) // 16], :, np.arange(c) % 16].transpose(1, 0, 2) for s, c in enumerate(ctx)] for name in ("k", "v")}
+    got = [from_bf16(run_tree(gpu, pkg, b, q, n_q, seen, workspace=part)) for part in (1.0, 0.3, 0)]
+    few = np.zeros(b.tokens, dtype=bool)        # every third sequence and the long one, against the formula
+    for s in range(n_seqs):
+        if s % 3 == 0 or s == n_seqs // 2: few[b.seq_start[s]:b.seq_start[s + 1]] = True
+    for s in range(n_seqs):
+        if not (s % 3 == 0 or s == n_seqs // 2): b.new[s] = 0       # (the formula's; what lies on the device stays)
+    want, bound = tree_attend(b, q, n_q, seen, rows=rows)
+    for y in got:
+        assert (np.abs(y - want) <= bound)[few].all()
+        # the others: two results, each off by a weight's and a result's rounding, 2^-8 of a mean of |v| (under 4) and of itself
+        assert (np.abs(y - got[0])[~few] <= 2.0 ** -6 * np.abs(got[0])[~few] + 4 * 2.0 ** -6).all()
+
+
+def test_two_streams_at_once(gpu, pkg):
+    """Two batches on streams and workspaces of their own, calls among each other: the bits of calls alone."""
+    torch, dev, lib = gpu
+    sides = []
+    for i in range(2):
+        b = Batch(i, E4M3, 128, 2, 16, [40, 4, 20], [3000 - 900 * i, 700, 1500 + 400 * i]).upload(torch, dev)
+        q = put(torch, dev, to_bf16(b.rng.standard_normal((b.tokens, 8 * 128))))
+        cache, words = b.descriptor(pkg), torch.from_numpy(bits(trees(b.rng, b.new), 1)).to(dev)
+        need = lib.attention_paged_tree_workspace_bytes(cache, 8, b.tokens, 40, max(b.ctx))
+        sides.append((b, q, torch.zeros_like(q), cache, words, need, torch.zeros(need, dtype=torch.uint8, device=dev), torch.cuda.Stream(device=dev)))
+    def call(b, q, y, cache, words, need, ws, _):
+        assert lib.attention_paged_tree(cache, ptr(q), ptr(y), ptr(words), 1, ptr(ws), need, 8, b.tokens, 40, max(b.ctx), 0, 0, 1024, 1024) == 0
+    want = []
+    for s in sides:
+        call(*s)
+        torch.cuda.synchronize()
+        want.append(s[2].clone())
+    lib.set_sync(False)
+    try:
+        for _ in range(20):
+            for s in sides: s[2].zero_()
+            torch.cuda.synchronize()
+            for _ in range(5):
+                for s in sides:
+                    lib.set_stream(s[-1].cuda_stream)
+                    call(*s)
+            torch.cuda.synchronize()
+            for s, w in zip(sides, want): assert torch.equal(s[2], w)
+    finally:
+        lib.set_stream(None)
+        lib.set_sync(True)
