@@ -52,6 +52,29 @@ __device__ __forceinline__ Beam beam_state(const BeamSelect& p, int row)
     return p.last && p.last[row] == p.eos ? Beam::ENDED : Beam::ALIVE;
 }
 
+// A value of each lane added up, or its largest, over the wave.
+template <int CTRL>
+__device__ __forceinline__ double beam_dpp(double v)
+{
+    const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bits, CTRL, 0xF, 0xF, true), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double beam_lane(double v, int lane)
+{
+    const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+    return __builtin_bit_cast(double, (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(bits >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)bits, lane));
+}
+template <class F>
+__device__ __forceinline__ double beam_over_wave(double v, F f)
+{
+    v = f(v, beam_dpp<0xB1>(v));                                            // quad_perm [1,0,3,2]
+    v = f(v, beam_dpp<0x4E>(v));                                            // quad_perm [2,3,0,1]
+    v = f(v, beam_dpp<0x141>(v));                                           // row_half_mirror
+    v = f(v, beam_dpp<0x140>(v));                                           // row_mirror
+    return f(f(beam_lane(v, 0), beam_lane(v, 16)), f(beam_lane(v, 32), beam_lane(v, 48)));
+}
+
 // Sum over 16 lanes.
 __device__ __forceinline__ int beam_sum16(int v)
 {
@@ -189,8 +212,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_chunk_kernel(const BeamSele
     uint32_t from = beam_kth(best, p.n_out, top);
     const float all_m = beam_logit(top >> 16);
     double all = m == all_m ? (double)sum : all_m < INFINITY && sum > 0.0f ? (double)(sum * beam_exp(m - all_m)) : 0.0;
-#pragma unroll
-    for (int d = 32; d >= 1; d /= 2) { all += __shfl_xor(all, d); }
+    all = beam_over_wave(all, [](double a, double b) { return a + b; });
     if (lane == 0) { sums[threadIdx.x >> 6] = all; }
     if (mine >= from) { winners[atomicAdd(counts + 2, 1)] = threadIdx.x; }
     __syncthreads();
@@ -253,7 +275,7 @@ struct BeamRank
     __device__ __forceinline__ bool operator>(const BeamRank& o) const { return total > o.total || (total == o.total && then > o.then); }
 };
 
-// The n_out best of what the chunks of a group's rows left, whose lists are in order.  With j + 1 of each list at least as large as its j-th, as many lists as n_out needs give a bound
+// The n_out best of what the chunks of a group's rows left, whose lists are in order.  The n_out-th largest of the lists' first entries, 256 in all, is a bound
 // that n_out continuations reach, and few more do: those are ranked by counting.  Where more reach it than there is room for (equal totals, such as minus infinity), the ranks are gone
 // through byte by byte, by how many have each value, until just n_out reach the bytes found.  Grid: groups.
 constexpr int BEAM_ROOM = 512;
@@ -274,16 +296,15 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
     __shared__ int bins[256];
     __shared__ int chosen[3];                                               // the byte, how many are above it, and with it
     __shared__ BeamRank picked[BEAM_ROOM];
-    __shared__ int from[BEAM_ROOM];
     __shared__ uint32_t heads[256];
     __shared__ int count;
     const int group = blockIdx.x, row0 = group * p.n_beams, per_row = p.chunks * p.n_out, n_all = p.n_beams * per_row;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // asked for beside the statistics: what the thread keeps, and its list's entry for the bound, to which the first 256 lists go
+    // asked for beside the statistics: what the thread keeps, and an entry for the bound, of the first 256 lists as many of each as make 256
     const uint32_t* const found = p.found + (size_t)row0 * per_row;
-    const int n_lists = min(p.n_beams * p.chunks, 256), deep = (p.n_out + n_lists - 1) / n_lists - 1, head = threadIdx.x * p.n_out + deep;
+    const int n_lists = min(p.n_beams * p.chunks, 256), deep = min(256 / n_lists, p.n_out), head = (int)threadIdx.x / deep * p.n_out + (int)threadIdx.x % deep;
     const bool holds = n_all <= HELD * BEAM_PICK_THREADS;
-    uint32_t words[HELD], head_word = (int)threadIdx.x < n_lists ? found[head] : 0u;
+    uint32_t words[HELD], head_word = (int)threadIdx.x < n_lists * deep ? found[head] : 0u;
 #pragma unroll
     for (int n = 0; n < HELD; n++)
     {
@@ -297,13 +318,11 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
         const double2 mine = lane < p.chunks ? of[lane] : make_double2(-INFINITY, 0.0);
         m = mine.x;
         for (int c = lane + 64; c < p.chunks; c += 64) { m = fmax(m, of[c].x); }
-        const int span = min(p.chunks, 64);
-        for (int d = 1; d < span; d *= 2) { m = fmax(m, __shfl_xor(m, d)); }
-        m = __shfl(m, 0);
+        m = beam_over_wave(m, [](double a, double b) { return fmax(a, b); });
         auto part = [&](const double2& c) { return c.x == m ? c.y : m < INFINITY && c.y > 0.0 ? c.y * exp(c.x - m) : 0.0; };
         sum = part(mine);
         for (int c = lane + 64; c < p.chunks; c += 64) { sum += part(of[c]); }
-        for (int d = 1; d < span; d *= 2) { sum += __shfl_xor(sum, d); }
+        sum = beam_over_wave(sum, [](double a, double b) { return a + b; });
         if (lane == 0)
         {
             states[b] = beam_state(p, row0 + b);
@@ -338,27 +357,23 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
         if (holds)
         {
 #pragma unroll
-            for (int n = 0; n < HELD; n++) { f(n * BEAM_PICK_THREADS + (int)threadIdx.x, held[n]); }
+            for (int n = 0; n < HELD; n++) { f(held[n]); }
         }
         else
         {
-            for (int i = threadIdx.x; i < n_all; i += BEAM_PICK_THREADS) { f(i, rank_of(i, found[i])); }
+            for (int i = threadIdx.x; i < n_all; i += BEAM_PICK_THREADS) { f(rank_of(i, found[i])); }
         }
     };
     // the bound, of the totals' upper halves
     if (threadIdx.x < 256) { heads[threadIdx.x] = (uint32_t)(rank_of(head, head_word).total >> 32); }
     __syncthreads();
     uint32_t top;
-    const uint32_t bound = beam_kth(heads, (p.n_out + deep) / (deep + 1), top);
-    each([&](int i, const BeamRank& r) {
+    const uint32_t bound = beam_kth(heads, p.n_out, top);
+    each([&](const BeamRank& r) {
         if ((uint32_t)(r.total >> 32) >= bound && (r.total | r.then) != 0)
         {
             const int at = atomicAdd(&count, 1);
-            if (at < BEAM_ROOM)
-            {
-                picked[at] = r;
-                from[at] = i;
-            }
+            if (at < BEAM_ROOM) { picked[at] = r; }
         }
     });
     __syncthreads();
@@ -375,7 +390,7 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
             const int shift = 56 - byte % 8 * 8;
             if (threadIdx.x < 256) { bins[threadIdx.x] = 0; }
             __syncthreads();
-            each([&](int, const BeamRank& r) {
+            each([&](const BeamRank& r) {
                 const unsigned long long word = byte < 8 ? r.total : r.then, known = byte < 8 ? least.total : least.then;
                 const bool open = (byte < 8 || r.total == least.total) && (shift == 56 || word >> (shift + 8) == known >> (shift + 8));
                 if (open && (r.total | r.then) != 0) { atomicAdd(bins + (word >> shift & 255), 1); }
@@ -417,12 +432,11 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
             if (chosen[2] == need) { break; }
         }
         // all from `least` on, n_out of them
-        each([&](int i, const BeamRank& r) {
+        each([&](const BeamRank& r) {
             if (!(least > r) && (r.total | r.then) != 0)
             {
                 const int at = atomicAdd(&count, 1);
                 picked[at] = r;
-                from[at] = i;
             }
         });
         __syncthreads();
@@ -437,9 +451,9 @@ __global__ __launch_bounds__(BEAM_PICK_THREADS) void beam_pick_kernel(const Beam
         place = beam_sum16(place);
         if (n < n_picked && threadIdx.x % 16 == 0 && place < p.n_out)
         {
-            const int i = from[n], to = group * p.n_out + place, b = beam_of(i);
-            p.parent_out[to] = row0 + b;
-            p.token_out[to] = token_of(i, b, found[i]);
+            const int to = group * p.n_out + place;
+            p.parent_out[to] = row0 + 0xFFFF - (int)(mine.then >> 48);
+            p.token_out[to] = (int)(0xFFFFFFFFu - (uint32_t)mine.then);
             p.score_out[to] = (float)__builtin_bit_cast(double, mine.total >> 63 ? mine.total & ~(1ull << 63) : ~mine.total);
         }
     }
