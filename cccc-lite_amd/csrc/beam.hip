@@ -10,8 +10,8 @@ namespace
 {
 inline bool aligned(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-// Logits per thread: 64, and fewer where that leaves the GPU with less than two workgroups per CU.  MI355X us, both launches: 128 rows of 128256 logits, n_out 16, with 64 / 32 / 16 29.6 / 34.7 / 34.4;
-// 4 rows of 151936, n_out 4, with 8 (300 workgroups) 14.6.
+// Logits per thread: 64, and fewer where that leaves the GPU with less than two workgroups per CU.  MI355X us, both launches: 128 rows of 128256 logits, n_out 16, with 64 / 16 29.6 / 34.4 (26.9 with 64 since the groups' launch became
+// faster); 4 rows of 151936, n_out 4, with 8 (300 workgroups) 13.8.
 int logits_per_thread(int rows, int vocab)
 {
     int per = 64;
