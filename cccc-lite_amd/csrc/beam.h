@@ -178,7 +178,7 @@ __global__ __launch_bounds__(BEAM_THREADS) void beam_chunk_kernel(const BeamSele
     if (left >= CHUNK) { take(std::false_type()); }
     else { take(std::true_type()); }
     const Beam state = beam_state(p, row);
-    const int eos = state == Beam::ENDED ? p.eos - first : -1;
+    const int eos = state == Beam::ENDED && p.eos >= first && p.eos - first < left ? p.eos - first : -1;       // (a place behind the vocabulary would count for the bound)
     auto number = [](uint32_t order, int at) { return order << 16 | (uint32_t)(0xFFFF - at); };
     auto number_of = [&](uint32_t bits, int at) { return number(state == Beam::ALIVE ? beam_order(bits) : at == eos ? BEAM_MOST : BEAM_LEAST, at); };
     uint32_t mine = number((uint32_t)((largest >> 16) + 0x8000), place(threadIdx.x, 63 - (largest & 0xFFFF)));
