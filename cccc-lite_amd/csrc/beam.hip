@@ -24,7 +24,8 @@ int chunks_of(int vocab, int per) { return (vocab + BEAM_THREADS * per - 1) / (B
 bool beam_sizes(int n_groups, int n_beams, int vocab, int n_out)
 {
     if (n_groups < 0 || n_beams <= 0 || n_beams > 64 || vocab <= 0 || vocab > 1 << 20 || n_out <= 0 || n_out > 128 || n_out > (long long)n_beams * vocab) { return false; }
-    return (long long)n_groups * n_beams * chunks_of(vocab, 8) <= 0xFFFFFF;
+    // grids of fewer than 2^32 lanes: of 256 for each chunk, of 1024 for each group
+    return (long long)n_groups * n_beams * chunks_of(vocab, 8) <= 0xFFFFFF && (long long)n_groups * BEAM_PICK_THREADS <= 0xFFFFFFFFLL;
 }
 
 template <int PER>
