@@ -46,11 +46,12 @@ unsigned long long hip_beam_select_workspace_bytes(int n_groups, int n_beams, in
 int hip_beam_select_bf16(const void* logits, long long ld, const void* score, const void* last, int eos, int n_groups, int n_beams, int vocab, int n_out, void* parent_out, void* token_out,
                          void* score_out, void* workspace, unsigned long long workspace_bytes)
 {
-    if (!beam_sizes(n_groups, n_beams, vocab, n_out) || !logits || !parent_out || !token_out || !score_out || !workspace || ld < vocab || ld % 8 != 0) { return -1; }
+    if (!beam_sizes(n_groups, n_beams, vocab, n_out)) { return -1; }
+    if (n_groups == 0) { return 0; }
+    if (!logits || !parent_out || !token_out || !score_out || !workspace || ld < vocab || ld % 8 != 0) { return -1; }
     if (!aligned(logits, 16) || !aligned(workspace, 16) || !aligned(score, 4) || !aligned(last, 4) || !aligned(parent_out, 4) || !aligned(token_out, 4) || !aligned(score_out, 4)) { return -1; }
     if (n_out != n_beams && (score_out == score || token_out == last)) { return -1; }
     if (workspace_bytes < hip_beam_select_workspace_bytes(n_groups, n_beams, vocab, n_out)) { return -1; }
-    if (n_groups == 0) { return 0; }
     const int rows = n_groups * n_beams, per = logits_per_thread(rows, vocab), chunks = chunks_of(vocab, per);
     double2* const stats = (double2*)workspace;
     const BeamSelect p = { (const uint16_t*)logits, (size_t)ld, (const float*)score, (const int*)last, eos, n_groups, n_beams, vocab, n_out, chunks, (int*)parent_out, (int*)token_out,

@@ -477,7 +477,8 @@ C_EXPORT int hip_kv_paged_fork(const hip_paged_kv* caches, int n_layers, int n_o
  *   last int32 [n_groups * n_beams] (NULL: none): a beam whose last token is `eos` has ended and goes on with eos at its score alone.  A beam whose score is not finite has not begun.  Continuations that cannot be (other
  * tokens of an ended beam, all of one that has not begun, logits of minus infinity or NaN) have minus infinity and come last, by beam and token; a logit of plus infinity leaves its beam's finite ones no weight.
  * n_beams up to 64, n_out up to 128 and n_beams * vocab, vocab up to 1048576, n_groups up to 4194303, n_groups * n_beams times the started 2048s of vocab up to 16777215 (else -1, and 0 bytes).  score_out may be score and token_out last if n_out is n_beams; other overlaps are not allowed.
- * workspace: hip_beam_select_workspace_bytes bytes, 16-byte aligned, content of no matter; calls that share one must be ordered.  logits 16-byte aligned.  0 for n_groups 0. */
+ * workspace: hip_beam_select_workspace_bytes bytes, 16-byte aligned, content of no matter; calls that share one must be ordered.  logits 16-byte aligned.  0 for n_groups 0, whatever
+ * the buffers (NULL too). */
 C_EXPORT unsigned long long hip_beam_select_workspace_bytes(int n_groups, int n_beams, int vocab, int n_out);
 C_EXPORT int hip_beam_select_bf16(const void* logits, long long ld, const void* score, const void* last, int eos, int n_groups, int n_beams, int vocab, int n_out,
                                   void* parent_out, void* token_out, void* score_out, void* workspace, unsigned long long workspace_bytes);

@@ -22,3 +22,13 @@ def test_beam_groups(setup):
         for groups in (4194304, 5000000, 16777215 // beams):
             assert lib.beam_select_workspace_bytes(groups, beams, vocab, 1) == 0 and select(lib, p, groups, beams, vocab) == -1, (groups, beams, vocab)
     assert not raw.any()
+
+
+def test_no_groups(setup):
+    """The workspace of no groups is 0 bytes, and its call has nothing to do, whatever the buffers."""
+    lib, _, p, raw = setup
+    assert lib.beam_select_workspace_bytes(0, 4, 1000, 4) == 0
+    nothing = dict(logits=None, score=None, last=None, parent=None, token=None, out=None)
+    assert select(lib, p, 0, 4, 1000, 4, ws=None, nb=0) == 0 and select(lib, p, 0, 4, 1000, 4, ws=None, nb=0, **nothing) == 0
+    assert select(lib, p, 0, 65, 1000, 4, ws=None, nb=0) == select(lib, p, 0, 4, 0, 4, ws=None, nb=0) == -1
+    assert not raw.any()
