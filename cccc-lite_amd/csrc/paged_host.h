@@ -14,6 +14,12 @@ constexpr long long MOST_BLOCKS = 0xFFFFFF;        // of 256 lanes: a grid has f
 
 inline bool aligned(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
+// Whether two buffers of so many bytes have any in common (NULL: none).
+inline bool overlap(const void* a, unsigned long long n_a, const void* b, unsigned long long n_b)
+{
+    return a && b && n_a && n_b && (uintptr_t)a < (uintptr_t)b + n_b && (uintptr_t)b < (uintptr_t)a + n_a;
+}
+
 // The descriptor as the kernels take it; false: refused.
 inline bool paged_args(const hip_paged_kv* c, PagedArgs& a)
 {

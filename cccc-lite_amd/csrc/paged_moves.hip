@@ -48,7 +48,14 @@ int hip_kv_paged_keep(const hip_paged_kv* caches, int n_layers, const void* keep
 {
     PagedArgs a;
     if (!layers_args(caches, n_layers, a) || !keep || !n_keep || n_tokens < 0 || max_new <= 0) { return -1; }
-    if (!aligned(keep, 4) || !aligned(n_keep, 4) || !aligned(ctx_out, 4) || ctx_out == caches->ctx_len) { return -1; }
+    if (!aligned(keep, 4) || !aligned(n_keep, 4) || !aligned(ctx_out, 4)) { return -1; }
+    // the lengths are written while other workgroups, and launches for further layers, read these
+    const unsigned long long n = 4ull * a.n_seqs;
+    if (overlap(ctx_out, n, keep, 4ull * n_tokens) || overlap(ctx_out, n, n_keep, n) || overlap(ctx_out, n, a.ctx_len, n) || overlap(ctx_out, n, a.seq_start, n + 4) ||
+        overlap(ctx_out, n, a.table, n * a.table_stride))
+    {
+        return -1;
+    }
     if (n_tokens == 0 && !ctx_out) { return 0; }
     const long long per_layer = 2LL * a.n_seqs;
     for (int first = 0; first < n_layers;)

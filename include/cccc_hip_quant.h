@@ -453,8 +453,8 @@ C_EXPORT int hip_attention_paged_tree_bf16(const hip_paged_kv* cache, const void
 /* The entries below take the caches of all layers of a model, `caches` in host memory, n_layers of them: alike but for k, v, k_scale and v_scale (else -1). */
 
 /* Of the new tokens of sequence s those at keep[seq_start[s] + i], i < n_keep[s] (int32, counted from its first new token, ascending), stay: the i-th one's row moves to where new token i is, in
- * all layers.  An index below its place i, or not below the sequence's number of new tokens, moves nothing; n_keep beyond that number is cut to it.  ctx_out int32 [n_seqs], not ctx_len itself (NULL: none):
- * the rows left, ctx_len less the tokens that do not stay.  A sequence with more new tokens than max_new is left as it is, its ctx_len too.  Rows behind the
+ * all layers.  An index below its place i, or not below the sequence's number of new tokens, moves nothing; n_keep beyond that number is cut to it.  ctx_out int32 [n_seqs], a buffer of its own (NULL: none; -1 where
+ * it overlaps keep, n_keep, ctx_len, seq_start or page_table): the rows left, ctx_len less the tokens that do not stay.  A sequence with more new tokens than max_new is left as it is, its ctx_len too.  Rows behind the
  * kept ones hold anything afterwards.  Pages that new tokens lie in belong to one sequence; rows whose source or place has no page do not move.  0 for n_tokens 0 without ctx_out. */
 C_EXPORT int hip_kv_paged_keep(const hip_paged_kv* caches, int n_layers, const void* keep, const void* n_keep, int n_tokens, int max_new, void* ctx_out);
 

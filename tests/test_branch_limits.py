@@ -32,3 +32,24 @@ def test_no_groups(setup):
     assert select(lib, p, 0, 4, 1000, 4, ws=None, nb=0) == 0 and select(lib, p, 0, 4, 1000, 4, ws=None, nb=0, **nothing) == 0
     assert select(lib, p, 0, 65, 1000, 4, ws=None, nb=0) == select(lib, p, 0, 4, 0, 4, ws=None, nb=0) == -1
     assert not raw.any()
+
+
+N_SEQS, STRIDE, TOKENS, LAYERS = 5, 6, 40, 3
+# where each buffer of a call begins, and its bytes
+AT = {"page_table": (4096, 4 * N_SEQS * STRIDE), "ctx_len": (8192, 4 * N_SEQS), "seq_start": (12288, 4 * N_SEQS + 4), "keep": (16384, 4 * TOKENS), "n_keep": (20480, 4 * N_SEQS)}
+
+
+def caches(capi, p):
+    one = capi.make_paged_kv(type=4, head_dim=128, n_kv_heads=2, page_size=16, n_pages=9, k=p, v=p, page_table=p + AT["page_table"][0], table_stride=STRIDE, ctx_len=p + AT["ctx_len"][0], seq_start=p + AT["seq_start"][0],
+                             n_seqs=N_SEQS, k_scale=p, v_scale=p)
+    return capi.paged_layers([one] * LAYERS)
+
+
+@pytest.mark.parametrize("name", ["page_table", "ctx_len", "seq_start", "keep", "n_keep"])
+def test_keep_writes_none_of_what_it_reads(setup, name):
+    """All workgroups of all layers read these; the lengths that are left are written by some of them."""
+    lib, capi, p, raw = setup
+    begin, size = AT[name]
+    for out in (begin, begin + 4, begin + size - 4, begin - 4, begin - 4 * N_SEQS + 4):
+        assert lib.kv_paged_keep(caches(capi, p), LAYERS, p + AT["keep"][0], p + AT["n_keep"][0], TOKENS, 8, p + out) == -1, out - begin
+    assert not raw.any()
