@@ -1,6 +1,7 @@
 // C-ABI entry points that move rows and pages of a paged key / value cache in all layers (kernels in paged_moves.h).
 #include "paged_host.h"
 #include "paged_moves.h"
+#include <iterator>
 
 using namespace ccq;
 
@@ -84,7 +85,24 @@ int hip_kv_paged_fork(const hip_paged_kv* caches, int n_layers, int n_out, const
     {
         if (!aligned(p, 4)) { return -1; }
     }
-    if ((long long)n_out * a.table_stride > 0x3FFFFFFFLL || !aligned(workspace, 16) || table_out == caches->page_table || ctx_out == caches->ctx_len || workspace_bytes < hip_kv_paged_fork_workspace_bytes(caches, n_layers, n_out)) { return -1; }
+    const unsigned long long need = hip_kv_paged_fork_workspace_bytes(caches, n_layers, n_out);
+    if ((long long)n_out * a.table_stride > 0x3FFFFFFFLL || !aligned(workspace, 16) || workspace_bytes < need) { return -1; }
+    // what a launch writes, the next one and other workgroups still read beside
+    struct Buffer
+    {
+        const void* at;
+        unsigned long long bytes;
+    };
+    const unsigned long long n = 4ull * n_out, n_old = 4ull * a.n_seqs;
+    const Buffer buffers[] = { { table_out, n * a.table_stride }, { ctx_out, n }, { missing, 4 }, { workspace, need },       // written
+                               { parent, n }, { rows, n }, { grow, n }, { reserved, (unsigned long long)a.n_pages }, { a.table, n_old * a.table_stride }, { a.ctx_len, n_old } };
+    for (int i = 0; i < 4; i++)
+    {
+        for (const Buffer* b = buffers + i + 1; b != std::end(buffers); b++)
+        {
+            if (overlap(buffers[i].at, buffers[i].bytes, b->at, b->bytes)) { return -1; }
+        }
+    }
     char* at = (char*)workspace;
     PagedFork f = { (const int*)parent, (const int*)rows, (const int*)grow, (const uint8_t*)reserved, (int*)table_out, (int*)ctx_out, (int*)missing, n_out };
     f.n_free = (int*)at;

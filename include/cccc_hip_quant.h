@@ -465,7 +465,7 @@ C_EXPORT int hip_kv_paged_keep(const hip_paged_kv* caches, int n_layers, const v
  *   New pages are those that no sequence of the new batch has taken over and that are not reserved (bytes [n_pages], not 0: reserved; NULL: none), lowest first, handed out in the order
  * of the sequences, to each its last page first.  So a sequence that nobody takes over is freed, and pages that the caller holds for other ends are to be reserved.
  *   Where pages run out, entries of table_out are -1 and counted in `missing` (0 otherwise).  Entries taken over that are no page are -1, those behind a sequence's pages too.
- * table_out and ctx_out are buffers of their own, not those of the caches.  workspace: hip_kv_paged_fork_workspace_bytes bytes, 16-byte aligned, content between calls of no matter; calls that
+ * table_out, ctx_out, missing and the workspace overlap neither each other nor the arrays that the call reads, those of the caches among them (else -1).  workspace: hip_kv_paged_fork_workspace_bytes bytes, 16-byte aligned, content between calls of no matter; calls that
  * share one must be ordered.  n_out up to 65536, n_out * table_stride below 2^30.  The new batch in place of the old one, a descriptor per layer with table_out and ctx_out serves the next step. */
 C_EXPORT unsigned long long hip_kv_paged_fork_workspace_bytes(const hip_paged_kv* caches, int n_layers, int n_out);
 C_EXPORT int hip_kv_paged_fork(const hip_paged_kv* caches, int n_layers, int n_out, const void* parent, const void* rows, const void* grow, const void* reserved,

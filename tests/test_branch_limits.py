@@ -53,3 +53,25 @@ def test_keep_writes_none_of_what_it_reads(setup, name):
     for out in (begin, begin + 4, begin + size - 4, begin - 4, begin - 4 * N_SEQS + 4):
         assert lib.kv_paged_keep(caches(capi, p), LAYERS, p + AT["keep"][0], p + AT["n_keep"][0], TOKENS, 8, p + out) == -1, out - begin
     assert not raw.any()
+
+
+N_OUT = 7
+FORK = {"page_table": AT["page_table"], "ctx_len": AT["ctx_len"], "parent": (24576, 4 * N_OUT), "rows": (25600, 4 * N_OUT), "grow": (26624, 4 * N_OUT), "reserved": (27648, 9),
+        "table_out": (32768, 4 * N_OUT * STRIDE), "ctx_out": (36864, 4 * N_OUT), "missing": (40960, 4), "workspace": (45056, None)}
+
+
+@pytest.mark.parametrize("written", ["table_out", "ctx_out", "missing", "workspace"])
+@pytest.mark.parametrize("name", list(FORK))
+def test_fork_writes_none_of_what_it_reads(setup, written, name):
+    """The second launch reads parents, rows, growth, lengths and tables anew; what is written lies in buffers of its own."""
+    lib, capi, p, raw = setup
+    if written == name: return
+    c = caches(capi, p)
+    need = lib.kv_paged_fork_workspace_bytes(c, LAYERS, N_OUT)
+    size = lambda n: FORK[n][1] or need  # noqa: E731
+    step = 16 if written == "workspace" else 4
+    begin, end = FORK[name][0], FORK[name][0] + size(name)
+    for first in {begin, (end - 1) // step * step, (begin - size(written)) // step * step + step}:      # its first byte, its last, what ends in it
+        a = {n: p + FORK[n][0] for n in FORK} | {written: p + first}
+        assert lib.kv_paged_fork(c, LAYERS, N_OUT, a["parent"], a["rows"], a["grow"], a["reserved"], a["table_out"], a["ctx_out"], a["missing"], a["workspace"], need) == -1, (first - begin)
+    assert not raw.any()
