@@ -122,8 +122,8 @@ __device__ __forceinline__ float beam_exp(float d) { return __builtin_amdgcn_exp
 
 // A chunk of 256 PER logits of a row, PER of them per thread, eight side by side; PER <= 64.  Each logit is seen once, as it arrives: the thread's largest number, and its sum
 // beside its largest logit so far (FP32 exponentials of exact differences, errors of both signs: the logarithm of a row's sum is off by 2e-9 to 6e-8 on average, over rows of five distributions).  The few threads that reach the
-// bound have their logits read once more, from the L2.  MI355X, 128 rows of 128256 logits 17.6 us (33 MB: 1.9 TB/s): all workgroups run at once, so that loads (6 us by their bytes), some 12 instructions
-// per logit (5 us by their count) and the search for the best come one after the other.  Grid: rows x chunks.  LDS: two lists of numbers.
+// bound have their logits read once more, from the L2.  MI355X, 128 rows of 128256 logits 17.6 us (33 MB: 1.9 TB/s): all workgroups run at once, so that loads (6 us by their bytes), the arithmetic
+// and the search for the best come one after the other: 17.6 vector instructions per logit, counted over the launch, 7 us of their issue.  Grid: rows x chunks.  LDS: two lists of numbers.
 template <int PER>
 __global__ __launch_bounds__(BEAM_THREADS) void beam_chunk_kernel(const BeamSelect p)
 {

@@ -574,6 +574,8 @@ __device__ __forceinline__ void add_parts(int n, uint16_t* y, Part part)
 //           of 16.  FP8 keys become BF16 in registers, times their power of two (a lane's operand is one key's): exact.
 //   V p:    the eight weights of a lane in 32 keys (4 g .. + 3 and 16 + 4 g .. + 3) are its column operand as they are; the row operand (dim, the same
 //           keys) comes from transposing reads.  FP8 values' powers of two go to the weights.
+// Weights are rounded to BF16 for that product, their sum is of the FP32 ones: the matrix cores' FP32 product has a sixteenth of BF16's rate.  At most half a step, 2^-8 of a weight, errors of both signs: trees of 4
+// to 60 tokens differ from 64 bits by 2.2e-3 - 2.3e-3 of the results' size, where FP32 weights leave the 1.7e-3 of the results' own rounding.
 // Rows are read once per kv head and kept out of the way of what is read again (nt): 64 sequences 114 us for 124 without.
 // LDS: chunk c (16 bytes) of row r lies at c ^ swizzle(r), so that the operand reads hit all banks.
 template <int TYPE, int DIM>
@@ -966,6 +968,7 @@ __device__ __forceinline__ void attend_part(const PagedArgs& a, const PagedAtten
 //           8 (i / 4) + 4 h + i % 4 of 32.
 //   V p:    registers 8 u .. + 7 of a lane are its column operand of the u-th 16 keys as they are; the row operand (dim, the same keys) comes from
 //           two transposing reads.
+// Weights are rounded to BF16 for that product as in the form above, and for its reason.
 // A row's statistics and sums stay in the two lanes that have it.
 template <int TYPE, int DIM>
 struct TileForm

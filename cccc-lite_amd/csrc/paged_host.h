@@ -145,7 +145,8 @@ inline int tile_ranges(long long workgroups, int blocks, size_t outputs, int dim
     return best;
 }
 
-// Workspace for each of the pieces per kv head that run at once.
+// Workspace for each of the pieces per kv head that run at once: two, since tiles of little more than one range's keys are in two.  Every slot has them,
+// whatever the call's lengths (8 kv heads of 128 on 256 CUs: 68 MB).
 inline size_t piece_bytes(const PagedArgs& a, int dim) { return (size_t)2 * a.n_kv * 128 * (dim + 2) * 4; }
 
 // False: more than a launch can have.
