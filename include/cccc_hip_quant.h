@@ -473,7 +473,8 @@ C_EXPORT int hip_kv_paged_fork(const hip_paged_kv* caches, int n_layers, int n_o
 
 /* The n_out best continuations of each of n_groups groups of n_beams beams: of beam b by token v with score[b] + log softmax(logits[b])[v], v < vocab.  logits BF16 [n_groups * n_beams] rows
  * with pitch ld (a multiple of 8), score FP32 [n_groups * n_beams] (NULL: zeros).  Per group, best first: parent_out int32 (the row, counted through all groups, so that hip_kv_paged_fork
- * takes it as it is), token_out int32 and score_out FP32, [n_groups][n_out] each.  Sums are compared in 64 bits, within a beam the logits themselves; equal ones go to the lower beam, then the lower token.
+ * takes it as it is), token_out int32 and score_out FP32, [n_groups][n_out] each.  Totals are compared in 64 bits, within a beam the logits themselves; equal ones go to the lower beam, then the lower token.
+ * The sum under a beam's logarithm is of FP32 exponentials: it moves all totals of the beam by some 1e-8 (7e-6 at most), the same for rows that are the same, so that beams of other logits closer than that may come in either order.
  *   last int32 [n_groups * n_beams] (NULL: none): a beam whose last token is `eos` has ended and goes on with eos at its score alone.  A beam whose score is not finite has not begun.  Continuations that cannot be (other
  * tokens of an ended beam, all of one that has not begun, logits of minus infinity or NaN) have minus infinity and come last, by beam and token; a logit of plus infinity leaves its beam's finite ones no weight.
  * n_beams up to 64, n_out up to 128 and n_beams * vocab, vocab up to 1048576, n_groups up to 4194303, n_groups * n_beams times the started 2048s of vocab up to 16777215 (else -1, and 0 bytes).  score_out may be score and token_out last if n_out is n_beams; other overlaps are not allowed.
