@@ -75,3 +75,18 @@ def test_fork_writes_none_of_what_it_reads(setup, written, name):
         a = {n: p + FORK[n][0] for n in FORK} | {written: p + first}
         assert lib.kv_paged_fork(c, LAYERS, N_OUT, a["parent"], a["rows"], a["grow"], a["reserved"], a["table_out"], a["ctx_out"], a["missing"], a["workspace"], need) == -1, (first - begin)
     assert not raw.any()
+
+
+def test_fork_arguments(setup):
+    """Each argument by itself, all buffers apart."""
+    lib, capi, p, raw = setup
+    c = caches(capi, p)
+    need = lib.kv_paged_fork_workspace_bytes(c, LAYERS, N_OUT)
+    def call(n_layers=LAYERS, n_out=N_OUT, nb=need, **other):
+        a = {n: p + FORK[n][0] for n in FORK} | other
+        return lib.kv_paged_fork(c, n_layers, n_out, a["parent"], a["rows"], a["grow"], a["reserved"], a["table_out"], a["ctx_out"], a["missing"], a["workspace"], nb)
+    missing = [{n: None} for n in ("parent", "grow", "table_out", "ctx_out", "missing", "workspace")]
+    odd = [{n: p + FORK[n][0] + by} for n in ("parent", "rows", "grow", "table_out", "ctx_out", "missing") for by in (1, 2)] + [dict(workspace=p + FORK["workspace"][0] + by) for by in (4, 8)]
+    for bad in missing + odd + [dict(nb=need - 1), dict(nb=0), dict(n_out=0), dict(n_out=-1), dict(n_out=65537, nb=1 << 40), dict(n_layers=0), dict(n_layers=65537)]:
+        assert call(**bad) == -1, bad
+    assert not raw.any()
